@@ -505,6 +505,65 @@ typedef struct tsg_rollout {
  * appended point, then one to notice that it is finished: P + max(20, default_len) steps finish every row. */
 int tsg_rollout_run(const tsg_model* m, const tsg_graph* g, const tsg_rollout* r, int32_t n_steps, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Operators over sequences, for fitting function G on whole trajectories (and for models built next to it): dropout
+ * with a recomputed mask, causal attention over packed sequences, cross entropy over the road vocabulary.
+ * ------------------------------------------------------------------------------------------ */
+#define TSG_F32 0
+#define TSG_BF16 1
+#define TSG_F16 2
+
+/* y[i] = keep(i) ? x[i] / (1 - p) : 0 for i in [0, n).  keep(i): word i & 3 of Philox4x32-10 with the key `seed` and the
+ * counter (i / 4 as 64 bits, site, step) is >= floor(p 2^32).  The mask is a function of (seed, site, step, i) alone and is
+ * stored nowhere: the backward is the same call on the gradient.  `site` tells the dropouts of a model apart, `step` the
+ * training steps; step_dev, when non-NULL, is a device int64 whose low 32 bits are used instead of `step`, so that
+ * a captured graph can advance it.  x may equal y; otherwise they must not overlap.  p == 1 drops everything. */
+typedef struct tsg_dropout_desc {
+  int64_t n;
+  int32_t dtype;           /* TSG_F32 / TSG_BF16 / TSG_F16 */
+  uint32_t site, step, reserved;
+  uint64_t seed;
+  double p;                /* in [0, 1] */
+  const int64_t* step_dev; /* or NULL */
+  const void* x;
+  void* y;
+} tsg_dropout_desc;
+
+int tsg_dropout(const tsg_dropout_desc* d, void* stream);
+
+/* Causal attention over packed sequences.  Sequence s has the query rows [q_ptr[s], q_ptr[s+1]) and the keys
+ * [k_ptr[s], k_ptr[s+1]) (device int32, non-decreasing; the two may be one array); its last row sees its last key, a row i
+ * places before it one key fewer for each place (so one row per sequence over a kept cache is the single-token form).
+ * Query head h reads key-value head h / (heads / kv_heads).  Rows that see no key, rows behind the last sequence
+ * and keys that nothing sees give zeros.  Pointer values outside the arrays are clamped to them, never followed.
+ * Strides are in elements, >= 0; the width runs contiguously.  Base addresses are 16-byte aligned, strides and dim
+ * multiples of 8 (16-bit types) or 4 (f32).  dim <= 512; n_q * heads and n_k * kv_heads below 2^31.
+ * stats [heads][n_q][2] f32 is written by the forward (a row's largest q.k, and the base-2 logarithm of the sum of
+ * exp(scale (q.k - largest)); 0 and +inf where a row sees nothing) and read, with out, by the backward, which writes
+ * delta [heads][n_q].
+ * workspace: what tsg_attn_workspace says, for the forward with few rows over many keys; 0 bytes = none needed. */
+typedef struct tsg_attn_desc {
+  int32_t dtype, n_seq, heads, kv_heads, dim;
+  float scale;             /* > 0 */
+  int64_t n_q, n_k;
+  const int32_t* q_ptr;    /* [n_seq+1] */
+  const int32_t* k_ptr;    /* [n_seq+1] */
+  const void *q, *k, *v;   /* [n_q][heads][dim], [n_k][kv_heads][dim] by the strides below */
+  void* out;               /* [n_q][heads][dim] */
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  float* stats;            /* [heads][n_q][2], 8-byte aligned */
+  void* workspace;
+  size_t workspace_bytes;
+  const void* d_out;       /* backward only from here on */
+  void *dq, *dk, *dv;
+  int64_t d_out_row, d_out_head, dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+  float* delta;
+} tsg_attn_desc;
+
+int tsg_attn_workspace(const tsg_attn_desc* d, size_t* bytes_host);
+int tsg_attn_forward(const tsg_attn_desc* d, void* stream);
+int tsg_attn_backward(const tsg_attn_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

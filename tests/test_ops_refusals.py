@@ -1,0 +1,71 @@
+"""What the sequence operators (ts_trajgen_amd.ops) refuse before anything is launched: no GPU needed."""
+import ctypes as C
+
+import pytest
+import torch
+
+from ts_trajgen_amd import _lib, ops
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 2, 64)
+    p = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        ops.dropout(x, 0.5, 1)
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        ops.causal_attention(x, x, x, p)
+    with pytest.raises(TypeError):
+        ops.dropout([1.0], 0.5, 1)
+
+
+@pytest.mark.parametrize('kw', [dict(p=-0.1), dict(p=1.5), dict(p=float('nan')), dict(seed=-1), dict(seed=1 << 64),
+                                dict(site=1 << 32), dict(step=-1), dict(step=1 << 32),
+                                dict(step=torch.zeros(2, dtype=torch.int64)), dict(step=torch.zeros(1))])
+def test_dropout_generator_arguments(kw):
+    a = dict(p=0.5, seed=1, site=0, step=0)
+    a.update(kw)
+    with pytest.raises(ValueError):
+        ops.check_rng('dropout', a['p'], a['seed'], a['site'], a['step'], torch.device('cpu'))
+
+
+def _dropout(**kw):
+    d = _lib.DropoutDesc()
+    d.n, d.dtype, d.p, d.x, d.y = 8, 0, 0.5, 4096, 4096
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return _lib.lib().tsg_dropout(C.byref(d), None)
+
+
+def test_dropout_descriptor():
+    assert _lib.lib().tsg_dropout(None, None) == -1
+    assert _dropout(n=0) == 0
+    for kw in (dict(n=-1), dict(dtype=3), dict(p=1.5), dict(p=float('nan')), dict(x=None), dict(y=None)):
+        assert _dropout(**kw) == -1
+
+
+def _attn(entry='tsg_attn_forward', **kw):
+    d = _lib.AttnDesc()
+    d.dtype, d.n_seq, d.heads, d.kv_heads, d.dim, d.scale, d.n_q, d.n_k = 1, 1, 4, 2, 64, 0.125, 10, 10
+    for n in ('q_ptr', 'k_ptr', 'q', 'k', 'v', 'out', 'stats', 'd_out', 'dq', 'dk', 'dv', 'delta'):
+        setattr(d, n, 4096)
+    for n in ('q', 'k', 'v', 'out', 'd_out', 'dq', 'dk', 'dv'):
+        setattr(d, n + '_row', 256)
+        setattr(d, n + '_head', 64)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return getattr(_lib.lib(), entry)(C.byref(d), None)
+
+
+@pytest.mark.parametrize('kw,rc', [
+    (dict(dtype=7), -1), (dict(heads=3), -1), (dict(heads=0), -1), (dict(kv_heads=0), -1), (dict(dim=0), -1),
+    (dict(dim=20), -1), (dict(dim=520), -3), (dict(scale=0.0), -1), (dict(scale=-1.0), -1), (dict(scale=float('nan')), -1),
+    (dict(scale=float('inf')), -1), (dict(n_seq=-1), -1), (dict(n_k=-1), -1), (dict(q=None), -1), (dict(v=None), -1),
+    (dict(out=None), -1), (dict(stats=None), -1), (dict(q_ptr=None), -1), (dict(k=4100), -1), (dict(q_row=252), -1),
+    (dict(v_head=-64), -1), (dict(n_q=1 << 31), -3), (dict(n_k=1 << 30, kv_heads=4), -3), (dict(n_q=1, n_k=100000), -2)])
+def test_attention_descriptor(kw, rc):
+    assert _attn(**kw) == rc
+
+
+def test_attention_backward_descriptor():
+    for kw in (dict(d_out=None), dict(dq=None), dict(dk=None), dict(dv=4), dict(delta=None), dict(d_out_row=3)):
+        assert _attn('tsg_attn_backward', **kw) == -1

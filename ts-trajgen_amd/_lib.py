@@ -19,7 +19,8 @@ ABI_VERSION = 2         # TSG_ABI_VERSION of include/tsg.h
 EXPORTS = ('tsg_version', 'tsg_gemm_f32', 'tsg_gat_forward', 'tsg_gat_forward_static', 'tsg_gat_train_forward', 'tsg_gat_train_backward', 'tsg_gat_build_input', 'tsg_lstm_step_batched',
            'tsg_score_candidates', 'tsg_engine_reset', 'tsg_engine_run', 'tsg_engine_run_profiled', 'tsg_engine_graph_create', 'tsg_engine_graph_launch',
            'tsg_engine_graph_destroy', 'tsg_frontier_expand_select',
-           'tsg_score_frontier', 'tsg_rollout_run', 'tsg_reconstruct_paths', 'tsg_h_pair_scores', 'tsg_geodesic_pairs')
+           'tsg_score_frontier', 'tsg_rollout_run', 'tsg_reconstruct_paths', 'tsg_h_pair_scores', 'tsg_geodesic_pairs',
+           'tsg_dropout', 'tsg_attn_workspace', 'tsg_attn_forward', 'tsg_attn_backward')
 
 _p = C.c_void_p
 _i32 = C.c_int32
@@ -103,6 +104,22 @@ class Rollout(C.Structure):
                 ('prev_idx', _p), ('out_idx', _p), ('rid', _p), ('tcode', _p)]
 
 
+class DropoutDesc(C.Structure):
+    _fields_ = [('n', C.c_int64), ('dtype', _i32), ('site', C.c_uint32), ('step', C.c_uint32), ('reserved', C.c_uint32),
+                ('seed', C.c_uint64), ('p', C.c_double), ('step_dev', _p), ('x', _p), ('y', _p)]
+
+
+class AttnDesc(C.Structure):
+    _fields_ = [('dtype', _i32), ('n_seq', _i32), ('heads', _i32), ('kv_heads', _i32), ('dim', _i32), ('scale', C.c_float),
+                ('n_q', C.c_int64), ('n_k', C.c_int64), ('q_ptr', _p), ('k_ptr', _p),
+                ('q', _p), ('k', _p), ('v', _p), ('out', _p)] + [
+                    (n, C.c_int64) for n in ('q_row', 'q_head', 'k_row', 'k_head', 'v_row', 'v_head', 'out_row', 'out_head')] + [
+                ('stats', _p), ('workspace', _p), ('workspace_bytes', _sz),
+                ('d_out', _p), ('dq', _p), ('dk', _p), ('dv', _p)] + [
+                    (n, C.c_int64) for n in ('d_out_row', 'd_out_head', 'dq_row', 'dq_head', 'dk_row', 'dk_head', 'dv_row',
+                                             'dv_head')] + [('delta', _p)]
+
+
 _lib = None
 
 
@@ -149,6 +166,10 @@ def lib():
     L.tsg_h_pair_scores.argtypes = [C.POINTER(Model), _i32, _p, _p, _p, _p, _p]
     L.tsg_geodesic_pairs.argtypes = [_p, _i32, _i32, _p, _p, _p, _p]
     L.tsg_rollout_run.argtypes = [C.POINTER(Model), C.POINTER(Graph), C.POINTER(Rollout), _i32, _p]
+    L.tsg_dropout.argtypes = [C.POINTER(DropoutDesc), _p]
+    for name in ('tsg_attn_forward', 'tsg_attn_backward'):
+        getattr(L, name).argtypes = [C.POINTER(AttnDesc), _p]
+    L.tsg_attn_workspace.argtypes = [C.POINTER(AttnDesc), C.POINTER(_sz)]
     for name in EXPORTS:
         getattr(L, name).restype = C.c_int
     _lib = L

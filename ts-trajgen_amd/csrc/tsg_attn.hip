@@ -1,0 +1,866 @@
+// Causal attention over packed sequences with grouped heads: forward, backward, and the form for few query rows.
+//
+//   p_ij = exp(scale (q_i . k_j - m_i)) / l_i,  o_i = sum_j p_ij v_j          over the keys j that row i sees
+//   delta_i = do_i . o_i,  dv_j = sum_i p_ij do_i,  ds_ij = p_ij (do_i . v_j - delta_i),
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i                       sums over the heads of a group too
+//
+// Sequences lie one behind the other (q_ptr / k_ptr).  Row t of sequence s sees keys [k0, k0 + (t - q0) + (lk - lq) + 1):
+// a contiguous interval of the packed keys, and both ends grow with t.  So a tile of query rows is simply a stretch of
+// the packed rows, whatever sequences it crosses: it walks the union of its rows' intervals and masks by the row's own.
+// Trajectories of a few dozen positions fill a tile of 128 that way.  The same holds for a tile of keys and the query
+// rows that see them.  No lengths are needed on the host.  Rows of no sequence give zeros.
+//
+// Tile kernels (dim <= 256): a workgroup of four waves owns 128 rows, 32 per wave; the wave computes the TRANSPOSED
+// score tile (A = keys, B = its rows), so that a lane holds one row: the softmax statistics are one register per
+// lane, and the probabilities feed the next product as they stand (tsg_mma.h).  Scores, statistics and outputs are held
+// in f32; p and ds are rounded to the operand type for the matrix cores (nearest even, 2^-9 relative for bf16, which is
+// what the output's own rounding costs too); for f32 operands nothing is rounded.
+// The backward is two kernels, one per output side (dq; dk and dv), each recomputing the scores: seven products instead
+// of five, no atomics, and results that do not depend on the order of workgroups.
+#include "tsg_mma.h"
+
+namespace {
+
+struct AttnArgs {
+  int n_seq, heads, kv_heads, group, dim, chunks;
+  int n_q, n_k;
+  const int* q_ptr;
+  const int* k_ptr;
+  const char *q, *k, *v, *o, *d_o;
+  char *out, *dq, *dk, *dv;
+  long q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head, dq_row, dq_head, dk_row, dk_head, dv_row,
+      dv_head;   // bytes
+  float2* stat;  // [heads][n_q]: largest product q.k of the row, log2 of the sum over it; (0, +inf) where a row sees nothing
+  float* delta;  // [heads][n_q]
+  float scale, scale2;
+  int n_split;
+  float* part;   // rows kernel: [n_q][heads][n_split][dim + 2]
+};
+
+// the sequence that position t belongs to, -1 for none (empty sequences share their start with the next one)
+__device__ __forceinline__ int seq_of(const int* ptr, int n_seq, int t) {
+  int lo = 0, hi = n_seq;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ptr[mid] <= t) lo = mid + 1;
+    else hi = mid;
+  }
+  return (lo > 0 && t < ptr[lo]) ? lo - 1 : -1;
+}
+__device__ __forceinline__ int clamp_to(long v, int n) { return v < 0 ? 0 : (v > n ? n : (int)v); }
+
+// keys [lo, hi) that query row t sees; always inside [0, n_k], whatever the pointers hold
+__device__ __forceinline__ void keys_of_row(const AttnArgs& a, int t, int& lo, int& hi) {
+  lo = hi = 0;
+  if (t >= a.n_q) return;
+  const int s = seq_of(a.q_ptr, a.n_seq, t);
+  if (s < 0) return;
+  const long q1 = a.q_ptr[s + 1], k0 = a.k_ptr[s], k1 = a.k_ptr[s + 1];
+  const long end = k1 - (q1 - 1 - t);  // the last row sees the last key
+  lo = clamp_to(k0, a.n_k);
+  hi = clamp_to(end < k1 ? end : k1, a.n_k);
+  if (hi <= lo) lo = hi = 0;
+}
+// query rows [lo, hi) that see key j
+__device__ __forceinline__ void rows_of_key(const AttnArgs& a, int j, int& lo, int& hi) {
+  lo = hi = 0;
+  if (j >= a.n_k) return;
+  const int s = seq_of(a.k_ptr, a.n_seq, j);
+  if (s < 0) return;
+  const long q0 = a.q_ptr[s], q1 = a.q_ptr[s + 1], k1 = a.k_ptr[s + 1];
+  const long first = q1 - (k1 - j);
+  lo = clamp_to(first > q0 ? first : q0, a.n_q);
+  hi = clamp_to(q1, a.n_q);
+  if (hi <= lo) lo = hi = 0;
+}
+
+// Interval bounds over a wave (lanes l and l + 32 hold the same row) and over the workgroup
+struct Bounds {
+  int wave_lo, wave_hi;  // union of the wave's intervals; empty: wave_lo >= wave_hi
+  int in_lo, in_hi;      // intersection; empty when a row of the wave is empty
+  int lo, hi;            // union over the workgroup
+};
+__device__ __forceinline__ Bounds bounds_of(int lo, int hi, int wave, int* shared /* [8] */) {
+  Bounds b;
+  const bool none = hi <= lo;
+  int ulo = none ? 0x7fffffff : lo, uhi = none ? 0 : hi, ilo = none ? 0x7fffffff : lo, ihi = none ? 0 : hi;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ulo = min(ulo, __shfl_xor(ulo, o, 64));
+    uhi = max(uhi, __shfl_xor(uhi, o, 64));
+    ilo = max(ilo, __shfl_xor(ilo, o, 64));
+    ihi = min(ihi, __shfl_xor(ihi, o, 64));
+  }
+  b.wave_lo = __builtin_amdgcn_readfirstlane(ulo);
+  b.wave_hi = __builtin_amdgcn_readfirstlane(uhi);
+  b.in_lo = __builtin_amdgcn_readfirstlane(ilo);
+  b.in_hi = __builtin_amdgcn_readfirstlane(ihi);
+  if ((threadIdx.x & 63) == 0) shared[wave] = ulo, shared[4 + wave] = uhi;
+  __syncthreads();
+  b.lo = min(min(shared[0], shared[1]), min(shared[2], shared[3]));
+  b.hi = max(max(shared[4], shared[5]), max(shared[6], shared[7]));
+  b.lo = __builtin_amdgcn_readfirstlane(b.lo);
+  b.hi = __builtin_amdgcn_readfirstlane(b.hi);
+  return b;
+}
+
+// operand fragments of one row per lane, straight from memory; zeros outside
+template <int NF> __device__ __forceinline__ void load_frags(tsg_u4 (&f)[NF], const char* row, bool ok, int chunks, int h) {
+#pragma unroll
+  for (int s = 0; s < NF; ++s) {
+    const int c = 2 * s + h;
+    const char* g = ok && c < chunks ? row + c * 16 : reinterpret_cast<const char*>(&tsg_zero_chunk);
+    f[s] = *reinterpret_cast<const tsg_u4*>(g);
+  }
+}
+
+template <typename D> __device__ __forceinline__ float frag_dot(tsg_u4 a, tsg_u4 b) {
+  float s = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (TsgElem<D>::BYTES == 4) {
+      s += __uint_as_float(a[w]) * __uint_as_float(b[w]);
+    } else {
+      typedef typename D::type T;
+      typedef T T2 __attribute__((ext_vector_type(2)));
+      const unsigned aw = a[w], bw = b[w];
+      const T2 x = __builtin_bit_cast(T2, TsgElem<D>::BYTES == 4 ? 0u : aw), y = __builtin_bit_cast(T2, TsgElem<D>::BYTES == 4 ? 0u : bw);
+      s += (float)x.x * (float)y.x + (float)x.y * (float)y.y;
+    }
+  }
+  return s;
+}
+template <> __device__ __forceinline__ float frag_dot<TsgF32>(tsg_u4 a, tsg_u4 b) {
+  float s = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) s += __uint_as_float(a[w]) * __uint_as_float(b[w]);
+  return s;
+}
+
+// four neighbouring elements of a row, f32 -> element type
+template <typename D> __device__ __forceinline__ void store4(char* at, float x, float y, float z, float w) {
+  uint2 v;
+  v.x = tsg_pack2<D>(x, y);
+  v.y = tsg_pack2<D>(z, w);
+  *reinterpret_cast<uint2*>(at) = v;
+}
+template <> __device__ __forceinline__ void store4<TsgF32>(char* at, float x, float y, float z, float w) {
+  *reinterpret_cast<float4*>(at) = make_float4(x, y, z, w);
+}
+// transposed accumulators [dim][row] -> one row per lane
+template <typename D, int ND> __device__ __forceinline__ void store_rows(const tsg_f32x16 (&acc)[ND], char* row, float by, int dim, int h) {
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * dt + 8 * g + 4 * h;
+      if (d < dim)
+        store4<D>(row + d * TsgElem<D>::BYTES, acc[dt][4 * g] * by, acc[dt][4 * g + 1] * by, acc[dt][4 * g + 2] * by, acc[dt][4 * g + 3] * by);
+    }
+}
+
+__device__ __forceinline__ float both_halves_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+__device__ __forceinline__ float both_halves_sum(float v) { return v + __shfl_xor(v, 32, 64); }
+
+// ------------------------------------------------------------------------------------------------- forward, tiles
+template <typename D, int DP, int BK>
+__global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
+  constexpr int CH = DP / TsgElem<D>::EPC, NF = CH / 2, ND = DP / 32, NB = BK / 32, TILE = BK * CH * 16;
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
+  __shared__ int edge[8];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane >> 5;
+  const int tiles = gridDim.x / a.heads;
+  const int tile = tiles - 1 - (int)(blockIdx.x / a.heads), head = blockIdx.x % a.heads;  // late rows see most keys: first
+  const int kvh = head / a.group;
+  const int t = tile * 128 + wave * 32 + (lane & 31);
+  int lo, hi;
+  keys_of_row(a, t, lo, hi);
+  const Bounds b = bounds_of(lo, hi, wave, edge);
+  tsg_u4 qf[NF];
+  load_frags(qf, a.q + (long)t * a.q_row + head * a.q_head, t < a.n_q, a.chunks, h);
+  tsg_f32x16 acc[ND];
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[dt][i] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  const char* kbase = a.k + kvh * a.k_head;
+  const char* vbase = a.v + kvh * a.v_head;
+  auto fetch = [&](int k0, int buf) {
+    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE, kbase + (long)k0 * a.k_row, a.k_row, 0, b.hi - k0, a.chunks, wave, lane);
+    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE + TILE, vbase + (long)k0 * a.v_row, a.v_row, 0, b.hi - k0, a.chunks, wave, lane);
+  };
+  if (b.lo < b.hi) fetch(b.lo, 0);
+  for (int k0 = b.lo, buf = 0; k0 < b.hi; k0 += BK, buf ^= 1) {
+    tsg_dma_wait();
+    __syncthreads();
+    if (k0 + BK < b.hi) fetch(k0 + BK, buf ^ 1);
+    if (k0 >= b.wave_hi || k0 + BK <= b.wave_lo) continue;  // nothing for this wave: uniform, the barriers are above
+    const char* kt = lds + buf * 2 * TILE;
+    const char* vt = kt + TILE;
+    tsg_f32x16 z[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) z[n][i] = 0.0f;
+#pragma unroll
+      for (int s = 0; s < NF; ++s) tsg_mma<D>(tsg_row_frag<CH>(kt, 32 * n + (lane & 31), 2 * s + h), qf[s], z[n]);
+    }
+    if (k0 < b.in_lo || k0 + BK > b.in_hi) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = k0 + 32 * n + (i & 3) + 8 * (i >> 2) + 4 * h;
+          if (key < lo || key >= hi) z[n][i] = -INFINITY;
+        }
+    }
+    float top = m;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, z[n][i]);
+    top = both_halves_max(top);
+    // The maximum is taken off before the scaling: products of the type's lowest value stay finite that way.
+    const float off = top == -INFINITY ? 0.0f : top;  // nothing seen yet: exp2(-inf) = 0, not NaN
+    if (__any(top > m)) {
+      const float fade = __builtin_amdgcn_exp2f((m - off) * a.scale2);
+      l *= fade;
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[dt][i] *= fade;
+    }
+    m = top;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        z[n][i] = __builtin_amdgcn_exp2f((z[n][i] - off) * a.scale2);
+        l += z[n][i];
+      }
+      TsgAccB<D> p;
+      p.set(z[n]);
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) p.template mma<CH>(vt, 32 * n, 32 * dt, acc[dt], lane);
+    }
+  }
+  l = both_halves_sum(l);
+  if (t < a.n_q) {
+    store_rows<D, ND>(acc, a.out + (long)t * a.o_row + head * a.o_head, l == 0.0f ? 0.0f : 1.0f / l, a.dim, h);
+    if (h == 0) a.stat[(long)head * a.n_q + t] = l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l));
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ backward, tiles: dq
+template <typename D, int DP, int BK>
+__global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
+  constexpr int CH = DP / TsgElem<D>::EPC, NF = CH / 2, ND = DP / 32, NB = BK / 32, TILE = BK * CH * 16;
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
+  __shared__ int edge[8];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane >> 5;
+  const int tiles = gridDim.x / a.heads;
+  const int tile = tiles - 1 - (int)(blockIdx.x / a.heads), head = blockIdx.x % a.heads;
+  const int kvh = head / a.group;
+  const int t = tile * 128 + wave * 32 + (lane & 31);
+  int lo, hi;
+  keys_of_row(a, t, lo, hi);
+  const Bounds b = bounds_of(lo, hi, wave, edge);
+  tsg_u4 qf[NF], gf[NF];
+  load_frags(qf, a.q + (long)t * a.q_row + head * a.q_head, t < a.n_q, a.chunks, h);
+  load_frags(gf, a.d_o + (long)t * a.do_row + head * a.do_head, t < a.n_q, a.chunks, h);
+  float delta = 0.0f;
+  float2 st = make_float2(0.0f, INFINITY);
+  {
+    const char* orow = a.o + (long)t * a.o_row + head * a.o_head;
+#pragma unroll
+    for (int s = 0; s < NF; ++s) {
+      const int c = 2 * s + h;
+      const char* g = t < a.n_q && c < a.chunks ? orow + c * 16 : reinterpret_cast<const char*>(&tsg_zero_chunk);
+      delta += frag_dot<D>(*reinterpret_cast<const tsg_u4*>(g), gf[s]);
+    }
+    delta = both_halves_sum(delta);
+    if (t < a.n_q) {
+      st = a.stat[(long)head * a.n_q + t];
+      if (h == 0) a.delta[(long)head * a.n_q + t] = delta;  // the dk / dv kernel, next on the stream, reads it
+    }
+  }
+  tsg_f32x16 acc[ND];
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[dt][i] = 0.0f;
+  const char* kbase = a.k + kvh * a.k_head;
+  const char* vbase = a.v + kvh * a.v_head;
+  auto fetch = [&](int k0, int buf) {
+    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE, kbase + (long)k0 * a.k_row, a.k_row, 0, b.hi - k0, a.chunks, wave, lane);
+    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE + TILE, vbase + (long)k0 * a.v_row, a.v_row, 0, b.hi - k0, a.chunks, wave, lane);
+  };
+  if (b.lo < b.hi) fetch(b.lo, 0);
+  for (int k0 = b.lo, buf = 0; k0 < b.hi; k0 += BK, buf ^= 1) {
+    tsg_dma_wait();
+    __syncthreads();
+    if (k0 + BK < b.hi) fetch(k0 + BK, buf ^ 1);
+    if (k0 >= b.wave_hi || k0 + BK <= b.wave_lo) continue;
+    const char* kt = lds + buf * 2 * TILE;
+    const char* vt = kt + TILE;
+    const bool edge_tile = k0 < b.in_lo || k0 + BK > b.in_hi;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      tsg_f32x16 z, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) z[i] = 0.0f, dp[i] = -delta;  // dp - delta comes out of the product
+#pragma unroll
+      for (int s = 0; s < NF; ++s) {
+        tsg_mma<D>(tsg_row_frag<CH>(kt, 32 * n + (lane & 31), 2 * s + h), qf[s], z);
+        tsg_mma<D>(tsg_row_frag<CH>(vt, 32 * n + (lane & 31), 2 * s + h), gf[s], dp);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = k0 + 32 * n + (i & 3) + 8 * (i >> 2) + 4 * h;
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i] - st.x, a.scale2, -st.y)) * dp[i];
+        if (edge_tile && (key < lo || key >= hi)) p = 0.0f;
+        z[i] = p;
+      }
+      TsgAccB<D> ds;
+      ds.set(z);
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) ds.template mma<CH>(kt, 32 * n, 32 * dt, acc[dt], lane);
+    }
+  }
+  if (t < a.n_q) store_rows<D, ND>(acc, a.dq + (long)t * a.dq_row + head * a.dq_head, a.scale, a.dim, h);
+}
+
+// ------------------------------------------------------------------------------------------ backward, tiles: dk and dv
+// PART 0: both; 1: dv only; 2: dk only (f32 at 256 wide: keys, values and both sums do not fit the registers at once)
+template <typename D, int DP, int BQ, int PART>
+__global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
+  constexpr int CH = DP / TsgElem<D>::EPC, NF = CH / 2, ND = DP / 32, NB = BQ / 32, TILE = BQ * CH * 16;
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
+  __shared__ __attribute__((aligned(16))) float stat[2][3][BQ];  // maximum, log2 of the sum, delta
+  __shared__ int edge[8];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane >> 5;
+  const int tile = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads;  // early keys are seen by most rows: first
+  const int j = tile * 128 + wave * 32 + (lane & 31);
+  int lo, hi;
+  rows_of_key(a, j, lo, hi);
+  const Bounds b = bounds_of(lo, hi, wave, edge);
+  tsg_u4 kf[NF], vf[PART == 1 ? 1 : NF];
+  load_frags(kf, a.k + (long)j * a.k_row + kvh * a.k_head, j < a.n_k, a.chunks, h);
+  if constexpr (PART != 1) load_frags(vf, a.v + (long)j * a.v_row + kvh * a.v_head, j < a.n_k, a.chunks, h);
+  tsg_f32x16 dk[PART == 1 ? 1 : ND], dv[PART == 2 ? 1 : ND];
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if constexpr (PART != 1) dk[dt][i] = 0.0f;
+      if constexpr (PART != 2) dv[dt][i] = 0.0f;
+    }
+  // the walk: for every head of the group the row tiles [b.lo, b.hi), as one sequence of steps
+  const int per = b.lo < b.hi ? (b.hi - b.lo + BQ - 1) / BQ : 0, steps = per * a.group;
+  auto fetch = [&](int step, int buf) {
+    const int head = kvh * a.group + step / per, t0 = b.lo + (step % per) * BQ;
+    tsg_load_tile<BQ, CH, 4>(lds + buf * 2 * TILE, a.q + head * a.q_head + (long)t0 * a.q_row, a.q_row, 0, b.hi - t0, a.chunks, wave, lane);
+    tsg_load_tile<BQ, CH, 4>(lds + buf * 2 * TILE + TILE, a.d_o + head * a.do_head + (long)t0 * a.do_row, a.do_row, 0, b.hi - t0, a.chunks,
+                             wave, lane);
+  };
+  auto stat_of = [&](int step, float2& st, float& delta) {
+    const int head = kvh * a.group + step / per, t = b.lo + (step % per) * BQ + tid;
+    st = make_float2(0.0f, INFINITY), delta = 0.0f;
+    if (tid < BQ && t < b.hi) st = a.stat[(long)head * a.n_q + t], delta = a.delta[(long)head * a.n_q + t];
+  };
+  auto stat_to = [&](int buf, float2 st, float delta) {
+    if (tid < BQ) stat[buf][0][tid] = st.x, stat[buf][1][tid] = st.y, stat[buf][2][tid] = delta;
+  };
+  float2 st;
+  float delta;
+  if (steps) {
+    fetch(0, 0);
+    stat_of(0, st, delta);
+    stat_to(0, st, delta);
+  }
+  for (int step = 0, buf = 0; step < steps; ++step, buf ^= 1) {
+    tsg_dma_wait();
+    __syncthreads();
+    const bool more = step + 1 < steps;
+    if (more) {
+      stat_of(step + 1, st, delta);
+      fetch(step + 1, buf ^ 1);
+    }
+    const int t0 = b.lo + (step % per) * BQ;
+    if (t0 < b.wave_hi && t0 + BQ > b.wave_lo) {
+      const char* qt = lds + buf * 2 * TILE;
+      const char* gt = qt + TILE;
+      const bool edge_tile = t0 < b.in_lo || t0 + BQ > b.in_hi;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        tsg_f32x16 z, dp;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 dl = *reinterpret_cast<const float4*>(&stat[buf][2][32 * n + 8 * g + 4 * h]);
+          z[4 * g] = z[4 * g + 1] = z[4 * g + 2] = z[4 * g + 3] = 0.0f;
+          dp[4 * g] = -dl.x, dp[4 * g + 1] = -dl.y, dp[4 * g + 2] = -dl.z, dp[4 * g + 3] = -dl.w;
+        }
+#pragma unroll
+        for (int s = 0; s < NF; ++s) {
+          tsg_mma<D>(tsg_row_frag<CH>(qt, 32 * n + (lane & 31), 2 * s + h), kf[s], z);
+          if constexpr (PART != 1) tsg_mma<D>(tsg_row_frag<CH>(gt, 32 * n + (lane & 31), 2 * s + h), vf[s], dp);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 ms = *reinterpret_cast<const float4*>(&stat[buf][0][32 * n + 8 * g + 4 * h]);
+          const float4 ls = *reinterpret_cast<const float4*>(&stat[buf][1][32 * n + 8 * g + 4 * h]);
+          const float mv[4] = {ms.x, ms.y, ms.z, ms.w}, lv[4] = {ls.x, ls.y, ls.z, ls.w};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int t = t0 + 32 * n + 8 * g + 4 * h + r;
+            const bool out = edge_tile && (t < lo || t >= hi);
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[4 * g + r] - mv[r], a.scale2, -lv[r]));
+            z[4 * g + r] = out ? 0.0f : p;
+            if constexpr (PART != 1) dp[4 * g + r] = out ? 0.0f : p * dp[4 * g + r];
+          }
+        }
+        if constexpr (PART != 2) {
+          TsgAccB<D> pb;
+          pb.set(z);
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) pb.template mma<CH>(gt, 32 * n, 32 * dt, dv[dt], lane);
+        }
+        if constexpr (PART != 1) {
+          TsgAccB<D> sb;
+          sb.set(dp);
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) sb.template mma<CH>(qt, 32 * n, 32 * dt, dk[dt], lane);
+        }
+      }
+    }
+    if (more) stat_to(buf ^ 1, st, delta);
+  }
+  if (j < a.n_k) {
+    if constexpr (PART != 1) store_rows<D, ND>(dk, a.dk + (long)j * a.dk_row + kvh * a.dk_head, a.scale, a.dim, h);
+    if constexpr (PART != 2) store_rows<D, ND>(dv, a.dv + (long)j * a.dv_row + kvh * a.dv_head, 1.0f, a.dim, h);
+  }
+}
+
+// --------------------------------------------------------------------------------- few rows: one row, keys split
+// One workgroup per (query row, key-value head, stretch of its heads, split of its keys).  LPR lanes hold a key (16 bytes
+// each, NC of them), so a wave reads 64 / LPR keys at once; every such lane group keeps its own running maximum, sum and
+// weighted values for the G heads that share the key, joined at the end through LDS, and over the splits by
+// attn_join_kernel.  Bound by reading the keys and values once.
+template <typename D> struct Chunk {
+  float v[TsgElem<D>::EPC];
+  __device__ __forceinline__ void set(tsg_u4 u) {
+    typedef typename D::type T;
+    typedef T T2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const unsigned x = u[w];
+      const T2 p = __builtin_bit_cast(T2, x);
+      v[2 * w] = (float)p.x;
+      v[2 * w + 1] = (float)p.y;
+    }
+  }
+};
+template <> struct Chunk<TsgF32> {
+  float v[4];
+  __device__ __forceinline__ void set(tsg_u4 u) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v[w] = __uint_as_float(u[w]);
+  }
+};
+
+template <typename D, int LPR, int NC, int G>
+__global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
+  constexpr int EPC = TsgElem<D>::EPC, NE = EPC * NC, PER = 64 / LPR, GROUPS = 4 * PER, U = G * NE > 32 ? 2 : 4;
+  __shared__ float st_m[GROUPS][G], st_l[GROUPS][G];
+  __shared__ float st_o[4][G][LPR * NE];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, part = lane % LPR, grp = wave * PER + lane / LPR;
+  const int stretches = (a.group + G - 1) / G;
+  int bid = blockIdx.x;
+  const int split = bid % a.n_split;
+  bid /= a.n_split;
+  const int st = bid % stretches;
+  bid /= stretches;
+  const int kvh = bid % a.kv_heads, t = bid / a.kv_heads;
+  const int head0 = kvh * a.group + st * G, n_heads = min(G, a.group - st * G);
+  int lo, hi;
+  keys_of_row(a, t, lo, hi);
+  const long span = hi - lo;
+  const int j0 = lo + (int)(span * split / a.n_split), j1 = lo + (int)(span * (split + 1) / a.n_split);
+  Chunk<D> qv[G][NC];
+  float o[G][NE], m[G], l[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    m[g] = -INFINITY, l[g] = 0.0f;
+    const char* row = a.q + (long)t * a.q_row + (head0 + g) * a.q_head;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int ch = part + c * LPR;
+      tsg_u4 u = {0u, 0u, 0u, 0u};
+      if (g < n_heads && ch < a.chunks) u = *reinterpret_cast<const tsg_u4*>(row + ch * 16);
+      qv[g][c].set(u);
+    }
+#pragma unroll
+    for (int e = 0; e < NE; ++e) o[g][e] = 0.0f;
+  }
+  const char* kb = a.k + kvh * a.k_head;
+  const char* vb = a.v + kvh * a.v_head;
+  for (int j = j0 + grp; j < j1; j += GROUPS * U) {
+    tsg_u4 kr[U][NC], vr[U][NC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int jj = min(j + u * GROUPS, j1 - 1);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int ch = part + c * LPR;
+        const bool in = ch < a.chunks;
+        kr[u][c] = *reinterpret_cast<const tsg_u4*>(in ? kb + (long)jj * a.k_row + ch * 16 : reinterpret_cast<const char*>(&tsg_zero_chunk));
+        vr[u][c] = *reinterpret_cast<const tsg_u4*>(in ? vb + (long)jj * a.v_row + ch * 16 : reinterpret_cast<const char*>(&tsg_zero_chunk));
+      }
+    }
+    float z[G][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      Chunk<D> kc[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) kc[c].set(kr[u][c]);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float s = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < EPC; ++e) s += kc[c].v[e] * qv[g][c].v[e];
+        z[g][u] = s;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int w = LPR / 2; w > 0; w >>= 1) z[g][u] += __shfl_xor(z[g][u], w, 64);
+        if (j + u * GROUPS >= j1) z[g][u] = -INFINITY;
+      }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float top = m[g];
+#pragma unroll
+      for (int u = 0; u < U; ++u) top = fmaxf(top, z[g][u]);
+      const float off = top == -INFINITY ? 0.0f : top;
+      const float fade = __builtin_amdgcn_exp2f((m[g] - off) * a.scale2);
+      m[g] = top;
+      l[g] *= fade;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) o[g][e] *= fade;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        z[g][u] = __builtin_amdgcn_exp2f((z[g][u] - off) * a.scale2);
+        l[g] += z[g][u];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      Chunk<D> vc[NC];
+      const bool in = j + u * GROUPS < j1;  // a key behind the end was read again: its value must not enter, not even times 0
+#pragma unroll
+      for (int c = 0; c < NC; ++c) vc[c].set(vr[u][c]);
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < EPC; ++e) o[g][c * EPC + e] += in ? z[g][u] * vc[c].v[e] : 0.0f;
+    }
+  }
+  // join the lane groups: common maximum, then sums over the groups of a wave (shuffles) and over the waves (LDS)
+  if (part == 0)
+#pragma unroll
+    for (int g = 0; g < G; ++g) st_m[grp][g] = m[g], st_l[grp][g] = l[g];
+  __syncthreads();
+  float top[G], sum[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    float v = -INFINITY;
+    for (int x = 0; x < GROUPS; ++x) v = fmaxf(v, st_m[x][g]);
+    top[g] = v;
+    const float off = v == -INFINITY ? 0.0f : v;
+    float s = 0.0f;
+    for (int x = 0; x < GROUPS; ++x) s += st_l[x][g] * __builtin_amdgcn_exp2f((st_m[x][g] - off) * a.scale2);
+    sum[g] = s;
+    const float by = __builtin_amdgcn_exp2f((m[g] - off) * a.scale2);
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      float v2 = o[g][e] * by;
+#pragma unroll
+      for (int w = LPR; w < 64; w <<= 1) v2 += __shfl_xor(v2, w, 64);
+      if (lane < LPR) st_o[wave][g][(part + (e / EPC) * LPR) * EPC + e % EPC] = v2;
+    }
+  }
+  __syncthreads();
+  for (int x = tid; x < G * a.dim; x += 256) {
+    const int g = x / a.dim, d = x % a.dim;
+    if (g >= n_heads) break;
+    const float v = (st_o[0][g][d] + st_o[1][g][d]) + (st_o[2][g][d] + st_o[3][g][d]);
+    float sg = 0.0f, tg = 0.0f;
+#pragma unroll
+    for (int y = 0; y < G; ++y)
+      if (y == g) sg = sum[y], tg = top[y];
+    if (a.n_split == 1) {
+      typedef typename D::type T;
+      reinterpret_cast<T*>(a.out + (long)t * a.o_row + (head0 + g) * a.o_head)[d] = (T)(v * (sg == 0.0f ? 0.0f : 1.0f / sg));
+      if (d == 0) a.stat[(long)(head0 + g) * a.n_q + t] = sg == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(tg, __builtin_amdgcn_logf(sg));
+    } else {
+      float* p = a.part + (((long)t * a.heads + head0 + g) * a.n_split + split) * (a.dim + 2);
+      p[d] = v;
+      if (d == 0) p[a.dim] = tg, p[a.dim + 1] = sg;
+    }
+  }
+}
+
+// one wave per (row, head): the splits' maxima, sums and weighted values
+template <typename D> __global__ __launch_bounds__(64) void attn_join_kernel(AttnArgs a) {
+  const int t = blockIdx.x / a.heads, head = blockIdx.x % a.heads, lane = threadIdx.x;
+  const float* p = a.part + ((long)t * a.heads + head) * a.n_split * (a.dim + 2);
+  float top = -INFINITY;
+  for (int s = lane; s < a.n_split; s += 64) top = fmaxf(top, p[(long)s * (a.dim + 2) + a.dim]);
+  top = tsg_wave_max(top);
+  const float off = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f;
+  for (int s = lane; s < a.n_split; s += 64)
+    l += p[(long)s * (a.dim + 2) + a.dim + 1] * __builtin_amdgcn_exp2f((p[(long)s * (a.dim + 2) + a.dim] - off) * a.scale2);
+  l = tsg_wave_sum(l);
+  const float by = l == 0.0f ? 0.0f : 1.0f / l;
+  typedef typename D::type T;
+  for (int d = lane; d < a.dim; d += 64) {
+    float v = 0.0f;
+    for (int s = 0; s < a.n_split; ++s)
+      v += p[(long)s * (a.dim + 2) + d] * __builtin_amdgcn_exp2f((p[(long)s * (a.dim + 2) + a.dim] - off) * a.scale2);
+    reinterpret_cast<T*>(a.out + (long)t * a.o_row + head * a.o_head)[d] = (T)(v * by);
+  }
+  if (lane == 0) a.stat[(long)head * a.n_q + t] = l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(top, __builtin_amdgcn_logf(l));
+}
+
+// -------------------------------------------------------------------------------- backward for heads wider than 256
+// One wave per row (dq) or key (dk, dv), lanes over the width.  Heads this wide are the largest recurrent states only.
+constexpr int WIDE = 8;  // elements per lane: dim <= 512
+template <typename T> __device__ __forceinline__ void load_wide(float (&x)[WIDE], const char* row, int dim, int lane) {
+#pragma unroll
+  for (int e = 0; e < WIDE; ++e) x[e] = lane + 64 * e < dim ? (float)reinterpret_cast<const T*>(row)[lane + 64 * e] : 0.0f;
+}
+template <typename T> __device__ __forceinline__ void store_wide(const float (&x)[WIDE], char* row, float by, int dim, int lane) {
+#pragma unroll
+  for (int e = 0; e < WIDE; ++e)
+    if (lane + 64 * e < dim) reinterpret_cast<T*>(row)[lane + 64 * e] = (T)(x[e] * by);
+}
+__device__ __forceinline__ float dot_wide(const float (&x)[WIDE], const float (&y)[WIDE]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int e = 0; e < WIDE; ++e) s += x[e] * y[e];
+  return tsg_wave_sum_u(s);
+}
+template <typename D> __global__ __launch_bounds__(64) void attn_wide_dq_kernel(AttnArgs a) {
+  typedef typename D::type T;
+  const int t = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kvh = head / a.group, lane = threadIdx.x;
+  int lo, hi;
+  keys_of_row(a, t, lo, hi);
+  float q[WIDE], g[WIDE], x[WIDE], acc[WIDE];
+  load_wide<T>(q, a.q + (long)t * a.q_row + head * a.q_head, a.dim, lane);
+  load_wide<T>(g, a.d_o + (long)t * a.do_row + head * a.do_head, a.dim, lane);
+  load_wide<T>(x, a.o + (long)t * a.o_row + head * a.o_head, a.dim, lane);
+  const float delta = dot_wide(g, x);
+  const float2 st = a.stat[(long)head * a.n_q + t];
+  if (lane == 0) a.delta[(long)head * a.n_q + t] = delta;
+#pragma unroll
+  for (int e = 0; e < WIDE; ++e) acc[e] = 0.0f;
+  for (int j = lo; j < hi; ++j) {
+    load_wide<T>(x, a.v + (long)j * a.v_row + kvh * a.v_head, a.dim, lane);
+    const float dp = dot_wide(g, x);
+    load_wide<T>(x, a.k + (long)j * a.k_row + kvh * a.k_head, a.dim, lane);
+    const float ds = __builtin_amdgcn_exp2f(__builtin_fmaf(dot_wide(q, x) - st.x, a.scale2, -st.y)) * (dp - delta);
+#pragma unroll
+    for (int e = 0; e < WIDE; ++e) acc[e] += ds * x[e];
+  }
+  store_wide<T>(acc, a.dq + (long)t * a.dq_row + head * a.dq_head, a.scale, a.dim, lane);
+}
+template <typename D> __global__ __launch_bounds__(64) void attn_wide_dkv_kernel(AttnArgs a) {
+  typedef typename D::type T;
+  const int j = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads, lane = threadIdx.x;
+  int lo, hi;
+  rows_of_key(a, j, lo, hi);
+  float k[WIDE], v[WIDE], x[WIDE], dk[WIDE], dv[WIDE];
+  load_wide<T>(k, a.k + (long)j * a.k_row + kvh * a.k_head, a.dim, lane);
+  load_wide<T>(v, a.v + (long)j * a.v_row + kvh * a.v_head, a.dim, lane);
+#pragma unroll
+  for (int e = 0; e < WIDE; ++e) dk[e] = dv[e] = 0.0f;
+  for (int head = kvh * a.group; head < (kvh + 1) * a.group; ++head)
+    for (int t = lo; t < hi; ++t) {
+      load_wide<T>(x, a.d_o + (long)t * a.do_row + head * a.do_head, a.dim, lane);
+      const float dp = dot_wide(v, x) - a.delta[(long)head * a.n_q + t];
+      float q[WIDE];
+      load_wide<T>(q, a.q + (long)t * a.q_row + head * a.q_head, a.dim, lane);
+      const float2 st = a.stat[(long)head * a.n_q + t];
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot_wide(q, k) - st.x, a.scale2, -st.y));
+#pragma unroll
+      for (int e = 0; e < WIDE; ++e) {
+        dv[e] += p * x[e];
+        dk[e] += p * dp * q[e];
+      }
+    }
+  store_wide<T>(dk, a.dk + (long)j * a.dk_row + kvh * a.dk_head, a.scale, a.dim, lane);
+  store_wide<T>(dv, a.dv + (long)j * a.dv_row + kvh * a.dv_head, 1.0f, a.dim, lane);
+}
+
+// ------------------------------------------------------------------------------------------------------ host side
+int rows_g(int group) { return group >= 8 ? 8 : (group >= 4 ? 4 : (group >= 2 ? 2 : 1)); }
+
+// The rows kernel reads a row's keys once per row; a tile kernel once per 128 rows, but spends 128 rows' worth of matrix
+// work on them.  Rows of one sequence share their keys, so the tile form wins as soon as a sequence has a few dozen rows,
+// and also where there are no more keys than rows around (short sequences lie side by side in a tile).
+bool use_rows(const tsg_attn_desc* d) {
+  if (d->dim > 256) return true;
+  return d->n_k >= 8 * d->n_q && d->n_q < 16 * (int64_t)d->n_seq;
+}
+int splits_of(const tsg_attn_desc* d) {
+  const int64_t wgs = d->n_q * (int64_t)d->kv_heads * tsg_cdiv(d->heads / d->kv_heads, rows_g(d->heads / d->kv_heads));
+  int64_t n = (2048 + wgs - 1) / wgs;
+  const int64_t mean = d->n_k / (d->n_seq > 0 ? d->n_seq : 1);
+  if (n > mean / 128) n = mean / 128;
+  return (int)(n < 1 ? 1 : (n > 1024 ? 1024 : n));
+}
+size_t workspace_of(const tsg_attn_desc* d) {
+  if (!use_rows(d)) return 0;
+  const int n = splits_of(d);
+  return n == 1 ? 0 : (size_t)d->n_q * d->heads * n * (d->dim + 2) * 4;
+}
+
+int check_attn(const tsg_attn_desc* d, bool backward) {
+  if (!d) return TSG_E_INVALID;
+  if (d->dtype != TSG_F32 && d->dtype != TSG_BF16 && d->dtype != TSG_F16) return TSG_E_INVALID;
+  if (d->n_seq < 0 || d->n_q < 0 || d->n_k < 0 || d->heads <= 0 || d->kv_heads <= 0 || d->dim <= 0) return TSG_E_INVALID;
+  if (d->heads % d->kv_heads) return TSG_E_INVALID;
+  if (!(d->scale > 0.0f) || !(d->scale < INFINITY)) return TSG_E_INVALID;
+  const int bytes = d->dtype == TSG_F32 ? 4 : 2, epc = 16 / bytes;
+  if (d->dim > 512 || d->n_q > 0x7ffffff0L || d->n_k > 0x7ffffff0L) return TSG_E_LIMIT;
+  if (d->n_q * (int64_t)d->heads > 0x7fffffffL || d->n_k * (int64_t)d->kv_heads > 0x7fffffffL) return TSG_E_LIMIT;
+  if (d->dim % epc) return TSG_E_INVALID;
+  if (!d->q_ptr || !d->k_ptr || !d->stats || (uintptr_t)d->stats % 8) return TSG_E_INVALID;
+  const void* p[9] = {d->q, d->k, d->v, d->out, backward ? d->d_out : nullptr, backward ? d->dq : nullptr,
+                      backward ? d->dk : nullptr, backward ? d->dv : nullptr, nullptr};
+  const int64_t s[16] = {d->q_row, d->q_head, d->k_row, d->k_head, d->v_row, d->v_head, d->out_row, d->out_head,
+                         backward ? d->d_out_row : 0, backward ? d->d_out_head : 0, backward ? d->dq_row : 0, backward ? d->dq_head : 0,
+                         backward ? d->dk_row : 0, backward ? d->dk_head : 0, backward ? d->dv_row : 0, backward ? d->dv_head : 0};
+  for (int i = 0; i < (backward ? 8 : 4); ++i)
+    if (!p[i] || (uintptr_t)p[i] % 16) return TSG_E_INVALID;
+  for (int i = 0; i < 16; ++i)
+    if (s[i] % epc || s[i] < 0) return TSG_E_INVALID;
+  if (backward && !d->delta) return TSG_E_INVALID;
+  return 0;
+}
+
+AttnArgs args_of(const tsg_attn_desc* d) {
+  AttnArgs a;
+  const long b = d->dtype == TSG_F32 ? 4 : 2;
+  a.n_seq = d->n_seq, a.heads = d->heads, a.kv_heads = d->kv_heads, a.group = d->heads / d->kv_heads;
+  a.dim = d->dim, a.chunks = (int)(d->dim * b / 16);
+  a.n_q = (int)d->n_q, a.n_k = (int)d->n_k;
+  a.q_ptr = d->q_ptr, a.k_ptr = d->k_ptr;
+  a.q = (const char*)d->q, a.k = (const char*)d->k, a.v = (const char*)d->v, a.o = (const char*)d->out, a.d_o = (const char*)d->d_out;
+  a.out = (char*)d->out, a.dq = (char*)d->dq, a.dk = (char*)d->dk, a.dv = (char*)d->dv;
+  a.q_row = d->q_row * b, a.q_head = d->q_head * b, a.k_row = d->k_row * b, a.k_head = d->k_head * b;
+  a.v_row = d->v_row * b, a.v_head = d->v_head * b, a.o_row = d->out_row * b, a.o_head = d->out_head * b;
+  a.do_row = d->d_out_row * b, a.do_head = d->d_out_head * b, a.dq_row = d->dq_row * b, a.dq_head = d->dq_head * b;
+  a.dk_row = d->dk_row * b, a.dk_head = d->dk_head * b, a.dv_row = d->dv_row * b, a.dv_head = d->dv_head * b;
+  a.stat = (float2*)d->stats, a.delta = d->delta;
+  a.scale = d->scale, a.scale2 = d->scale * 1.44269504088896340736f;
+  a.n_split = 1;
+  a.part = (float*)d->workspace;
+  return a;
+}
+
+template <typename D, int LPR, int NC> void launch_rows(const AttnArgs& a, hipStream_t s) {
+  const int g = rows_g(a.group);
+  const dim3 grid((unsigned)((long)a.n_q * a.kv_heads * tsg_cdiv(a.group, g) * a.n_split)), block(256);
+  if (g == 8) {
+    if constexpr (NC == 1) hipLaunchKernelGGL((attn_rows_kernel<D, LPR, NC, 8>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((attn_rows_kernel<D, LPR, NC, 4>), dim3(grid.x / tsg_cdiv(a.group, 8) * tsg_cdiv(a.group, 4)), block, 0, s, a);
+  } else if (g == 4) hipLaunchKernelGGL((attn_rows_kernel<D, LPR, NC, 4>), grid, block, 0, s, a);
+  else if (g == 2) hipLaunchKernelGGL((attn_rows_kernel<D, LPR, NC, 2>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((attn_rows_kernel<D, LPR, NC, 1>), grid, block, 0, s, a);
+}
+
+template <typename D> int forward_of(const tsg_attn_desc* d, hipStream_t s) {
+  AttnArgs a = args_of(d);
+  if (use_rows(d)) {
+    a.n_split = splits_of(d);
+    if ((long)a.n_q * a.kv_heads * tsg_cdiv(a.group, rows_g(a.group)) * 2 * a.n_split > 0x7fffffffL) return TSG_E_LIMIT;
+    constexpr int F = TsgElem<D>::BYTES / 2;  // 1: 16-bit types, 2: f32
+    if (a.dim <= 64) launch_rows<D, 8 * F, 1>(a, s);
+    else if (a.dim <= 128) launch_rows<D, 16 * F, 1>(a, s);
+    else if (a.dim <= 256) launch_rows<D, 32 * F, 1>(a, s);
+    else launch_rows<D, 64, F>(a, s);
+    if (a.n_split > 1) hipLaunchKernelGGL(attn_join_kernel<D>, dim3((unsigned)((long)a.n_q * a.heads)), dim3(64), 0, s, a);
+  } else {
+    const dim3 grid((unsigned)(tsg_cdiv(a.n_q, 128) * a.heads)), block(256);
+    constexpr bool F32 = TsgElem<D>::BYTES == 4;
+    if (a.dim <= 64) hipLaunchKernelGGL((attn_fwd_kernel<D, 64, 64>), grid, block, 0, s, a);
+    else if (a.dim <= 128) hipLaunchKernelGGL((attn_fwd_kernel<D, 128, F32 ? 32 : 64>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((attn_fwd_kernel<D, 256, 32>), grid, block, 0, s, a);
+  }
+  TSG_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
+  const AttnArgs a = args_of(d);
+  const dim3 block(256);
+  if (a.dim > 256) {
+    if (a.n_q) hipLaunchKernelGGL(attn_wide_dq_kernel<D>, dim3((unsigned)((long)a.n_q * a.heads)), dim3(64), 0, s, a);
+    if (a.n_k) hipLaunchKernelGGL(attn_wide_dkv_kernel<D>, dim3((unsigned)((long)a.n_k * a.kv_heads)), dim3(64), 0, s, a);
+    TSG_LAUNCH_CHECK();
+    return 0;
+  }
+  const dim3 gq((unsigned)(tsg_cdiv(a.n_q, 128) * a.heads)), gk((unsigned)(tsg_cdiv(a.n_k, 128) * a.kv_heads));
+  constexpr bool F32 = TsgElem<D>::BYTES == 4;
+  if (a.n_q) {
+    if (a.dim <= 64) hipLaunchKernelGGL((attn_dq_kernel<D, 64, 64>), gq, block, 0, s, a);
+    else if (a.dim <= 128) hipLaunchKernelGGL((attn_dq_kernel<D, 128, F32 ? 32 : 64>), gq, block, 0, s, a);
+    else hipLaunchKernelGGL((attn_dq_kernel<D, 256, 32>), gq, block, 0, s, a);
+  }
+  if (a.n_k) {
+    if (a.dim <= 64) hipLaunchKernelGGL((attn_dkv_kernel<D, 64, 32, 0>), gk, block, 0, s, a);
+    else if (a.dim <= 128) hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0>), gk, block, 0, s, a);
+    else if constexpr (F32) {
+      hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 1>), gk, block, 0, s, a);
+      hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 2>), gk, block, 0, s, a);
+    } else hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 0>), gk, block, 0, s, a);
+  }
+  TSG_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int tsg_attn_workspace(const tsg_attn_desc* d, size_t* bytes_host) {
+  if (!d || !bytes_host || d->n_q < 0 || d->n_k < 0 || d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads) return TSG_E_INVALID;
+  *bytes_host = d->n_q ? workspace_of(d) : 0;
+  return 0;
+}
+
+extern "C" int tsg_attn_forward(const tsg_attn_desc* d, void* stream) {
+  if (d && d->n_q == 0 && d->heads > 0) return 0;
+  const int rc = check_attn(d, false);
+  if (rc) return rc;
+  const size_t need = workspace_of(d);
+  if (need && (!d->workspace || d->workspace_bytes < need)) return TSG_E_TOO_SMALL;
+  hipStream_t s = (hipStream_t)stream;
+  return d->dtype == TSG_F32 ? forward_of<TsgF32>(d, s) : (d->dtype == TSG_BF16 ? forward_of<TsgBf16>(d, s) : forward_of<TsgF16>(d, s));
+}
+
+extern "C" int tsg_attn_backward(const tsg_attn_desc* d, void* stream) {
+  if (d && d->n_q == 0 && d->n_k == 0) return 0;
+  const int rc = check_attn(d, true);
+  if (rc) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  return d->dtype == TSG_F32 ? backward_of<TsgF32>(d, s) : (d->dtype == TSG_BF16 ? backward_of<TsgBf16>(d, s) : backward_of<TsgF16>(d, s));
+}
