@@ -564,6 +564,34 @@ int tsg_attn_workspace(const tsg_attn_desc* d, size_t* bytes_host);
 int tsg_attn_forward(const tsg_attn_desc* d, void* stream);
 int tsg_attn_backward(const tsg_attn_desc* d, void* stream);
 
+/* Softmax cross entropy of states against a vocabulary: z = h W^T + bias, row_loss[t] = log sum exp z[t] - z[t][target[t]],
+ * without the logits being kept; loss is their sum (reduction 1) or mean over the rows that count (2; none: 0 / 0 = NaN).
+ * A row whose target is ignore_index has loss 0 and adds nothing to any gradient, whatever its state holds.  Any
+ * other target outside [0, n_vocab) makes the row's loss and gradients NaN.  bias (may be NULL) and the gradients
+ * have the type of h and w.  The backward takes d_loss (one number, or one per row for reduction 0) and the stats that
+ * the forward left, takes the vocabulary in pieces and writes dh, dw and dbias whole.
+ * Base addresses of h and w are 16-byte aligned, rows a multiple of 16 bytes apart, hidden a multiple of 8 (pad with
+ * zeros), the workspace 256-byte aligned; tsg_xent_workspace says how much.  n_rows >= 1. */
+typedef struct tsg_xent_desc {
+  int32_t dtype, hidden, reduction, reserved;
+  int64_t n_rows, n_vocab, ignore_index;
+  const void *h, *w, *bias;  /* [n_rows][hidden], [n_vocab][hidden], [n_vocab] */
+  int64_t h_row, w_row;      /* elements */
+  const int64_t* target;     /* [n_rows] */
+  float* row_loss;           /* [n_rows] out */
+  float* loss;               /* [1] out, reduction 1 and 2 */
+  float* stats;              /* [n_rows][2], 8-byte aligned: written by the forward, read by the backward */
+  void* workspace;
+  size_t workspace_bytes;
+  const float* d_loss;       /* backward only from here on */
+  void *dh, *dw, *dbias;
+  int64_t dh_row, dw_row;
+} tsg_xent_desc;
+
+int tsg_xent_workspace(const tsg_xent_desc* d, size_t* forward_bytes_host, size_t* backward_bytes_host);
+int tsg_xent_forward(const tsg_xent_desc* d, void* stream);
+int tsg_xent_backward(const tsg_xent_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,13 @@ def bound(dt):
     return 1e-5 if dt == torch.float32 else torch.finfo(dt).eps + 2e-6
 
 
+def bound_of(dt, want):
+    """f16 below 2^-14 has a fixed step of 2^-24: an element is off by up to half of it however small it is (gradients of means
+    over hundreds of rows lie there), which is 2^-25 sqrt(n) in the 2-norm over n elements, on top of bound()."""
+    norm = float(want.norm())
+    return bound(dt) + (2.0 ** -25 * math.sqrt(want.numel()) / norm if dt == torch.float16 and norm else 0.0)
+
+
 def rel(x, y):
     x, y = x.detach().double().cpu(), y.detach().double().cpu()
     assert x.shape == y.shape and torch.isfinite(x).all()
@@ -309,3 +316,225 @@ def test_capture_over_a_living_eager_graph_is_refused():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(dx, want)
+
+
+# ---------------------------------------------------------------------------------------------------- cross entropy
+def plain_cross_entropy(h, w, b, target, ignore, d_row):
+    """64-bit losses per row, and the gradients for the row gradients d_row."""
+    h, w = h.detach().double().cpu(), w.detach().double().cpu()
+    b = torch.zeros(w.shape[0], dtype=torch.double) if b is None else b.detach().double().cpu()
+    target, d_row = target.cpu(), d_row.double().cpu()
+    used = target != ignore
+    h = torch.where(used.unsqueeze(1), h, torch.zeros((), dtype=torch.double))
+    lp = torch.log_softmax(h @ w.t() + b, dim=1)
+    at = torch.where(used, target, 0)
+    rows = torch.where(used, -lp.gather(1, at.unsqueeze(1)).squeeze(1), torch.zeros((), dtype=torch.double))
+    dz = lp.exp()
+    dz[torch.arange(len(at)), at] -= 1.0
+    dz = dz * (d_row * used).unsqueeze(1)
+    return rows, dz @ w, dz.t() @ h, dz.sum(0)
+
+
+def entropy_case(dt, t, v, k, bias=True, reduction='mean', ignored=0.2, seed=0, h_by=1.0, w_by=None, spread=None):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.tanh(torch.randn(t, k, generator=g)) * h_by
+    if spread is not None:
+        h = h * spread(t).unsqueeze(1)
+    h = h.to(dt).to(DEV).requires_grad_(True)
+    w = (torch.randn(v, k, generator=g) * (w_by or 1.5 / math.sqrt(k))).to(dt).to(DEV).requires_grad_(True)
+    b = (torch.randn(v, generator=g) * 0.5).to(dt).to(DEV).requires_grad_(True) if bias else None
+    target = torch.randint(0, v, (t,), generator=g)
+    target[torch.rand(t, generator=g) < ignored] = -100
+    target[0] = v - 1
+    return h, w, b, target.to(DEV)
+
+
+def check_entropy(dt, h, w, b, target, reduction='mean'):
+    from ts_trajgen_amd import ops
+    loss = ops.linear_cross_entropy(h, w, target, bias=b, reduction=reduction)
+    up = torch.randn(loss.shape, generator=torch.Generator().manual_seed(1)).to(DEV) if reduction == 'none' else torch.full((), 1.7, device=DEV)
+    got = torch.autograd.grad(loss, [h, w] + ([b] if b is not None else []), up)
+    used = target != -100
+    n = float(used.sum())
+    d_row = up if reduction == 'none' else torch.full((len(target),), 1.7 / (n if reduction == 'mean' else 1.0), device=DEV)
+    rows, dh, dw, db = plain_cross_entropy(h, w, b, target, -100, d_row)
+    want = rows if reduction == 'none' else rows.sum() / (n if reduction == 'mean' else 1.0)
+    # the loss itself is f32: products of exact operands, one rounding per addition
+    assert rel(loss, want) < 1e-5
+    for a, e in zip(got, (dh, dw, db)):
+        assert rel(a, e) < bound_of(dt, e), (a.shape, rel(a, e))
+    return loss, got
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('t,v,k', [(1, 1, 8), (1, 300, 64), (61, 1000, 256), (129, 129, 72), (300, 5003, 100), (128, 128, 128),
+                                   (257, 4097, 320), (5, 11096, 256), (700, 640, 1000), (64, 2048, 3)])
+def test_cross_entropy_sizes(dt, t, v, k):
+    check_entropy(dt, *entropy_case(dt, t, v, k, seed=t + v))
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('reduction', ['none', 'sum', 'mean'])
+@pytest.mark.parametrize('bias', [True, False])
+def test_cross_entropy_reductions(dt, reduction, bias):
+    check_entropy(dt, *entropy_case(dt, 200, 1500, 128, bias=bias, seed=3), reduction=reduction)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_cross_entropy_of_sharp_and_flat_rows(dt):
+    check_entropy(dt, *entropy_case(dt, 150, 2000, 64, w_by=2.0, seed=4), reduction='sum')       # logits up to ~60
+    check_entropy(dt, *entropy_case(dt, 150, 2000, 64, w_by=1e-3, seed=5), reduction='mean')     # almost uniform
+    check_entropy(torch.float32, *entropy_case(torch.float32, 150, 2000, 64, h_by=1e-6, w_by=1e4, seed=6), reduction='mean')
+    check_entropy(torch.float32, *entropy_case(torch.float32, 90, 700, 64, seed=7, spread=lambda t: torch.logspace(-3, 1, t)), reduction='none')
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_cross_entropy_several_pieces(dt, monkeypatch):
+    # 20000 rows: 2^30 bytes of dz are a piece of 26752 (16-bit) or 13312 (f32) entries
+    g = torch.Generator(device=DEV).manual_seed(1)
+    t, v, k = 20000, 27000, 16
+    from ts_trajgen_amd import ops
+    h = torch.randn(t, k, generator=g, device=DEV).to(dt).requires_grad_(True)
+    w = (torch.randn(v, k, generator=g, device=DEV) * 0.3).to(dt).requires_grad_(True)
+    b = (torch.randn(v, generator=g, device=DEV) * 0.3).to(dt).requires_grad_(True)
+    target = torch.randint(0, v, (t,), generator=g, device=DEV)
+    loss = ops.linear_cross_entropy(h, w, target, bias=b)
+    got = torch.autograd.grad(loss, [h, w, b])
+    with torch.no_grad():
+        z = h.double() @ w.double().t() + b.double()
+        lp = torch.log_softmax(z, dim=1)
+        assert rel(loss, -lp.gather(1, target.unsqueeze(1)).mean()) < 1e-5
+        dz = lp.exp_()
+        dz[torch.arange(t, device=DEV), target] -= 1.0
+        dz /= t
+        for a, e in zip(got, (dz @ w.double(), dz.t() @ h.double(), dz.sum(0))):
+            assert rel(a, e) < bound_of(dt, e)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_cross_entropy_rows_left_out_hold_anything(dt):
+    from ts_trajgen_amd import ops
+    h, w, b, target = entropy_case(dt, 130, 900, 64, seed=8)
+    loss, grads = check_entropy(dt, h, w, b, target)
+    bad = h.detach().clone()
+    bad[target == -100] = float('nan')
+    bad[torch.nonzero(target == -100)[0]] = float('inf')
+    bad.requires_grad_(True)
+    loss2 = ops.linear_cross_entropy(bad, w, target, bias=b)
+    got = torch.autograd.grad(loss2, [bad, w, b], torch.full((), 1.7, device=DEV))
+    assert torch.equal(loss, loss2)
+    for a, e in zip(got, grads):
+        assert torch.equal(a, e)
+    assert float(got[0][target == -100].abs().sum()) == 0.0
+
+
+def test_cross_entropy_masked_entries_empty_means_and_bad_targets():
+    from ts_trajgen_amd import ops
+    for dt in TYPES:
+        h, w, b, target = entropy_case(dt, 40, 300, 64, seed=9, ignored=0.0)
+        with torch.no_grad():
+            b[7:200] = float('-inf')                    # entries that cannot be chosen
+        target = torch.where((target >= 7) & (target < 200), torch.full_like(target, 3), target)
+        loss = ops.linear_cross_entropy(h, w, target, bias=b)
+        want, dh, dw, db = plain_cross_entropy(h, w, b, target, -100, torch.full((40,), 1 / 40.0))
+        got = torch.autograd.grad(loss, [h, w, b])
+        assert rel(loss, want.mean()) < 1e-5
+        for a, e in zip(got, (dh, dw, db)):
+            assert rel(a, e) < bound_of(dt, e)
+        assert float(got[1][7:200].abs().sum()) == 0.0
+        with torch.no_grad():
+            b.fill_(torch.finfo(dt).min)                # the type's lowest value everywhere: uniform
+        none = torch.full_like(target, -100)
+        rows = ops.linear_cross_entropy(h, w, none, reduction='none')
+        assert float(rows.detach().abs().sum()) == 0.0
+        assert math.isnan(float(ops.linear_cross_entropy(h, w, none)))
+        off = target.clone()
+        off[5] = 300
+        rows = ops.linear_cross_entropy(h, w, off, reduction='none')
+        assert torch.isnan(rows[5]) and torch.isfinite(rows[torch.arange(40, device=DEV) != 5]).all()
+        off[5] = -1
+        dh, = torch.autograd.grad(ops.linear_cross_entropy(h, w, off, reduction='sum'), [h])
+        assert torch.isnan(dh[5].float()).all() and torch.isfinite(dh[torch.arange(40, device=DEV) != 5].float()).all()
+
+
+def test_cross_entropy_views_and_repeats():
+    from ts_trajgen_amd import ops
+    for dt in TYPES:
+        h, w, b, target = entropy_case(dt, 100, 700, 64, seed=10)
+        wide = torch.randn(100, 200, device=DEV).to(dt)
+        hv = wide[:, 24:88]                             # rows 200 apart
+        a = ops.linear_cross_entropy(hv, w, target, bias=b, reduction='none')
+        assert torch.equal(a, ops.linear_cross_entropy(hv.contiguous(), w, target, bias=b, reduction='none'))
+        assert torch.equal(ops.linear_cross_entropy(hv, w.t().contiguous().t(), target, bias=b, reduction='none'), a)
+        assert torch.equal(ops.linear_cross_entropy(wide[:, 23:87], w, target, reduction='none'),
+                           ops.linear_cross_entropy(wide[:, 23:87].contiguous(), w, target, reduction='none'))
+        one = torch.randn(1, 64, device=DEV).to(dt).requires_grad_(True)
+        loss = ops.linear_cross_entropy(one.expand(100, 64), w, target, bias=b)
+        loss.backward()
+        assert one.grad.shape == one.shape
+        w.grad = b.grad = None
+
+        def step():
+            loss = ops.linear_cross_entropy(h, w, target, bias=b)
+            return (loss.detach(),) + torch.autograd.grad(loss, [h, w, b])
+        del loss, a
+        first = step()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            third = step()
+        for _ in range(3):
+            for t in third:
+                t.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            second = step()
+            for x, y, z in zip(first, second, third):
+                assert torch.equal(x, y) and torch.equal(x, z)
+
+
+def test_cross_entropy_gradient_against_differences():
+    from ts_trajgen_amd import ops
+    h, w, b, target = entropy_case(torch.float32, 30, 50, 16, seed=11)
+    loss = ops.linear_cross_entropy(h, w, target, bias=b)
+    grads = torch.autograd.grad(loss, [h, w, b])
+    n = float((target != -100).sum())
+    for i, g in enumerate(grads):
+        d = torch.randn_like(g)
+        args = [[x.detach().clone() for x in (h, w, b)] for _ in range(2)]
+        args[0][i] += 1e-3 * d
+        args[1][i] -= 1e-3 * d
+        hi, lo = (float(plain_cross_entropy(*a, target, -100, torch.ones(30))[0].sum()) / n for a in args)
+        # e^2 / 6 of the third derivative, and f32 rounding of the shifted arguments over 2 e
+        assert abs((hi - lo) / 2e-3 - float((g * d).sum())) < 1e-3 * (1.0 + abs(hi - lo) / 2e-3)
+
+
+def test_the_operators_together_over_packed_trajectories():
+    """states -> dropout -> attention -> dropout -> loss, as function G is fitted, against autograd through 64-bit forms."""
+    from ts_trajgen_amd import ops
+    lens = [5, 1, 33, 20]
+    n, width, vocab = sum(lens), 64, 400
+    g = torch.Generator().manual_seed(2)
+    x = (torch.randn(n, width, generator=g) * 0.5).to(DEV).requires_grad_(True)
+    w = (torch.randn(vocab, width, generator=g) * 0.2).to(DEV).requires_grad_(True)
+    b = (torch.randn(vocab, generator=g) * 0.2).to(DEV).requires_grad_(True)
+    target = torch.randint(0, vocab, (n,), generator=g).to(DEV)
+    target[torch.tensor(np.cumsum(lens) - 1)] = -100
+    p = torch.tensor(ptr(lens), dtype=torch.int32, device=DEV)
+
+    def fused():
+        s = ops.dropout(x, 0.3, 5, 0, 1)
+        a = ops.causal_attention(s.unsqueeze(1), s.unsqueeze(1), s.unsqueeze(1), p, scale=1.0).squeeze(1)
+        return ops.linear_cross_entropy(ops.dropout(a, 0.3, 5, 1, 1), w, target, bias=b)
+    loss = fused()
+    got = torch.autograd.grad(loss, [x, w, b])
+    xd, wd, bd = (t.detach().double().cpu().requires_grad_(True) for t in (x, w, b))
+    s = xd * keep_of(n * width, 0.3, 5, 0, 1).view(n, width) / 0.7
+    seq = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(lens))
+    pos = torch.arange(n)
+    z = (s @ s.t()).masked_fill((seq.unsqueeze(1) != seq) | (pos.unsqueeze(1) < pos), -math.inf)
+    a = (torch.softmax(z, 1) @ s) * keep_of(n * width, 0.3, 5, 1, 1).view(n, width) / 0.7
+    want = torch.nn.functional.cross_entropy(a @ wd.t() + bd, target.cpu())
+    assert rel(loss, want) < 1e-5
+    for a, e in zip(got, torch.autograd.grad(want, [xd, wd, bd])):
+        assert rel(a, e) < 1e-5

@@ -20,7 +20,8 @@ EXPORTS = ('tsg_version', 'tsg_gemm_f32', 'tsg_gat_forward', 'tsg_gat_forward_st
            'tsg_score_candidates', 'tsg_engine_reset', 'tsg_engine_run', 'tsg_engine_run_profiled', 'tsg_engine_graph_create', 'tsg_engine_graph_launch',
            'tsg_engine_graph_destroy', 'tsg_frontier_expand_select',
            'tsg_score_frontier', 'tsg_rollout_run', 'tsg_reconstruct_paths', 'tsg_h_pair_scores', 'tsg_geodesic_pairs',
-           'tsg_dropout', 'tsg_attn_workspace', 'tsg_attn_forward', 'tsg_attn_backward')
+           'tsg_dropout', 'tsg_attn_workspace', 'tsg_attn_forward', 'tsg_attn_backward', 'tsg_xent_workspace',
+           'tsg_xent_forward', 'tsg_xent_backward')
 
 _p = C.c_void_p
 _i32 = C.c_int32
@@ -120,6 +121,14 @@ class AttnDesc(C.Structure):
                                              'dv_head')] + [('delta', _p)]
 
 
+class XentDesc(C.Structure):
+    _fields_ = [('dtype', _i32), ('hidden', _i32), ('reduction', _i32), ('reserved', _i32), ('n_rows', C.c_int64),
+                ('n_vocab', C.c_int64), ('ignore_index', C.c_int64), ('h', _p), ('w', _p), ('bias', _p),
+                ('h_row', C.c_int64), ('w_row', C.c_int64), ('target', _p), ('row_loss', _p), ('loss', _p), ('stats', _p),
+                ('workspace', _p), ('workspace_bytes', _sz), ('d_loss', _p), ('dh', _p), ('dw', _p), ('dbias', _p),
+                ('dh_row', C.c_int64), ('dw_row', C.c_int64)]
+
+
 _lib = None
 
 
@@ -170,6 +179,9 @@ def lib():
     for name in ('tsg_attn_forward', 'tsg_attn_backward'):
         getattr(L, name).argtypes = [C.POINTER(AttnDesc), _p]
     L.tsg_attn_workspace.argtypes = [C.POINTER(AttnDesc), C.POINTER(_sz)]
+    L.tsg_xent_workspace.argtypes = [C.POINTER(XentDesc), C.POINTER(_sz), C.POINTER(_sz)]
+    for name in ('tsg_xent_forward', 'tsg_xent_backward'):
+        getattr(L, name).argtypes = [C.POINTER(XentDesc), _p]
     for name in EXPORTS:
         getattr(L, name).restype = C.c_int
     _lib = L

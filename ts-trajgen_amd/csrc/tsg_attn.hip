@@ -187,8 +187,8 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   const char* kbase = a.k + kvh * a.k_head;
   const char* vbase = a.v + kvh * a.v_head;
   auto fetch = [&](int k0, int buf) {
-    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE, kbase + (long)k0 * a.k_row, a.k_row, 0, b.hi - k0, a.chunks, wave, lane);
-    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE + TILE, vbase + (long)k0 * a.v_row, a.v_row, 0, b.hi - k0, a.chunks, wave, lane);
+    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE, kbase + (long)k0 * a.k_row, a.k_row, b.hi - k0, a.chunks, wave, lane);
+    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE + TILE, vbase + (long)k0 * a.v_row, a.v_row, b.hi - k0, a.chunks, wave, lane);
   };
   if (b.lo < b.hi) fetch(b.lo, 0);
   for (int k0 = b.lo, buf = 0; k0 < b.hi; k0 += BK, buf ^= 1) {
@@ -293,8 +293,8 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   const char* kbase = a.k + kvh * a.k_head;
   const char* vbase = a.v + kvh * a.v_head;
   auto fetch = [&](int k0, int buf) {
-    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE, kbase + (long)k0 * a.k_row, a.k_row, 0, b.hi - k0, a.chunks, wave, lane);
-    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE + TILE, vbase + (long)k0 * a.v_row, a.v_row, 0, b.hi - k0, a.chunks, wave, lane);
+    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE, kbase + (long)k0 * a.k_row, a.k_row, b.hi - k0, a.chunks, wave, lane);
+    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE + TILE, vbase + (long)k0 * a.v_row, a.v_row, b.hi - k0, a.chunks, wave, lane);
   };
   if (b.lo < b.hi) fetch(b.lo, 0);
   for (int k0 = b.lo, buf = 0; k0 < b.hi; k0 += BK, buf ^= 1) {
@@ -360,8 +360,8 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   const int per = b.lo < b.hi ? (b.hi - b.lo + BQ - 1) / BQ : 0, steps = per * a.group;
   auto fetch = [&](int step, int buf) {
     const int head = kvh * a.group + step / per, t0 = b.lo + (step % per) * BQ;
-    tsg_load_tile<BQ, CH, 4>(lds + buf * 2 * TILE, a.q + head * a.q_head + (long)t0 * a.q_row, a.q_row, 0, b.hi - t0, a.chunks, wave, lane);
-    tsg_load_tile<BQ, CH, 4>(lds + buf * 2 * TILE + TILE, a.d_o + head * a.do_head + (long)t0 * a.do_row, a.do_row, 0, b.hi - t0, a.chunks,
+    tsg_load_tile<BQ, CH, 4>(lds + buf * 2 * TILE, a.q + head * a.q_head + (long)t0 * a.q_row, a.q_row, b.hi - t0, a.chunks, wave, lane);
+    tsg_load_tile<BQ, CH, 4>(lds + buf * 2 * TILE + TILE, a.d_o + head * a.do_head + (long)t0 * a.do_row, a.do_row, b.hi - t0, a.chunks,
                              wave, lane);
   };
   auto stat_of = [&](int step, float2& st, float& delta) {

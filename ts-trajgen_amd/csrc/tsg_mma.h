@@ -129,17 +129,20 @@ template <> struct TsgAccB<TsgF32> {
 // tsg_dma_wait() before the barrier that hands the tile over.
 static __device__ const tsg_u4 tsg_zero_chunk = {0u, 0u, 0u, 0u};  // what chunks outside an operand are read from
 __device__ __forceinline__ void tsg_dma16(const void* g, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :
+  unsigned keep;  // m0 holds the LDS base of such a load; what the compiler has in it is put back
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(g)
-               : "memory", "m0");
+               : "memory");
 }
 __device__ __forceinline__ void tsg_dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// Tile [ROWS][CH] of a row-major operand: row r of the tile is src + r * stride bytes for r0 <= r < r1 and zeros elsewhere,
+// Tile [ROWS][CH] of a row-major operand: row r of the tile is src + r * stride bytes for r < r1 and zeros from there on,
 // chunks from `chunks` on are zeros.  All WAVES waves take part.
-template <int ROWS, int CH, int WAVES>
-__device__ __forceinline__ void tsg_load_tile(char* tile, const char* src, long stride, int r0, int r1, int chunks, int wave, int lane) {
+// MASKED: row r is zeros also where bit r of `used` is clear.
+template <int ROWS, int CH, int WAVES, bool MASKED = false>
+__device__ __forceinline__ void tsg_load_tile(char* tile, const char* src, long stride, int r1, int chunks, int wave, int lane,
+                                              unsigned long long used = 0) {
   constexpr int N = ROWS * CH / 64;  // instructions of 64 chunks
   static_assert(ROWS * CH % 64 == 0, "whole wave loads");
 #pragma unroll
@@ -148,7 +151,7 @@ __device__ __forceinline__ void tsg_load_tile(char* tile, const char* src, long 
     if (N % WAVES == 0 || ins < N) {
       const int at = ins * 64 + lane, r = at / CH, c = (at % CH) ^ tsg_swz<CH>(r);
       const char* g = src + (long)r * stride + c * 16;
-      if (r < r0 || r >= r1 || c >= chunks) g = reinterpret_cast<const char*>(&tsg_zero_chunk);
+      if (r >= r1 || c >= chunks || (MASKED && !(used >> r & 1))) g = reinterpret_cast<const char*>(&tsg_zero_chunk);
       tsg_dma16(g, tsg_lds_addr(tile) + ins * 1024);
     }
   }

@@ -2,6 +2,7 @@
 
     dropout(x, p, seed, site, step)                        mask recomputed from a counter, never stored
     causal_attention(q, k, v, seq_ptr, kv_ptr, scale)      packed sequences, grouped heads, forward and backward
+    linear_cross_entropy(h, weight, target, bias, ...)     loss over a large vocabulary, logits never kept
 
 They take tensors on a HIP device (f32, bf16 or f16), run on torch's current stream of that device, allocate their results and
 workspaces through torch's allocator and never synchronise, so they can be captured in a graph (forward and backward
@@ -216,7 +217,7 @@ class _CausalAttention(torch.autograd.Function):
         return tuple(t if wide == dim else t[..., :dim].contiguous() for t in (dq, dk, dv)) + (None, None, None)
 
 
-def _check_ptr(name, p, dev):
+def _check_ptr(name, p):
     if p.dtype != torch.int32 or p.dim() != 1 or p.numel() < 1 or not p.is_contiguous():
         raise ValueError('causal_attention: %s is a contiguous int32 vector of sequence starts, one more than sequences' % name)
 
@@ -233,7 +234,7 @@ def causal_attention(q, k, v, seq_ptr, kv_ptr=None, scale=None):
     nothing, and rows behind the last sequence, give zeros.  scale defaults to 1 / sqrt(dim) and is positive; function G's
     attention (function_g_fc.py:31-35) is one head with scale 1.  dim <= 512."""
     kv_ptr = seq_ptr if kv_ptr is None else kv_ptr
-    dev = _on_device('causal_attention', q, k, v, seq_ptr, kv_ptr)
+    _on_device('causal_attention', q, k, v, seq_ptr, kv_ptr)
     _dtype('causal_attention', q, k, v)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
         raise ValueError('causal_attention: q [n_q][heads][dim] and k, v [n_k][kv_heads][dim], got %s, %s, %s'
@@ -242,8 +243,8 @@ def causal_attention(q, k, v, seq_ptr, kv_ptr=None, scale=None):
         raise ValueError('causal_attention: heads of 1 to 512, got %d' % q.shape[2])
     if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
         raise ValueError('causal_attention: %d heads over %d key-value heads' % (q.shape[1], k.shape[1]))
-    _check_ptr('seq_ptr', seq_ptr, dev)
-    _check_ptr('kv_ptr', kv_ptr, dev)
+    _check_ptr('seq_ptr', seq_ptr)
+    _check_ptr('kv_ptr', kv_ptr)
     if seq_ptr.numel() != kv_ptr.numel():
         raise ValueError('causal_attention: %d and %d sequences' % (seq_ptr.numel() - 1, kv_ptr.numel() - 1))
     if seq_ptr is kv_ptr and q.shape[0] != k.shape[0]:
@@ -255,3 +256,107 @@ def causal_attention(q, k, v, seq_ptr, kv_ptr=None, scale=None):
     out = _CausalAttention.apply(q, k, v, seq_ptr, kv_ptr, scale)
     del held
     return out
+
+
+# ---------------------------------------------------------------------------------------------------- cross entropy
+REDUCTIONS = {'none': 0, 'sum': 1, 'mean': 2}
+
+
+def _rows_for(x, wide):
+    """x [rows][width] as the kernels read it: rows 16-byte aligned, padded with zeros to `wide`."""
+    per = 4 if x.dtype == torch.float32 else 8
+    if x.shape[1] != wide:
+        return torch.nn.functional.pad(x, (0, wide - x.shape[1]))
+    if x.stride(1) == 1 and x.stride(0) >= wide and x.stride(0) % per == 0 and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _xent_desc(h, w, bias, target, ignore, reduction, stats):
+    d = _lib.XentDesc()
+    d.dtype, d.hidden, d.reduction = DTYPES[h.dtype], h.shape[1], reduction
+    d.n_rows, d.n_vocab, d.ignore_index = h.shape[0], w.shape[0], ignore
+    d.h, d.w, d.bias = _lib.ptr(h), _lib.ptr(w), _lib.ptr(bias)
+    d.h_row, d.w_row = max(h.stride(0), h.shape[1]), max(w.stride(0), w.shape[1])
+    d.target, d.stats = _lib.ptr(target), _lib.ptr(stats)
+    return d
+
+
+def _xent_workspace(d, dev, backward):
+    sizes = C.c_size_t(), C.c_size_t()
+    _lib.check(_lib.lib().tsg_xent_workspace(C.byref(d), C.byref(sizes[0]), C.byref(sizes[1])), 'tsg_xent_workspace')
+    ws = torch.empty(sizes[backward].value, dtype=torch.uint8, device=dev)
+    d.workspace, d.workspace_bytes = _lib.ptr(ws), ws.numel()
+    return ws
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, w, bias, target, ignore, reduction):
+        wide = -(-h.shape[1] // 8) * 8
+        hl, wl = _rows_for(h.detach(), wide), _rows_for(w.detach(), wide)
+        bl = None if bias is None else bias.detach().contiguous()
+        target = target.contiguous()
+        stats = torch.empty((h.shape[0], 2), dtype=torch.float32, device=h.device)
+        rows = torch.empty(h.shape[0], dtype=torch.float32, device=h.device)
+        loss = rows if reduction == 0 else torch.empty((), dtype=torch.float32, device=h.device)
+        d = _xent_desc(hl, wl, bl, target, ignore, reduction, stats)
+        d.row_loss, d.loss = _lib.ptr(rows), _lib.ptr(loss)
+        ws = _xent_workspace(d, h.device, 0)
+        with torch.cuda.device(h.device):
+            _lib.check(_lib.lib().tsg_xent_forward(C.byref(d), _lib.current_stream()), 'tsg_xent_forward')
+        del ws
+        if any(ctx.needs_input_grad[:3]):
+            ctx.save_for_backward(h, w, bias, target, stats)
+            ctx.cfg = (ignore, reduction)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_loss):
+        h, w, bias, target, stats = ctx.saved_tensors
+        width, wide = h.shape[1], -(-h.shape[1] // 8) * 8
+        hl, wl = _rows_for(h.detach(), wide), _rows_for(w.detach(), wide)
+        bl = None if bias is None else bias.detach().contiguous()
+        d_loss = d_loss.contiguous().float()
+        d = _xent_desc(hl, wl, bl, target, ctx.cfg[0], ctx.cfg[1], stats)
+        dh = torch.empty((h.shape[0], wide), dtype=h.dtype, device=h.device)
+        dw = torch.empty((w.shape[0], wide), dtype=h.dtype, device=h.device)
+        db = None if bias is None else torch.empty_like(bl)
+        d.d_loss, d.dh, d.dw, d.dbias = _lib.ptr(d_loss), _lib.ptr(dh), _lib.ptr(dw), _lib.ptr(db)
+        d.dh_row = d.dw_row = wide
+        ws = _xent_workspace(d, h.device, 1)
+        with torch.cuda.device(h.device):
+            _lib.check(_lib.lib().tsg_xent_backward(C.byref(d), _lib.current_stream()), 'tsg_xent_backward')
+        del ws
+        if wide != width:
+            dh, dw = dh[:, :width].contiguous(), dw[:, :width].contiguous()
+        return dh, dw, db, None, None, None
+
+
+def linear_cross_entropy(h, weight, target, bias=None, ignore_index=-100, reduction='mean'):
+    """Cross entropy of softmax(h weight^T + bias) against target, differentiable in h, weight and bias, without the
+    [rows][vocabulary] logits being kept (they exist in pieces of the vocabulary, in the backward only).
+
+    h [rows][hidden], weight [vocabulary][hidden] (function G's out_fc.weight, function_g_fc.py:134), bias [vocabulary] or
+    None, all of one type (f32, bf16 or f16); target int64 [rows].  The loss is f32: per row ('none'), their sum
+    ('sum') or their mean over the rows whose target is not ignore_index ('mean'; NaN when there is none).  Rows with
+    ignore_index have loss 0 and add nothing to any gradient.  A target outside the vocabulary cannot be refused without
+    waiting for the device: it makes its row's loss and gradients NaN."""
+    _on_device('linear_cross_entropy', h, weight, bias, target)
+    _dtype('linear_cross_entropy', h, weight, bias)
+    if h.dim() != 2 or weight.dim() != 2 or h.shape[1] != weight.shape[1] or h.shape[1] < 1:
+        raise ValueError('linear_cross_entropy: h [rows][hidden] and weight [vocabulary][hidden], got %s and %s'
+                         % (tuple(h.shape), tuple(weight.shape)))
+    if h.shape[0] < 1 or weight.shape[0] < 1:
+        raise ValueError('linear_cross_entropy: at least one row and one entry, got %d and %d' % (h.shape[0], weight.shape[0]))
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError('linear_cross_entropy: bias of %d entries, got %s' % (weight.shape[0], tuple(bias.shape)))
+    if target.dtype != torch.int64 or tuple(target.shape) != (h.shape[0],):
+        raise ValueError('linear_cross_entropy: target is int64 [rows], got %s %s' % (target.dtype, tuple(target.shape)))
+    if reduction not in REDUCTIONS:
+        raise ValueError("linear_cross_entropy: reduction is 'none', 'sum' or 'mean', got %r" % (reduction,))
+    held = _hold_leaves(h, weight, bias)
+    loss = _LinearCrossEntropy.apply(h, weight, bias, target, int(ignore_index), REDUCTIONS[reduction])
+    del held
+    return loss
