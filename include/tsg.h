@@ -552,6 +552,8 @@ typedef struct tsg_attn_desc {
   void* out;               /* [n_q][heads][dim] */
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
   float* stats;            /* [heads][n_q][2], 8-byte aligned */
+  void* out_rest;          /* or NULL; 16-bit types: [n_q][heads][dim] contiguous, 16-byte aligned: what rounding took off out, written by
+                              the forward and read by the backward, whose d_out.out then is that of the unrounded out */
   void* workspace;
   size_t workspace_bytes;
   const void* d_out;       /* backward only from here on */

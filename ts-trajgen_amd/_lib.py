@@ -115,7 +115,7 @@ class AttnDesc(C.Structure):
                 ('n_q', C.c_int64), ('n_k', C.c_int64), ('q_ptr', _p), ('k_ptr', _p),
                 ('q', _p), ('k', _p), ('v', _p), ('out', _p)] + [
                     (n, C.c_int64) for n in ('q_row', 'q_head', 'k_row', 'k_head', 'v_row', 'v_head', 'out_row', 'out_head')] + [
-                ('stats', _p), ('workspace', _p), ('workspace_bytes', _sz),
+                ('stats', _p), ('out_rest', _p), ('workspace', _p), ('workspace_bytes', _sz),
                 ('d_out', _p), ('dq', _p), ('dk', _p), ('dv', _p)] + [
                     (n, C.c_int64) for n in ('d_out_row', 'd_out_head', 'dq_row', 'dq_head', 'dk_row', 'dk_head', 'dv_row',
                                              'dv_head')] + [('delta', _p)]

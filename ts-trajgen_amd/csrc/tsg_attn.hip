@@ -7,10 +7,10 @@
 // Sequences lie one behind the other (q_ptr / k_ptr).  Row t of sequence s sees keys [k0, k0 + (t - q0) + (lk - lq) + 1):
 // a contiguous interval of the packed keys, and both ends grow with t.  So a tile of query rows is simply a stretch of
 // the packed rows, whatever sequences it crosses: it walks the union of its rows' intervals and masks by the row's own.
-// Trajectories of a few dozen positions fill a tile of 128 that way.  The same holds for a tile of keys and the query
+// Trajectories of a few dozen positions fill a tile that way.  The same holds for a tile of keys and the query
 // rows that see them.  No lengths are needed on the host.  Rows of no sequence give zeros.
 //
-// Tile kernels (dim <= 256): a workgroup of four waves owns 128 rows, 32 per wave; the wave computes the TRANSPOSED
+// Tile kernels (dim <= 256): a workgroup of four waves owns 128 rows, 32 per wave (f32: 64 and 16); the wave computes the TRANSPOSED
 // score tile (A = keys, B = its rows), so that a lane holds one row: the softmax statistics are one register per
 // lane, and the probabilities feed the next product as they stand (tsg_mma.h).  Scores, statistics and outputs are held
 // in f32; p and ds are rounded to the operand type for the matrix cores (nearest even, 2^-9 relative for bf16, which is
@@ -27,6 +27,7 @@ struct AttnArgs {
   const int* q_ptr;
   const int* k_ptr;
   const char *q, *k, *v, *o, *d_o;
+  char* rest;    // [n_q][heads][dim] 16-bit, or null: what the rounding of out left over (o + rest is out to 2^-16)
   char *out, *dq, *dk, *dv;
   long q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head, dq_row, dq_head, dk_row, dk_head, dv_row,
       dv_head;   // bytes
@@ -74,18 +75,18 @@ __device__ __forceinline__ void rows_of_key(const AttnArgs& a, int j, int& lo, i
   if (hi <= lo) lo = hi = 0;
 }
 
-// Interval bounds over a wave (lanes l and l + 32 hold the same row) and over the workgroup
+// Interval bounds over a wave (lanes W apart hold the same row) and over the workgroup
 struct Bounds {
   int wave_lo, wave_hi;  // union of the wave's intervals; empty: wave_lo >= wave_hi
   int in_lo, in_hi;      // intersection; empty when a row of the wave is empty
   int lo, hi;            // union over the workgroup
 };
-__device__ __forceinline__ Bounds bounds_of(int lo, int hi, int wave, int* shared /* [8] */) {
+template <int W> __device__ __forceinline__ Bounds bounds_of(int lo, int hi, int wave, int* shared /* [8] */) {
   Bounds b;
   const bool none = hi <= lo;
   int ulo = none ? 0x7fffffff : lo, uhi = none ? 0 : hi, ilo = none ? 0x7fffffff : lo, ihi = none ? 0 : hi;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = W / 2; o > 0; o >>= 1) {
     ulo = min(ulo, __shfl_xor(ulo, o, 64));
     uhi = max(uhi, __shfl_xor(uhi, o, 64));
     ilo = max(ilo, __shfl_xor(ilo, o, 64));
@@ -105,10 +106,10 @@ __device__ __forceinline__ Bounds bounds_of(int lo, int hi, int wave, int* share
 }
 
 // operand fragments of one row per lane, straight from memory; zeros outside
-template <int NF> __device__ __forceinline__ void load_frags(tsg_u4 (&f)[NF], const char* row, bool ok, int chunks, int h) {
+template <int PARTS, int NF> __device__ __forceinline__ void load_frags(tsg_u4 (&f)[NF], const char* row, bool ok, int chunks, int h) {
 #pragma unroll
   for (int s = 0; s < NF; ++s) {
-    const int c = 2 * s + h;
+    const int c = PARTS * s + h;
     const char* g = ok && c < chunks ? row + c * 16 : reinterpret_cast<const char*>(&tsg_zero_chunk);
     f[s] = *reinterpret_cast<const tsg_u4*>(g);
   }
@@ -147,48 +148,67 @@ template <typename D> __device__ __forceinline__ void store4(char* at, float x, 
 template <> __device__ __forceinline__ void store4<TsgF32>(char* at, float x, float y, float z, float w) {
   *reinterpret_cast<float4*>(at) = make_float4(x, y, z, w);
 }
-// transposed accumulators [dim][row] -> one row per lane
-template <typename D, int ND> __device__ __forceinline__ void store_rows(const tsg_f32x16 (&acc)[ND], char* row, float by, int dim, int h) {
+// transposed accumulators [dim][row] -> one row per lane; REST: what the rounding left over instead
+template <typename D, int ND, bool REST = false>
+__device__ __forceinline__ void store_rows(const typename TsgElem<D>::Acc (&acc)[ND], char* row, float by, int dim, int h) {
+  typedef TsgElem<D> E;
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * dt + 8 * g + 4 * h;
-      if (d < dim)
-        store4<D>(row + d * TsgElem<D>::BYTES, acc[dt][4 * g] * by, acc[dt][4 * g + 1] * by, acc[dt][4 * g + 2] * by, acc[dt][4 * g + 3] * by);
+    for (int g = 0; g < E::REGS / 4; ++g) {
+      const int d = E::W * dt + 8 * g + 4 * h;
+      float x[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[r] = acc[dt][4 * g + r] * by;
+        if (REST) x[r] -= (float)(typename E::T)x[r];
+      }
+      if (d < dim) store4<D>(row + d * E::BYTES, x[0], x[1], x[2], x[3]);
     }
 }
 
-__device__ __forceinline__ float both_halves_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
-__device__ __forceinline__ float both_halves_sum(float v) { return v + __shfl_xor(v, 32, 64); }
+template <int W> __device__ __forceinline__ float parts_max(float v) {
+#pragma unroll
+  for (int o = W; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+template <int W> __device__ __forceinline__ float parts_sum(float v) {
+#pragma unroll
+  for (int o = W; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+template <typename D> constexpr int rows_per_wg() { return 4 * TsgElem<D>::W; }
 
 // ------------------------------------------------------------------------------------------------- forward, tiles
 template <typename D, int DP, int BK>
 __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
-  constexpr int CH = DP / TsgElem<D>::EPC, NF = CH / 2, ND = DP / 32, NB = BK / 32, TILE = BK * CH * 16;
+  typedef TsgElem<D> E;
+  typedef typename E::Acc Acc;
+  constexpr bool F32 = E::BYTES == 4;
+  constexpr int W = E::W, PARTS = 64 / W, CH = DP / E::EPC, NF = CH / PARTS, ND = DP / W, NB = BK / W, TILE = BK * CH * 16;
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
   __shared__ int edge[8];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane >> 5;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane / W;
   const int tiles = gridDim.x / a.heads;
   const int tile = tiles - 1 - (int)(blockIdx.x / a.heads), head = blockIdx.x % a.heads;  // late rows see most keys: first
   const int kvh = head / a.group;
-  const int t = tile * 128 + wave * 32 + (lane & 31);
+  const int t = tile * (4 * W) + wave * W + lane % W;
   int lo, hi;
   keys_of_row(a, t, lo, hi);
-  const Bounds b = bounds_of(lo, hi, wave, edge);
+  const Bounds b = bounds_of<W>(lo, hi, wave, edge);
   tsg_u4 qf[NF];
-  load_frags(qf, a.q + (long)t * a.q_row + head * a.q_head, t < a.n_q, a.chunks, h);
-  tsg_f32x16 acc[ND];
+  load_frags<PARTS>(qf, a.q + (long)t * a.q_row + head * a.q_head, t < a.n_q, a.chunks, h);
+  Acc acc[ND];
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[dt][i] = 0.0f;
+    for (int i = 0; i < E::REGS; ++i) acc[dt][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
   const char* kbase = a.k + kvh * a.k_head;
   const char* vbase = a.v + kvh * a.v_head;
   auto fetch = [&](int k0, int buf) {
-    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE, kbase + (long)k0 * a.k_row, a.k_row, b.hi - k0, a.chunks, wave, lane);
-    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE + TILE, vbase + (long)k0 * a.v_row, a.v_row, b.hi - k0, a.chunks, wave, lane);
+    tsg_load_tile<BK, CH, 4, false, F32>(lds + buf * 2 * TILE, kbase + (long)k0 * a.k_row, a.k_row, b.hi - k0, a.chunks, wave, lane);
+    tsg_load_tile<BK, CH, 4, false, F32>(lds + buf * 2 * TILE + TILE, vbase + (long)k0 * a.v_row, a.v_row, b.hi - k0, a.chunks, wave, lane);
   };
   if (b.lo < b.hi) fetch(b.lo, 0);
   for (int k0 = b.lo, buf = 0; k0 < b.hi; k0 += BK, buf ^= 1) {
@@ -198,20 +218,20 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
     if (k0 >= b.wave_hi || k0 + BK <= b.wave_lo) continue;  // nothing for this wave: uniform, the barriers are above
     const char* kt = lds + buf * 2 * TILE;
     const char* vt = kt + TILE;
-    tsg_f32x16 z[NB];
+    Acc z[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) z[n][i] = 0.0f;
+      for (int i = 0; i < E::REGS; ++i) z[n][i] = 0.0f;
 #pragma unroll
-      for (int s = 0; s < NF; ++s) tsg_mma<D>(tsg_row_frag<CH>(kt, 32 * n + (lane & 31), 2 * s + h), qf[s], z[n]);
+      for (int s = 0; s < NF; ++s) tsg_mma<D>(tsg_row_frag<CH, F32>(kt, W * n + lane % W, PARTS * s + h), qf[s], z[n]);
     }
     if (k0 < b.in_lo || k0 + BK > b.in_hi) {
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = k0 + 32 * n + (i & 3) + 8 * (i >> 2) + 4 * h;
+        for (int i = 0; i < E::REGS; ++i) {
+          const int key = k0 + W * n + (i & 3) + 8 * (i >> 2) + 4 * h;
           if (key < lo || key >= hi) z[n][i] = -INFINITY;
         }
     }
@@ -219,8 +239,8 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, z[n][i]);
-    top = both_halves_max(top);
+      for (int i = 0; i < E::REGS; ++i) top = fmaxf(top, z[n][i]);
+    top = parts_max<W>(top);
     // The maximum is taken off before the scaling: products of the type's lowest value stay finite that way.
     const float off = top == -INFINITY ? 0.0f : top;  // nothing seen yet: exp2(-inf) = 0, not NaN
     if (__any(top > m)) {
@@ -229,25 +249,27 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[dt][i] *= fade;
+        for (int i = 0; i < E::REGS; ++i) acc[dt][i] *= fade;
     }
     m = top;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < E::REGS; ++i) {
         z[n][i] = __builtin_amdgcn_exp2f((z[n][i] - off) * a.scale2);
         l += z[n][i];
       }
       TsgAccB<D> p;
       p.set(z[n]);
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt) p.template mma<CH>(vt, 32 * n, 32 * dt, acc[dt], lane);
+      for (int dt = 0; dt < ND; ++dt) p.template mma<CH>(vt, W * n, W * dt, acc[dt], lane);
     }
   }
-  l = both_halves_sum(l);
+  l = parts_sum<W>(l);
   if (t < a.n_q) {
-    store_rows<D, ND>(acc, a.out + (long)t * a.o_row + head * a.o_head, l == 0.0f ? 0.0f : 1.0f / l, a.dim, h);
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    store_rows<D, ND>(acc, a.out + (long)t * a.o_row + head * a.o_head, by, a.dim, h);
+    if (!F32 && a.rest) store_rows<D, ND, true>(acc, a.rest + ((long)t * a.heads + head) * a.dim * E::BYTES, by, a.dim, h);
     if (h == 0) a.stat[(long)head * a.n_q + t] = l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l));
   }
 }
@@ -255,46 +277,53 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
 // ------------------------------------------------------------------------------------------------ backward, tiles: dq
 template <typename D, int DP, int BK>
 __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
-  constexpr int CH = DP / TsgElem<D>::EPC, NF = CH / 2, ND = DP / 32, NB = BK / 32, TILE = BK * CH * 16;
+  typedef TsgElem<D> E;
+  typedef typename E::Acc Acc;
+  constexpr bool F32 = E::BYTES == 4;
+  constexpr int W = E::W, PARTS = 64 / W, CH = DP / E::EPC, NF = CH / PARTS, ND = DP / W, NB = BK / W, TILE = BK * CH * 16;
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
   __shared__ int edge[8];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane >> 5;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane / W;
   const int tiles = gridDim.x / a.heads;
   const int tile = tiles - 1 - (int)(blockIdx.x / a.heads), head = blockIdx.x % a.heads;
   const int kvh = head / a.group;
-  const int t = tile * 128 + wave * 32 + (lane & 31);
+  const int t = tile * (4 * W) + wave * W + lane % W;
   int lo, hi;
   keys_of_row(a, t, lo, hi);
-  const Bounds b = bounds_of(lo, hi, wave, edge);
+  const Bounds b = bounds_of<W>(lo, hi, wave, edge);
   tsg_u4 qf[NF], gf[NF];
-  load_frags(qf, a.q + (long)t * a.q_row + head * a.q_head, t < a.n_q, a.chunks, h);
-  load_frags(gf, a.d_o + (long)t * a.do_row + head * a.do_head, t < a.n_q, a.chunks, h);
+  load_frags<PARTS>(qf, a.q + (long)t * a.q_row + head * a.q_head, t < a.n_q, a.chunks, h);
+  load_frags<PARTS>(gf, a.d_o + (long)t * a.do_row + head * a.do_head, t < a.n_q, a.chunks, h);
   float delta = 0.0f;
   float2 st = make_float2(0.0f, INFINITY);
   {
     const char* orow = a.o + (long)t * a.o_row + head * a.o_head;
 #pragma unroll
     for (int s = 0; s < NF; ++s) {
-      const int c = 2 * s + h;
+      const int c = PARTS * s + h;
       const char* g = t < a.n_q && c < a.chunks ? orow + c * 16 : reinterpret_cast<const char*>(&tsg_zero_chunk);
       delta += frag_dot<D>(*reinterpret_cast<const tsg_u4*>(g), gf[s]);
+      if (!F32 && a.rest) {
+        g = t < a.n_q && c < a.chunks ? a.rest + (((long)t * a.heads + head) * a.dim) * E::BYTES + c * 16 : reinterpret_cast<const char*>(&tsg_zero_chunk);
+        delta += frag_dot<D>(*reinterpret_cast<const tsg_u4*>(g), gf[s]);
+      }
     }
-    delta = both_halves_sum(delta);
+    delta = parts_sum<W>(delta);
     if (t < a.n_q) {
       st = a.stat[(long)head * a.n_q + t];
       if (h == 0) a.delta[(long)head * a.n_q + t] = delta;  // the dk / dv kernel, next on the stream, reads it
     }
   }
-  tsg_f32x16 acc[ND];
+  Acc acc[ND];
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[dt][i] = 0.0f;
+    for (int i = 0; i < E::REGS; ++i) acc[dt][i] = 0.0f;
   const char* kbase = a.k + kvh * a.k_head;
   const char* vbase = a.v + kvh * a.v_head;
   auto fetch = [&](int k0, int buf) {
-    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE, kbase + (long)k0 * a.k_row, a.k_row, b.hi - k0, a.chunks, wave, lane);
-    tsg_load_tile<BK, CH, 4>(lds + buf * 2 * TILE + TILE, vbase + (long)k0 * a.v_row, a.v_row, b.hi - k0, a.chunks, wave, lane);
+    tsg_load_tile<BK, CH, 4, false, F32>(lds + buf * 2 * TILE, kbase + (long)k0 * a.k_row, a.k_row, b.hi - k0, a.chunks, wave, lane);
+    tsg_load_tile<BK, CH, 4, false, F32>(lds + buf * 2 * TILE + TILE, vbase + (long)k0 * a.v_row, a.v_row, b.hi - k0, a.chunks, wave, lane);
   };
   if (b.lo < b.hi) fetch(b.lo, 0);
   for (int k0 = b.lo, buf = 0; k0 < b.hi; k0 += BK, buf ^= 1) {
@@ -307,17 +336,17 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
     const bool edge_tile = k0 < b.in_lo || k0 + BK > b.in_hi;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      tsg_f32x16 z, dp;
+      Acc z, dp;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) z[i] = 0.0f, dp[i] = -delta;  // dp - delta comes out of the product
+      for (int i = 0; i < E::REGS; ++i) z[i] = 0.0f, dp[i] = -delta;  // dp - delta comes out of the product
 #pragma unroll
       for (int s = 0; s < NF; ++s) {
-        tsg_mma<D>(tsg_row_frag<CH>(kt, 32 * n + (lane & 31), 2 * s + h), qf[s], z);
-        tsg_mma<D>(tsg_row_frag<CH>(vt, 32 * n + (lane & 31), 2 * s + h), gf[s], dp);
+        tsg_mma<D>(tsg_row_frag<CH, F32>(kt, W * n + lane % W, PARTS * s + h), qf[s], z);
+        tsg_mma<D>(tsg_row_frag<CH, F32>(vt, W * n + lane % W, PARTS * s + h), gf[s], dp);
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = k0 + 32 * n + (i & 3) + 8 * (i >> 2) + 4 * h;
+      for (int i = 0; i < E::REGS; ++i) {
+        const int key = k0 + W * n + (i & 3) + 8 * (i >> 2) + 4 * h;
         float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i] - st.x, a.scale2, -st.y)) * dp[i];
         if (edge_tile && (key < lo || key >= hi)) p = 0.0f;
         z[i] = p;
@@ -325,34 +354,37 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
       TsgAccB<D> ds;
       ds.set(z);
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt) ds.template mma<CH>(kt, 32 * n, 32 * dt, acc[dt], lane);
+      for (int dt = 0; dt < ND; ++dt) ds.template mma<CH>(kt, W * n, W * dt, acc[dt], lane);
     }
   }
   if (t < a.n_q) store_rows<D, ND>(acc, a.dq + (long)t * a.dq_row + head * a.dq_head, a.scale, a.dim, h);
 }
 
 // ------------------------------------------------------------------------------------------ backward, tiles: dk and dv
-// PART 0: both; 1: dv only; 2: dk only (f32 at 256 wide: keys, values and both sums do not fit the registers at once)
+// PART 0: both; 1: dv only; 2: dk only (16-bit types at 256 wide: keys, values and both sums do not fit the registers at once)
 template <typename D, int DP, int BQ, int PART>
 __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
-  constexpr int CH = DP / TsgElem<D>::EPC, NF = CH / 2, ND = DP / 32, NB = BQ / 32, TILE = BQ * CH * 16;
+  typedef TsgElem<D> E;
+  typedef typename E::Acc Acc;
+  constexpr bool F32 = E::BYTES == 4;
+  constexpr int W = E::W, PARTS = 64 / W, CH = DP / E::EPC, NF = CH / PARTS, ND = DP / W, NB = BQ / W, TILE = BQ * CH * 16;
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
   __shared__ __attribute__((aligned(16))) float stat[2][3][BQ];  // maximum, log2 of the sum, delta
   __shared__ int edge[8];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane >> 5;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane / W;
   const int tile = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads;  // early keys are seen by most rows: first
-  const int j = tile * 128 + wave * 32 + (lane & 31);
+  const int j = tile * (4 * W) + wave * W + lane % W;
   int lo, hi;
   rows_of_key(a, j, lo, hi);
-  const Bounds b = bounds_of(lo, hi, wave, edge);
+  const Bounds b = bounds_of<W>(lo, hi, wave, edge);
   tsg_u4 kf[NF], vf[PART == 1 ? 1 : NF];
-  load_frags(kf, a.k + (long)j * a.k_row + kvh * a.k_head, j < a.n_k, a.chunks, h);
-  if constexpr (PART != 1) load_frags(vf, a.v + (long)j * a.v_row + kvh * a.v_head, j < a.n_k, a.chunks, h);
-  tsg_f32x16 dk[PART == 1 ? 1 : ND], dv[PART == 2 ? 1 : ND];
+  load_frags<PARTS>(kf, a.k + (long)j * a.k_row + kvh * a.k_head, j < a.n_k, a.chunks, h);
+  if constexpr (PART != 1) load_frags<PARTS>(vf, a.v + (long)j * a.v_row + kvh * a.v_head, j < a.n_k, a.chunks, h);
+  Acc dk[PART == 1 ? 1 : ND], dv[PART == 2 ? 1 : ND];
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < E::REGS; ++i) {
       if constexpr (PART != 1) dk[dt][i] = 0.0f;
       if constexpr (PART != 2) dv[dt][i] = 0.0f;
     }
@@ -360,8 +392,8 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   const int per = b.lo < b.hi ? (b.hi - b.lo + BQ - 1) / BQ : 0, steps = per * a.group;
   auto fetch = [&](int step, int buf) {
     const int head = kvh * a.group + step / per, t0 = b.lo + (step % per) * BQ;
-    tsg_load_tile<BQ, CH, 4>(lds + buf * 2 * TILE, a.q + head * a.q_head + (long)t0 * a.q_row, a.q_row, b.hi - t0, a.chunks, wave, lane);
-    tsg_load_tile<BQ, CH, 4>(lds + buf * 2 * TILE + TILE, a.d_o + head * a.do_head + (long)t0 * a.do_row, a.do_row, b.hi - t0, a.chunks,
+    tsg_load_tile<BQ, CH, 4, false, F32>(lds + buf * 2 * TILE, a.q + head * a.q_head + (long)t0 * a.q_row, a.q_row, b.hi - t0, a.chunks, wave, lane);
+    tsg_load_tile<BQ, CH, 4, false, F32>(lds + buf * 2 * TILE + TILE, a.d_o + head * a.do_head + (long)t0 * a.do_row, a.do_row, b.hi - t0, a.chunks,
                              wave, lane);
   };
   auto stat_of = [&](int step, float2& st, float& delta) {
@@ -394,26 +426,26 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
       const bool edge_tile = t0 < b.in_lo || t0 + BQ > b.in_hi;
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        tsg_f32x16 z, dp;
+        Acc z, dp;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 dl = *reinterpret_cast<const float4*>(&stat[buf][2][32 * n + 8 * g + 4 * h]);
+        for (int g = 0; g < E::REGS / 4; ++g) {
+          const float4 dl = *reinterpret_cast<const float4*>(&stat[buf][2][W * n + 8 * g + 4 * h]);
           z[4 * g] = z[4 * g + 1] = z[4 * g + 2] = z[4 * g + 3] = 0.0f;
           dp[4 * g] = -dl.x, dp[4 * g + 1] = -dl.y, dp[4 * g + 2] = -dl.z, dp[4 * g + 3] = -dl.w;
         }
 #pragma unroll
         for (int s = 0; s < NF; ++s) {
-          tsg_mma<D>(tsg_row_frag<CH>(qt, 32 * n + (lane & 31), 2 * s + h), kf[s], z);
-          if constexpr (PART != 1) tsg_mma<D>(tsg_row_frag<CH>(gt, 32 * n + (lane & 31), 2 * s + h), vf[s], dp);
+          tsg_mma<D>(tsg_row_frag<CH, F32>(qt, W * n + lane % W, PARTS * s + h), kf[s], z);
+          if constexpr (PART != 1) tsg_mma<D>(tsg_row_frag<CH, F32>(gt, W * n + lane % W, PARTS * s + h), vf[s], dp);
         }
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 ms = *reinterpret_cast<const float4*>(&stat[buf][0][32 * n + 8 * g + 4 * h]);
-          const float4 ls = *reinterpret_cast<const float4*>(&stat[buf][1][32 * n + 8 * g + 4 * h]);
+        for (int g = 0; g < E::REGS / 4; ++g) {
+          const float4 ms = *reinterpret_cast<const float4*>(&stat[buf][0][W * n + 8 * g + 4 * h]);
+          const float4 ls = *reinterpret_cast<const float4*>(&stat[buf][1][W * n + 8 * g + 4 * h]);
           const float mv[4] = {ms.x, ms.y, ms.z, ms.w}, lv[4] = {ls.x, ls.y, ls.z, ls.w};
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int t = t0 + 32 * n + 8 * g + 4 * h + r;
+            const int t = t0 + W * n + 8 * g + 4 * h + r;
             const bool out = edge_tile && (t < lo || t >= hi);
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[4 * g + r] - mv[r], a.scale2, -lv[r]));
             z[4 * g + r] = out ? 0.0f : p;
@@ -424,13 +456,13 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
           TsgAccB<D> pb;
           pb.set(z);
 #pragma unroll
-          for (int dt = 0; dt < ND; ++dt) pb.template mma<CH>(gt, 32 * n, 32 * dt, dv[dt], lane);
+          for (int dt = 0; dt < ND; ++dt) pb.template mma<CH>(gt, W * n, W * dt, dv[dt], lane);
         }
         if constexpr (PART != 1) {
           TsgAccB<D> sb;
           sb.set(dp);
 #pragma unroll
-          for (int dt = 0; dt < ND; ++dt) sb.template mma<CH>(qt, 32 * n, 32 * dt, dk[dt], lane);
+          for (int dt = 0; dt < ND; ++dt) sb.template mma<CH>(qt, W * n, W * dt, dk[dt], lane);
         }
       }
     }
@@ -608,7 +640,9 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
       if (y == g) sg = sum[y], tg = top[y];
     if (a.n_split == 1) {
       typedef typename D::type T;
-      reinterpret_cast<T*>(a.out + (long)t * a.o_row + (head0 + g) * a.o_head)[d] = (T)(v * (sg == 0.0f ? 0.0f : 1.0f / sg));
+      const float x = v * (sg == 0.0f ? 0.0f : 1.0f / sg);
+      reinterpret_cast<T*>(a.out + (long)t * a.o_row + (head0 + g) * a.o_head)[d] = (T)x;
+      if (a.rest) reinterpret_cast<T*>(a.rest)[((long)t * a.heads + head0 + g) * a.dim + d] = (T)(x - (float)(T)x);
       if (d == 0) a.stat[(long)(head0 + g) * a.n_q + t] = sg == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(tg, __builtin_amdgcn_logf(sg));
     } else {
       float* p = a.part + (((long)t * a.heads + head0 + g) * a.n_split + split) * (a.dim + 2);
@@ -636,7 +670,9 @@ template <typename D> __global__ __launch_bounds__(64) void attn_join_kernel(Att
     float v = 0.0f;
     for (int s = 0; s < a.n_split; ++s)
       v += p[(long)s * (a.dim + 2) + d] * __builtin_amdgcn_exp2f((p[(long)s * (a.dim + 2) + a.dim] - off) * a.scale2);
-    reinterpret_cast<T*>(a.out + (long)t * a.o_row + head * a.o_head)[d] = (T)(v * by);
+    v *= by;
+    reinterpret_cast<T*>(a.out + (long)t * a.o_row + head * a.o_head)[d] = (T)v;
+    if (a.rest) reinterpret_cast<T*>(a.rest)[((long)t * a.heads + head) * a.dim + d] = (T)(v - (float)(T)v);
   }
   if (lane == 0) a.stat[(long)head * a.n_q + t] = l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(top, __builtin_amdgcn_logf(l));
 }
@@ -668,7 +704,11 @@ template <typename D> __global__ __launch_bounds__(64) void attn_wide_dq_kernel(
   load_wide<T>(q, a.q + (long)t * a.q_row + head * a.q_head, a.dim, lane);
   load_wide<T>(g, a.d_o + (long)t * a.do_row + head * a.do_head, a.dim, lane);
   load_wide<T>(x, a.o + (long)t * a.o_row + head * a.o_head, a.dim, lane);
-  const float delta = dot_wide(g, x);
+  float delta = dot_wide(g, x);
+  if (a.rest) {
+    load_wide<T>(x, a.rest + ((long)t * a.heads + head) * a.dim * sizeof(T), a.dim, lane);
+    delta += dot_wide(g, x);
+  }
   const float2 st = a.stat[(long)head * a.n_q + t];
   if (lane == 0) a.delta[(long)head * a.n_q + t] = delta;
 #pragma unroll
@@ -755,6 +795,7 @@ int check_attn(const tsg_attn_desc* d, bool backward) {
   for (int i = 0; i < 16; ++i)
     if (s[i] % epc || s[i] < 0) return TSG_E_INVALID;
   if (backward && !d->delta) return TSG_E_INVALID;
+  if ((uintptr_t)d->out_rest % 16) return TSG_E_INVALID;
   return 0;
 }
 
@@ -773,6 +814,7 @@ AttnArgs args_of(const tsg_attn_desc* d) {
   a.dk_row = d->dk_row * b, a.dk_head = d->dk_head * b, a.dv_row = d->dv_row * b, a.dv_head = d->dv_head * b;
   a.stat = (float2*)d->stats, a.delta = d->delta;
   a.scale = d->scale, a.scale2 = d->scale * 1.44269504088896340736f;
+  a.rest = d->dtype == TSG_F32 ? nullptr : (char*)d->out_rest;
   a.n_split = 1;
   a.part = (float*)d->workspace;
   return a;
@@ -801,10 +843,10 @@ template <typename D> int forward_of(const tsg_attn_desc* d, hipStream_t s) {
     else launch_rows<D, 64, F>(a, s);
     if (a.n_split > 1) hipLaunchKernelGGL(attn_join_kernel<D>, dim3((unsigned)((long)a.n_q * a.heads)), dim3(64), 0, s, a);
   } else {
-    const dim3 grid((unsigned)(tsg_cdiv(a.n_q, 128) * a.heads)), block(256);
-    constexpr bool F32 = TsgElem<D>::BYTES == 4;
+    const dim3 grid((unsigned)(tsg_cdiv(a.n_q, rows_per_wg<D>()) * a.heads)), block(256);
+    constexpr int BK = TsgElem<D>::BYTES == 4 ? 32 : 64;
     if (a.dim <= 64) hipLaunchKernelGGL((attn_fwd_kernel<D, 64, 64>), grid, block, 0, s, a);
-    else if (a.dim <= 128) hipLaunchKernelGGL((attn_fwd_kernel<D, 128, F32 ? 32 : 64>), grid, block, 0, s, a);
+    else if (a.dim <= 128) hipLaunchKernelGGL((attn_fwd_kernel<D, 128, BK>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((attn_fwd_kernel<D, 256, 32>), grid, block, 0, s, a);
   }
   TSG_LAUNCH_CHECK();
@@ -820,7 +862,8 @@ template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
     TSG_LAUNCH_CHECK();
     return 0;
   }
-  const dim3 gq((unsigned)(tsg_cdiv(a.n_q, 128) * a.heads)), gk((unsigned)(tsg_cdiv(a.n_k, 128) * a.kv_heads));
+  constexpr int R = rows_per_wg<D>();
+  const dim3 gq((unsigned)(tsg_cdiv(a.n_q, R) * a.heads)), gk((unsigned)(tsg_cdiv(a.n_k, R) * a.kv_heads));
   constexpr bool F32 = TsgElem<D>::BYTES == 4;
   if (a.n_q) {
     if (a.dim <= 64) hipLaunchKernelGGL((attn_dq_kernel<D, 64, 64>), gq, block, 0, s, a);
@@ -830,10 +873,11 @@ template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
   if (a.n_k) {
     if (a.dim <= 64) hipLaunchKernelGGL((attn_dkv_kernel<D, 64, 32, 0>), gk, block, 0, s, a);
     else if (a.dim <= 128) hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0>), gk, block, 0, s, a);
-    else if constexpr (F32) {
+    else if constexpr (F32) hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 0>), gk, block, 0, s, a);
+    else {
       hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 1>), gk, block, 0, s, a);
       hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 2>), gk, block, 0, s, a);
-    } else hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 0>), gk, block, 0, s, a);
+    }
   }
   TSG_LAUNCH_CHECK();
   return 0;

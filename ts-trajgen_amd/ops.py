@@ -175,6 +175,10 @@ class _CausalAttention(torch.autograd.Function):
         out = torch.empty((q.shape[0], q.shape[1], wide), dtype=q.dtype, device=q.device)
         stats = torch.empty((q.shape[1], q.shape[0], 2), dtype=torch.float32, device=q.device)
         d = _attn_desc(ql, kl, vl, q_ptr, k_ptr, scale, out, stats)
+        rest = None
+        if q.dtype != torch.float32 and any(ctx.needs_input_grad[:3]):
+            rest = torch.empty(out.shape, dtype=q.dtype, device=q.device)
+            d.out_rest = _lib.ptr(rest)
         need = C.c_size_t()
         _lib.check(L.tsg_attn_workspace(C.byref(d), C.byref(need)), 'tsg_attn_workspace')
         if need.value:
@@ -188,20 +192,21 @@ class _CausalAttention(torch.autograd.Function):
         if any(ctx.needs_input_grad[:3]):
             ctx.scale, ctx.dim = scale, dim
             res = out if wide == dim else out[..., :dim].contiguous()
-            ctx.save_for_backward(q, k, v, q_ptr, k_ptr, res, stats)
+            ctx.save_for_backward(q, k, v, q_ptr, k_ptr, res, stats, rest)
             return res
         return out if wide == dim else out[..., :dim].contiguous()
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        q, k, v, q_ptr, k_ptr, out, stats = ctx.saved_tensors
+        q, k, v, q_ptr, k_ptr, out, stats, rest = ctx.saved_tensors
         dim, per = ctx.dim, 4 if q.dtype == torch.float32 else 8
         wide = -(-dim // per) * per
         ql, kl, vl, ol, gl = (_laid_out(t.detach(), per, wide) for t in (q, k, v, out, d_out))
         dq, dk, dv = (torch.empty(t.shape[:2] + (wide,), dtype=t.dtype, device=t.device) for t in (q, k, v))
         if q.shape[0] and k.shape[0]:
             d = _attn_desc(ql, kl, vl, q_ptr, k_ptr, ctx.scale, ol, stats)
+            d.out_rest = _lib.ptr(rest)
             delta = torch.empty(stats.shape[:2], dtype=torch.float32, device=q.device)
             d.d_out, d.d_out_row, d.d_out_head = _lib.ptr(gl), gl.stride(0), gl.stride(1)
             for name, t in (('dq', dq), ('dk', dk), ('dv', dv)):
