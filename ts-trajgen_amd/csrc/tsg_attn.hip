@@ -177,6 +177,8 @@ template <int W> __device__ __forceinline__ float parts_sum(float v) {
   for (int o = W; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
+// in a branch that is seldom taken: keeps the compiler from running both sides and selecting
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
 template <typename D> constexpr int rows_per_wg() { return 4 * TsgElem<D>::W; }
 
 // ------------------------------------------------------------------------------------------------- forward, tiles
@@ -186,9 +188,10 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   typedef typename E::Acc Acc;
   constexpr bool F32 = E::BYTES == 4;
   constexpr int W = E::W, PARTS = 64 / W, CH = DP / E::EPC, NF = CH / PARTS, ND = DP / W, NB = BK / W, TILE = BK * CH * 16;
-  __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
   __shared__ int edge[8];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane / W;
+  const unsigned row0 = tsg_lds_addr(lds) + TsgLane<D, CH>::row(lane), col0 = tsg_lds_addr(lds) + TsgLane<D, CH>::col(lane);
   const int tiles = gridDim.x / a.heads;
   const int tile = tiles - 1 - (int)(blockIdx.x / a.heads), head = blockIdx.x % a.heads;  // late rows see most keys: first
   const int kvh = head / a.group;
@@ -216,23 +219,24 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
     __syncthreads();
     if (k0 + BK < b.hi) fetch(k0 + BK, buf ^ 1);
     if (k0 >= b.wave_hi || k0 + BK <= b.wave_lo) continue;  // nothing for this wave: uniform, the barriers are above
-    const char* kt = lds + buf * 2 * TILE;
-    const char* vt = kt + TILE;
+    const unsigned row = tsg_opaque(row0) + buf * 2 * TILE, col = tsg_opaque(col0) + buf * 2 * TILE;
     Acc z[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
 #pragma unroll
       for (int i = 0; i < E::REGS; ++i) z[n][i] = 0.0f;
 #pragma unroll
-      for (int s = 0; s < NF; ++s) tsg_mma<D>(tsg_row_frag<CH, F32>(kt, W * n + lane % W, PARTS * s + h), qf[s], z[n]);
+      for (int s = 0; s < NF; ++s) tsg_mma<D>(tsg_row_frag<D>(row, s, W * n * CH * 16), qf[s], z[n]);
     }
     if (k0 < b.in_lo || k0 + BK > b.in_hi) {
+      keep_branch();
+      const int first = lo - k0 - 4 * h, last = hi - k0 - 4 * h;
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int i = 0; i < E::REGS; ++i) {
-          const int key = k0 + W * n + (i & 3) + 8 * (i >> 2) + 4 * h;
-          if (key < lo || key >= hi) z[n][i] = -INFINITY;
+          const int key = W * n + (i & 3) + 8 * (i >> 2);
+          if (key < first || key >= last) z[n][i] = -INFINITY;
         }
     }
     float top = m;
@@ -241,28 +245,46 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
 #pragma unroll
       for (int i = 0; i < E::REGS; ++i) top = fmaxf(top, z[n][i]);
     top = parts_max<W>(top);
-    // The maximum is taken off before the scaling: products of the type's lowest value stay finite that way.
-    const float off = top == -INFINITY ? 0.0f : top;  // nothing seen yet: exp2(-inf) = 0, not NaN
-    if (__any(top > m)) {
-      const float fade = __builtin_amdgcn_exp2f((m - off) * a.scale2);
+    // A row's reference m follows its maximum only when that has run 2^8 ahead: the sums and products of p <= 2^8 are as
+    // exact as those of p <= 1, and most tiles then leave the 32 x dim accumulators alone.
+    if (__any((top - m) * a.scale2 > 8.0f)) {
+      keep_branch();
+      const float fade = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - top) * a.scale2);
       l *= fade;
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
         for (int i = 0; i < E::REGS; ++i) acc[dt][i] *= fade;
+      m = top;
     }
-    m = top;
+    const float off = m == -INFINITY ? 0.0f : m;  // nothing seen yet: exp2(-inf) = 0, not NaN
+    // f32 takes the reference off before the scaling (all of z - m's bits; products of the type's lowest value stay finite); for
+    // the 16-bit types one fused operation does, where the scaling cannot overflow, and what rounding m scale2 leaves over goes
+    // into the row's logarithm at the end.
+    if (!F32 && a.scale2 <= 1.0f) {
+      const float off2 = off * a.scale2;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < E::REGS; ++i) z[n][i] = __builtin_fmaf(z[n][i], a.scale2, -off2);
+    } else {
+      keep_branch();
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < E::REGS; ++i) z[n][i] = (z[n][i] - off) * a.scale2;
+    }
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
 #pragma unroll
       for (int i = 0; i < E::REGS; ++i) {
-        z[n][i] = __builtin_amdgcn_exp2f((z[n][i] - off) * a.scale2);
+        z[n][i] = __builtin_amdgcn_exp2f(z[n][i]);
         l += z[n][i];
       }
       TsgAccB<D> p;
       p.set(z[n]);
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt) p.template mma<CH>(vt, W * n, W * dt, acc[dt], lane);
+      for (int dt = 0; dt < ND; ++dt) p.template mma<CH>(col, dt, TILE + W * n * CH * 16, acc[dt]);
     }
   }
   l = parts_sum<W>(l);
@@ -270,7 +292,8 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
     store_rows<D, ND>(acc, a.out + (long)t * a.o_row + head * a.o_head, by, a.dim, h);
     if (!F32 && a.rest) store_rows<D, ND, true>(acc, a.rest + ((long)t * a.heads + head) * a.dim * E::BYTES, by, a.dim, h);
-    if (h == 0) a.stat[(long)head * a.n_q + t] = l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l));
+    const float left = !F32 && a.scale2 <= 1.0f ? __builtin_fmaf(m, a.scale2, -(m * a.scale2)) : 0.0f;
+    if (h == 0) a.stat[(long)head * a.n_q + t] = l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l) - left);
   }
 }
 
@@ -281,9 +304,10 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   typedef typename E::Acc Acc;
   constexpr bool F32 = E::BYTES == 4;
   constexpr int W = E::W, PARTS = 64 / W, CH = DP / E::EPC, NF = CH / PARTS, ND = DP / W, NB = BK / W, TILE = BK * CH * 16;
-  __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
   __shared__ int edge[8];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane / W;
+  const unsigned row0 = tsg_lds_addr(lds) + TsgLane<D, CH>::row(lane), col0 = tsg_lds_addr(lds) + TsgLane<D, CH>::col(lane);
   const int tiles = gridDim.x / a.heads;
   const int tile = tiles - 1 - (int)(blockIdx.x / a.heads), head = blockIdx.x % a.heads;
   const int kvh = head / a.group;
@@ -331,8 +355,7 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
     __syncthreads();
     if (k0 + BK < b.hi) fetch(k0 + BK, buf ^ 1);
     if (k0 >= b.wave_hi || k0 + BK <= b.wave_lo) continue;
-    const char* kt = lds + buf * 2 * TILE;
-    const char* vt = kt + TILE;
+    const unsigned row = tsg_opaque(row0) + buf * 2 * TILE, col = tsg_opaque(col0) + buf * 2 * TILE;
     const bool edge_tile = k0 < b.in_lo || k0 + BK > b.in_hi;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -341,20 +364,24 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
       for (int i = 0; i < E::REGS; ++i) z[i] = 0.0f, dp[i] = -delta;  // dp - delta comes out of the product
 #pragma unroll
       for (int s = 0; s < NF; ++s) {
-        tsg_mma<D>(tsg_row_frag<CH, F32>(kt, W * n + lane % W, PARTS * s + h), qf[s], z);
-        tsg_mma<D>(tsg_row_frag<CH, F32>(vt, W * n + lane % W, PARTS * s + h), gf[s], dp);
+        tsg_mma<D>(tsg_row_frag<D>(row, s, W * n * CH * 16), qf[s], z);
+        tsg_mma<D>(tsg_row_frag<D>(row, s, TILE + W * n * CH * 16), gf[s], dp);
       }
 #pragma unroll
-      for (int i = 0; i < E::REGS; ++i) {
-        const int key = k0 + W * n + (i & 3) + 8 * (i >> 2) + 4 * h;
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i] - st.x, a.scale2, -st.y)) * dp[i];
-        if (edge_tile && (key < lo || key >= hi)) p = 0.0f;
-        z[i] = p;
+      for (int i = 0; i < E::REGS; ++i) z[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i] - st.x, a.scale2, -st.y)) * dp[i];
+      if (edge_tile) {
+        keep_branch();
+        const int first = lo - k0 - W * n - 4 * h, last = hi - k0 - W * n - 4 * h;
+#pragma unroll
+        for (int i = 0; i < E::REGS; ++i) {
+          const int key = (i & 3) + 8 * (i >> 2);
+          if (key < first || key >= last) z[i] = 0.0f;
+        }
       }
       TsgAccB<D> ds;
       ds.set(z);
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt) ds.template mma<CH>(kt, W * n, W * dt, acc[dt], lane);
+      for (int dt = 0; dt < ND; ++dt) ds.template mma<CH>(col, dt, W * n * CH * 16, acc[dt]);
     }
   }
   if (t < a.n_q) store_rows<D, ND>(acc, a.dq + (long)t * a.dq_row + head * a.dq_head, a.scale, a.dim, h);
@@ -362,24 +389,31 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
 
 // ------------------------------------------------------------------------------------------ backward, tiles: dk and dv
 // PART 0: both; 1: dv only; 2: dk only (16-bit types at 256 wide: keys, values and both sums do not fit the registers at once)
-template <typename D, int DP, int BQ, int PART>
+// VL: the values' fragments are read from LDS in every step instead of held in registers, which then suffice without spills
+// (16-bit types 128 wide at two waves a SIMD, 256 wide at one; f32 256 wide).
+template <typename D, int DP, int BQ, int PART, bool VL>
 __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
   typedef TsgElem<D> E;
   typedef typename E::Acc Acc;
   constexpr bool F32 = E::BYTES == 4;
   constexpr int W = E::W, PARTS = 64 / W, CH = DP / E::EPC, NF = CH / PARTS, ND = DP / W, NB = BQ / W, TILE = BQ * CH * 16;
-  __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + (VL ? 4 * W * CH * 16 : 0)];
   __shared__ __attribute__((aligned(16))) float stat[2][3][BQ];  // maximum, log2 of the sum, delta
   __shared__ int edge[8];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane / W;
+  const unsigned row0 = tsg_lds_addr(lds) + TsgLane<D, CH>::row(lane), col0 = tsg_lds_addr(lds) + TsgLane<D, CH>::col(lane);
   const int tile = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads;  // early keys are seen by most rows: first
   const int j = tile * (4 * W) + wave * W + lane % W;
   int lo, hi;
   rows_of_key(a, j, lo, hi);
   const Bounds b = bounds_of<W>(lo, hi, wave, edge);
-  tsg_u4 kf[NF], vf[PART == 1 ? 1 : NF];
+  tsg_u4 kf[NF], vf[PART == 1 || VL ? 1 : NF];
   load_frags<PARTS>(kf, a.k + (long)j * a.k_row + kvh * a.k_head, j < a.n_k, a.chunks, h);
-  if constexpr (PART != 1) load_frags<PARTS>(vf, a.v + (long)j * a.v_row + kvh * a.v_head, j < a.n_k, a.chunks, h);
+  if constexpr (PART != 1 && VL) {
+    // the wave's own rows: no other wave reads them, and the first step waits for them
+    tsg_load_tile<W, CH, 1, false, F32>(lds + 4 * TILE + wave * W * CH * 16, a.v + (long)(tile * (4 * W) + wave * W) * a.v_row + kvh * a.v_head,
+                                        a.v_row, a.n_k - (tile * (4 * W) + wave * W), a.chunks, 0, lane);
+  } else if constexpr (PART != 1) load_frags<PARTS>(vf, a.v + (long)j * a.v_row + kvh * a.v_head, j < a.n_k, a.chunks, h);
   Acc dk[PART == 1 ? 1 : ND], dv[PART == 2 ? 1 : ND];
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
@@ -410,63 +444,74 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
     fetch(0, 0);
     stat_of(0, st, delta);
     stat_to(0, st, delta);
+    if (steps > 1) stat_of(1, st, delta);  // held until the next step's buffer is free
   }
   for (int step = 0, buf = 0; step < steps; ++step, buf ^= 1) {
     tsg_dma_wait();
     __syncthreads();
-    const bool more = step + 1 < steps;
-    if (more) {
-      stat_of(step + 1, st, delta);
+    if (step + 1 < steps) {
+      stat_to(buf ^ 1, st, delta);
       fetch(step + 1, buf ^ 1);
+      if (step + 2 < steps) stat_of(step + 2, st, delta);
     }
     const int t0 = b.lo + (step % per) * BQ;
-    if (t0 < b.wave_hi && t0 + BQ > b.wave_lo) {
-      const char* qt = lds + buf * 2 * TILE;
-      const char* gt = qt + TILE;
-      const bool edge_tile = t0 < b.in_lo || t0 + BQ > b.in_hi;
+    if (t0 >= b.wave_hi || t0 + BQ <= b.wave_lo) continue;
+    const unsigned row = tsg_opaque(row0) + buf * 2 * TILE, col = tsg_opaque(col0) + buf * 2 * TILE;
+    const unsigned vrow = tsg_opaque(row0) + 4 * TILE + wave * W * CH * 16;
+    const bool edge_tile = t0 < b.in_lo || t0 + BQ > b.in_hi;
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        Acc z, dp;
+    for (int n = 0; n < NB; ++n) {
+      Acc z, dp;
 #pragma unroll
-        for (int g = 0; g < E::REGS / 4; ++g) {
-          const float4 dl = *reinterpret_cast<const float4*>(&stat[buf][2][W * n + 8 * g + 4 * h]);
-          z[4 * g] = z[4 * g + 1] = z[4 * g + 2] = z[4 * g + 3] = 0.0f;
-          dp[4 * g] = -dl.x, dp[4 * g + 1] = -dl.y, dp[4 * g + 2] = -dl.z, dp[4 * g + 3] = -dl.w;
-        }
-#pragma unroll
-        for (int s = 0; s < NF; ++s) {
-          tsg_mma<D>(tsg_row_frag<CH, F32>(qt, W * n + lane % W, PARTS * s + h), kf[s], z);
-          if constexpr (PART != 1) tsg_mma<D>(tsg_row_frag<CH, F32>(gt, W * n + lane % W, PARTS * s + h), vf[s], dp);
-        }
-#pragma unroll
-        for (int g = 0; g < E::REGS / 4; ++g) {
-          const float4 ms = *reinterpret_cast<const float4*>(&stat[buf][0][W * n + 8 * g + 4 * h]);
-          const float4 ls = *reinterpret_cast<const float4*>(&stat[buf][1][W * n + 8 * g + 4 * h]);
-          const float mv[4] = {ms.x, ms.y, ms.z, ms.w}, lv[4] = {ls.x, ls.y, ls.z, ls.w};
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int t = t0 + W * n + 8 * g + 4 * h + r;
-            const bool out = edge_tile && (t < lo || t >= hi);
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[4 * g + r] - mv[r], a.scale2, -lv[r]));
-            z[4 * g + r] = out ? 0.0f : p;
-            if constexpr (PART != 1) dp[4 * g + r] = out ? 0.0f : p * dp[4 * g + r];
-          }
-        }
-        if constexpr (PART != 2) {
-          TsgAccB<D> pb;
-          pb.set(z);
-#pragma unroll
-          for (int dt = 0; dt < ND; ++dt) pb.template mma<CH>(gt, W * n, W * dt, dv[dt], lane);
-        }
+      for (int g = 0; g < E::REGS / 4; ++g) {
+        z[4 * g] = z[4 * g + 1] = z[4 * g + 2] = z[4 * g + 3] = 0.0f;
         if constexpr (PART != 1) {
-          TsgAccB<D> sb;
-          sb.set(dp);
-#pragma unroll
-          for (int dt = 0; dt < ND; ++dt) sb.template mma<CH>(qt, W * n, W * dt, dk[dt], lane);
+          const float4 dl = *reinterpret_cast<const float4*>(&stat[buf][2][W * n + 8 * g + 4 * h]);
+          dp[4 * g] = -dl.x, dp[4 * g + 1] = -dl.y, dp[4 * g + 2] = -dl.z, dp[4 * g + 3] = -dl.w;  // dp - delta comes out of the product
         }
       }
+#pragma unroll
+      for (int s = 0; s < NF; ++s) {
+        tsg_mma<D>(tsg_row_frag<D>(row, s, W * n * CH * 16), kf[s], z);
+        if constexpr (PART != 1)
+          tsg_mma<D>(tsg_row_frag<D>(row, s, TILE + W * n * CH * 16),
+                     VL ? tsg_row_frag<D>(vrow, s, 0) : vf[VL ? 0 : s], dp);
+      }
+#pragma unroll
+      for (int g = 0; g < E::REGS / 4; ++g) {
+        const float4 ms = *reinterpret_cast<const float4*>(&stat[buf][0][W * n + 8 * g + 4 * h]);
+        const float4 ls = *reinterpret_cast<const float4*>(&stat[buf][1][W * n + 8 * g + 4 * h]);
+        const float mv[4] = {ms.x, ms.y, ms.z, ms.w}, lv[4] = {ls.x, ls.y, ls.z, ls.w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z[4 * g + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[4 * g + r] - mv[r], a.scale2, -lv[r]));
+      }
+      if (edge_tile) {
+        keep_branch();
+        const int first = lo - t0 - W * n - 4 * h, last = hi - t0 - W * n - 4 * h;
+#pragma unroll
+        for (int i = 0; i < E::REGS; ++i) {
+          const int t = (i & 3) + 8 * (i >> 2);
+          if (t < first || t >= last) {
+            z[i] = 0.0f;
+            if constexpr (PART != 1) dp[i] = 0.0f;
+          }
+        }
+      }
+      if constexpr (PART != 2) {
+        TsgAccB<D> pb;
+        pb.set(z);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) pb.template mma<CH>(col, dt, TILE + W * n * CH * 16, dv[dt]);
+      }
+      if constexpr (PART != 1) {
+#pragma unroll
+        for (int i = 0; i < E::REGS; ++i) dp[i] *= z[i];
+        TsgAccB<D> sb;
+        sb.set(dp);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) sb.template mma<CH>(col, dt, W * n * CH * 16, dk[dt]);
+      }
     }
-    if (more) stat_to(buf ^ 1, st, delta);
   }
   if (j < a.n_k) {
     if constexpr (PART != 1) store_rows<D, ND>(dk, a.dk + (long)j * a.dk_row + kvh * a.dk_head, a.scale, a.dim, h);
@@ -871,12 +916,12 @@ template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
     else hipLaunchKernelGGL((attn_dq_kernel<D, 256, 32>), gq, block, 0, s, a);
   }
   if (a.n_k) {
-    if (a.dim <= 64) hipLaunchKernelGGL((attn_dkv_kernel<D, 64, 32, 0>), gk, block, 0, s, a);
-    else if (a.dim <= 128) hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0>), gk, block, 0, s, a);
-    else if constexpr (F32) hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 0>), gk, block, 0, s, a);
+    if (a.dim <= 64) hipLaunchKernelGGL((attn_dkv_kernel<D, 64, 32, 0, false>), gk, block, 0, s, a);
+    else if (a.dim <= 128) hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0, !F32>), gk, block, 0, s, a);
+    else if constexpr (F32) hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 16, 0, true>), gk, block, 0, s, a);
     else {
-      hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 1>), gk, block, 0, s, a);
-      hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 2>), gk, block, 0, s, a);
+      hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 1, false>), gk, block, 0, s, a);
+      hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 2, true>), gk, block, 0, s, a);
     }
   }
   TSG_LAUNCH_CHECK();

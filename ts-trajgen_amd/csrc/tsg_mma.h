@@ -75,40 +75,56 @@ template <int CH, bool F32 = false> __device__ __forceinline__ int tsg_swz(int r
 typedef __attribute__((address_space(3))) char tsg_lds_char;
 __device__ __forceinline__ unsigned tsg_lds_addr(const void* p) { return (unsigned)(uintptr_t)(tsg_lds_char*)p; }
 
-template <int CH, bool F32 = false> __device__ __forceinline__ tsg_u4 tsg_row_frag(const char* tile, int row, int chunk) {
-  return *reinterpret_cast<const tsg_u4*>(tile + ((size_t)row * CH + (chunk ^ tsg_swz<CH, F32>(row))) * 16);
+// Where a lane's fragments lie, as LDS byte addresses.  A row takes CH * 16 bytes, a power of two, and tiles start at
+// multiples of that, so the swizzle is an exclusive-or on the address: a fragment's address is the lane's own start, `^` a
+// constant of the k step or column block, plus an offset the load instruction carries.  tsg_opaque() inside a loop keeps the
+// compiler from holding every such address in a register of its own (which costs more than the one operation).
+__device__ __forceinline__ unsigned tsg_opaque(unsigned v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+template <typename D, int CH> struct TsgLane {
+  static constexpr bool F32 = TsgElem<D>::BYTES == 4;
+  static constexpr int W = TsgElem<D>::W, PARTS = 64 / W, ROW = CH * 16;
+  // first row fragment of row l % W of the tile
+  static __device__ __forceinline__ unsigned row(int lane) {
+    const int r = lane % W, h = lane / W;
+    return r * ROW + ((h ^ tsg_swz<CH, F32>(r)) << 4);
+  }
+  // first column fragment of the W rows from the tile's start, numbered as an accumulator's registers number them
+  static __device__ __forceinline__ unsigned col(int lane) {
+    if (F32) return 4 * (lane >> 4) * ROW + (((((lane & 15) >> 2) ^ tsg_swz<CH, true>(4 * (lane >> 4))) << 4) | ((lane & 3) << 2));
+    const int i = lane & 15, r = 4 * (lane >> 5) + (i >> 2);  // ds_read_b64_tr_b16: 16 lanes hand in 4 rows x 16 columns
+    return r * ROW + (((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ tsg_swz<CH>(r)) << 4) + 8 * (i & 1);
+  }
+  // the same with k = 8 (l / 32) + 0..7 (16-bit types): the order that a row fragment has
+  static __device__ __forceinline__ unsigned col_in_order(int lane) {
+    const int i = lane & 15, r = 8 * (lane >> 5) + (i >> 2);
+    return r * ROW + (((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ tsg_swz<CH>(r)) << 4) + 8 * (i & 1);
+  }
+};
+typedef __attribute__((address_space(3))) const tsg_u4 tsg_lds_u4;
+typedef __attribute__((address_space(3))) const float tsg_lds_f32;
+typedef __attribute__((address_space(3))) tsg_s4 tsg_lds_s4;
+// row fragment of k step s; offset: of the tile and the row block
+template <typename D> __device__ __forceinline__ tsg_u4 tsg_row_frag(unsigned row, int s, int offset) {
+  return *reinterpret_cast<tsg_lds_u4*>((uintptr_t)((row ^ (s * (64 / TsgElem<D>::W) * 16)) + offset));
+}
+__device__ __forceinline__ tsg_u4 tsg_join4(tsg_s4 x, tsg_s4 y) {
+  typedef short s8 __attribute__((ext_vector_type(8)));
+  const s8 a = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_bit_cast(tsg_u4, a);
+}
+// 16 rows x 32 columns from row fragment order (TsgLane::col_in_order); block: 32-column block
+template <int CH> __device__ __forceinline__ tsg_u4 tsg_col_frag(unsigned col, int block, int offset) {
+  const unsigned at = col ^ (block * 64);
+  const tsg_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tsg_lds_s4*>((uintptr_t)(at + offset)));
+  const tsg_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tsg_lds_s4*>((uintptr_t)((at ^ 16) + offset + 4 * CH * 16)));
+  return tsg_join4(x, y);
 }
 
-// acc[m][n] += sum over the 32 rows row0.. of tile: tile[row][col0 + m] * p(row, n), p in accumulator layout
-template <typename D, int CH>
-__device__ __forceinline__ void tsg_mma_cols(const char* tile, int row0, int col0, const tsg_u4 (&p)[2], tsg_f32x16& acc, int lane) {
-  const int h = lane >> 5, i = lane & 15, part = (lane >> 4) & 1;
-  const int col = col0 + 16 * part + 4 * (i & 3);  // ds_read_b64_tr_b16: 16 lanes hand in 4 rows x 16 columns
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    tsg_s4 v[2];
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const int row = row0 + 16 * t + 8 * g + 4 * h + (i >> 2);
-      const char* at = tile + ((size_t)row * CH + ((col >> 3) ^ tsg_swz<CH>(row))) * 16 + (col & 7) * 2;
-      v[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tsg_s4*)at);
-    }
-    typedef short s8 __attribute__((ext_vector_type(8)));
-    const s8 a = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
-    tsg_mma<D>(__builtin_bit_cast(tsg_u4, a), p[t], acc);
-  }
-}
-template <int CH>
-__device__ __forceinline__ void tsg_mma_cols_f32(const char* tile, int row0, int col0, const tsg_f4& p, tsg_f4& acc, int lane) {
-  const int col = col0 + (lane & 15);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = row0 + 4 * (lane >> 4) + i;
-    const float a = *reinterpret_cast<const float*>(tile + ((size_t)row * CH + ((col >> 2) ^ tsg_swz<CH, true>(row))) * 16 + (col & 3) * 4);
-    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a, p[i], acc, 0, 0, 0);
-  }
-}
-// the accumulator as the B operand: rounded to the operand type (nearest even)
+// acc[m][n] += sum over W rows of a tile: tile[row][W block + m] * p(row, n), p in accumulator layout, rounded to the
+// operand type (nearest even)
 template <typename D> struct TsgAccB {
   tsg_u4 v[2];
   __device__ __forceinline__ void set(const tsg_f32x16& p) {
@@ -117,17 +133,25 @@ template <typename D> struct TsgAccB {
 #pragma unroll
       for (int w = 0; w < 4; ++w) v[t][w] = tsg_pack2<D>(p[8 * t + 2 * w], p[8 * t + 2 * w + 1]);
   }
-  template <int CH>
-  __device__ __forceinline__ void mma(const char* tile, int row0, int col0, tsg_f32x16& acc, int lane) const {
-    tsg_mma_cols<D, CH>(tile, row0, col0, v, acc, lane);
+  template <int CH> __device__ __forceinline__ void mma(unsigned col, int block, int offset, tsg_f32x16& acc) const {
+    const unsigned at = col ^ (block * 64);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const tsg_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tsg_lds_s4*>((uintptr_t)(at + offset + 16 * t * CH * 16)));
+      const tsg_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tsg_lds_s4*>((uintptr_t)((at ^ 32) + offset + (16 * t + 8) * CH * 16)));
+      tsg_mma<D>(tsg_join4(x, y), v[t], acc);
+    }
   }
 };
 template <> struct TsgAccB<TsgF32> {
   tsg_f4 v;
   __device__ __forceinline__ void set(const tsg_f4& p) { v = p; }
-  template <int CH>
-  __device__ __forceinline__ void mma(const char* tile, int row0, int col0, tsg_f4& acc, int lane) const {
-    tsg_mma_cols_f32<CH>(tile, row0, col0, v, acc, lane);
+  template <int CH> __device__ __forceinline__ void mma(unsigned col, int block, int offset, tsg_f4& acc) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = *reinterpret_cast<tsg_lds_f32*>((uintptr_t)((col ^ (block * 64) ^ (i * 16)) + offset + i * CH * 16));
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a, v[i], acc, 0, 0, 0);
+    }
   }
 };
 

@@ -64,21 +64,6 @@ struct XentArgs {
   long dw_row;
 };
 
-// natural order: lane half h holds k = 16 s + 8 h + 0..7 of column col0 + (lane & 31), from a tile whose rows are k
-template <int CH> __device__ __forceinline__ tsg_u4 col_frag(const char* tile, int k0, int col0, int lane) {
-  const int h = lane >> 5, i = lane & 15, col = col0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
-  tsg_s4 v[2];
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const int row = k0 + 8 * h + 4 * g + (i >> 2);
-    const char* at = tile + ((size_t)row * CH + ((col >> 3) ^ tsg_swz<CH>(row))) * 16 + (col & 7) * 2;
-    v[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tsg_s4*)at);
-  }
-  typedef short s8 __attribute__((ext_vector_type(8)));
-  const s8 a = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
-  return __builtin_bit_cast(tsg_u4, a);
-}
-
 struct Operand {
   const char* p;   // element (0, 0) of the workgroup's stretch
   long row, plane;
@@ -92,7 +77,10 @@ template <typename D, bool AC, bool BC, bool MASKED = false>
 __device__ __forceinline__ void product(tsg_f32x16 (&acc)[2][2], char* lds, const Operand& a, const Operand& b, int K, int passes, int wave, int lane) {
   constexpr int TILE = TM * TK * 2;
   const int per = (K + TK - 1) / TK, steps = per * passes;
-  const int h = lane >> 5, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  // a wave's 64 rows or columns: rows lie 128 bytes apart, columns 2
+  const unsigned a0 = tsg_lds_addr(lds) + (AC ? TsgLane<D, TM / 8>::col_in_order(lane) ^ (wm * 2) : TsgLane<D, TK / 8>::row(lane) + wm * TK * 2);
+  const unsigned b0 = tsg_lds_addr(lds) + TILE + (BC ? TsgLane<D, TN / 8>::col_in_order(lane) ^ (wn * 2) : TsgLane<D, TK / 8>::row(lane) + wn * TK * 2);
   auto fetch = [&](int step, int buf) {
     const int pass = step / per, k0 = (step % per) * TK;
     char* at = lds + buf * 2 * TILE;
@@ -110,15 +98,14 @@ __device__ __forceinline__ void product(tsg_f32x16 (&acc)[2][2], char* lds, cons
     tsg_dma_wait();
     __syncthreads();
     if (step + 1 < steps) fetch(step + 1, buf ^ 1);
-    const char* at = lds + buf * 2 * TILE;
-    const char* bt = at + TILE;
+    const unsigned at = tsg_opaque(a0) + buf * 2 * TILE, bt = tsg_opaque(b0) + buf * 2 * TILE;
 #pragma unroll
     for (int s = 0; s < TK / 16; ++s) {
       tsg_u4 fa[2], fb[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        fa[x] = AC ? col_frag<TM / 8>(at, 16 * s, wm + 32 * x, lane) : tsg_row_frag<TK / 8>(at, wm + 32 * x + (lane & 31), 2 * s + h);
-        fb[x] = BC ? col_frag<TN / 8>(bt, 16 * s, wn + 32 * x, lane) : tsg_row_frag<TK / 8>(bt, wn + 32 * x + (lane & 31), 2 * s + h);
+        fa[x] = AC ? tsg_col_frag<TM / 8>(at, x, 16 * s * TM * 2) : tsg_row_frag<D>(at, s, 32 * x * TK * 2);
+        fb[x] = BC ? tsg_col_frag<TN / 8>(bt, x, 16 * s * TN * 2) : tsg_row_frag<D>(bt, s, 32 * x * TK * 2);
       }
 #pragma unroll
       for (int x = 0; x < 2; ++x)
@@ -171,7 +158,7 @@ template <typename D> __device__ __forceinline__ void logits(const XentArgs& a, 
 
 template <typename D>
 __global__ __launch_bounds__(256, 2) void xent_stat_kernel(XentArgs a, int tiles_m, int tiles_n) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * TM * TK * 2];
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TM * TK * 2];
   __shared__ float2 join[2][TN];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
   int tm, tn;
@@ -293,7 +280,7 @@ __global__ __launch_bounds__(1024) void xent_grad_kernel(XentArgs a, const float
 
 template <typename D>
 __global__ __launch_bounds__(256, 2) void xent_dz_kernel(XentArgs a, int tiles_m, int tiles_n) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * TM * TK * 2 + 2 * 16 * TM];
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TM * TK * 2 + 2 * 16 * TM];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
   int tm, tn;
   tile_of(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
@@ -378,7 +365,7 @@ __global__ __launch_bounds__(256, 2) void xent_dz_kernel(XentArgs a, int tiles_m
 // dW of the piece: rows v, columns k', summed over the states
 template <typename D, typename OUT>
 __global__ __launch_bounds__(256, 2) void xent_dw_kernel(XentArgs a, int tiles_m, int tiles_n) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * TM * TK * 2];
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TM * TK * 2];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
   int tm, tn;
   tile_of(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
@@ -405,7 +392,7 @@ __global__ __launch_bounds__(256, 2) void xent_dw_kernel(XentArgs a, int tiles_m
 // dh: rows t, columns k', summed over a stretch of the piece; the stretches' sums are added up over the pieces
 template <typename D>
 __global__ __launch_bounds__(256, 2) void xent_dh_kernel(XentArgs a, int tiles_m, int tiles_n) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * TM * TK * 2];
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TM * TK * 2];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
   const int split_id = blockIdx.x / (tiles_m * tiles_n);
   int tm, tn;
