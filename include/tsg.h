@@ -537,7 +537,7 @@ int tsg_dropout(const tsg_dropout_desc* d, void* stream);
  * Query head h reads key-value head h / (heads / kv_heads).  Rows that see no key, rows behind the last sequence
  * and keys that nothing sees give zeros.  Pointer values outside the arrays are clamped to them, never followed.
  * Strides are in elements, >= 0; the width runs contiguously.  Base addresses are 16-byte aligned, strides and dim
- * multiples of 8 (16-bit types) or 4 (f32).  dim <= 512; n_q * heads and n_k * kv_heads below 2^31.
+ * multiples of 8 (16-bit types) or 4 (f32), row strides below 2^24 bytes.  dim <= 512; n_q * heads and n_k * kv_heads below 2^31.
  * stats [heads][n_q][2] f32 is written by the forward (a row's largest q.k, and the base-2 logarithm of the sum of
  * exp(scale (q.k - largest)); 0 and +inf where a row sees nothing) and read, with out, by the backward, which writes
  * delta [heads][n_q].
@@ -572,7 +572,7 @@ int tsg_attn_backward(const tsg_attn_desc* d, void* stream);
  * other target outside [0, n_vocab) makes the row's loss and gradients NaN.  bias (may be NULL) and the gradients
  * have the type of h and w.  The backward takes d_loss (one number, or one per row for reduction 0) and the stats that
  * the forward left, takes the vocabulary in pieces and writes dh, dw and dbias whole.
- * Base addresses of h and w are 16-byte aligned, rows a multiple of 16 bytes apart, hidden a multiple of 8 (pad with
+ * Base addresses of h and w are 16-byte aligned, rows a multiple of 16 and less than 2^23 bytes apart, hidden a multiple of 8 (pad with
  * zeros), the workspace 256-byte aligned; tsg_xent_workspace says how much.  n_rows >= 1. */
 typedef struct tsg_xent_desc {
   int32_t dtype, hidden, reduction, reserved;

@@ -105,13 +105,17 @@ template <int W> __device__ __forceinline__ Bounds bounds_of(int lo, int hi, int
   return b;
 }
 
+__device__ __forceinline__ tsg_u4 chunk_of(const char* row, int c, bool ok) {
+  tsg_u4 v = {0u, 0u, 0u, 0u};
+  if (ok) v = *reinterpret_cast<const tsg_u4*>(row + c * 16);
+  return v;
+}
 // operand fragments of one row per lane, straight from memory; zeros outside
 template <int PARTS, int NF> __device__ __forceinline__ void load_frags(tsg_u4 (&f)[NF], const char* row, bool ok, int chunks, int h) {
 #pragma unroll
   for (int s = 0; s < NF; ++s) {
     const int c = PARTS * s + h;
-    const char* g = ok && c < chunks ? row + c * 16 : reinterpret_cast<const char*>(&tsg_zero_chunk);
-    f[s] = *reinterpret_cast<const tsg_u4*>(g);
+    f[s] = chunk_of(row, c, ok && c < chunks);
   }
 }
 
@@ -209,10 +213,14 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   float m = -INFINITY, l = 0.0f;
   const char* kbase = a.k + kvh * a.k_head;
   const char* vbase = a.v + kvh * a.v_head;
+  TsgLoader<BK, CH, 4, F32> kl, vl;
+  kl.init(a.k_row, a.chunks, tsg_lds_addr(lds), wave, lane);
+  vl.init(a.v_row, a.chunks, tsg_lds_addr(lds) + TILE, wave, lane);
   auto fetch = [&](int k0, int buf) {
-    tsg_load_tile<BK, CH, 4, false, F32>(lds + buf * 2 * TILE, kbase + (long)k0 * a.k_row, a.k_row, b.hi - k0, a.chunks, wave, lane);
-    tsg_load_tile<BK, CH, 4, false, F32>(lds + buf * 2 * TILE + TILE, vbase + (long)k0 * a.v_row, a.v_row, b.hi - k0, a.chunks, wave, lane);
+    kl.load(kbase + (long)k0 * a.k_row, b.hi - k0, a.chunks * 16, buf * 2 * TILE);
+    vl.load(vbase + (long)k0 * a.v_row, b.hi - k0, a.chunks * 16, buf * 2 * TILE);
   };
+  tsg_settle(qf);
   if (b.lo < b.hi) fetch(b.lo, 0);
   for (int k0 = b.lo, buf = 0; k0 < b.hi; k0 += BK, buf ^= 1) {
     tsg_dma_wait();
@@ -325,12 +333,9 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
 #pragma unroll
     for (int s = 0; s < NF; ++s) {
       const int c = PARTS * s + h;
-      const char* g = t < a.n_q && c < a.chunks ? orow + c * 16 : reinterpret_cast<const char*>(&tsg_zero_chunk);
-      delta += frag_dot<D>(*reinterpret_cast<const tsg_u4*>(g), gf[s]);
-      if (!F32 && a.rest) {
-        g = t < a.n_q && c < a.chunks ? a.rest + (((long)t * a.heads + head) * a.dim) * E::BYTES + c * 16 : reinterpret_cast<const char*>(&tsg_zero_chunk);
-        delta += frag_dot<D>(*reinterpret_cast<const tsg_u4*>(g), gf[s]);
-      }
+      const bool ok = t < a.n_q && c < a.chunks;
+      delta += frag_dot<D>(chunk_of(orow, c, ok), gf[s]);
+      if (!F32 && a.rest) delta += frag_dot<D>(chunk_of(a.rest + ((long)t * a.heads + head) * a.dim * E::BYTES, c, ok), gf[s]);
     }
     delta = parts_sum<W>(delta);
     if (t < a.n_q) {
@@ -345,10 +350,16 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
     for (int i = 0; i < E::REGS; ++i) acc[dt][i] = 0.0f;
   const char* kbase = a.k + kvh * a.k_head;
   const char* vbase = a.v + kvh * a.v_head;
+  TsgLoader<BK, CH, 4, F32> kl, vl;
+  kl.init(a.k_row, a.chunks, tsg_lds_addr(lds), wave, lane);
+  vl.init(a.v_row, a.chunks, tsg_lds_addr(lds) + TILE, wave, lane);
   auto fetch = [&](int k0, int buf) {
-    tsg_load_tile<BK, CH, 4, false, F32>(lds + buf * 2 * TILE, kbase + (long)k0 * a.k_row, a.k_row, b.hi - k0, a.chunks, wave, lane);
-    tsg_load_tile<BK, CH, 4, false, F32>(lds + buf * 2 * TILE + TILE, vbase + (long)k0 * a.v_row, a.v_row, b.hi - k0, a.chunks, wave, lane);
+    kl.load(kbase + (long)k0 * a.k_row, b.hi - k0, a.chunks * 16, buf * 2 * TILE);
+    vl.load(vbase + (long)k0 * a.v_row, b.hi - k0, a.chunks * 16, buf * 2 * TILE);
   };
+  tsg_settle(qf);
+  tsg_settle(gf);
+  asm volatile("" : "+v"(st.x), "+v"(st.y), "+v"(delta));
   if (b.lo < b.hi) fetch(b.lo, 0);
   for (int k0 = b.lo, buf = 0; k0 < b.hi; k0 += BK, buf ^= 1) {
     tsg_dma_wait();
@@ -411,8 +422,10 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   load_frags<PARTS>(kf, a.k + (long)j * a.k_row + kvh * a.k_head, j < a.n_k, a.chunks, h);
   if constexpr (PART != 1 && VL) {
     // the wave's own rows: no other wave reads them, and the first step waits for them
-    tsg_load_tile<W, CH, 1, false, F32>(lds + 4 * TILE + wave * W * CH * 16, a.v + (long)(tile * (4 * W) + wave * W) * a.v_row + kvh * a.v_head,
-                                        a.v_row, a.n_k - (tile * (4 * W) + wave * W), a.chunks, 0, lane);
+    TsgLoader<W, CH, 1, F32> vl;
+    vl.init(a.v_row, a.chunks, tsg_lds_addr(lds) + 4 * TILE + wave * W * CH * 16, 0, lane);
+    const int j0 = tile * (4 * W) + wave * W;
+    vl.load(a.v + (long)j0 * a.v_row + kvh * a.v_head, a.n_k - j0, a.chunks * 16, 0);
   } else if constexpr (PART != 1) load_frags<PARTS>(vf, a.v + (long)j * a.v_row + kvh * a.v_head, j < a.n_k, a.chunks, h);
   Acc dk[PART == 1 ? 1 : ND], dv[PART == 2 ? 1 : ND];
 #pragma unroll
@@ -423,38 +436,51 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
       if constexpr (PART != 2) dv[dt][i] = 0.0f;
     }
   // the walk: for every head of the group the row tiles [b.lo, b.hi), as one sequence of steps
-  const int per = b.lo < b.hi ? (b.hi - b.lo + BQ - 1) / BQ : 0, steps = per * a.group;
-  auto fetch = [&](int step, int buf) {
-    const int head = kvh * a.group + step / per, t0 = b.lo + (step % per) * BQ;
-    tsg_load_tile<BQ, CH, 4, false, F32>(lds + buf * 2 * TILE, a.q + head * a.q_head + (long)t0 * a.q_row, a.q_row, b.hi - t0, a.chunks, wave, lane);
-    tsg_load_tile<BQ, CH, 4, false, F32>(lds + buf * 2 * TILE + TILE, a.d_o + head * a.do_head + (long)t0 * a.do_row, a.do_row, b.hi - t0, a.chunks,
-                             wave, lane);
+  const int steps = b.lo < b.hi ? (b.hi - b.lo + BQ - 1) / BQ * a.group : 0;
+  struct Step {
+    int head, t0;
   };
-  auto stat_of = [&](int step, float2& st, float& delta) {
-    const int head = kvh * a.group + step / per, t = b.lo + (step % per) * BQ + tid;
+  auto after = [&](Step p) {
+    p.t0 += BQ;
+    if (p.t0 >= b.hi) p.t0 = b.lo, ++p.head;
+    return p;
+  };
+  TsgLoader<BQ, CH, 4, F32> ql, gl;
+  ql.init(a.q_row, a.chunks, tsg_lds_addr(lds), wave, lane);
+  gl.init(a.do_row, a.chunks, tsg_lds_addr(lds) + TILE, wave, lane);
+  auto fetch = [&](Step p, int buf) {
+    ql.load(a.q + p.head * a.q_head + (long)p.t0 * a.q_row, b.hi - p.t0, a.chunks * 16, buf * 2 * TILE);
+    gl.load(a.d_o + p.head * a.do_head + (long)p.t0 * a.do_row, b.hi - p.t0, a.chunks * 16, buf * 2 * TILE);
+  };
+  auto stat_of = [&](Step p, float2& st, float& delta) {
+    const int t = p.t0 + tid;
     st = make_float2(0.0f, INFINITY), delta = 0.0f;
-    if (tid < BQ && t < b.hi) st = a.stat[(long)head * a.n_q + t], delta = a.delta[(long)head * a.n_q + t];
+    if (tid < BQ && t < b.hi) st = a.stat[(long)p.head * a.n_q + t], delta = a.delta[(long)p.head * a.n_q + t];
   };
   auto stat_to = [&](int buf, float2 st, float delta) {
     if (tid < BQ) stat[buf][0][tid] = st.x, stat[buf][1][tid] = st.y, stat[buf][2][tid] = delta;
   };
-  float2 st;
-  float delta;
+  float2 st = make_float2(0.0f, INFINITY);
+  float delta = 0.0f;
+  Step now = {kvh * a.group, b.lo};
+  tsg_settle(kf);
+  if constexpr (PART != 1 && !VL) tsg_settle(vf);
   if (steps) {
-    fetch(0, 0);
-    stat_of(0, st, delta);
+    stat_of(now, st, delta);
     stat_to(0, st, delta);
-    if (steps > 1) stat_of(1, st, delta);  // held until the next step's buffer is free
+    if (steps > 1) stat_of(after(now), st, delta);  // held until the next step's buffer is free
+    fetch(now, 0);
   }
   for (int step = 0, buf = 0; step < steps; ++step, buf ^= 1) {
     tsg_dma_wait();
     __syncthreads();
+    const int t0 = now.t0;
+    now = after(now);
     if (step + 1 < steps) {
       stat_to(buf ^ 1, st, delta);
-      fetch(step + 1, buf ^ 1);
-      if (step + 2 < steps) stat_of(step + 2, st, delta);
+      if (step + 2 < steps) stat_of(after(now), st, delta);  // before the tile's loads: a wait for these does not drain those
+      fetch(now, buf ^ 1);
     }
-    const int t0 = b.lo + (step % per) * BQ;
     if (t0 >= b.wave_hi || t0 + BQ <= b.wave_lo) continue;
     const unsigned row = tsg_opaque(row0) + buf * 2 * TILE, col = tsg_opaque(col0) + buf * 2 * TILE;
     const unsigned vrow = tsg_opaque(row0) + 4 * TILE + wave * W * CH * 16;
@@ -589,11 +615,19 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
       const int jj = min(j + u * GROUPS, j1 - 1);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const int ch = part + c * LPR;
-        const bool in = ch < a.chunks;
-        kr[u][c] = *reinterpret_cast<const tsg_u4*>(in ? kb + (long)jj * a.k_row + ch * 16 : reinterpret_cast<const char*>(&tsg_zero_chunk));
-        vr[u][c] = *reinterpret_cast<const tsg_u4*>(in ? vb + (long)jj * a.v_row + ch * 16 : reinterpret_cast<const char*>(&tsg_zero_chunk));
+        const int ch = min(part + c * LPR, a.chunks - 1);  // lanes behind the width read its last chunk, and drop it below
+        kr[u][c] = *reinterpret_cast<const tsg_u4*>(kb + (long)jj * a.k_row + ch * 16);
+        vr[u][c] = *reinterpret_cast<const tsg_u4*>(vb + (long)jj * a.v_row + ch * 16);
       }
+    }
+    if (a.chunks < LPR * NC) {
+      keep_branch();
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (part + c * LPR >= a.chunks) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) kr[u][c] = vr[u][c] = tsg_u4{0u, 0u, 0u, 0u};
+        }
     }
     float z[G][U];
 #pragma unroll
@@ -840,6 +874,8 @@ int check_attn(const tsg_attn_desc* d, bool backward) {
   for (int i = 0; i < 16; ++i)
     if (s[i] % epc || s[i] < 0) return TSG_E_INVALID;
   if (backward && !d->delta) return TSG_E_INVALID;
+  for (int i = 0; i < 16; i += 2)
+    if (s[i] * bytes >= (1 << 24)) return TSG_E_LIMIT;  // offsets inside a tile of 64 rows are 32-bit
   if ((uintptr_t)d->out_rest % 16) return TSG_E_INVALID;
   return 0;
 }
@@ -917,7 +953,13 @@ template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
   }
   if (a.n_k) {
     if (a.dim <= 64) hipLaunchKernelGGL((attn_dkv_kernel<D, 64, 32, 0, false>), gk, block, 0, s, a);
-    else if (a.dim <= 128) hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0, !F32>), gk, block, 0, s, a);
+    else if (a.dim <= 128) {
+      if constexpr (F32) hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0, false>), gk, block, 0, s, a);
+      else {
+        hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 64, 1, false>), gk, block, 0, s, a);
+        hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 2, false>), gk, block, 0, s, a);
+      }
+    }
     else if constexpr (F32) hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 16, 0, true>), gk, block, 0, s, a);
     else {
       hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 1, false>), gk, block, 0, s, a);

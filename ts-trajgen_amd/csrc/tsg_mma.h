@@ -155,34 +155,103 @@ template <> struct TsgAccB<TsgF32> {
   }
 };
 
-// 16 bytes per lane straight into LDS at lds + 16 * lane (lds wave-uniform).  The compiler does not see these loads:
-// tsg_dma_wait() before the barrier that hands the tile over.
-static __device__ const tsg_u4 tsg_zero_chunk = {0u, 0u, 0u, 0u};  // what chunks outside an operand are read from
-__device__ __forceinline__ void tsg_dma16(const void* g, unsigned lds) {
-  unsigned keep;  // m0 holds the LDS base of such a load; what the compiler has in it is put back
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+// ---- tiles from memory straight into LDS (buffer_load_dwordx4 ... lds: lane l's 16 bytes go to m0 + 16 l).
+// The compiler does not see these loads: tsg_dma_wait() before the barrier that hands the tile over, and no load of its
+// own left in flight across a tile loop (tsg_settle), or its waits would drain these too.
+// A buffer descriptor bounds the operand: what lies behind its last valid byte is written to LDS as zeros.
+__device__ __forceinline__ void tsg_dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int N> __device__ __forceinline__ void tsg_settle(tsg_u4 (&f)[N]) {
+#pragma unroll
+  for (int s = 0; s < N; ++s) asm volatile("" : "+v"(f[s]));
+}
+
+__device__ __forceinline__ tsg_u4 tsg_descriptor(const char* base, unsigned bytes) {
+  const unsigned long long p = reinterpret_cast<unsigned long long>(base);
+  tsg_u4 d;
+  d[0] = __builtin_amdgcn_readfirstlane((unsigned)p);
+  d[1] = __builtin_amdgcn_readfirstlane((unsigned)(p >> 32)) & 0xffffu;
+  d[2] = __builtin_amdgcn_readfirstlane(bytes);
+  d[3] = 0x00020000u;  // raw buffer, no stride
+  return d;
+}
+// m0 holds the LDS address of such a load; what the compiler has in it is put back
+__device__ __forceinline__ void tsg_dma(tsg_u4 d, unsigned off, unsigned lds) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
                : "=&s"(keep)
-               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(g)
+               : "s"(lds), "v"(off), "s"(d)
                : "memory");
 }
-__device__ __forceinline__ void tsg_dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int STEP> __device__ __forceinline__ void tsg_dma2(tsg_u4 d, unsigned o0, unsigned o1, unsigned lds) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %4, 0 offen lds\n\ts_add_u32 m0, m0, %5\n\ts_nop 0\n\t"
+               "buffer_load_dwordx4 %3, %4, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
+               : "s"(lds), "v"(o0), "v"(o1), "s"(d), "n"(STEP)
+               : "memory", "scc");
+}
+template <int STEP> __device__ __forceinline__ void tsg_dma4(tsg_u4 d, unsigned o0, unsigned o1, unsigned o2, unsigned o3, unsigned lds) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %6, 0 offen lds\n\ts_add_u32 m0, m0, %7\n\ts_nop 0\n\t"
+               "buffer_load_dwordx4 %3, %6, 0 offen lds\n\ts_add_u32 m0, m0, %7\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %6, 0 offen lds\n\t"
+               "s_add_u32 m0, m0, %7\n\ts_nop 0\n\tbuffer_load_dwordx4 %5, %6, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
+               : "s"(lds), "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(d), "n"(STEP)
+               : "memory", "scc");
+}
 
-// Tile [ROWS][CH] of a row-major operand: row r of the tile is src + r * stride bytes for r < r1 and zeros from there on,
-// chunks from `chunks` on are zeros.  All WAVES waves take part.
-// MASKED: row r is zeros also where bit r of `used` is clear.
-template <int ROWS, int CH, int WAVES, bool MASKED = false, bool F32 = false>
-__device__ __forceinline__ void tsg_load_tile(char* tile, const char* src, long stride, int r1, int chunks, int wave, int lane,
-                                              unsigned long long used = 0) {
-  constexpr int N = ROWS * CH / 64;  // instructions of 64 chunks
-  static_assert(ROWS * CH % 64 == 0, "whole wave loads");
+// The loads of a [ROWS][CH] tile by WAVES waves: a lane's byte offsets within the operand's rows, kept over the tile loop.
+// ROWS * stride must stay below 2^31 bytes.
+template <int ROWS, int CH, int WAVES, bool F32 = false> struct TsgLoader {
+  static constexpr int N = ROWS * CH / 64 / WAVES, DOWN = 64 * WAVES / CH;  // loads per wave; rows from one to the next
+  static constexpr bool EVEN = DOWN % 16 == 0;  // the swizzle repeats: one offset serves all
+  static_assert(N >= 1 && ROWS * CH % (64 * WAVES) == 0, "whole wave loads");
+  unsigned off[EVEN ? 1 : N], stride, lds;
+  int row;  // of the first load
+  __device__ __forceinline__ void init(long row_bytes, int chunks, unsigned tile, int wave, int lane) {
+    stride = __builtin_amdgcn_readfirstlane((unsigned)row_bytes);
+    lds = __builtin_amdgcn_readfirstlane(tile + wave * 1024);
+    row = (wave * 64 + lane) / CH;
 #pragma unroll
-  for (int n = 0; n < (N + WAVES - 1) / WAVES; ++n) {
-    const int ins = n * WAVES + wave;
-    if (N % WAVES == 0 || ins < N) {
-      const int at = ins * 64 + lane, r = at / CH, c = (at % CH) ^ tsg_swz<CH, F32>(r);
-      const char* g = src + (long)r * stride + c * 16;
-      if (r >= r1 || c >= chunks || (MASKED && !(used >> r & 1))) g = reinterpret_cast<const char*>(&tsg_zero_chunk);
-      tsg_dma16(g, tsg_lds_addr(tile) + ins * 1024);
+    for (int n = 0; n < (EVEN ? 1 : N); ++n) {
+      const int r = row + n * DOWN, c = ((wave * 64 + lane) % CH) ^ tsg_swz<CH, F32>(r);
+      off[n] = c < chunks ? r * stride + c * 16 : 0x80000000u;  // behind every bound
     }
+  }
+  __device__ __forceinline__ unsigned at(int n) const { return EVEN ? off[0] + n * DOWN * stride : off[EVEN ? 0 : n]; }
+  __device__ __forceinline__ unsigned at(int n, unsigned long long used) const { return used >> (row + n * DOWN) & 1 ? at(n) : 0x80000000u; }
+  // rows [0, left) of the operand at base exist, `width` bytes each; shift: of the LDS address, for the buffer
+  __device__ __forceinline__ tsg_u4 bound(const char* base, long left, int width) const {
+    const int rows = left < ROWS ? (int)left : ROWS;
+    return tsg_descriptor(base, rows > 0 ? (rows - 1) * stride + width : 0u);
+  }
+  __device__ __forceinline__ void load(const char* base, long left, int width, int shift) const {
+    const tsg_u4 d = bound(base, left, width);
+    issue(d, shift, [&](int n) { return at(n); });
+  }
+  __device__ __forceinline__ void load(const char* base, long left, int width, int shift, unsigned long long used) const {
+    const tsg_u4 d = bound(base, left, width);
+    issue(d, shift, [&](int n) { return at(n, used); });
+  }
+  template <typename F> __device__ __forceinline__ void issue(tsg_u4 d, int shift, F off_of) const {
+    const unsigned to = __builtin_amdgcn_readfirstlane(lds + shift);
+    if constexpr (N == 1) tsg_dma(d, off_of(0), to);
+    else if constexpr (N == 2) tsg_dma2<WAVES * 1024>(d, off_of(0), off_of(1), to);
+    else {
+      static_assert(N % 4 == 0, "");
+#pragma unroll
+      for (int n = 0; n < N; n += 4) tsg_dma4<WAVES * 1024>(d, off_of(n), off_of(n + 1), off_of(n + 2), off_of(n + 3), to + n * WAVES * 1024);
+    }
+  }
+};
+
+// Order of the instructions of a block: `first` LDS reads, then one matrix product for every `per` more, so that a product never
+// waits for the read just before it.
+template <int READS, int PRODUCTS, int FIRST, int PER> __device__ __forceinline__ void tsg_interleave() {
+  __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
+#pragma unroll
+  for (int n = 0; n < PRODUCTS; ++n) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (FIRST + n * PER < READS) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
   }
 }

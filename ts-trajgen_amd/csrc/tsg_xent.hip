@@ -81,23 +81,42 @@ __device__ __forceinline__ void product(tsg_f32x16 (&acc)[2][2], char* lds, cons
   // a wave's 64 rows or columns: rows lie 128 bytes apart, columns 2
   const unsigned a0 = tsg_lds_addr(lds) + (AC ? TsgLane<D, TM / 8>::col_in_order(lane) ^ (wm * 2) : TsgLane<D, TK / 8>::row(lane) + wm * TK * 2);
   const unsigned b0 = tsg_lds_addr(lds) + TILE + (BC ? TsgLane<D, TN / 8>::col_in_order(lane) ^ (wn * 2) : TsgLane<D, TK / 8>::row(lane) + wn * TK * 2);
-  auto fetch = [&](int step, int buf) {
-    const int pass = step / per, k0 = (step % per) * TK;
-    char* at = lds + buf * 2 * TILE;
+  TsgLoader<AC ? TK : TM, (AC ? TM : TK) / 8, 4> al;
+  TsgLoader<BC ? TK : TN, (BC ? TN : TK) / 8, 4> bl;
+  // a tile whose memory rows are k is as wide as the operand is; one whose columns are k ends where k ends (its last step: below)
+  al.init(a.row, AC ? a.cols / 8 : TK / 8, tsg_lds_addr(lds), wave, lane);
+  bl.init(b.row, BC ? b.cols / 8 : TK / 8, tsg_lds_addr(lds) + TILE, wave, lane);
+  auto fetch = [&](int pass, int k0, int buf) {
     const char* ap = a.p + (pass == 2 ? a.plane : 0);
     const char* bp = b.p + (pass == 1 ? b.plane : 0);
-    if (AC) tsg_load_tile<TK, TM / 8, 4>(at, ap + (long)k0 * a.row, a.row, a.rows - k0, a.cols / 8, wave, lane);
-    else tsg_load_tile<TM, TK / 8, 4>(at, ap + k0 * 2, a.row, a.rows, (a.cols - k0) / 8, wave, lane);
-    if (BC)
-      tsg_load_tile<TK, TN / 8, 4, MASKED>(at + TILE, bp + (long)k0 * b.row, b.row, b.rows - k0, b.cols / 8, wave, lane,
-                                           MASKED ? b.used[k0 / TK] : 0ull);
-    else tsg_load_tile<TN, TK / 8, 4>(at + TILE, bp + k0 * 2, b.row, b.rows, (b.cols - k0) / 8, wave, lane);
+    if (!AC || !BC) {
+      if (K - k0 < TK && K % TK) {  // the last, narrower step
+        if (!AC) al.init(a.row, (a.cols - k0) / 8, tsg_lds_addr(lds), wave, lane);
+        if (!BC) bl.init(b.row, (b.cols - k0) / 8, tsg_lds_addr(lds) + TILE, wave, lane);
+      }
+    }
+    if (AC) al.load(ap + (long)k0 * a.row, a.rows - k0, a.cols * 2, buf * 2 * TILE);
+    else al.load(ap + k0 * 2, a.rows, min(a.cols - k0, TK) * 2, buf * 2 * TILE);
+    if (BC && MASKED) bl.load(bp + (long)k0 * b.row, b.rows - k0, b.cols * 2, buf * 2 * TILE, b.used[k0 / TK]);
+    else if (BC) bl.load(bp + (long)k0 * b.row, b.rows - k0, b.cols * 2, buf * 2 * TILE);
+    else bl.load(bp + k0 * 2, b.rows, min(b.cols - k0, TK) * 2, buf * 2 * TILE);
+    if (!AC || !BC) {
+      if (K - k0 < TK && K % TK) {
+        if (!AC) al.init(a.row, TK / 8, tsg_lds_addr(lds), wave, lane);
+        if (!BC) bl.init(b.row, TK / 8, tsg_lds_addr(lds) + TILE, wave, lane);
+      }
+    }
   };
-  if (steps) fetch(0, 0);
+  int pass = 0, k0 = 0;
+  if (steps) fetch(0, 0, 0);
   for (int step = 0, buf = 0; step < steps; ++step, buf ^= 1) {
     tsg_dma_wait();
     __syncthreads();
-    if (step + 1 < steps) fetch(step + 1, buf ^ 1);
+    if (step + 1 < steps) {
+      k0 += TK;
+      if (k0 >= K) k0 = 0, ++pass;
+      fetch(pass, k0, buf ^ 1);
+    }
     const unsigned at = tsg_opaque(a0) + buf * 2 * TILE, bt = tsg_opaque(b0) + buf * 2 * TILE;
 #pragma unroll
     for (int s = 0; s < TK / 16; ++s) {
@@ -523,6 +542,7 @@ Layout layout_of(const tsg_xent_desc* d, bool backward) {
     if (vc < TM) vc = TM;
     const size_t all = (V + TM - 1) / TM * TM;
     if (vc > all) vc = all;
+    if (vc > ((size_t)1 << 22)) vc = (size_t)1 << 22;  // 128 rows of dz stay below 2^31 bytes
     const size_t pieces = (all + vc - 1) / vc;  // even pieces
     vc = ((all + pieces - 1) / pieces + TM - 1) / TM * TM;
     l.vc = (int)vc;
@@ -554,6 +574,7 @@ int check_xent(const tsg_xent_desc* d, bool backward) {
   const int epc = d->dtype == TSG_F32 ? 4 : 8;
   if (!d->h || !d->w || !d->target || !d->stats || (uintptr_t)d->h % 16 || (uintptr_t)d->w % 16 || (uintptr_t)d->stats % 8) return TSG_E_INVALID;
   if (d->h_row < d->hidden || d->w_row < d->hidden || d->h_row % epc || d->w_row % epc) return TSG_E_INVALID;
+  if (d->h_row * 4 >= (1 << 23) || d->w_row * 4 >= (1 << 23)) return TSG_E_LIMIT;  // offsets inside a tile are 32-bit
   if (!backward && !d->row_loss) return TSG_E_INVALID;
   if (!backward && d->reduction && !d->loss) return TSG_E_INVALID;
   if (backward && (!d->d_loss || !d->dh || !d->dw || (d->bias && !d->dbias))) return TSG_E_INVALID;

@@ -139,7 +139,7 @@ def dropout(x, p, seed, site=0, step=0):
 def _fits(x, per):
     """Whether the kernels can read x [rows][heads][dim] where it lies."""
     return (x.stride(2) == 1 and x.shape[2] % per == 0 and x.stride(0) % per == 0 and x.stride(1) % per == 0
-            and x.data_ptr() % 16 == 0)
+            and x.stride(0) * x.element_size() < 1 << 24 and x.data_ptr() % 16 == 0)
 
 
 def _laid_out(x, per, dim):
@@ -272,7 +272,7 @@ def _rows_for(x, wide):
     per = 4 if x.dtype == torch.float32 else 8
     if x.shape[1] != wide:
         return torch.nn.functional.pad(x, (0, wide - x.shape[1]))
-    if x.stride(1) == 1 and x.stride(0) >= wide and x.stride(0) % per == 0 and x.data_ptr() % 16 == 0:
+    if x.stride(1) == 1 and x.stride(0) >= wide and x.stride(0) % per == 0 and x.stride(0) < 1 << 21 and x.data_ptr() % 16 == 0:
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
