@@ -541,7 +541,8 @@ int tsg_dropout(const tsg_dropout_desc* d, void* stream);
  * stats [heads][n_q][2] f32 is written by the forward (a row's largest q.k, and the base-2 logarithm of the sum of
  * exp(scale (q.k - largest)); 0 and +inf where a row sees nothing) and read, with out, by the backward, which writes
  * delta [heads][n_q].
- * workspace: what tsg_attn_workspace says, for the forward with few rows over many keys; 0 bytes = none needed. */
+ * workspace: what tsg_attn_workspace says, 16-byte aligned, for the forward with few rows over many keys and for the
+ * backward of few long sequences; 0 bytes = none needed. */
 typedef struct tsg_attn_desc {
   int32_t dtype, n_seq, heads, kv_heads, dim;
   float scale;             /* > 0 */
@@ -562,7 +563,7 @@ typedef struct tsg_attn_desc {
   float* delta;
 } tsg_attn_desc;
 
-int tsg_attn_workspace(const tsg_attn_desc* d, size_t* bytes_host);
+int tsg_attn_workspace(const tsg_attn_desc* d, size_t* forward_bytes_host, size_t* backward_bytes_host);
 int tsg_attn_forward(const tsg_attn_desc* d, void* stream);
 int tsg_attn_backward(const tsg_attn_desc* d, void* stream);
 

@@ -196,6 +196,13 @@ def test_attention_single_rows_over_long_keys(dt, heads, kv_heads, dim):
     attend(dt, [1, 1, 0, 2, 1], [1500, 33, 70, 700, 1], heads, kv_heads, dim, seed=dim, grad=dim <= 256)
 
 
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('lens,heads,kv_heads,dim', [([3100], 2, 1, 64), ([1700, 1500], 4, 2, 128), ([2000], 1, 1, 256), ([4000], 1, 1, 40)])
+def test_attention_long_sequences(dt, lens, heads, kv_heads, dim):
+    # few long sequences: the backward's walk over the rows is cut into stretches
+    attend(dt, lens, lens, heads, kv_heads, dim, seed=dim)
+
+
 def test_attention_rows_behind_the_last_sequence_are_zero_and_unread():
     from ts_trajgen_amd import ops
     for dt in TYPES:

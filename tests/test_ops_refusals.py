@@ -100,3 +100,8 @@ def test_cross_entropy_backward_descriptor():
 def test_cross_entropy_refuses_cpu_tensors():
     with pytest.raises(RuntimeError, match='no CPU fallback'):
         ops.linear_cross_entropy(torch.zeros(2, 8), torch.zeros(5, 8), torch.zeros(2, dtype=torch.int64))
+
+
+def test_attention_backward_of_one_long_sequence_needs_its_workspace():
+    assert _attn('tsg_attn_backward', n_q=4096, n_k=4096) == -2
+    assert _attn('tsg_attn_backward', n_q=4096, n_k=4096, workspace=4104, workspace_bytes=1 << 40) == -2

@@ -178,7 +178,7 @@ def lib():
     L.tsg_dropout.argtypes = [C.POINTER(DropoutDesc), _p]
     for name in ('tsg_attn_forward', 'tsg_attn_backward'):
         getattr(L, name).argtypes = [C.POINTER(AttnDesc), _p]
-    L.tsg_attn_workspace.argtypes = [C.POINTER(AttnDesc), C.POINTER(_sz)]
+    L.tsg_attn_workspace.argtypes = [C.POINTER(AttnDesc), C.POINTER(_sz), C.POINTER(_sz)]
     L.tsg_xent_workspace.argtypes = [C.POINTER(XentDesc), C.POINTER(_sz), C.POINTER(_sz)]
     for name in ('tsg_xent_forward', 'tsg_xent_backward'):
         getattr(L, name).argtypes = [C.POINTER(XentDesc), _p]

@@ -35,7 +35,7 @@ struct AttnArgs {
   float* delta;  // [heads][n_q]
   float scale, scale2;
   int n_split;
-  float* part;   // rows kernel: [n_q][heads][n_split][dim + 2]
+  float* part;   // rows kernel: [n_q][heads][n_split][dim + 2]; dk and dv: [2][n_split][n_k][kv_heads][dim]
 };
 
 // the sequence that position t belongs to, -1 for none (empty sequences share their start with the next one)
@@ -171,6 +171,17 @@ __device__ __forceinline__ void store_rows(const typename TsgElem<D>::Acc (&acc)
     }
 }
 
+template <typename D, int ND> __device__ __forceinline__ void store_sums(const typename TsgElem<D>::Acc (&acc)[ND], float* row, int dim, int h) {
+  typedef TsgElem<D> E;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int g = 0; g < E::REGS / 4; ++g) {
+      const int d = E::W * dt + 8 * g + 4 * h;
+      if (d < dim) *reinterpret_cast<float4*>(row + d) = make_float4(acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]);
+    }
+}
+
 template <int W> __device__ __forceinline__ float parts_max(float v) {
 #pragma unroll
   for (int o = W; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
@@ -236,6 +247,7 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
 #pragma unroll
       for (int s = 0; s < NF; ++s) tsg_mma<D>(tsg_row_frag<D>(row, s, W * n * CH * 16), qf[s], z[n]);
     }
+    if constexpr (!F32) tsg_interleave<NB * NF, NB * NF, 6, 1>();
     if (k0 < b.in_lo || k0 + BK > b.in_hi) {
       keep_branch();
       const int first = lo - k0 - 4 * h, last = hi - k0 - 4 * h;
@@ -294,6 +306,7 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) p.template mma<CH>(col, dt, TILE + W * n * CH * 16, acc[dt]);
     }
+    if constexpr (!F32) tsg_interleave<NB * ND * 4, NB * ND * 2, 8, 2>();
   }
   l = parts_sum<W>(l);
   if (t < a.n_q) {
@@ -378,6 +391,7 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
         tsg_mma<D>(tsg_row_frag<D>(row, s, W * n * CH * 16), qf[s], z);
         tsg_mma<D>(tsg_row_frag<D>(row, s, TILE + W * n * CH * 16), gf[s], dp);
       }
+      if constexpr (!F32) tsg_interleave<2 * NF, 2 * NF, 6, 1>();
 #pragma unroll
       for (int i = 0; i < E::REGS; ++i) z[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i] - st.x, a.scale2, -st.y)) * dp[i];
       if (edge_tile) {
@@ -393,6 +407,7 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
       ds.set(z);
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) ds.template mma<CH>(col, dt, W * n * CH * 16, acc[dt]);
+      if constexpr (!F32) tsg_interleave<ND * 4, ND * 2, 8, 2>();
     }
   }
   if (t < a.n_q) store_rows<D, ND>(acc, a.dq + (long)t * a.dq_row + head * a.dq_head, a.scale, a.dim, h);
@@ -413,7 +428,8 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   __shared__ int edge[8];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane / W;
   const unsigned row0 = tsg_lds_addr(lds) + TsgLane<D, CH>::row(lane), col0 = tsg_lds_addr(lds) + TsgLane<D, CH>::col(lane);
-  const int tile = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads;  // early keys are seen by most rows: first
+  // early keys are seen by most rows: first.  With n_split > 1 the walk over the rows is cut into that many stretches.
+  const int split = blockIdx.x / a.kv_heads % a.n_split, tile = blockIdx.x / a.kv_heads / a.n_split, kvh = blockIdx.x % a.kv_heads;
   const int j = tile * (4 * W) + wave * W + lane % W;
   int lo, hi;
   rows_of_key(a, j, lo, hi);
@@ -436,7 +452,8 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
       if constexpr (PART != 2) dv[dt][i] = 0.0f;
     }
   // the walk: for every head of the group the row tiles [b.lo, b.hi), as one sequence of steps
-  const int steps = b.lo < b.hi ? (b.hi - b.lo + BQ - 1) / BQ * a.group : 0;
+  const int per = b.lo < b.hi ? (b.hi - b.lo + BQ - 1) / BQ : 0, all = per * a.group;
+  const int first = (int)((long)all * split / a.n_split), steps = (int)((long)all * (split + 1) / a.n_split) - first;
   struct Step {
     int head, t0;
   };
@@ -462,7 +479,7 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   };
   float2 st = make_float2(0.0f, INFINITY);
   float delta = 0.0f;
-  Step now = {kvh * a.group, b.lo};
+  Step now = {kvh * a.group + (steps ? first / per : 0), b.lo + (steps ? first % per : 0) * BQ};
   tsg_settle(kf);
   if constexpr (PART != 1 && !VL) tsg_settle(vf);
   if (steps) {
@@ -503,6 +520,7 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
           tsg_mma<D>(tsg_row_frag<D>(row, s, TILE + W * n * CH * 16),
                      VL ? tsg_row_frag<D>(vrow, s, 0) : vf[VL ? 0 : s], dp);
       }
+      if constexpr (!F32) tsg_interleave<(PART == 1 ? 1 : VL ? 3 : 2) * NF, (PART == 1 ? 1 : 2) * NF, 6, PART != 1 && VL ? 2 : 1>();
 #pragma unroll
       for (int g = 0; g < E::REGS / 4; ++g) {
         const float4 ms = *reinterpret_cast<const float4*>(&stat[buf][0][W * n + 8 * g + 4 * h]);
@@ -539,10 +557,31 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
       }
     }
   }
-  if (j < a.n_k) {
+  if (j < a.n_k && a.n_split > 1) {
+    float* p = a.part + (((long)split * a.n_k + j) * a.kv_heads + kvh) * a.dim;
+    if constexpr (PART != 1) store_sums<D, ND>(dk, p, a.dim, h);
+    if constexpr (PART != 2) store_sums<D, ND>(dv, p + (long)a.n_split * a.n_k * a.kv_heads * a.dim, a.dim, h);
+  } else if (j < a.n_k) {
     if constexpr (PART != 1) store_rows<D, ND>(dk, a.dk + (long)j * a.dk_row + kvh * a.dk_head, a.scale, a.dim, h);
     if constexpr (PART != 2) store_rows<D, ND>(dv, a.dv + (long)j * a.dv_row + kvh * a.dv_head, 1.0f, a.dim, h);
   }
+}
+
+// dk and dv from the stretches' sums: four elements per thread, blockIdx.y 0: dk, 1: dv
+template <typename D> __global__ __launch_bounds__(256) void attn_dkv_join_kernel(AttnArgs a) {
+  const long all = (long)a.n_k * a.kv_heads * a.dim, i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= all) return;
+  const float* p = a.part + (long)blockIdx.y * a.n_split * all + i;
+  float4 s = *reinterpret_cast<const float4*>(p);
+  for (int n = 1; n < a.n_split; ++n) {
+    const float4 v = *reinterpret_cast<const float4*>(p + n * all);
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  const int d = (int)(i % a.dim), kvh = (int)(i / a.dim % a.kv_heads);
+  const long j = i / a.dim / a.kv_heads;
+  const float by = blockIdx.y ? 1.0f : a.scale;
+  char* to = blockIdx.y ? a.dv + j * a.dv_row + kvh * a.dv_head : a.dk + j * a.dk_row + kvh * a.dk_head;
+  store4<D>(to + d * TsgElem<D>::BYTES, s.x * by, s.y * by, s.z * by, s.w * by);
 }
 
 // --------------------------------------------------------------------------------- few rows: one row, keys split
@@ -853,6 +892,22 @@ size_t workspace_of(const tsg_attn_desc* d) {
   return n == 1 ? 0 : (size_t)d->n_q * d->heads * n * (d->dim + 2) * 4;
 }
 
+// A tile of keys walks every row that sees it, for all heads of its group: the first keys of a long sequence walk twice the mean,
+// and a workgroup's walk is one chain.  Cut until there are three rounds of workgroups, but no shorter than eight steps of
+// 64 rows in the mean; the sums then meet in f32 (4 sequences of 2.5-4 k positions, 16 heads over 4, 128 wide).
+int dkv_splits_of(const tsg_attn_desc* d) {
+  if (d->dim > 256 || d->n_seq <= 0) return 1;
+  const int64_t wgs = (int64_t)tsg_cdiv(d->n_k, d->dtype == TSG_F32 ? 64 : 128) * d->kv_heads;
+  const int64_t steps = d->n_q / d->n_seq * (d->heads / d->kv_heads) / 64 / 2;
+  int64_t n = wgs ? 1536 / wgs : 1;
+  if (n > steps / 8) n = steps / 8;
+  return (int)(n < 1 ? 1 : (n > 16 ? 16 : n));
+}
+size_t backward_workspace_of(const tsg_attn_desc* d) {
+  const int n = dkv_splits_of(d);
+  return n == 1 ? 0 : (size_t)2 * n * d->n_k * d->kv_heads * d->dim * 4;
+}
+
 int check_attn(const tsg_attn_desc* d, bool backward) {
   if (!d) return TSG_E_INVALID;
   if (d->dtype != TSG_F32 && d->dtype != TSG_BF16 && d->dtype != TSG_F16) return TSG_E_INVALID;
@@ -935,7 +990,8 @@ template <typename D> int forward_of(const tsg_attn_desc* d, hipStream_t s) {
 }
 
 template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
-  const AttnArgs a = args_of(d);
+  AttnArgs a = args_of(d);
+  a.n_split = dkv_splits_of(d);
   const dim3 block(256);
   if (a.dim > 256) {
     if (a.n_q) hipLaunchKernelGGL(attn_wide_dq_kernel<D>, dim3((unsigned)((long)a.n_q * a.heads)), dim3(64), 0, s, a);
@@ -944,7 +1000,7 @@ template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
     return 0;
   }
   constexpr int R = rows_per_wg<D>();
-  const dim3 gq((unsigned)(tsg_cdiv(a.n_q, R) * a.heads)), gk((unsigned)(tsg_cdiv(a.n_k, R) * a.kv_heads));
+  const dim3 gq((unsigned)(tsg_cdiv(a.n_q, R) * a.heads)), gk((unsigned)(tsg_cdiv(a.n_k, R) * a.kv_heads * a.n_split));
   constexpr bool F32 = TsgElem<D>::BYTES == 4;
   if (a.n_q) {
     if (a.dim <= 64) hipLaunchKernelGGL((attn_dq_kernel<D, 64, 64>), gq, block, 0, s, a);
@@ -965,6 +1021,8 @@ template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
       hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 1, false>), gk, block, 0, s, a);
       hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 2, true>), gk, block, 0, s, a);
     }
+    if (a.n_split > 1)
+      hipLaunchKernelGGL(attn_dkv_join_kernel<D>, dim3((unsigned)(((long)a.n_k * a.kv_heads * a.dim / 4 + 255) / 256), 2), block, 0, s, a);
   }
   TSG_LAUNCH_CHECK();
   return 0;
@@ -972,9 +1030,11 @@ template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
 
 }  // namespace
 
-extern "C" int tsg_attn_workspace(const tsg_attn_desc* d, size_t* bytes_host) {
-  if (!d || !bytes_host || d->n_q < 0 || d->n_k < 0 || d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads) return TSG_E_INVALID;
-  *bytes_host = d->n_q ? workspace_of(d) : 0;
+extern "C" int tsg_attn_workspace(const tsg_attn_desc* d, size_t* forward_bytes_host, size_t* backward_bytes_host) {
+  if (!d || !forward_bytes_host || !backward_bytes_host) return TSG_E_INVALID;
+  if (d->n_q < 0 || d->n_k < 0 || d->dim <= 0 || d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads) return TSG_E_INVALID;
+  *forward_bytes_host = d->n_q ? workspace_of(d) : 0;
+  *backward_bytes_host = d->n_k ? backward_workspace_of(d) : 0;
   return 0;
 }
 
@@ -992,6 +1052,8 @@ extern "C" int tsg_attn_backward(const tsg_attn_desc* d, void* stream) {
   if (d && d->n_q == 0 && d->n_k == 0) return 0;
   const int rc = check_attn(d, true);
   if (rc) return rc;
+  const size_t need = backward_workspace_of(d);
+  if (need && (!d->workspace || (uintptr_t)d->workspace % 16 || d->workspace_bytes < need)) return TSG_E_TOO_SMALL;
   hipStream_t s = (hipStream_t)stream;
   return d->dtype == TSG_F32 ? backward_of<TsgF32>(d, s) : (d->dtype == TSG_BF16 ? backward_of<TsgBf16>(d, s) : backward_of<TsgF16>(d, s));
 }

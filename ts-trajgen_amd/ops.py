@@ -165,6 +165,15 @@ def _attn_desc(q, k, v, q_ptr, k_ptr, scale, out, stats):
     return d
 
 
+def _attn_workspace(d, dev, backward):
+    sizes = C.c_size_t(), C.c_size_t()
+    _lib.check(_lib.lib().tsg_attn_workspace(C.byref(d), C.byref(sizes[0]), C.byref(sizes[1])), 'tsg_attn_workspace')
+    need = sizes[backward].value
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    d.workspace, d.workspace_bytes = _lib.ptr(ws), need
+    return ws
+
+
 class _CausalAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_ptr, k_ptr, scale):
@@ -179,11 +188,7 @@ class _CausalAttention(torch.autograd.Function):
         if q.dtype != torch.float32 and any(ctx.needs_input_grad[:3]):
             rest = torch.empty(out.shape, dtype=q.dtype, device=q.device)
             d.out_rest = _lib.ptr(rest)
-        need = C.c_size_t()
-        _lib.check(L.tsg_attn_workspace(C.byref(d), C.byref(need)), 'tsg_attn_workspace')
-        if need.value:
-            ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-            d.workspace, d.workspace_bytes = _lib.ptr(ws), need.value
+        ws = _attn_workspace(d, q.device, 0)  # noqa: F841  (held until the launches are on the stream)
         if q.shape[0] and k.shape[0]:
             with torch.cuda.device(q.device):
                 _lib.check(L.tsg_attn_forward(C.byref(d), _lib.current_stream()), 'tsg_attn_forward')
@@ -214,6 +219,7 @@ class _CausalAttention(torch.autograd.Function):
                 setattr(d, name + '_row', t.stride(0))
                 setattr(d, name + '_head', t.stride(1))
             d.delta = _lib.ptr(delta)
+            ws = _attn_workspace(d, q.device, 1)  # noqa: F841
             with torch.cuda.device(q.device):
                 _lib.check(_lib.lib().tsg_attn_backward(C.byref(d), _lib.current_stream()), 'tsg_attn_backward')
         else:
