@@ -38,23 +38,37 @@ struct AttnArgs {
   float* part;   // rows kernel: [n_q][heads][n_split][dim + 2]; dk and dv: [2][n_split][n_k][kv_heads][dim]
 };
 
-// the sequence that position t belongs to, -1 for none (empty sequences share their start with the next one)
-__device__ __forceinline__ int seq_of(const int* ptr, int n_seq, int t) {
+// The sequence that position t belongs to, -1 for none (empty sequences share their start with the next one).  One position,
+// alike in all lanes of a wave: every lane probes, so 4096 sequences take two loads one behind the other.
+__device__ __forceinline__ int starts_until(const int* ptr, int n_seq, int t) {  // how many starts are <= t
+  const int lane = threadIdx.x & 63;
   int lo = 0, hi = n_seq;
   while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (ptr[mid] <= t) lo = mid + 1;
+    const int w = (hi - lo + 64) / 65, at = lo + (lane + 1) * w - 1;
+    const int n = __popcll(__ballot(at < hi && ptr[at < hi ? at : lo] <= t));
+    lo += n * w;
+    hi = min(hi, lo + w - 1);
+  }
+  return lo;
+}
+__device__ __forceinline__ int seq_from(const int* ptr, int n_seq, int s, int t) {  // s: starts_until of a position before t
+  for (int n = 0; n < 8 && s < n_seq && ptr[s] <= t; ++n) ++s;
+  int hi = s < n_seq && ptr[s] <= t ? n_seq : s;  // not among the next few: bisect
+  while (s < hi) {
+    const int mid = (s + hi) >> 1;
+    if (ptr[mid] <= t) s = mid + 1;
     else hi = mid;
   }
-  return (lo > 0 && t < ptr[lo]) ? lo - 1 : -1;
+  return (s > 0 && t < ptr[s]) ? s - 1 : -1;
 }
 __device__ __forceinline__ int clamp_to(long v, int n) { return v < 0 ? 0 : (v > n ? n : (int)v); }
 
-// keys [lo, hi) that query row t sees; always inside [0, n_k], whatever the pointers hold
-__device__ __forceinline__ void keys_of_row(const AttnArgs& a, int t, int& lo, int& hi) {
+// keys [lo, hi) that query row t sees; always inside [0, n_k], whatever the pointers hold.  t0 <= t: alike in the wave
+__device__ __forceinline__ void keys_of_row(const AttnArgs& a, int t0, int t, int& lo, int& hi) {
   lo = hi = 0;
+  const int from = starts_until(a.q_ptr, a.n_seq, t0);
   if (t >= a.n_q) return;
-  const int s = seq_of(a.q_ptr, a.n_seq, t);
+  const int s = seq_from(a.q_ptr, a.n_seq, from, t);
   if (s < 0) return;
   const long q1 = a.q_ptr[s + 1], k0 = a.k_ptr[s], k1 = a.k_ptr[s + 1];
   const long end = k1 - (q1 - 1 - t);  // the last row sees the last key
@@ -63,10 +77,11 @@ __device__ __forceinline__ void keys_of_row(const AttnArgs& a, int t, int& lo, i
   if (hi <= lo) lo = hi = 0;
 }
 // query rows [lo, hi) that see key j
-__device__ __forceinline__ void rows_of_key(const AttnArgs& a, int j, int& lo, int& hi) {
+__device__ __forceinline__ void rows_of_key(const AttnArgs& a, int j0, int j, int& lo, int& hi) {
   lo = hi = 0;
+  const int from = starts_until(a.k_ptr, a.n_seq, j0);
   if (j >= a.n_k) return;
-  const int s = seq_of(a.k_ptr, a.n_seq, j);
+  const int s = seq_from(a.k_ptr, a.n_seq, from, j);
   if (s < 0) return;
   const long q0 = a.q_ptr[s], q1 = a.q_ptr[s + 1], k1 = a.k_ptr[s + 1];
   const long first = q1 - (k1 - j);
@@ -198,7 +213,7 @@ template <typename D> constexpr int rows_per_wg() { return 4 * TsgElem<D>::W; }
 
 // ------------------------------------------------------------------------------------------------- forward, tiles
 template <typename D, int DP, int BK>
-__global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, (DP > 128 && TsgElem<D>::BYTES == 2) ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
   typedef TsgElem<D> E;
   typedef typename E::Acc Acc;
   constexpr bool F32 = E::BYTES == 4;
@@ -210,12 +225,13 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   const int tiles = gridDim.x / a.heads;
   const int tile = tiles - 1 - (int)(blockIdx.x / a.heads), head = blockIdx.x % a.heads;  // late rows see most keys: first
   const int kvh = head / a.group;
-  const int t = tile * (4 * W) + wave * W + lane % W;
-  int lo, hi;
-  keys_of_row(a, t, lo, hi);
-  const Bounds b = bounds_of<W>(lo, hi, wave, edge);
+  const int w0 = __builtin_amdgcn_readfirstlane(tile * (4 * W) + wave * W), t = w0 + lane % W;
+  // the row's own operands first: their way here covers the search for its sequence
   tsg_u4 qf[NF];
   load_frags<PARTS>(qf, a.q + (long)t * a.q_row + head * a.q_head, t < a.n_q, a.chunks, h);
+  int lo, hi;
+  keys_of_row(a, w0, t, lo, hi);
+  const Bounds b = bounds_of<W>(lo, hi, wave, edge);
   Acc acc[ND];
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
@@ -231,14 +247,15 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
     kl.load(kbase + (long)k0 * a.k_row, b.hi - k0, a.chunks * 16, buf * 2 * TILE);
     vl.load(vbase + (long)k0 * a.v_row, b.hi - k0, a.chunks * 16, buf * 2 * TILE);
   };
-  tsg_settle(qf);
   if (b.lo < b.hi) fetch(b.lo, 0);
+  tsg_settle(qf);
   for (int k0 = b.lo, buf = 0; k0 < b.hi; k0 += BK, buf ^= 1) {
     tsg_dma_wait();
     __syncthreads();
     if (k0 + BK < b.hi) fetch(k0 + BK, buf ^ 1);
     if (k0 >= b.wave_hi || k0 + BK <= b.wave_lo) continue;  // nothing for this wave: uniform, the barriers are above
     const unsigned row = tsg_opaque(row0) + buf * 2 * TILE, col = tsg_opaque(col0) + buf * 2 * TILE;
+    __builtin_amdgcn_s_setprio(1);  // matrix phases ahead of the other wave's softmax: 2 % of the forward
     Acc z[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -248,6 +265,7 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
       for (int s = 0; s < NF; ++s) tsg_mma<D>(tsg_row_frag<D>(row, s, W * n * CH * 16), qf[s], z[n]);
     }
     if constexpr (!F32) tsg_interleave<NB * NF, NB * NF, 6, 1>();
+    __builtin_amdgcn_s_setprio(0);
     if (k0 < b.in_lo || k0 + BK > b.in_hi) {
       keep_branch();
       const int first = lo - k0 - 4 * h, last = hi - k0 - 4 * h;
@@ -301,12 +319,14 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
         z[n][i] = __builtin_amdgcn_exp2f(z[n][i]);
         l += z[n][i];
       }
+      __builtin_amdgcn_s_setprio(1);
       TsgAccB<D> p;
       p.set(z[n]);
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) p.template mma<CH>(col, dt, TILE + W * n * CH * 16, acc[dt]);
     }
     if constexpr (!F32) tsg_interleave<NB * ND * 4, NB * ND * 2, 8, 2>();
+    __builtin_amdgcn_s_setprio(0);
   }
   l = parts_sum<W>(l);
   if (t < a.n_q) {
@@ -320,7 +340,7 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
 
 // ------------------------------------------------------------------------------------------------ backward, tiles: dq
 template <typename D, int DP, int BK>
-__global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, (DP > 128 && TsgElem<D>::BYTES == 2) ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
   typedef TsgElem<D> E;
   typedef typename E::Acc Acc;
   constexpr bool F32 = E::BYTES == 4;
@@ -332,10 +352,7 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   const int tiles = gridDim.x / a.heads;
   const int tile = tiles - 1 - (int)(blockIdx.x / a.heads), head = blockIdx.x % a.heads;
   const int kvh = head / a.group;
-  const int t = tile * (4 * W) + wave * W + lane % W;
-  int lo, hi;
-  keys_of_row(a, t, lo, hi);
-  const Bounds b = bounds_of<W>(lo, hi, wave, edge);
+  const int w0 = __builtin_amdgcn_readfirstlane(tile * (4 * W) + wave * W), t = w0 + lane % W;
   tsg_u4 qf[NF], gf[NF];
   load_frags<PARTS>(qf, a.q + (long)t * a.q_row + head * a.q_head, t < a.n_q, a.chunks, h);
   load_frags<PARTS>(gf, a.d_o + (long)t * a.do_row + head * a.do_head, t < a.n_q, a.chunks, h);
@@ -356,6 +373,9 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
       if (h == 0) a.delta[(long)head * a.n_q + t] = delta;  // the dk / dv kernel, next on the stream, reads it
     }
   }
+  int lo, hi;
+  keys_of_row(a, w0, t, lo, hi);
+  const Bounds b = bounds_of<W>(lo, hi, wave, edge);
   Acc acc[ND];
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
@@ -370,10 +390,10 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
     kl.load(kbase + (long)k0 * a.k_row, b.hi - k0, a.chunks * 16, buf * 2 * TILE);
     vl.load(vbase + (long)k0 * a.v_row, b.hi - k0, a.chunks * 16, buf * 2 * TILE);
   };
+  if (b.lo < b.hi) fetch(b.lo, 0);
   tsg_settle(qf);
   tsg_settle(gf);
   asm volatile("" : "+v"(st.x), "+v"(st.y), "+v"(delta));
-  if (b.lo < b.hi) fetch(b.lo, 0);
   for (int k0 = b.lo, buf = 0; k0 < b.hi; k0 += BK, buf ^= 1) {
     tsg_dma_wait();
     __syncthreads();
@@ -418,7 +438,7 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
 // VL: the values' fragments are read from LDS in every step instead of held in registers, which then suffice without spills
 // (16-bit types 128 wide at two waves a SIMD, 256 wide at one; f32 256 wide).
 template <typename D, int DP, int BQ, int PART, bool VL>
-__global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP * TsgElem<D>::BYTES > 256 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
   typedef TsgElem<D> E;
   typedef typename E::Acc Acc;
   constexpr bool F32 = E::BYTES == 4;
@@ -430,10 +450,7 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   const unsigned row0 = tsg_lds_addr(lds) + TsgLane<D, CH>::row(lane), col0 = tsg_lds_addr(lds) + TsgLane<D, CH>::col(lane);
   // early keys are seen by most rows: first.  With n_split > 1 the walk over the rows is cut into that many stretches.
   const int split = blockIdx.x / a.kv_heads % a.n_split, tile = blockIdx.x / a.kv_heads / a.n_split, kvh = blockIdx.x % a.kv_heads;
-  const int j = tile * (4 * W) + wave * W + lane % W;
-  int lo, hi;
-  rows_of_key(a, j, lo, hi);
-  const Bounds b = bounds_of<W>(lo, hi, wave, edge);
+  const int w0 = __builtin_amdgcn_readfirstlane(tile * (4 * W) + wave * W), j = w0 + lane % W;
   tsg_u4 kf[NF], vf[PART == 1 || VL ? 1 : NF];
   load_frags<PARTS>(kf, a.k + (long)j * a.k_row + kvh * a.k_head, j < a.n_k, a.chunks, h);
   if constexpr (PART != 1 && VL) {
@@ -443,6 +460,9 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
     const int j0 = tile * (4 * W) + wave * W;
     vl.load(a.v + (long)j0 * a.v_row + kvh * a.v_head, a.n_k - j0, a.chunks * 16, 0);
   } else if constexpr (PART != 1) load_frags<PARTS>(vf, a.v + (long)j * a.v_row + kvh * a.v_head, j < a.n_k, a.chunks, h);
+  int lo, hi;
+  rows_of_key(a, w0, j, lo, hi);
+  const Bounds b = bounds_of<W>(lo, hi, wave, edge);
   Acc dk[PART == 1 ? 1 : ND], dv[PART == 2 ? 1 : ND];
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
@@ -480,14 +500,14 @@ __global__ __launch_bounds__(256, (DP > 128 || TsgElem<D>::BYTES == 4) ? 1 : 2) 
   float2 st = make_float2(0.0f, INFINITY);
   float delta = 0.0f;
   Step now = {kvh * a.group + (steps ? first / per : 0), b.lo + (steps ? first % per : 0) * BQ};
-  tsg_settle(kf);
-  if constexpr (PART != 1 && !VL) tsg_settle(vf);
   if (steps) {
+    fetch(now, 0);
     stat_of(now, st, delta);
     stat_to(0, st, delta);
     if (steps > 1) stat_of(after(now), st, delta);  // held until the next step's buffer is free
-    fetch(now, 0);
   }
+  tsg_settle(kf);
+  if constexpr (PART != 1 && !VL) tsg_settle(vf);
   for (int step = 0, buf = 0; step < steps; ++step, buf ^= 1) {
     tsg_dma_wait();
     __syncthreads();
@@ -626,7 +646,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
   const int kvh = bid % a.kv_heads, t = bid / a.kv_heads;
   const int head0 = kvh * a.group + st * G, n_heads = min(G, a.group - st * G);
   int lo, hi;
-  keys_of_row(a, t, lo, hi);
+  keys_of_row(a, t, t, lo, hi);
   const long span = hi - lo;
   const int j0 = lo + (int)(span * split / a.n_split), j1 = lo + (int)(span * (split + 1) / a.n_split);
   Chunk<D> qv[G][NC];
@@ -817,7 +837,7 @@ template <typename D> __global__ __launch_bounds__(64) void attn_wide_dq_kernel(
   typedef typename D::type T;
   const int t = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kvh = head / a.group, lane = threadIdx.x;
   int lo, hi;
-  keys_of_row(a, t, lo, hi);
+  keys_of_row(a, t, t, lo, hi);
   float q[WIDE], g[WIDE], x[WIDE], acc[WIDE];
   load_wide<T>(q, a.q + (long)t * a.q_row + head * a.q_head, a.dim, lane);
   load_wide<T>(g, a.d_o + (long)t * a.do_row + head * a.do_head, a.dim, lane);
@@ -845,7 +865,7 @@ template <typename D> __global__ __launch_bounds__(64) void attn_wide_dkv_kernel
   typedef typename D::type T;
   const int j = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads, lane = threadIdx.x;
   int lo, hi;
-  rows_of_key(a, j, lo, hi);
+  rows_of_key(a, j, j, lo, hi);
   float k[WIDE], v[WIDE], x[WIDE], dk[WIDE], dv[WIDE];
   load_wide<T>(k, a.k + (long)j * a.k_row + kvh * a.k_head, a.dim, lane);
   load_wide<T>(v, a.v + (long)j * a.v_row + kvh * a.v_head, a.dim, lane);
@@ -983,7 +1003,7 @@ template <typename D> int forward_of(const tsg_attn_desc* d, hipStream_t s) {
     constexpr int BK = TsgElem<D>::BYTES == 4 ? 32 : 64;
     if (a.dim <= 64) hipLaunchKernelGGL((attn_fwd_kernel<D, 64, 64>), grid, block, 0, s, a);
     else if (a.dim <= 128) hipLaunchKernelGGL((attn_fwd_kernel<D, 128, BK>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((attn_fwd_kernel<D, 256, 32>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((attn_fwd_kernel<D, 256, BK / 2>), grid, block, 0, s, a);
   }
   TSG_LAUNCH_CHECK();
   return 0;
@@ -1005,17 +1025,12 @@ template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
   if (a.n_q) {
     if (a.dim <= 64) hipLaunchKernelGGL((attn_dq_kernel<D, 64, 64>), gq, block, 0, s, a);
     else if (a.dim <= 128) hipLaunchKernelGGL((attn_dq_kernel<D, 128, F32 ? 32 : 64>), gq, block, 0, s, a);
-    else hipLaunchKernelGGL((attn_dq_kernel<D, 256, 32>), gq, block, 0, s, a);
+    else hipLaunchKernelGGL((attn_dq_kernel<D, 256, F32 ? 16 : 32>), gq, block, 0, s, a);
   }
   if (a.n_k) {
     if (a.dim <= 64) hipLaunchKernelGGL((attn_dkv_kernel<D, 64, 32, 0, false>), gk, block, 0, s, a);
-    else if (a.dim <= 128) {
-      if constexpr (F32) hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0, false>), gk, block, 0, s, a);
-      else {
-        hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 64, 1, false>), gk, block, 0, s, a);
-        hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 2, false>), gk, block, 0, s, a);
-      }
-    }
+    else if (a.dim <= 128)
+      hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0, !F32>), gk, block, 0, s, a);
     else if constexpr (F32) hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 16, 0, true>), gk, block, 0, s, a);
     else {
       hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 1, false>), gk, block, 0, s, a);
