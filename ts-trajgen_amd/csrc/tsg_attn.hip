@@ -96,7 +96,7 @@ struct Bounds {
   int in_lo, in_hi;      // intersection; empty when a row of the wave is empty
   int lo, hi;            // union over the workgroup
 };
-template <int W> __device__ __forceinline__ Bounds bounds_of(int lo, int hi, int wave, int* shared /* [8] */) {
+template <int W> __device__ __forceinline__ Bounds wave_bounds(int lo, int hi) {
   Bounds b;
   const bool none = hi <= lo;
   int ulo = none ? 0x7fffffff : lo, uhi = none ? 0 : hi, ilo = none ? 0x7fffffff : lo, ihi = none ? 0 : hi;
@@ -111,12 +111,14 @@ template <int W> __device__ __forceinline__ Bounds bounds_of(int lo, int hi, int
   b.wave_hi = __builtin_amdgcn_readfirstlane(uhi);
   b.in_lo = __builtin_amdgcn_readfirstlane(ilo);
   b.in_hi = __builtin_amdgcn_readfirstlane(ihi);
-  if ((threadIdx.x & 63) == 0) shared[wave] = ulo, shared[4 + wave] = uhi;
+  return b;
+}
+template <int W> __device__ __forceinline__ Bounds bounds_of(int lo, int hi, int wave, int* shared /* [8] */) {
+  Bounds b = wave_bounds<W>(lo, hi);
+  if ((threadIdx.x & 63) == 0) shared[wave] = b.wave_lo, shared[4 + wave] = b.wave_hi;
   __syncthreads();
-  b.lo = min(min(shared[0], shared[1]), min(shared[2], shared[3]));
-  b.hi = max(max(shared[4], shared[5]), max(shared[6], shared[7]));
-  b.lo = __builtin_amdgcn_readfirstlane(b.lo);
-  b.hi = __builtin_amdgcn_readfirstlane(b.hi);
+  b.lo = __builtin_amdgcn_readfirstlane(min(min(shared[0], shared[1]), min(shared[2], shared[3])));
+  b.hi = __builtin_amdgcn_readfirstlane(max(max(shared[4], shared[5]), max(shared[6], shared[7])));
   return b;
 }
 
@@ -209,7 +211,7 @@ template <int W> __device__ __forceinline__ float parts_sum(float v) {
 }
 // in a branch that is seldom taken: keeps the compiler from running both sides and selecting
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }
-template <typename D> constexpr int rows_per_wg() { return 4 * TsgElem<D>::W; }
+template <typename D> constexpr int rows_per_wg() { return TsgElem<D>::BYTES == 4 ? 16 : 128; }
 
 // ------------------------------------------------------------------------------------------------- forward, tiles
 template <typename D, int DP, int BK>
@@ -587,6 +589,265 @@ __global__ __launch_bounds__(256, DP * TsgElem<D>::BYTES > 256 ? 1 : 2) void att
   }
 }
 
+// ------------------------------------------------------------------------------------------ f32: 16 rows, 64 wide a wave
+// The f32 matrix cores are a sixteenth as fast as the 16-bit ones: operands straight from the caches keep them fed (32 bytes a
+// clock per CU), and what costs is idle waves.  So a workgroup owns only 16 rows, which see little more than they need
+// (trajectories of a few dozen positions: three blocks of 16 keys), and its waves share the work of every block evenly: each has
+// 64 of the width, forms its part of the 16 x 16 products q.k, and, once the parts have met in LDS, its 64 columns of the
+// sums.  A wave then holds 16 registers of each operand, so five to eight workgroups a CU cover the loads.
+// Row fragments as in tsg_mma.h.  Column fragments are read 16 bytes a lane: row m of product e of four stands for column
+// 4 m + e, so that one load serves four products and a lane's results are 16 bytes side by side.
+// Buffers bound the operands: rows behind the interval and chunks behind the width read as zeros.
+struct Rows16 {  // one block of 16 rows, 64 columns
+  __amdgpu_buffer_rsrc_t d;
+  unsigned row, col, stride;  // the lane's byte offsets: its row fragment, its column fragment
+  int chunks, left;           // chunks of the width; row fragments of this lane
+  __device__ __forceinline__ Rows16(long row_bytes, int n_chunks, int wave, int lane) {
+    stride = (unsigned)row_bytes, chunks = n_chunks, left = n_chunks - 16 * wave - (lane >> 4);
+    row = (lane & 15) * stride + wave * 256 + (lane >> 4) * 16;
+    col = (lane >> 4) * 4 * stride + wave * 256 + (lane & 15) * 16;
+  }
+  __device__ __forceinline__ void at(const char* base, int rows) {
+    const int n = rows < 16 ? rows : 16;
+    d = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, n > 0 ? (n - 1) * (int)stride + chunks * 16 : 0, 0x00020000);
+  }
+  __device__ __forceinline__ void rows(tsg_u4 (&f)[4]) const {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      f[s] = __builtin_bit_cast(tsg_u4, __builtin_amdgcn_raw_buffer_load_b128(d, 4 * s < left ? (int)(row + s * 64) : (int)0x80000000, 0, 0));
+  }
+  // f[i]: row 4 h + i; columns behind the width only reach sums that are not stored
+  __device__ __forceinline__ void cols(tsg_f4 (&f)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __builtin_bit_cast(tsg_f4, __builtin_amdgcn_raw_buffer_load_b128(d, (int)(col + i * stride), 0, 0));
+  }
+};
+typedef tsg_f4 Sum16[4];
+__device__ __forceinline__ tsg_f4 dot16(const tsg_u4 (&a)[4], const tsg_u4 (&b)[4], tsg_f4 z) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) tsg_mma<TsgF32>(a[s], b[s], z);
+  return z;
+}
+__device__ __forceinline__ void add16(Sum16& acc, const tsg_f4 (&v)[4], const tsg_f4& p) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][e], p[i], acc[e], 0, 0, 0);
+}
+__device__ __forceinline__ void zero16(Sum16& acc) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] = tsg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+__device__ __forceinline__ void store16(const Sum16& acc, char* row, float by, int dim, int wave, int h) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = 64 * wave + 16 * h + 4 * i;
+    if (c < dim) *reinterpret_cast<float4*>(row + c * 4) = make_float4(acc[0][i] * by, acc[1][i] * by, acc[2][i] * by, acc[3][i] * by);
+  }
+}
+// the waves' parts of a value, summed in the same order by all of them; slot: another one than the last call's
+template <int NW, typename V> __device__ __forceinline__ V over_waves(V (*slot)[64], V part, int wave, int lane) {
+  if (NW == 1) return part;
+  slot[wave][lane] = part;
+  __syncthreads();
+  V sum = slot[0][lane];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) sum += slot[w][lane];
+  return sum;
+}
+
+template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_fwd_kernel(AttnArgs a) {
+  __shared__ tsg_f4 meet[2][NW][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 4;
+  const int tiles = gridDim.x / a.heads;
+  const int t0 = (tiles - 1 - (int)(blockIdx.x / a.heads)) * 16, head = blockIdx.x % a.heads, kvh = head / a.group;
+  const int t = t0 + (lane & 15);
+  tsg_u4 qf[4];
+  Rows16 q(a.q_row, a.chunks, wave, lane), k(a.k_row, a.chunks, wave, lane), v(a.v_row, a.chunks, wave, lane);
+  q.at(a.q + (long)t0 * a.q_row + head * a.q_head, a.n_q - t0);
+  q.rows(qf);
+  int lo, hi;
+  keys_of_row(a, t0, t, lo, hi);
+  const Bounds b = wave_bounds<16>(lo, hi);
+  Sum16 acc;
+  zero16(acc);
+  float m = -INFINITY, l = 0.0f;
+  for (int k0 = b.wave_lo, buf = 0; k0 < b.wave_hi; k0 += 16, buf ^= 1) {
+    tsg_u4 kf[4];
+    tsg_f4 vf[4];
+    k.at(a.k + kvh * a.k_head + (long)k0 * a.k_row, b.wave_hi - k0);
+    v.at(a.v + kvh * a.v_head + (long)k0 * a.v_row, b.wave_hi - k0);
+    k.rows(kf);
+    v.cols(vf);
+    tsg_f4 z = over_waves<NW>(meet[buf], dot16(kf, qf, tsg_f4{0.0f, 0.0f, 0.0f, 0.0f}), wave, lane);
+    if (k0 < b.in_lo || k0 + 16 > b.in_hi) {
+      keep_branch();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (k0 + 4 * h + i < lo || k0 + 4 * h + i >= hi) z[i] = -INFINITY;
+    }
+    const float top = parts_max<16>(fmaxf(fmaxf(m, fmaxf(z[0], z[1])), fmaxf(z[2], z[3])));
+    if (__any((top - m) * a.scale2 > 8.0f)) {  // as in attn_fwd_kernel
+      keep_branch();
+      const float fade = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - top) * a.scale2);
+      l *= fade;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] *= fade;
+      m = top;
+    }
+    const float off = m == -INFINITY ? 0.0f : m;
+    // the reference comes off before the scaling: all of z - m's bits, and products of the type's lowest value stay finite
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      z[i] = __builtin_amdgcn_exp2f((z[i] - off) * a.scale2);
+      l += z[i];
+    }
+    add16(acc, vf, z);
+  }
+  l = parts_sum<16>(l);
+  if (t < a.n_q) {
+    store16(acc, a.out + (long)t * a.o_row + head * a.o_head, l == 0.0f ? 0.0f : 1.0f / l, a.dim, wave, h);
+    if (threadIdx.x < 16) a.stat[(long)head * a.n_q + t] = l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l));
+  }
+}
+
+template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_dq_kernel(AttnArgs a) {
+  __shared__ tsg_f4 meet[4][NW][64];
+  __shared__ float meet_delta[NW][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 4;
+  const int tiles = gridDim.x / a.heads;
+  const int t0 = (tiles - 1 - (int)(blockIdx.x / a.heads)) * 16, head = blockIdx.x % a.heads, kvh = head / a.group;
+  const int t = t0 + (lane & 15);
+  tsg_u4 qf[4], gf[4];
+  float delta = 0.0f;
+  {
+    Rows16 q(a.q_row, a.chunks, wave, lane), g(a.do_row, a.chunks, wave, lane), o(a.o_row, a.chunks, wave, lane);
+    q.at(a.q + (long)t0 * a.q_row + head * a.q_head, a.n_q - t0);
+    g.at(a.d_o + (long)t0 * a.do_row + head * a.do_head, a.n_q - t0);
+    o.at(a.o + (long)t0 * a.o_row + head * a.o_head, a.n_q - t0);
+    tsg_u4 of[4];
+    q.rows(qf);
+    g.rows(gf);
+    o.rows(of);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) delta += frag_dot<TsgF32>(of[s], gf[s]);
+  }
+  int lo, hi;
+  keys_of_row(a, t0, t, lo, hi);
+  const Bounds b = wave_bounds<16>(lo, hi);
+  delta = over_waves<NW>(meet_delta, parts_sum<16>(delta), wave, lane);
+  float2 st = make_float2(0.0f, INFINITY);
+  if (t < a.n_q) {
+    st = a.stat[(long)head * a.n_q + t];
+    if (threadIdx.x < 16) a.delta[(long)head * a.n_q + t] = delta;  // the dk / dv kernel, next on the stream, reads it
+  }
+  Sum16 acc;
+  zero16(acc);
+  Rows16 k(a.k_row, a.chunks, wave, lane), v(a.v_row, a.chunks, wave, lane);
+  for (int k0 = b.wave_lo, buf = 0; k0 < b.wave_hi; k0 += 16, buf ^= 2) {
+    tsg_u4 kf[4], vf[4];
+    tsg_f4 kc[4];
+    k.at(a.k + kvh * a.k_head + (long)k0 * a.k_row, b.wave_hi - k0);
+    v.at(a.v + kvh * a.v_head + (long)k0 * a.v_row, b.wave_hi - k0);
+    k.rows(kf);
+    v.rows(vf);
+    k.cols(kc);
+    tsg_f4 z = dot16(kf, qf, tsg_f4{0.0f, 0.0f, 0.0f, 0.0f}), dp = dot16(vf, gf, tsg_f4{0.0f, 0.0f, 0.0f, 0.0f});
+    if (NW > 1) meet[buf][wave][lane] = z;
+    dp = over_waves<NW>(meet[buf + 1], dp, wave, lane);
+    if (NW > 1) {
+      z = meet[buf][0][lane];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) z += meet[buf][w][lane];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i] - st.x, a.scale2, -st.y)) * (dp[i] - delta);
+    if (k0 < b.in_lo || k0 + 16 > b.in_hi) {
+      keep_branch();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (k0 + 4 * h + i < lo || k0 + 4 * h + i >= hi) z[i] = 0.0f;
+    }
+    add16(acc, kc, z);
+  }
+  if (t < a.n_q) store16(acc, a.dq + (long)t * a.dq_row + head * a.dq_head, a.scale, a.dim, wave, h);
+}
+
+template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_dkv_kernel(AttnArgs a) {
+  __shared__ tsg_f4 meet[4][NW][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 4;
+  const int split = blockIdx.x / a.kv_heads % a.n_split, j0 = blockIdx.x / a.kv_heads / a.n_split * 16, kvh = blockIdx.x % a.kv_heads;
+  const int j = j0 + (lane & 15);
+  tsg_u4 kf[4], vf[4];
+  {
+    Rows16 k(a.k_row, a.chunks, wave, lane), v(a.v_row, a.chunks, wave, lane);
+    k.at(a.k + (long)j0 * a.k_row + kvh * a.k_head, a.n_k - j0);
+    v.at(a.v + (long)j0 * a.v_row + kvh * a.v_head, a.n_k - j0);
+    k.rows(kf);
+    v.rows(vf);
+  }
+  int lo, hi;
+  rows_of_key(a, j0, j, lo, hi);
+  const Bounds b = wave_bounds<16>(lo, hi);
+  Sum16 dk, dv;
+  zero16(dk);
+  zero16(dv);
+  const int per = b.wave_lo < b.wave_hi ? (b.wave_hi - b.wave_lo + 15) / 16 : 0, all = per * a.group;
+  const int first = (int)((long)all * split / a.n_split), last = (int)((long)all * (split + 1) / a.n_split);
+  int head = kvh * a.group + (all ? first / per : 0), t0 = b.wave_lo + (all ? first % per : 0) * 16;
+  Rows16 q(a.q_row, a.chunks, wave, lane), g(a.do_row, a.chunks, wave, lane);
+  for (int step = first, buf = 0; step < last; ++step, buf ^= 2) {
+    tsg_u4 qf[4], gf[4];
+    tsg_f4 qc[4], gc[4];
+    q.at(a.q + head * a.q_head + (long)t0 * a.q_row, b.wave_hi - t0);
+    g.at(a.d_o + head * a.do_head + (long)t0 * a.do_row, b.wave_hi - t0);
+    q.rows(qf);
+    g.rows(gf);
+    g.cols(gc);
+    q.cols(qc);
+    float2 st[4];
+    float delta[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long at = (long)head * a.n_q + min(t0 + 4 * h + i, b.wave_hi - 1);  // rows behind the interval are masked below
+      st[i] = a.stat[at];
+      delta[i] = a.delta[at];
+    }
+    tsg_f4 z = dot16(qf, kf, tsg_f4{0.0f, 0.0f, 0.0f, 0.0f}), dp = dot16(gf, vf, tsg_f4{0.0f, 0.0f, 0.0f, 0.0f});
+    if (NW > 1) meet[buf][wave][lane] = z;
+    dp = over_waves<NW>(meet[buf + 1], dp, wave, lane);
+    if (NW > 1) {
+      z = meet[buf][0][lane];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) z += meet[buf][w][lane];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      z[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i] - st[i].x, a.scale2, -st[i].y));
+      dp[i] = z[i] * (dp[i] - delta[i]);
+    }
+    if (t0 < b.in_lo || t0 + 16 > b.in_hi) {
+      keep_branch();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t0 + 4 * h + i < lo || t0 + 4 * h + i >= hi) z[i] = dp[i] = 0.0f;
+    }
+    add16(dv, gc, z);
+    add16(dk, qc, dp);
+    t0 += 16;
+    if (t0 >= b.wave_hi) t0 = b.wave_lo, ++head;
+  }
+  if (j >= a.n_k) return;
+  if (a.n_split > 1) {
+    char* p = reinterpret_cast<char*>(a.part + (((long)split * a.n_k + j) * a.kv_heads + kvh) * a.dim);
+    store16(dk, p, 1.0f, a.dim, wave, h);
+    store16(dv, p + (long)a.n_split * a.n_k * a.kv_heads * a.dim * 4, 1.0f, a.dim, wave, h);
+  } else {
+    store16(dk, a.dk + (long)j * a.dk_row + kvh * a.dk_head, a.scale, a.dim, wave, h);
+    store16(dv, a.dv + (long)j * a.dv_row + kvh * a.dv_head, 1.0f, a.dim, wave, h);
+  }
+}
+
 // dk and dv from the stretches' sums: four elements per thread, blockIdx.y 0: dk, 1: dv
 template <typename D> __global__ __launch_bounds__(256) void attn_dkv_join_kernel(AttnArgs a) {
   const long all = (long)a.n_k * a.kv_heads * a.dim, i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
@@ -917,7 +1178,7 @@ size_t workspace_of(const tsg_attn_desc* d) {
 // 64 rows in the mean; the sums then meet in f32 (4 sequences of 2.5-4 k positions, 16 heads over 4, 128 wide).
 int dkv_splits_of(const tsg_attn_desc* d) {
   if (d->dim > 256 || d->n_seq <= 0) return 1;
-  const int64_t wgs = (int64_t)tsg_cdiv(d->n_k, d->dtype == TSG_F32 ? 64 : 128) * d->kv_heads;
+  const int64_t wgs = (int64_t)tsg_cdiv(d->n_k, d->dtype == TSG_F32 ? 16 : 128) * d->kv_heads;
   const int64_t steps = d->n_q / d->n_seq * (d->heads / d->kv_heads) / 64 / 2;
   int64_t n = wgs ? 1536 / wgs : 1;
   if (n > steps / 8) n = steps / 8;
@@ -1001,6 +1262,11 @@ template <typename D> int forward_of(const tsg_attn_desc* d, hipStream_t s) {
   } else {
     const dim3 grid((unsigned)(tsg_cdiv(a.n_q, rows_per_wg<D>()) * a.heads)), block(256);
     constexpr int BK = TsgElem<D>::BYTES == 4 ? 32 : 64;
+    if constexpr (__is_same(D, TsgF32)) {
+      if (a.dim <= 64) hipLaunchKernelGGL(attn_f32_fwd_kernel<1>, grid, dim3(64), 0, s, a);
+      else if (a.dim <= 128) hipLaunchKernelGGL(attn_f32_fwd_kernel<2>, grid, dim3(128), 0, s, a);
+      else hipLaunchKernelGGL(attn_f32_fwd_kernel<4>, grid, dim3(256), 0, s, a);
+    } else
     if (a.dim <= 64) hipLaunchKernelGGL((attn_fwd_kernel<D, 64, 64>), grid, block, 0, s, a);
     else if (a.dim <= 128) hipLaunchKernelGGL((attn_fwd_kernel<D, 128, BK>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((attn_fwd_kernel<D, 256, BK / 2>), grid, block, 0, s, a);
@@ -1021,13 +1287,23 @@ template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
   }
   constexpr int R = rows_per_wg<D>();
   const dim3 gq((unsigned)(tsg_cdiv(a.n_q, R) * a.heads)), gk((unsigned)(tsg_cdiv(a.n_k, R) * a.kv_heads * a.n_split));
-  constexpr bool F32 = TsgElem<D>::BYTES == 4;
+  constexpr bool F32 = __is_same(D, TsgF32);
   if (a.n_q) {
+    if constexpr (F32) {
+      if (a.dim <= 64) hipLaunchKernelGGL(attn_f32_dq_kernel<1>, gq, dim3(64), 0, s, a);
+      else if (a.dim <= 128) hipLaunchKernelGGL(attn_f32_dq_kernel<2>, gq, dim3(128), 0, s, a);
+      else hipLaunchKernelGGL(attn_f32_dq_kernel<4>, gq, dim3(256), 0, s, a);
+    } else
     if (a.dim <= 64) hipLaunchKernelGGL((attn_dq_kernel<D, 64, 64>), gq, block, 0, s, a);
     else if (a.dim <= 128) hipLaunchKernelGGL((attn_dq_kernel<D, 128, F32 ? 32 : 64>), gq, block, 0, s, a);
     else hipLaunchKernelGGL((attn_dq_kernel<D, 256, F32 ? 16 : 32>), gq, block, 0, s, a);
   }
   if (a.n_k) {
+    if constexpr (F32) {
+      if (a.dim <= 64) hipLaunchKernelGGL(attn_f32_dkv_kernel<1>, gk, dim3(64), 0, s, a);
+      else if (a.dim <= 128) hipLaunchKernelGGL(attn_f32_dkv_kernel<2>, gk, dim3(128), 0, s, a);
+      else hipLaunchKernelGGL(attn_f32_dkv_kernel<4>, gk, dim3(256), 0, s, a);
+    } else
     if (a.dim <= 64) hipLaunchKernelGGL((attn_dkv_kernel<D, 64, 32, 0, false>), gk, block, 0, s, a);
     else if (a.dim <= 128)
       hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0, !F32>), gk, block, 0, s, a);
