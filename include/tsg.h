@@ -584,6 +584,7 @@ typedef struct tsg_xent_desc {
   float* row_loss;           /* [n_rows] out */
   float* loss;               /* [1] out, reduction 1 and 2 */
   float* stats;              /* [n_rows][2], 8-byte aligned: written by the forward, read by the backward */
+  float* scales;             /* [2], f32 only (else NULL): likewise */
   void* workspace;
   size_t workspace_bytes;
   const float* d_loss;       /* backward only from here on */

@@ -74,7 +74,7 @@ def test_attention_backward_descriptor():
 def _xent(entry='tsg_xent_forward', **kw):
     d = _lib.XentDesc()
     d.dtype, d.hidden, d.reduction, d.n_rows, d.n_vocab, d.ignore_index = 0, 64, 2, 10, 100, -100
-    for n in ('h', 'w', 'bias', 'target', 'row_loss', 'loss', 'stats', 'd_loss', 'dh', 'dw', 'dbias', 'workspace'):
+    for n in ('h', 'w', 'bias', 'target', 'row_loss', 'loss', 'stats', 'scales', 'd_loss', 'dh', 'dw', 'dbias', 'workspace'):
         setattr(d, n, 4096)
     d.h_row = d.w_row = d.dh_row = d.dw_row = 64
     for k, v in kw.items():
@@ -85,7 +85,7 @@ def _xent(entry='tsg_xent_forward', **kw):
 @pytest.mark.parametrize('kw,rc', [
     (dict(dtype=3), -1), (dict(hidden=0), -1), (dict(hidden=60), -1), (dict(reduction=3), -1), (dict(n_rows=0), -1),
     (dict(n_rows=-1), -1), (dict(n_vocab=0), -1), (dict(n_rows=1 << 31), -3), (dict(n_vocab=1 << 31), -3), (dict(h=None), -1),
-    (dict(w=None), -1), (dict(target=None), -1), (dict(stats=None), -1), (dict(row_loss=None), -1), (dict(loss=None), -1),
+    (dict(w=None), -1), (dict(target=None), -1), (dict(stats=None), -1), (dict(row_loss=None), -1), (dict(loss=None), -1), (dict(scales=None), -1),
     (dict(h=4100), -1), (dict(h_row=56), -1), (dict(w_row=66), -1), (dict(workspace=None), -2), (dict(workspace_bytes=8), -2)])
 def test_cross_entropy_descriptor(kw, rc):
     assert _xent(**kw) == rc

@@ -125,7 +125,7 @@ class XentDesc(C.Structure):
     _fields_ = [('dtype', _i32), ('hidden', _i32), ('reduction', _i32), ('reserved', _i32), ('n_rows', C.c_int64),
                 ('n_vocab', C.c_int64), ('ignore_index', C.c_int64), ('h', _p), ('w', _p), ('bias', _p),
                 ('h_row', C.c_int64), ('w_row', C.c_int64), ('target', _p), ('row_loss', _p), ('loss', _p), ('stats', _p),
-                ('workspace', _p), ('workspace_bytes', _sz), ('d_loss', _p), ('dh', _p), ('dw', _p), ('dbias', _p),
+                ('scales', _p), ('workspace', _p), ('workspace_bytes', _sz), ('d_loss', _p), ('dh', _p), ('dw', _p), ('dbias', _p),
                 ('dh_row', C.c_int64), ('dw_row', C.c_int64)]
 
 

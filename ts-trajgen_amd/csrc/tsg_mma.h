@@ -69,6 +69,7 @@ template <> __device__ __forceinline__ void tsg_mma<TsgF32>(tsg_u4 a, tsg_u4 b, 
 template <int CH, bool F32 = false> __device__ __forceinline__ int tsg_swz(int r) {
   if (F32) return r & 15;
   if (CH >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+  if (CH == 4) return (r >> 2) & 3;
   return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
 }
 

@@ -21,12 +21,10 @@
 
 namespace {
 
-constexpr int TM = 128, TN = 128, TK = 64;  // tile of a workgroup: four waves of 64 x 64
-
-struct XentScales {   // device words of the workspace
-  unsigned amax_h, amax_w, gmax;  // bits of the largest magnitudes (non-negative floats order like their bits)
-  float count;        // rows that are not left out
-};
+#ifndef V_TK
+#define V_TK 64
+#endif
+constexpr int TM = 128, TN = 128, TK = V_TK;  // tile of a workgroup: four waves of 64 x 64
 
 // 2^(15 - e) for 2^(e-1) <= v < 2^e: brings the largest magnitude into [2^14, 2^15)
 __device__ __forceinline__ float scale_of(unsigned bits) {
@@ -49,7 +47,8 @@ struct XentArgs {
   long ignore;
   int rows, hidden, vocab;
   int v0, vc;                   // this piece of the vocabulary
-  XentScales* sc;
+  const float* scales;          // f32: what h and w were multiplied by
+  unsigned* gmax;               // backward: bits of the largest |g|
   float2* part;                 // forward: [vocab tiles][rows]
   float* zt;                    // forward: [rows] the target's logit
   float2* stat;                 // [rows] maximum, log2 of the sum
@@ -97,7 +96,7 @@ __device__ __forceinline__ void product(tsg_f32x16 (&acc)[2][2], char* lds, cons
     }
     if (AC) al.load(ap + (long)k0 * a.row, a.rows - k0, a.cols * 2, buf * 2 * TILE);
     else al.load(ap + k0 * 2, a.rows, min(a.cols - k0, TK) * 2, buf * 2 * TILE);
-    if (BC && MASKED) bl.load(bp + (long)k0 * b.row, b.rows - k0, b.cols * 2, buf * 2 * TILE, b.used[k0 / TK]);
+    if (BC && MASKED) bl.load(bp + (long)k0 * b.row, b.rows - k0, b.cols * 2, buf * 2 * TILE, b.used[k0 / 64] >> (k0 % 64));
     else if (BC) bl.load(bp + (long)k0 * b.row, b.rows - k0, b.cols * 2, buf * 2 * TILE);
     else bl.load(bp + k0 * 2, b.rows, min(b.cols - k0, TK) * 2, buf * 2 * TILE);
     if (!AC || !BC) {
@@ -162,7 +161,7 @@ template <typename D> __device__ __forceinline__ void logits(const XentArgs& a, 
   const Operand B = {a.h + (long)n0 * a.h_row, a.h_row, a.h_plane, a.rows - n0, a.hidden, nullptr};
   product<D, false, false>(acc, lds, A, B, a.hidden, split ? 3 : 1, wave, lane);
   const int h = lane >> 5, wm = (wave >> 1) * 64;
-  const float by = split ? 1.0f / (scale_of(a.sc->amax_h) * scale_of(a.sc->amax_w)) : 1.0f;
+  const float by = split ? 1.0f / (a.scales[0] * a.scales[1]) : 1.0f;
 #pragma unroll
   for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -294,23 +293,23 @@ __global__ __launch_bounds__(1024) void xent_grad_kernel(XentArgs a, const float
   __syncthreads();
   if (threadIdx.x) return;
   for (int w = 1; w < 16; ++w) m = fmaxf(m, top[w]);
-  a.sc->gmax = __float_as_uint(m);
+  *a.gmax = __float_as_uint(m);
 }
 
-template <typename D>
+template <typename D, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void xent_dz_kernel(XentArgs a, int tiles_m, int tiles_n) {
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TM * TK * 2 + 2 * 16 * TM];
+  __shared__ __attribute__((aligned(1024))) char lds[SPLIT || TK == 64 ? 4 * TM * 64 * 2 + 2 * 16 * TM : TN * (TM * 2 + 16)];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
   int tm, tn;
   tile_of(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
-  const bool split = a.h_plane != 0;
+  constexpr bool split = SPLIT;
   const int m0 = a.v0 + tm * TM;
   tsg_f32x16 z[2][2];
   logits<D>(a, z, lds, m0, tn * TN, wave, lane, split);
   const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
   // rows of 128 entries, 16 bytes of padding: [128 states][272 bytes], hi and (f32) lo
   constexpr int ROW = TM * 2 + 16, PLANE = TN * ROW;
-  const float gs = __is_same(D, TsgBf16) ? 1.0f : scale_of(a.sc->gmax);
+  const float gs = __is_same(D, TsgBf16) ? 1.0f : scale_of(*a.gmax);
 #pragma unroll
   for (int y = 0; y < 2; ++y) {
     const int n = wn + 32 * y + (lane & 31), t = tn * TN + n;
@@ -394,8 +393,8 @@ __global__ __launch_bounds__(256, 2) void xent_dw_kernel(XentArgs a, int tiles_m
   const Operand A = {a.dz + (long)tm * TM * 2, a.ldz * 2, a.dz_plane, a.rows, (int)a.ldz - tm * TM, nullptr};
   const Operand B = {a.h + (long)tn * TN * 2, a.h_row, a.h_plane, a.rows, a.hidden - tn * TN, a.used};
   product<D, true, true, true>(acc, lds, A, B, a.rows, split ? 3 : 1, wave, lane);
-  float by = __is_same(D, TsgBf16) ? 1.0f : 1.0f / scale_of(a.sc->gmax);
-  if (split) by /= scale_of(a.sc->amax_h);
+  float by = __is_same(D, TsgBf16) ? 1.0f : 1.0f / scale_of(*a.gmax);
+  if (split) by /= a.scales[0];
   const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
 #pragma unroll
   for (int x = 0; x < 2; ++x)
@@ -448,8 +447,8 @@ __global__ __launch_bounds__(256) void xent_dh_out_kernel(XentArgs a, OUT* dh, l
   if (i >= n) return;
   float s = 0.0f;
   for (int p = 0; p < a.splits; ++p) s += a.dh_part[p * n + i];
-  if (scaled) s /= scale_of(a.sc->gmax);
-  if (a.h_plane) s /= scale_of(a.sc->amax_w);
+  if (scaled) s /= scale_of(*a.gmax);
+  if (a.h_plane) s /= a.scales[1];
   dh[(i / a.hidden) * dh_row + i % a.hidden] = (OUT)s;
 }
 
@@ -458,49 +457,74 @@ template <typename OUT> __global__ __launch_bounds__(256) void xent_db_out_kerne
   if (v >= a.vc) return;
   float s = 0.0f;
   for (int t = 0; t < tiles_n; ++t) s += a.db_part[(long)t * a.vc + v];
-  if (scaled) s /= scale_of(a.sc->gmax);
+  if (scaled) s /= scale_of(*a.gmax);
   db[a.v0 + v] = (OUT)s;
 }
 
 // ---- f32 operands: largest magnitudes, then the two planes
-__global__ void xent_init_kernel(XentScales* s) { s->amax_h = s->amax_w = s->gmax = 0u, s->count = 0.0f; }
-
 __device__ __forceinline__ float4 row4(const float* x, long row, long i, int chunks) {
   return *reinterpret_cast<const float4*>(x + (i / chunks) * row + (i % chunks) * 4);
 }
-// blocks [0, hb): h (without the rows left out, which may hold anything), the others: w
-__global__ __launch_bounds__(256) void xent_amax_kernel(const float* h, long h_row, long n_h, const float* w, long w_row, long n_w, int chunks, int hb, XentScales* sc,
-                                                        const long* target, long ignore) {
-  const bool first = (int)blockIdx.x < hb;
-  const float* x = first ? h : w;
-  const long row = first ? h_row : w_row, n = (first ? n_h : n_w) * chunks;
-  const long b = first ? blockIdx.x : blockIdx.x - hb, nb = first ? hb : gridDim.x - hb;
+struct Planes {
+  const float *h, *w;
+  long h_row, n_h, w_row, n_w;
+  int chunks, hb, wb;  // blocks [0, hb): h, hb + [0, wb): w
+  float* amax;         // [hb + wb] a maximum per block
+  const long* target;
+  long ignore;
+  char *hp, *wp;
+  long h_plane, w_plane;
+  float* scales;       // [2] the two scales, for the products and for the backward
+};
+__device__ __forceinline__ float block_max(float m, float* shared) {
+  m = tsg_wave_max(m);
+  if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = m;
+  __syncthreads();
+  return fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
+}
+// rows of h that are left out may hold anything: they have no say
+__global__ __launch_bounds__(256) void xent_amax_kernel(Planes a) {
+  __shared__ float join[4];
+  const bool first = (int)blockIdx.x < a.hb;
+  const float* x = first ? a.h : a.w;
+  const long row = first ? a.h_row : a.w_row, n = (first ? a.n_h : a.n_w) * a.chunks;
+  const long b = first ? blockIdx.x : blockIdx.x - a.hb, nb = first ? a.hb : a.wb;
   float m = 0.0f;
   for (long i = b * 256 + threadIdx.x; i < n; i += nb * 256) {
-    if (first && target[i / chunks] == ignore) continue;
-    const float4 v = row4(x, row, i, chunks);
+    if (first && a.target[i / a.chunks] == a.ignore) continue;
+    const float4 v = row4(x, row, i, a.chunks);
     m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
   }
-  m = tsg_wave_max(m);
-  if ((threadIdx.x & 63) == 0) atomicMax(first ? &sc->amax_h : &sc->amax_w, __float_as_uint(m));  // a maximum: any order
+  m = block_max(m, join);
+  if (threadIdx.x == 0) a.amax[blockIdx.x] = m;
 }
-__global__ __launch_bounds__(256) void xent_planes_kernel(const float* h, long h_row, long n_h, const float* w, long w_row, long n_w, int chunks, int hb, const XentScales* sc,
-                                                          char* hp, long h_plane, char* wp, long w_plane) {
-  const bool first = (int)blockIdx.x < hb;
-  const float* x = first ? h : w;
-  const long row = first ? h_row : w_row, n = (first ? n_h : n_w) * chunks;
-  const long b = first ? blockIdx.x : blockIdx.x - hb, nb = first ? hb : gridDim.x - hb;
-  char* out = first ? hp : wp;
-  const long plane = first ? h_plane : w_plane;
-  const float by = scale_of(first ? sc->amax_h : sc->amax_w);
+// forward: the scales from the blocks' maxima (every block joins them itself); backward (amax null): as the forward left them
+__global__ __launch_bounds__(256) void xent_planes_kernel(Planes a) {
+  __shared__ float join[4];
+  const bool first = (int)blockIdx.x < a.hb;
+  const float* x = first ? a.h : a.w;
+  const long row = first ? a.h_row : a.w_row, n = (first ? a.n_h : a.n_w) * a.chunks;
+  const long b = first ? blockIdx.x : blockIdx.x - a.hb, nb = first ? a.hb : a.wb;
+  char* out = first ? a.hp : a.wp;
+  const long plane = first ? a.h_plane : a.w_plane;
+  float by;
+  if (a.amax) {
+    const float* from = a.amax + (first ? 0 : a.hb);
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < nb; i += 256) m = fmaxf(m, from[i]);
+    by = scale_of(__float_as_uint(block_max(m, join)));
+    if (b == 0 && threadIdx.x == 0) a.scales[first ? 0 : 1] = by;
+  } else {
+    by = a.scales[first ? 0 : 1];
+  }
   for (long i = b * 256 + threadIdx.x; i < n; i += nb * 256) {
-    const float4 v = row4(x, row, i, chunks);
-    const float a[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
+    const float4 v = row4(x, row, i, a.chunks);
+    const float s[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
     float r[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = a[e] - (float)(_Float16)a[e];
+    for (int e = 0; e < 4; ++e) r[e] = s[e] - (float)(_Float16)s[e];
     uint2 hi, lo;
-    hi.x = tsg_pack2<TsgF16>(a[0], a[1]), hi.y = tsg_pack2<TsgF16>(a[2], a[3]);
+    hi.x = tsg_pack2<TsgF16>(s[0], s[1]), hi.y = tsg_pack2<TsgF16>(s[2], s[3]);
     lo.x = tsg_pack2<TsgF16>(r[0], r[1]), lo.y = tsg_pack2<TsgF16>(r[2], r[3]);
     *reinterpret_cast<uint2*>(out + i * 8) = hi;
     *reinterpret_cast<uint2*>(out + plane + i * 8) = lo;
@@ -509,13 +533,14 @@ __global__ __launch_bounds__(256) void xent_planes_kernel(const float* h, long h
 
 // ------------------------------------------------------------------------------------------------------ host side
 struct Layout {
-  size_t scales, planes, h_plane, w_plane, part, zt, g, used, dz, dz_plane, db, dh, total;
+  size_t gmax, amax, planes, h_plane, w_plane, part, zt, g, used, dz, dz_plane, db, dh, total;
   int vc, splits, split_len;
 };
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // dz of a piece takes at most `budget` bytes (but 128 vocabulary rows at least): large pieces fill the chip, small ones keep
 // the workspace small.
+constexpr int PLANE_BLOCKS = 512;
 constexpr size_t DZ_BUDGET = (size_t)1 << 30;
 
 Layout layout_of(const tsg_xent_desc* d, bool backward) {
@@ -528,8 +553,9 @@ Layout layout_of(const tsg_xent_desc* d, bool backward) {
     at += up256(n);
     return p;
   };
-  l.scales = take(sizeof(XentScales));
+  l.gmax = take(4);
   if (f32) {
+    l.amax = take(2 * PLANE_BLOCKS * 4);
     l.h_plane = up256(T * K * 2), l.w_plane = up256(V * K * 2);
     l.planes = take(2 * (l.h_plane + l.w_plane));
   }
@@ -553,7 +579,7 @@ Layout layout_of(const tsg_xent_desc* d, bool backward) {
     l.db = d->bias ? take((size_t)tsg_cdiv(T, TN) * vc * 4) : 0;
     const size_t tiles = (size_t)tsg_cdiv(T, TM) * tsg_cdiv(K, TN);
     size_t s = (512 + tiles - 1) / tiles;  // two workgroups a CU
-    if (s > vc / 512) s = vc / 512;
+    if (s > vc / TM) s = vc / TM;
     if (s < 1) s = 1;
     l.split_len = (int)(((vc + s - 1) / s + TK - 1) / TK * TK);
     l.splits = (int)((vc + l.split_len - 1) / l.split_len);
@@ -577,6 +603,7 @@ int check_xent(const tsg_xent_desc* d, bool backward) {
   if (d->h_row * 4 >= (1 << 23) || d->w_row * 4 >= (1 << 23)) return TSG_E_LIMIT;  // offsets inside a tile are 32-bit
   if (!backward && !d->row_loss) return TSG_E_INVALID;
   if (!backward && d->reduction && !d->loss) return TSG_E_INVALID;
+  if (d->dtype == TSG_F32 && !d->scales) return TSG_E_INVALID;
   if (backward && (!d->d_loss || !d->dh || !d->dw || (d->bias && !d->dbias))) return TSG_E_INVALID;
   if (backward && (d->dh_row < d->hidden || d->dw_row < d->hidden)) return TSG_E_INVALID;
   return 0;
@@ -586,7 +613,8 @@ XentArgs args_of(const tsg_xent_desc* d, const Layout& l) {
   XentArgs a = {};
   char* ws = (char*)d->workspace;
   const bool f32 = d->dtype == TSG_F32;
-  a.sc = (XentScales*)(ws + l.scales);
+  a.gmax = (unsigned*)(ws + l.gmax);
+  a.scales = d->scales;
   if (f32) {
     a.h = ws + l.planes, a.h_plane = (long)l.h_plane, a.h_row = d->hidden * 2L;
     a.w = ws + l.planes + 2 * l.h_plane, a.w_plane = (long)l.w_plane, a.w_row = d->hidden * 2L;
@@ -601,17 +629,22 @@ XentArgs args_of(const tsg_xent_desc* d, const Layout& l) {
   return a;
 }
 
-void make_planes(const tsg_xent_desc* d, const XentArgs& a, hipStream_t s) {
-  const int chunks = d->hidden / 4;
+void make_planes(const tsg_xent_desc* d, const XentArgs& a, const Layout& l, bool backward, hipStream_t s) {
+  Planes p;
+  p.h = (const float*)d->h, p.w = (const float*)d->w, p.h_row = d->h_row, p.w_row = d->w_row, p.n_h = d->n_rows, p.n_w = d->n_vocab;
+  p.chunks = d->hidden / 4;
   auto blocks = [&](int64_t n) {
-    const int64_t b = (n * chunks + 1023) / 1024;
-    return (int)(b > 1024 ? 1024 : b);
+    const int64_t b = (n * p.chunks + 1023) / 1024;
+    return (int)(b > PLANE_BLOCKS ? PLANE_BLOCKS : b);
   };
-  const int hb = blocks(d->n_rows), wb = blocks(d->n_vocab);
-  hipLaunchKernelGGL(xent_amax_kernel, dim3(hb + wb), dim3(256), 0, s, (const float*)d->h, (long)d->h_row, (long)d->n_rows, (const float*)d->w, (long)d->w_row,
-                     (long)d->n_vocab, chunks, hb, a.sc, a.target, a.ignore);
-  hipLaunchKernelGGL(xent_planes_kernel, dim3(hb + wb), dim3(256), 0, s, (const float*)d->h, (long)d->h_row, (long)d->n_rows, (const float*)d->w, (long)d->w_row,
-                     (long)d->n_vocab, chunks, hb, (const XentScales*)a.sc, (char*)a.h, a.h_plane, (char*)a.w, a.w_plane);
+  p.hb = blocks(p.n_h), p.wb = blocks(p.n_w);
+  p.amax = backward ? nullptr : (float*)((char*)d->workspace + l.amax);
+  p.target = (const long*)d->target, p.ignore = d->ignore_index;
+  p.hp = (char*)a.h, p.wp = (char*)a.w, p.h_plane = a.h_plane, p.w_plane = a.w_plane;
+  p.scales = d->scales;
+  const dim3 grid((unsigned)(p.hb + p.wb));
+  if (!backward) hipLaunchKernelGGL(xent_amax_kernel, grid, dim3(256), 0, s, p);
+  hipLaunchKernelGGL(xent_planes_kernel, grid, dim3(256), 0, s, p);
 }
 
 template <typename D> void launch_stat(const XentArgs& a, int tm, int tn, hipStream_t s) {
@@ -621,7 +654,7 @@ template <typename D> void launch_stat(const XentArgs& a, int tm, int tn, hipStr
 template <typename D, typename OUT> void backward_piece(XentArgs a, const tsg_xent_desc* d, const Layout& l, hipStream_t s) {
   const int tv = tsg_cdiv(a.vc, TM), tt = tsg_cdiv(a.rows, TN), tk = tsg_cdiv(a.hidden, TN);
   const int scaled = !__is_same(D, TsgBf16);
-  hipLaunchKernelGGL(xent_dz_kernel<D>, dim3((unsigned)(tv * tt)), dim3(256), 0, s, a, tv, tt);
+  hipLaunchKernelGGL((xent_dz_kernel<D, __is_same(OUT, float)>), dim3((unsigned)(tv * tt)), dim3(256), 0, s, a, tv, tt);
   hipLaunchKernelGGL((xent_dw_kernel<D, OUT>), dim3((unsigned)(tv * tk)), dim3(256), 0, s, a, tv, tk);
   hipLaunchKernelGGL(xent_dh_kernel<D>, dim3((unsigned)(tt * tk * l.splits)), dim3(256), 0, s, a, tt, tk);
   if (d->bias) hipLaunchKernelGGL(xent_db_out_kernel<OUT>, dim3(tsg_cdiv(a.vc, 256)), dim3(256), 0, s, a, (OUT*)d->dbias, tt, scaled);
@@ -648,10 +681,7 @@ extern "C" int tsg_xent_forward(const tsg_xent_desc* d, void* stream) {
   XentArgs a = args_of(d, l);
   a.part = (float2*)((char*)d->workspace + l.part);
   a.zt = (float*)((char*)d->workspace + l.zt);
-  if (d->dtype == TSG_F32) {
-    hipLaunchKernelGGL(xent_init_kernel, dim3(1), dim3(1), 0, s, a.sc);
-    make_planes(d, a, s);
-  }
+  if (d->dtype == TSG_F32) make_planes(d, a, l, false, s);
   const int tm = tsg_cdiv(a.vocab, TM), tn = tsg_cdiv(a.rows, TN);
   if (d->dtype == TSG_BF16) launch_stat<TsgBf16>(a, tm, tn, s);
   else launch_stat<TsgF16>(a, tm, tn, s);
@@ -678,8 +708,7 @@ extern "C" int tsg_xent_backward(const tsg_xent_desc* d, void* stream) {
   a.splits = l.splits, a.split_len = l.split_len;
   a.dw = (char*)d->dw, a.dw_row = d->dw_row * (d->dtype == TSG_F32 ? 4 : 2);
   a.ldz = l.vc;
-  hipLaunchKernelGGL(xent_init_kernel, dim3(1), dim3(1), 0, s, a.sc);
-  if (d->dtype == TSG_F32) make_planes(d, a, s);
+  if (d->dtype == TSG_F32) make_planes(d, a, l, true, s);
   hipLaunchKernelGGL(xent_grad_kernel, dim3(1), dim3(1024), 0, s, a, d->d_loss, d->reduction);
   for (int64_t v0 = 0; v0 < d->n_vocab; v0 += l.vc) {
     a.v0 = (int)v0;

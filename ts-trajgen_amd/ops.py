@@ -283,13 +283,13 @@ def _rows_for(x, wide):
     return x.clone(memory_format=torch.contiguous_format)
 
 
-def _xent_desc(h, w, bias, target, ignore, reduction, stats):
+def _xent_desc(h, w, bias, target, ignore, reduction, stats, scales):
     d = _lib.XentDesc()
     d.dtype, d.hidden, d.reduction = DTYPES[h.dtype], h.shape[1], reduction
     d.n_rows, d.n_vocab, d.ignore_index = h.shape[0], w.shape[0], ignore
     d.h, d.w, d.bias = _lib.ptr(h), _lib.ptr(w), _lib.ptr(bias)
     d.h_row, d.w_row = max(h.stride(0), h.shape[1]), max(w.stride(0), w.shape[1])
-    d.target, d.stats = _lib.ptr(target), _lib.ptr(stats)
+    d.target, d.stats, d.scales = _lib.ptr(target), _lib.ptr(stats), _lib.ptr(scales)
     return d
 
 
@@ -311,26 +311,27 @@ class _LinearCrossEntropy(torch.autograd.Function):
         stats = torch.empty((h.shape[0], 2), dtype=torch.float32, device=h.device)
         rows = torch.empty(h.shape[0], dtype=torch.float32, device=h.device)
         loss = rows if reduction == 0 else torch.empty((), dtype=torch.float32, device=h.device)
-        d = _xent_desc(hl, wl, bl, target, ignore, reduction, stats)
+        scales = torch.empty(2, dtype=torch.float32, device=h.device) if h.dtype == torch.float32 else None
+        d = _xent_desc(hl, wl, bl, target, ignore, reduction, stats, scales)
         d.row_loss, d.loss = _lib.ptr(rows), _lib.ptr(loss)
         ws = _xent_workspace(d, h.device, 0)
         with torch.cuda.device(h.device):
             _lib.check(_lib.lib().tsg_xent_forward(C.byref(d), _lib.current_stream()), 'tsg_xent_forward')
         del ws
         if any(ctx.needs_input_grad[:3]):
-            ctx.save_for_backward(h, w, bias, target, stats)
+            ctx.save_for_backward(h, w, bias, target, stats, scales)
             ctx.cfg = (ignore, reduction)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss):
-        h, w, bias, target, stats = ctx.saved_tensors
+        h, w, bias, target, stats, scales = ctx.saved_tensors
         width, wide = h.shape[1], -(-h.shape[1] // 8) * 8
         hl, wl = _rows_for(h.detach(), wide), _rows_for(w.detach(), wide)
         bl = None if bias is None else bias.detach().contiguous()
         d_loss = d_loss.contiguous().float()
-        d = _xent_desc(hl, wl, bl, target, ctx.cfg[0], ctx.cfg[1], stats)
+        d = _xent_desc(hl, wl, bl, target, ctx.cfg[0], ctx.cfg[1], stats, scales)
         dh = torch.empty((h.shape[0], wide), dtype=h.dtype, device=h.device)
         dw = torch.empty((w.shape[0], wide), dtype=h.dtype, device=h.device)
         db = None if bias is None else torch.empty_like(bl)
