@@ -397,9 +397,9 @@ def test_cross_entropy_of_sharp_and_flat_rows(dt):
 
 @pytest.mark.parametrize('dt', TYPES)
 def test_cross_entropy_several_pieces(dt, monkeypatch):
-    # 20000 rows: 2^30 bytes of dz are a piece of 26752 (16-bit) or 13312 (f32) entries
+    # 40000 rows: 2^31 bytes of dz are a piece of 26624 (16-bit) or 13312 (f32) entries
     g = torch.Generator(device=DEV).manual_seed(1)
-    t, v, k = 20000, 27000, 16
+    t, v, k = 40000, 27000, 16
     from ts_trajgen_amd import ops
     h = torch.randn(t, k, generator=g, device=DEV).to(dt).requires_grad_(True)
     w = (torch.randn(v, k, generator=g, device=DEV) * 0.3).to(dt).requires_grad_(True)

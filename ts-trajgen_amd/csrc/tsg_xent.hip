@@ -19,12 +19,21 @@
 // All sums, maxima and logarithms are f32.  Nothing depends on the order of workgroups: no floating-point atomics.
 #include "tsg_mma.h"
 
+#include <type_traits>
+
 namespace {
 
-#ifndef V_TK
-#define V_TK 64
-#endif
-constexpr int TM = 128, TN = 128, TK = V_TK;  // tile of a workgroup: four waves of 64 x 64
+constexpr int TK = 64;  // k of one step
+// A workgroup's tile: WM x WN waves of XM x XN products of 32 x 32
+template <int XM_, int XN_, int WM_, int WN_> struct Tile {
+  static constexpr int XM = XM_, XN = XN_, WM = WM_, WN = WN_, WAVES = WM * WN, TM = 32 * XM * WM, TN = 32 * XN * WN;
+  static constexpr int A = TM * TK * 2, STAGE = (TM + TN) * TK * 2;  // bytes of one step's tiles
+};
+// 256 x 256 reads half as much per product from the L2 as 128 x 128 (which the L2's rate bounds at about 900 TFLOP/s), but needs two
+// rounds of tiles for the 256 CUs; 64 x 64 is for the products of a few rows, where the chip would otherwise stand empty.
+typedef Tile<4, 2, 2, 4> Big;
+typedef Tile<2, 2, 2, 2> Mid;
+typedef Tile<1, 1, 2, 2> Few;
 
 // 2^(15 - e) for 2^(e-1) <= v < 2^e: brings the largest magnitude into [2^14, 2^15)
 __device__ __forceinline__ float scale_of(unsigned bits) {
@@ -42,7 +51,6 @@ struct XentArgs {
   long h_row, w_row;            // bytes
   long h_plane, w_plane;        // bytes from hi to lo; 0 for 16-bit types
   const char* bias;             // in the caller's type, or null
-  int bias_f32;
   const long* target;
   long ignore;
   int rows, hidden, vocab;
@@ -72,38 +80,36 @@ struct Operand {
 
 // acc[m][n] += A B over k in [0, K): AC / BC: the operand's memory rows are k.  passes: 1, or 3 with two planes each.
 // MASKED: B's memory rows are read as zeros where its `used` bit is clear.
-template <typename D, bool AC, bool BC, bool MASKED = false>
-__device__ __forceinline__ void product(tsg_f32x16 (&acc)[2][2], char* lds, const Operand& a, const Operand& b, int K, int passes, int wave, int lane) {
-  constexpr int TILE = TM * TK * 2;
+template <typename T> using Acc = tsg_f32x16[T::XM][T::XN];
+template <typename D, typename T, bool AC, bool BC, bool MASKED = false>
+__device__ __forceinline__ void product(Acc<T>& acc, char* lds, const Operand& a, const Operand& b, int K, int passes, int wave, int lane) {
   const int per = (K + TK - 1) / TK, steps = per * passes;
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  // a wave's 64 rows or columns: rows lie 128 bytes apart, columns 2
-  const unsigned a0 = tsg_lds_addr(lds) + (AC ? TsgLane<D, TM / 8>::col_in_order(lane) ^ (wm * 2) : TsgLane<D, TK / 8>::row(lane) + wm * TK * 2);
-  const unsigned b0 = tsg_lds_addr(lds) + TILE + (BC ? TsgLane<D, TN / 8>::col_in_order(lane) ^ (wn * 2) : TsgLane<D, TK / 8>::row(lane) + wn * TK * 2);
-  TsgLoader<AC ? TK : TM, (AC ? TM : TK) / 8, 4> al;
-  TsgLoader<BC ? TK : TN, (BC ? TN : TK) / 8, 4> bl;
+  const int wm = wave / T::WN * 32 * T::XM, wn = wave % T::WN * 32 * T::XN;
+  // a wave's rows or columns: rows lie 128 bytes apart, columns 2
+  const unsigned a0 = tsg_lds_addr(lds) + (AC ? TsgLane<D, T::TM / 8>::col_in_order(lane) ^ (wm * 2) : TsgLane<D, TK / 8>::row(lane) + wm * TK * 2);
+  const unsigned b0 = tsg_lds_addr(lds) + T::A + (BC ? TsgLane<D, T::TN / 8>::col_in_order(lane) ^ (wn * 2) : TsgLane<D, TK / 8>::row(lane) + wn * TK * 2);
+  TsgLoader<AC ? TK : T::TM, (AC ? T::TM : TK) / 8, T::WAVES> al;
+  TsgLoader<BC ? TK : T::TN, (BC ? T::TN : TK) / 8, T::WAVES> bl;
   // a tile whose memory rows are k is as wide as the operand is; one whose columns are k ends where k ends (its last step: below)
-  al.init(a.row, AC ? a.cols / 8 : TK / 8, tsg_lds_addr(lds), wave, lane);
-  bl.init(b.row, BC ? b.cols / 8 : TK / 8, tsg_lds_addr(lds) + TILE, wave, lane);
+  const unsigned at0 = tsg_lds_addr(lds), bt0 = tsg_lds_addr(lds) + T::A;
+  al.init(a.row, AC ? a.cols / 8 : TK / 8, at0, wave, lane);
+  bl.init(b.row, BC ? b.cols / 8 : TK / 8, bt0, wave, lane);
   auto fetch = [&](int pass, int k0, int buf) {
     const char* ap = a.p + (pass == 2 ? a.plane : 0);
     const char* bp = b.p + (pass == 1 ? b.plane : 0);
-    if (!AC || !BC) {
-      if (K - k0 < TK && K % TK) {  // the last, narrower step
-        if (!AC) al.init(a.row, (a.cols - k0) / 8, tsg_lds_addr(lds), wave, lane);
-        if (!BC) bl.init(b.row, (b.cols - k0) / 8, tsg_lds_addr(lds) + TILE, wave, lane);
-      }
+    const bool narrow = (!AC || !BC) && K - k0 < TK;  // the last step of a K that is no multiple of 64
+    if (narrow) {
+      if (!AC) al.init(a.row, (a.cols - k0) / 8, at0, wave, lane);
+      if (!BC) bl.init(b.row, (b.cols - k0) / 8, bt0, wave, lane);
     }
-    if (AC) al.load(ap + (long)k0 * a.row, a.rows - k0, a.cols * 2, buf * 2 * TILE);
-    else al.load(ap + k0 * 2, a.rows, min(a.cols - k0, TK) * 2, buf * 2 * TILE);
-    if (BC && MASKED) bl.load(bp + (long)k0 * b.row, b.rows - k0, b.cols * 2, buf * 2 * TILE, b.used[k0 / 64] >> (k0 % 64));
-    else if (BC) bl.load(bp + (long)k0 * b.row, b.rows - k0, b.cols * 2, buf * 2 * TILE);
-    else bl.load(bp + k0 * 2, b.rows, min(b.cols - k0, TK) * 2, buf * 2 * TILE);
-    if (!AC || !BC) {
-      if (K - k0 < TK && K % TK) {
-        if (!AC) al.init(a.row, TK / 8, tsg_lds_addr(lds), wave, lane);
-        if (!BC) bl.init(b.row, TK / 8, tsg_lds_addr(lds) + TILE, wave, lane);
-      }
+    if (AC) al.load(ap + (long)k0 * a.row, a.rows - k0, a.cols * 2, buf * T::STAGE);
+    else al.load(ap + k0 * 2, a.rows, min(a.cols - k0, TK) * 2, buf * T::STAGE);
+    if (BC && MASKED) bl.load(bp + (long)k0 * b.row, b.rows - k0, b.cols * 2, buf * T::STAGE, b.used[k0 / 64]);
+    else if (BC) bl.load(bp + (long)k0 * b.row, b.rows - k0, b.cols * 2, buf * T::STAGE);
+    else bl.load(bp + k0 * 2, b.rows, min(b.cols - k0, TK) * 2, buf * T::STAGE);
+    if (narrow) {
+      if (!AC) al.init(a.row, TK / 8, at0, wave, lane);
+      if (!BC) bl.init(b.row, TK / 8, bt0, wave, lane);
     }
   };
   int pass = 0, k0 = 0;
@@ -116,29 +122,28 @@ __device__ __forceinline__ void product(tsg_f32x16 (&acc)[2][2], char* lds, cons
       if (k0 >= K) k0 = 0, ++pass;
       fetch(pass, k0, buf ^ 1);
     }
-    const unsigned at = tsg_opaque(a0) + buf * 2 * TILE, bt = tsg_opaque(b0) + buf * 2 * TILE;
+    const unsigned at = tsg_opaque(a0) + buf * T::STAGE, bt = tsg_opaque(b0) + buf * T::STAGE;
 #pragma unroll
     for (int s = 0; s < TK / 16; ++s) {
-      tsg_u4 fa[2], fb[2];
+      tsg_u4 fa[T::XM], fb[T::XN];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        fa[x] = AC ? tsg_col_frag<TM / 8>(at, x, 16 * s * TM * 2) : tsg_row_frag<D>(at, s, 32 * x * TK * 2);
-        fb[x] = BC ? tsg_col_frag<TN / 8>(bt, x, 16 * s * TN * 2) : tsg_row_frag<D>(bt, s, 32 * x * TK * 2);
-      }
+      for (int x = 0; x < T::XM; ++x) fa[x] = AC ? tsg_col_frag<T::TM / 8>(at, x, 16 * s * T::TM * 2) : tsg_row_frag<D>(at, s, 32 * x * TK * 2);
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+      for (int y = 0; y < T::XN; ++y) fb[y] = BC ? tsg_col_frag<T::TN / 8>(bt, y, 16 * s * T::TN * 2) : tsg_row_frag<D>(bt, s, 32 * y * TK * 2);
 #pragma unroll
-        for (int y = 0; y < 2; ++y) tsg_mma<D>(fa[x], fb[y], acc[x][y]);
+      for (int x = 0; x < T::XM; ++x)
+#pragma unroll
+        for (int y = 0; y < T::XN; ++y) tsg_mma<D>(fa[x], fb[y], acc[x][y]);
     }
   }
   __syncthreads();  // the epilogue may use the tiles' memory
 }
 
-__device__ __forceinline__ void zero_acc(tsg_f32x16 (&acc)[2][2]) {
+template <typename T> __device__ __forceinline__ void zero_acc(Acc<T>& acc) {
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int x = 0; x < T::XM; ++x)
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+    for (int y = 0; y < T::XN; ++y)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[x][y][i] = 0.0f;
 }
@@ -154,68 +159,75 @@ __device__ __forceinline__ void tile_of(int b, int total, int tiles_m, int tiles
 }
 
 // The two products over h and w have the vocabulary down the accumulator's rows and the states across its columns, so that a
-// lane's 32 registers of a state are reduced without leaving the lane.
-template <typename D> __device__ __forceinline__ void logits(const XentArgs& a, tsg_f32x16 (&acc)[2][2], char* lds, int m0, int n0, int wave, int lane, bool split) {
-  zero_acc(acc);
+// lane's registers of a state are reduced without leaving the lane.
+template <typename D, typename T, bool SPLIT> __device__ __forceinline__ void logits(const XentArgs& a, Acc<T>& acc, char* lds, int m0, int n0, int wave, int lane) {
+  zero_acc<T>(acc);
   const Operand A = {a.w + (long)m0 * a.w_row, a.w_row, a.w_plane, a.vocab - m0, a.hidden, nullptr};
   const Operand B = {a.h + (long)n0 * a.h_row, a.h_row, a.h_plane, a.rows - n0, a.hidden, nullptr};
-  product<D, false, false>(acc, lds, A, B, a.hidden, split ? 3 : 1, wave, lane);
-  const int h = lane >> 5, wm = (wave >> 1) * 64;
-  const float by = split ? 1.0f / (a.scales[0] * a.scales[1]) : 1.0f;
+  product<D, T, false, false>(acc, lds, A, B, a.hidden, SPLIT ? 3 : 1, wave, lane);
+  const int h = lane >> 5, wm = wave / T::WN * 32 * T::XM;
+  const float by = SPLIT ? 1.0f / (a.scales[0] * a.scales[1]) : 1.0f;
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int x = 0; x < T::XM; ++x)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int v = m0 + wm + 32 * x + (i & 3) + 8 * (i >> 2) + 4 * h;
       float b = 0.0f;
-      if (a.bias && v < a.vocab) b = a.bias_f32 ? reinterpret_cast<const float*>(a.bias)[v] : (float)reinterpret_cast<const typename D::type*>(a.bias)[v];
+      if (a.bias && v < a.vocab) b = SPLIT ? reinterpret_cast<const float*>(a.bias)[v] : (float)reinterpret_cast<const typename D::type*>(a.bias)[v];
 #pragma unroll
-      for (int y = 0; y < 2; ++y) acc[x][y][i] = v < a.vocab ? (split ? acc[x][y][i] * by : acc[x][y][i]) + b : -INFINITY;
+      for (int y = 0; y < T::XN; ++y) acc[x][y][i] = v < a.vocab ? (SPLIT ? acc[x][y][i] * by : acc[x][y][i]) + b : -INFINITY;
     }
 }
 
-template <typename D>
-__global__ __launch_bounds__(256, 2) void xent_stat_kernel(XentArgs a, int tiles_m, int tiles_n) {
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TM * TK * 2];
-  __shared__ float2 join[2][TN];
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
+
+template <typename D, typename T, bool SPLIT>
+__global__ __launch_bounds__(64 * T::WAVES, 2) void xent_stat_kernel(XentArgs a, int tiles_m, int tiles_n) {
+  __shared__ __attribute__((aligned(1024))) char lds[2 * T::STAGE];
+  __shared__ float2 join[T::WM][T::TN];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
   int tm, tn;
   tile_of(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
-  tsg_f32x16 z[2][2];
-  logits<D>(a, z, lds, tm * TM, tn * TN, wave, lane, a.h_plane != 0);
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  Acc<T> z;
+  logits<D, T, SPLIT>(a, z, lds, tm * T::TM, tn * T::TN, wave, lane);
+  const int wm = wave / T::WN * 32 * T::XM, wn = wave % T::WN * 32 * T::XN;
 #pragma unroll
-  for (int y = 0; y < 2; ++y) {
-    const int n = wn + 32 * y + (lane & 31), t = tn * TN + n;
+  for (int y = 0; y < T::XN; ++y) {
+    const int n = wn + 32 * y + (lane & 31), t = tn * T::TN + n;
     float top = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < T::XM; ++x)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, z[x][y][i]);
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float off = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
-    const long at = (t < a.rows ? a.target[t] : -1) - (tm * TM + wm + 4 * h);
+    const long target = t < a.rows ? a.target[t] : -1;
+    const int at = target >= 0 && target < a.vocab ? (int)target - (tm * T::TM + wm + 4 * h) : -1;
     float zt = 0.0f;
     bool mine = false;
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < T::XM; ++x)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         if (at == 32 * x + (i & 3) + 8 * (i >> 2)) zt = z[x][y][i], mine = true;
-        sum += __builtin_amdgcn_exp2f((z[x][y][i] - off) * 1.44269504088896340736f);
+        sum += __builtin_amdgcn_exp2f((z[x][y][i] - off) * LOG2E);
       }
     sum += __shfl_xor(sum, 32, 64);
-    if (mine && t < a.rows && a.target[t] < a.vocab) a.zt[t] = zt;
-    if (h == 0) join[wave >> 1][n] = make_float2(top, sum);
+    if (mine) a.zt[t] = zt;
+    if (h == 0) join[wave / T::WN][n] = make_float2(top, sum);
   }
   __syncthreads();
-  const int n = threadIdx.x, t = tn * TN + n;
-  if (n < TN && t < a.rows) {
-    const float2 p = join[0][n], q = join[1][n];
-    const float top = fmaxf(p.x, q.x), off = top == -INFINITY ? 0.0f : top;
-    a.part[(long)tm * a.rows + t] = make_float2(top, p.y * __builtin_amdgcn_exp2f((p.x - off) * 1.44269504088896340736f) +
-                                                         q.y * __builtin_amdgcn_exp2f((q.x - off) * 1.44269504088896340736f));
+  for (int n = threadIdx.x; n < T::TN; n += 64 * T::WAVES) {
+    const int t = tn * T::TN + n;
+    if (t >= a.rows) break;
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < T::WM; ++w) top = fmaxf(top, join[w][n].x);
+    const float off = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < T::WM; ++w) sum += join[w][n].y * __builtin_amdgcn_exp2f((join[w][n].x - off) * LOG2E);
+    a.part[(long)tm * a.rows + t] = make_float2(top, sum);
   }
 }
 
@@ -228,7 +240,7 @@ __global__ __launch_bounds__(256) void xent_join_kernel(XentArgs a, int tiles_m,
     for (int m = part; m < tiles_m; m += 8) {
       const float2 p = a.part[(long)m * a.rows + t];
       const float to = fmaxf(top, p.x), off = to == -INFINITY ? 0.0f : to;
-      sum = sum * __builtin_amdgcn_exp2f((top - off) * 1.44269504088896340736f) + p.y * __builtin_amdgcn_exp2f((p.x - off) * 1.44269504088896340736f);
+      sum = sum * __builtin_amdgcn_exp2f((top - off) * LOG2E) + p.y * __builtin_amdgcn_exp2f((p.x - off) * LOG2E);
       top = to;
     }
   join[part][n] = make_float2(top, sum);
@@ -238,12 +250,12 @@ __global__ __launch_bounds__(256) void xent_join_kernel(XentArgs a, int tiles_m,
   for (int p = 0; p < 8; ++p) top = fmaxf(top, join[p][n].x);
   const float off = top == -INFINITY ? 0.0f : top;
   sum = 0.0f;
-  for (int p = 0; p < 8; ++p) sum += join[p][n].y * __builtin_amdgcn_exp2f((join[p][n].x - off) * 1.44269504088896340736f);
+  for (int p = 0; p < 8; ++p) sum += join[p][n].y * __builtin_amdgcn_exp2f((join[p][n].x - off) * LOG2E);
   const float l2 = __builtin_amdgcn_logf(sum);
   a.stat[t] = make_float2(off, l2);
   const long tg = a.target[t];
   float l = 0.0f;
-  if (tg != a.ignore) l = tg >= 0 && tg < a.vocab ? (off - a.zt[t]) + l2 * 0.693147180559945309417f : NAN;
+  if (tg != a.ignore) l = tg >= 0 && tg < a.vocab ? (off - a.zt[t]) + l2 * LN2 : NAN;
   loss[t] = l;
 }
 
@@ -296,144 +308,161 @@ __global__ __launch_bounds__(1024) void xent_grad_kernel(XentArgs a, const float
   *a.gmax = __float_as_uint(m);
 }
 
-template <typename D, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void xent_dz_kernel(XentArgs a, int tiles_m, int tiles_n) {
-  __shared__ __attribute__((aligned(1024))) char lds[SPLIT || TK == 64 ? 4 * TM * 64 * 2 + 2 * 16 * TM : TN * (TM * 2 + 16)];
+template <typename D, typename T, bool SPLIT>
+__global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dz_kernel(XentArgs a, int tiles_m, int tiles_n) {
+  constexpr int ROW = T::TM * 2 + 16;  // a state's dz of the tile in LDS, 16 bytes of padding
+  __shared__ __attribute__((aligned(1024))) char lds[T::TN * ROW > 2 * T::STAGE ? T::TN * ROW : 2 * T::STAGE];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
   int tm, tn;
   tile_of(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
-  constexpr bool split = SPLIT;
-  const int m0 = a.v0 + tm * TM;
-  tsg_f32x16 z[2][2];
-  logits<D>(a, z, lds, m0, tn * TN, wave, lane, split);
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  // rows of 128 entries, 16 bytes of padding: [128 states][272 bytes], hi and (f32) lo
-  constexpr int ROW = TM * 2 + 16, PLANE = TN * ROW;
+  const int m0 = a.v0 + tm * T::TM;
+  Acc<T> z;
+  logits<D, T, SPLIT>(a, z, lds, m0, tn * T::TN, wave, lane);
+  const int wm = wave / T::WN * 32 * T::XM, wn = wave % T::WN * 32 * T::XN;
   const float gs = __is_same(D, TsgBf16) ? 1.0f : scale_of(*a.gmax);
 #pragma unroll
-  for (int y = 0; y < 2; ++y) {
-    const int n = wn + 32 * y + (lane & 31), t = tn * TN + n;
+  for (int y = 0; y < T::XN; ++y) {
+    const int n = wn + 32 * y + (lane & 31), t = tn * T::TN + n;
     const bool in = t < a.rows;
     const float2 st = in ? a.stat[t] : make_float2(0.0f, INFINITY);
     const float g = in ? a.g[t] * gs : 0.0f;
-    const long at = (in ? a.target[t] : -1) - (m0 + wm + 4 * h);
+    const long target = in ? a.target[t] : -1;
+    const int at = target >= 0 && target < a.vocab ? (int)target - (m0 + wm + 4 * h) : -1;
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < T::XM; ++x)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float d[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[x][y][4 * q + r] - st.x, 1.44269504088896340736f, -st.y));
-          d[r] = g == 0.0f ? 0.0f : (at == 32 * x + 8 * q + r ? p - 1.0f : p) * g;  // a row left out adds nothing, whatever it holds
-          z[x][y][4 * q + r] = d[r];
-        }
-        char* to = lds + n * ROW + (wm + 32 * x + 8 * q + 4 * h) * 2;
-        uint2 hi;
-        hi.x = tsg_pack2<D>(d[0], d[1]);
-        hi.y = tsg_pack2<D>(d[2], d[3]);
-        *reinterpret_cast<uint2*>(to) = hi;
-        if (split) {
-          typedef typename D::type T;
-          uint2 lo;
-          lo.x = tsg_pack2<D>(d[0] - (float)(T)d[0], d[1] - (float)(T)d[1]);
-          lo.y = tsg_pack2<D>(d[2] - (float)(T)d[2], d[3] - (float)(T)d[3]);
-          *reinterpret_cast<uint2*>(to + PLANE) = lo;
-        }
+      for (int i = 0; i < 16; ++i) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[x][y][i] - st.x, LOG2E, -st.y));
+        // a row left out adds nothing, whatever it holds
+        z[x][y][i] = g == 0.0f ? 0.0f : (at == 32 * x + (i & 3) + 8 * (i >> 2) ? p - 1.0f : p) * g;
       }
   }
-  float sums[32];
-  if (a.db_part) {
-    // sums over the states: 32 registers x 32 lanes -> one register per lane, halving both in every step
+#pragma unroll 1
+  for (int plane = 0; plane < (SPLIT ? 2 : 1); ++plane) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int y = 0; y < T::XN; ++y)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sums[16 * x + i] = z[x][0][i] + z[x][1][i];
+      for (int x = 0; x < T::XM; ++x)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+        for (int q = 0; q < 4; ++q) {
+          typedef typename D::type E;
+          float d[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            d[r] = z[x][y][4 * q + r];
+            if (SPLIT && plane) d[r] -= (float)(E)d[r];
+          }
+          uint2 v;
+          v.x = tsg_pack2<D>(d[0], d[1]);
+          v.y = tsg_pack2<D>(d[2], d[3]);
+          *reinterpret_cast<uint2*>(lds + (wn + 32 * y + (lane & 31)) * ROW + (wm + 32 * x + 8 * q + 4 * h) * 2) = v;
+        }
+    __syncthreads();
+    constexpr int CH = T::TM / 8;
+#pragma unroll
+    for (int k = 0; k < T::TN * CH / (64 * T::WAVES); ++k) {
+      const int id = k * 64 * T::WAVES + threadIdx.x, n = id / CH, c = id % CH, t = tn * T::TN + n;
+      if (t < a.rows && tm * T::TM + c * 8 < a.ldz)
+        *reinterpret_cast<tsg_u4*>(a.dz + plane * a.dz_plane + ((long)t * a.ldz + tm * T::TM + c * 8) * 2) = *reinterpret_cast<const tsg_u4*>(lds + n * ROW + c * 16);
+    }
+    __syncthreads();
+  }
+  if (!a.db_part) return;
+  // sums over the states: 16 XM registers x 32 lanes, halving the registers with every bit of the lane while there are two left
+  float sums[16 * T::XM];
+#pragma unroll
+  for (int x = 0; x < T::XM; ++x)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float v = z[x][0][i];
+#pragma unroll
+      for (int y = 1; y < T::XN; ++y) v += z[x][y][i];
+      sums[16 * x + i] = v;
+    }
+  int n = 16 * T::XM;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (n > 1) {
+      n /= 2;
       const bool up = lane & o;
 #pragma unroll
-      for (int i = 0; i < o; ++i) {
-        const float keep = up ? sums[i + o] : sums[i], send = up ? sums[i] : sums[i + o];
-        sums[i] = keep + __shfl_xor(send, o, 64);
-      }
+      for (int i = 0; i < 8 * T::XM; ++i)
+        if (i < n) {
+          const float keep = up ? sums[i + n] : sums[i], send = up ? sums[i] : sums[i + n];
+          sums[i] = keep + __shfl_xor(send, o, 64);
+        }
+    } else {
+      sums[0] += __shfl_xor(sums[0], o, 64);
     }
   }
-  __syncthreads();
-  for (int p = 0; p < (split ? 2 : 1); ++p)
+  float* join = reinterpret_cast<float*>(lds);  // [WN][TM]
 #pragma unroll
-    for (int k = 0; k < TN * 16 / 256; ++k) {
-      const int id = k * 256 + threadIdx.x, n = id >> 4, c = id & 15, t = tn * TN + n;
-      if (t < a.rows)
-        *reinterpret_cast<tsg_u4*>(a.dz + p * a.dz_plane + ((long)t * a.ldz + tm * TM + c * 8) * 2) =
-            *reinterpret_cast<const tsg_u4*>(lds + p * PLANE + n * ROW + c * 16);
-    }
-  if (a.db_part) {
-    __syncthreads();
-    float* join = reinterpret_cast<float*>(lds);  // [2 column waves][128]
-    const int r = lane & 31;  // the step that looked at bit o of the lane kept the registers with bit o set like it
-    const int i = r & 15, x = r >> 4;
-    join[(wave & 1) * TM + wm + 32 * x + (i & 3) + 8 * (i >> 2) + 4 * h] = sums[0];
-    __syncthreads();
-    const int v = tm * TM + threadIdx.x;
-    if (threadIdx.x < TM && v < a.vc) a.db_part[(long)tn * a.vc + v] = join[threadIdx.x] + join[TM + threadIdx.x];
+  for (int k = 0; k < (T::XM > 2 ? T::XM / 2 : 1); ++k) {
+    const int id = T::XM == 1 ? (lane & 31) >> 1 : (lane & 31) * (T::XM / 2) + k, x = id >> 4, i = id & 15;
+    join[wave % T::WN * T::TM + wm + 32 * x + (i & 3) + 8 * (i >> 2) + 4 * h] = sums[k];
+  }
+  __syncthreads();
+  for (int m = threadIdx.x; m < T::TM && tm * T::TM + m < a.vc; m += 64 * T::WAVES) {
+    float v = join[m];
+#pragma unroll
+    for (int w = 1; w < T::WN; ++w) v += join[w * T::TM + m];
+    a.db_part[(long)tn * a.vc + tm * T::TM + m] = v;
   }
 }
 
 // dW of the piece: rows v, columns k', summed over the states
-template <typename D, typename OUT>
-__global__ __launch_bounds__(256, 2) void xent_dw_kernel(XentArgs a, int tiles_m, int tiles_n) {
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TM * TK * 2];
+template <typename D, typename T, typename OUT>
+__global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dw_kernel(XentArgs a, int tiles_m, int tiles_n) {
+  constexpr bool SPLIT = __is_same(OUT, float);
+  __shared__ __attribute__((aligned(1024))) char lds[2 * T::STAGE];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
   int tm, tn;
   tile_of(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
-  const bool split = a.h_plane != 0;
-  tsg_f32x16 acc[2][2];
-  zero_acc(acc);
-  const Operand A = {a.dz + (long)tm * TM * 2, a.ldz * 2, a.dz_plane, a.rows, (int)a.ldz - tm * TM, nullptr};
-  const Operand B = {a.h + (long)tn * TN * 2, a.h_row, a.h_plane, a.rows, a.hidden - tn * TN, a.used};
-  product<D, true, true, true>(acc, lds, A, B, a.rows, split ? 3 : 1, wave, lane);
+  Acc<T> acc;
+  zero_acc<T>(acc);
+  const Operand A = {a.dz + (long)tm * T::TM * 2, a.ldz * 2, a.dz_plane, a.rows, (int)a.ldz - tm * T::TM, nullptr};
+  const Operand B = {a.h + (long)tn * T::TN * 2, a.h_row, a.h_plane, a.rows, a.hidden - tn * T::TN, a.used};
+  product<D, T, true, true, true>(acc, lds, A, B, a.rows, SPLIT ? 3 : 1, wave, lane);
   float by = __is_same(D, TsgBf16) ? 1.0f : 1.0f / scale_of(*a.gmax);
-  if (split) by /= a.scales[0];
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  if (SPLIT) by /= a.scales[0];
+  const int wm = wave / T::WN * 32 * T::XM, wn = wave % T::WN * 32 * T::XN;
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int x = 0; x < T::XM; ++x)
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+    for (int y = 0; y < T::XN; ++y)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int v = a.v0 + tm * TM + wm + 32 * x + (i & 3) + 8 * (i >> 2) + 4 * h, k = tn * TN + wn + 32 * y + (lane & 31);
-        if (v < a.vocab && k < a.hidden) reinterpret_cast<OUT*>(a.dw + (long)v * a.dw_row)[k] = (OUT)(acc[x][y][i] * by);
+        const int m = tm * T::TM + wm + 32 * x + (i & 3) + 8 * (i >> 2) + 4 * h, k = tn * T::TN + wn + 32 * y + (lane & 31);
+        if (m < a.vc && k < a.hidden) reinterpret_cast<OUT*>(a.dw + (long)(a.v0 + m) * a.dw_row)[k] = (OUT)(acc[x][y][i] * by);
       }
 }
 
 // dh: rows t, columns k', summed over a stretch of the piece; the stretches' sums are added up over the pieces
-template <typename D>
-__global__ __launch_bounds__(256, 2) void xent_dh_kernel(XentArgs a, int tiles_m, int tiles_n) {
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TM * TK * 2];
+template <typename D, typename T, bool SPLIT>
+__global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dh_kernel(XentArgs a, int tiles_m, int tiles_n) {
+  __shared__ __attribute__((aligned(1024))) char lds[2 * T::STAGE];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
   const int split_id = blockIdx.x / (tiles_m * tiles_n);
   int tm, tn;
   tile_of(blockIdx.x % (tiles_m * tiles_n), tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
-  const bool split = a.h_plane != 0;
   const int c0 = split_id * a.split_len, len = min(a.split_len, a.vc - c0);
-  tsg_f32x16 acc[2][2];
-  zero_acc(acc);
+  Acc<T> acc;
+  zero_acc<T>(acc);
   if (len > 0) {
-    // ldz covers the piece up to a multiple of 128 with zeros, W ends at its last row: the shorter one decides
-    const Operand A = {a.dz + ((long)tm * TM * a.ldz + c0) * 2, a.ldz * 2, a.dz_plane, a.rows - tm * TM, (len + 7) / 8 * 8, nullptr};
-    const Operand B = {a.w + (long)(a.v0 + c0) * a.w_row + (long)tn * TN * 2, a.w_row, a.w_plane, len, a.hidden - tn * TN, nullptr};
-    product<D, false, true>(acc, lds, A, B, len, split ? 3 : 1, wave, lane);
+    // dz is zero behind the vocabulary up to a multiple of 64, W ends at its last row
+    const Operand A = {a.dz + ((long)tm * T::TM * a.ldz + c0) * 2, a.ldz * 2, a.dz_plane, a.rows - tm * T::TM, (len + 7) / 8 * 8, nullptr};
+    const Operand B = {a.w + (long)(a.v0 + c0) * a.w_row + (long)tn * T::TN * 2, a.w_row, a.w_plane, len, a.hidden - tn * T::TN, nullptr};
+    product<D, T, false, true>(acc, lds, A, B, len, SPLIT ? 3 : 1, wave, lane);
   }
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  const int wm = wave / T::WN * 32 * T::XM, wn = wave % T::WN * 32 * T::XN;
   float* out = a.dh_part + (long)split_id * a.rows * a.hidden;
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int x = 0; x < T::XM; ++x)
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+    for (int y = 0; y < T::XN; ++y)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int t = tm * TM + wm + 32 * x + (i & 3) + 8 * (i >> 2) + 4 * h, k = tn * TN + wn + 32 * y + (lane & 31);
+        const int t = tm * T::TM + wm + 32 * x + (i & 3) + 8 * (i >> 2) + 4 * h, k = tn * T::TN + wn + 32 * y + (lane & 31);
         if (t < a.rows && k < a.hidden) {
           float* p = out + (long)t * a.hidden + k;
           *p = a.first ? acc[x][y][i] : *p + acc[x][y][i];
@@ -441,22 +470,50 @@ __global__ __launch_bounds__(256, 2) void xent_dh_kernel(XentArgs a, int tiles_m
       }
 }
 
-template <typename OUT>
+// Four elements per thread; PARTS of the workgroup's waves share the stretches (1 or 4)
+template <typename OUT, int PARTS>
 __global__ __launch_bounds__(256) void xent_dh_out_kernel(XentArgs a, OUT* dh, long dh_row, int scaled) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x, n = (long)a.rows * a.hidden;
+  constexpr int WIDE = 256 / PARTS;
+  __shared__ float4 join[PARTS][WIDE];
+  const int part = threadIdx.x / WIDE, lane = threadIdx.x % WIDE;
+  const long i = ((long)blockIdx.x * WIDE + lane) * 4, n = (long)a.rows * a.hidden;
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (i < n)
+#pragma unroll 4
+    for (int p = part; p < a.splits; p += PARTS) {
+      const float4 v = *reinterpret_cast<const float4*>(a.dh_part + p * n + i);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+  if (PARTS > 1) {
+    join[part][lane] = s;
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int p = 1; p < PARTS; ++p) {
+      const float4 v = join[p][lane];
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+  }
   if (i >= n) return;
-  float s = 0.0f;
-  for (int p = 0; p < a.splits; ++p) s += a.dh_part[p * n + i];
-  if (scaled) s /= scale_of(*a.gmax);
-  if (a.h_plane) s /= a.scales[1];
-  dh[(i / a.hidden) * dh_row + i % a.hidden] = (OUT)s;
+  float by = scaled ? 1.0f / scale_of(*a.gmax) : 1.0f;
+  if (__is_same(OUT, float)) by /= a.scales[1];
+  OUT* to = dh + (i / a.hidden) * dh_row + i % a.hidden;
+  OUT v[4] = {(OUT)(s.x * by), (OUT)(s.y * by), (OUT)(s.z * by), (OUT)(s.w * by)};
+  if (sizeof(OUT) == 4) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(v);
+  else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(v);
 }
 
 template <typename OUT> __global__ __launch_bounds__(256) void xent_db_out_kernel(XentArgs a, OUT* db, int tiles_n, int scaled) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v >= a.vc) return;
+  __shared__ float join[4][64];
+  const int part = threadIdx.x >> 6, lane = threadIdx.x & 63, v = blockIdx.x * 64 + lane;
   float s = 0.0f;
-  for (int t = 0; t < tiles_n; ++t) s += a.db_part[(long)t * a.vc + v];
+  if (v < a.vc)
+#pragma unroll 4
+    for (int t = part; t < tiles_n; t += 4) s += a.db_part[(long)t * a.vc + v];
+  join[part][lane] = s;
+  __syncthreads();
+  if (part || v >= a.vc) return;
+  s = (join[0][lane] + join[1][lane]) + (join[2][lane] + join[3][lane]);
   if (scaled) s /= scale_of(*a.gmax);
   db[a.v0 + v] = (OUT)s;
 }
@@ -534,14 +591,21 @@ __global__ __launch_bounds__(256) void xent_planes_kernel(Planes a) {
 // ------------------------------------------------------------------------------------------------------ host side
 struct Layout {
   size_t gmax, amax, planes, h_plane, w_plane, part, zt, g, used, dz, dz_plane, db, dh, total;
-  int vc, splits, split_len;
+  int vc, splits, split_len, dh_shape;
 };
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // dz of a piece takes at most `budget` bytes (but 128 vocabulary rows at least): large pieces fill the chip, small ones keep
 // the workspace small.
+// The largest tile that still gives every CU a workgroup (256 x 256 fill one, of 128 x 128 two fit), else the next
+enum Shape { FEW, MID, BIG };
+Shape shape_of(int64_t m, int64_t n, int64_t times = 1) {
+  if ((int64_t)tsg_cdiv(m, Big::TM) * tsg_cdiv(n, Big::TN) * times >= 256) return BIG;
+  if ((int64_t)tsg_cdiv(m, Mid::TM) * tsg_cdiv(n, Mid::TN) * times >= 256) return MID;
+  return FEW;
+}
 constexpr int PLANE_BLOCKS = 512;
-constexpr size_t DZ_BUDGET = (size_t)1 << 30;
+constexpr size_t DZ_BUDGET = (size_t)2 << 30;
 
 Layout layout_of(const tsg_xent_desc* d, bool backward) {
   Layout l = {};
@@ -560,26 +624,29 @@ Layout layout_of(const tsg_xent_desc* d, bool backward) {
     l.planes = take(2 * (l.h_plane + l.w_plane));
   }
   if (!backward) {
-    l.part = take((size_t)tsg_cdiv(V, TM) * T * 8);
+    l.part = take((size_t)tsg_cdiv(V, shape_of(V, T) == FEW ? Few::TM : shape_of(V, T) == MID ? Mid::TM : Big::TM) * T * 8);
     l.zt = take(T * 4);
   } else {
     const size_t each = f32 ? 4 : 2;
-    size_t vc = DZ_BUDGET / (T * each) / TM * TM;
-    if (vc < TM) vc = TM;
-    const size_t all = (V + TM - 1) / TM * TM;
+    size_t vc = DZ_BUDGET / (T * each) / 256 * 256;
+    if (vc < 256) vc = 256;
+    const size_t all = (V + 63) / 64 * 64;
     if (vc > all) vc = all;
-    if (vc > ((size_t)1 << 22)) vc = (size_t)1 << 22;  // 128 rows of dz stay below 2^31 bytes
+    if (vc > ((size_t)1 << 21)) vc = (size_t)1 << 21;  // 256 rows of dz stay below 2^31 bytes
     const size_t pieces = (all + vc - 1) / vc;  // even pieces
-    vc = ((all + pieces - 1) / pieces + TM - 1) / TM * TM;
+    if (pieces > 1) vc = ((all + pieces - 1) / pieces + 255) / 256 * 256;
     l.vc = (int)vc;
     l.dz_plane = f32 ? up256(T * vc * 2) : 0;
     l.dz = take(f32 ? 2 * l.dz_plane : T * vc * 2);
     l.g = take(T * 4);
     l.used = take((T + 63) / 64 * 8);
-    l.db = d->bias ? take((size_t)tsg_cdiv(T, TN) * vc * 4) : 0;
-    const size_t tiles = (size_t)tsg_cdiv(T, TM) * tsg_cdiv(K, TN);
-    size_t s = (512 + tiles - 1) / tiles;  // two workgroups a CU
-    if (s > vc / TM) s = vc / TM;
+    l.db = d->bias ? take((size_t)tsg_cdiv(T, 64) * vc * 4) : 0;
+    // dh has few tiles and a long sum: cut it until the chip is full, in stretches of 128 entries at least
+    l.dh_shape = T >= 2048 ? BIG : T > 64 ? MID : FEW;
+    const int tm = l.dh_shape == BIG ? Big::TM : l.dh_shape == MID ? Mid::TM : Few::TM;
+    const size_t tiles = (size_t)tsg_cdiv(T, tm) * tsg_cdiv(K, tm);
+    size_t s = ((l.dh_shape == BIG ? 256 : 512) + tiles - 1) / tiles;
+    if (s > vc / 128) s = vc / 128;
     if (s < 1) s = 1;
     l.split_len = (int)(((vc + s - 1) / s + TK - 1) / TK * TK);
     l.splits = (int)((vc + l.split_len - 1) / l.split_len);
@@ -594,8 +661,8 @@ int check_xent(const tsg_xent_desc* d, bool backward) {
   if (d->dtype != TSG_F32 && d->dtype != TSG_BF16 && d->dtype != TSG_F16) return TSG_E_INVALID;
   if (d->n_rows < 0 || d->n_vocab <= 0 || d->hidden <= 0 || d->reduction < 0 || d->reduction > 2) return TSG_E_INVALID;
   if (d->n_rows > 0x7fffff00L || d->n_vocab > 0x7fffff00L) return TSG_E_LIMIT;
-  if ((int64_t)tsg_cdiv(d->n_rows, TN) * tsg_cdiv(d->n_vocab, TM) > 0x7fffffffL) return TSG_E_LIMIT;
-  if (d->n_rows * (int64_t)d->hidden > ((int64_t)1 << 38)) return TSG_E_LIMIT;
+  if ((int64_t)tsg_cdiv(d->n_rows, 64) * tsg_cdiv(d->n_vocab, 64) > 0x7fffffffL) return TSG_E_LIMIT;
+  if (d->n_rows * (int64_t)d->hidden > ((int64_t)1 << 36)) return TSG_E_LIMIT;
   if (d->hidden % 8) return TSG_E_INVALID;
   const int epc = d->dtype == TSG_F32 ? 4 : 8;
   if (!d->h || !d->w || !d->target || !d->stats || (uintptr_t)d->h % 16 || (uintptr_t)d->w % 16 || (uintptr_t)d->stats % 8) return TSG_E_INVALID;
@@ -605,7 +672,7 @@ int check_xent(const tsg_xent_desc* d, bool backward) {
   if (!backward && d->reduction && !d->loss) return TSG_E_INVALID;
   if (d->dtype == TSG_F32 && !d->scales) return TSG_E_INVALID;
   if (backward && (!d->d_loss || !d->dh || !d->dw || (d->bias && !d->dbias))) return TSG_E_INVALID;
-  if (backward && (d->dh_row < d->hidden || d->dw_row < d->hidden)) return TSG_E_INVALID;
+  if (backward && (d->dh_row < d->hidden || d->dw_row < d->hidden || d->dh_row % 4 || (uintptr_t)d->dh % 16)) return TSG_E_INVALID;
   return 0;
 }
 
@@ -621,7 +688,7 @@ XentArgs args_of(const tsg_xent_desc* d, const Layout& l) {
   } else {
     a.h = (const char*)d->h, a.w = (const char*)d->w, a.h_row = d->h_row * 2, a.w_row = d->w_row * 2;
   }
-  a.bias = (const char*)d->bias, a.bias_f32 = f32;
+  a.bias = (const char*)d->bias;
   a.target = (const long*)d->target, a.ignore = d->ignore_index;
   a.rows = (int)d->n_rows, a.hidden = d->hidden, a.vocab = (int)d->n_vocab;
   a.stat = (float2*)d->stats;
@@ -647,19 +714,53 @@ void make_planes(const tsg_xent_desc* d, const XentArgs& a, const Layout& l, boo
   hipLaunchKernelGGL(xent_planes_kernel, grid, dim3(256), 0, s, p);
 }
 
-template <typename D> void launch_stat(const XentArgs& a, int tm, int tn, hipStream_t s) {
-  hipLaunchKernelGGL(xent_stat_kernel<D>, dim3((unsigned)(tm * tn)), dim3(256), 0, s, a, tm, tn);
+// f(Tile<...>) for the shape
+template <typename F> void with_tile(int shape, F f) {
+  if (shape == BIG) f(Big());
+  else if (shape == MID) f(Mid());
+  else f(Few());
+}
+
+template <typename D, bool SPLIT> int launch_stat(const XentArgs& a, hipStream_t s) {
+  int tm = 0;
+  with_tile(shape_of(a.vocab, a.rows), [&](auto t) {
+    typedef decltype(t) T;
+    tm = tsg_cdiv(a.vocab, T::TM);
+    const int tn = tsg_cdiv(a.rows, T::TN);
+    hipLaunchKernelGGL((xent_stat_kernel<D, T, SPLIT>), dim3((unsigned)(tm * tn)), dim3(64 * T::WAVES), 0, s, a, tm, tn);
+  });
+  return tm;
 }
 
 template <typename D, typename OUT> void backward_piece(XentArgs a, const tsg_xent_desc* d, const Layout& l, hipStream_t s) {
-  const int tv = tsg_cdiv(a.vc, TM), tt = tsg_cdiv(a.rows, TN), tk = tsg_cdiv(a.hidden, TN);
+  constexpr bool SPLIT = __is_same(OUT, float);
   const int scaled = !__is_same(D, TsgBf16);
-  hipLaunchKernelGGL((xent_dz_kernel<D, __is_same(OUT, float)>), dim3((unsigned)(tv * tt)), dim3(256), 0, s, a, tv, tt);
-  hipLaunchKernelGGL((xent_dw_kernel<D, OUT>), dim3((unsigned)(tv * tk)), dim3(256), 0, s, a, tv, tk);
-  hipLaunchKernelGGL(xent_dh_kernel<D>, dim3((unsigned)(tt * tk * l.splits)), dim3(256), 0, s, a, tt, tk);
-  if (d->bias) hipLaunchKernelGGL(xent_db_out_kernel<OUT>, dim3(tsg_cdiv(a.vc, 256)), dim3(256), 0, s, a, (OUT*)d->dbias, tt, scaled);
+  int tt = 0;
+  int shape = shape_of(a.vc, a.rows);
+  if (SPLIT && shape == BIG) shape = MID;  // 256 x 256 and the two planes of dz do not fit the registers
+  with_tile(shape, [&](auto t) {
+    typedef std::conditional_t<SPLIT && __is_same(decltype(t), Big), Mid, decltype(t)> T;
+    tt = tsg_cdiv(a.rows, T::TN);
+    const int tv = tsg_cdiv(a.vc, T::TM);
+    hipLaunchKernelGGL((xent_dz_kernel<D, T, SPLIT>), dim3((unsigned)(tv * tt)), dim3(64 * T::WAVES), 0, s, a, tv, tt);
+  });
+  with_tile(shape_of(a.vc, a.hidden), [&](auto t) {
+    typedef decltype(t) T;
+    const int tv = tsg_cdiv(a.vc, T::TM), tk = tsg_cdiv(a.hidden, T::TN);
+    hipLaunchKernelGGL((xent_dw_kernel<D, T, OUT>), dim3((unsigned)(tv * tk)), dim3(64 * T::WAVES), 0, s, a, tv, tk);
+  });
+  with_tile(l.dh_shape, [&](auto t) {
+    typedef decltype(t) T;
+    const int tr = tsg_cdiv(a.rows, T::TM), tk = tsg_cdiv(a.hidden, T::TN);
+    hipLaunchKernelGGL((xent_dh_kernel<D, T, SPLIT>), dim3((unsigned)(tr * tk * l.splits)), dim3(64 * T::WAVES), 0, s, a, tr, tk);
+  });
+  if (d->bias) hipLaunchKernelGGL(xent_db_out_kernel<OUT>, dim3(tsg_cdiv(a.vc, 64)), dim3(256), 0, s, a, (OUT*)d->dbias, tt, scaled);
   if (a.v0 + a.vc >= a.vocab)
-    hipLaunchKernelGGL(xent_dh_out_kernel<OUT>, dim3((unsigned)(((long)a.rows * a.hidden + 255) / 256)), dim3(256), 0, s, a, (OUT*)d->dh, (long)d->dh_row, scaled);
+  {
+    const long quads = (long)a.rows * a.hidden / 4;
+    if (l.splits >= 16) hipLaunchKernelGGL((xent_dh_out_kernel<OUT, 4>), dim3((unsigned)((quads + 63) / 64)), dim3(256), 0, s, a, (OUT*)d->dh, (long)d->dh_row, scaled);
+    else hipLaunchKernelGGL((xent_dh_out_kernel<OUT, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, a, (OUT*)d->dh, (long)d->dh_row, scaled);
+  }
 }
 
 }  // namespace
@@ -682,9 +783,9 @@ extern "C" int tsg_xent_forward(const tsg_xent_desc* d, void* stream) {
   a.part = (float2*)((char*)d->workspace + l.part);
   a.zt = (float*)((char*)d->workspace + l.zt);
   if (d->dtype == TSG_F32) make_planes(d, a, l, false, s);
-  const int tm = tsg_cdiv(a.vocab, TM), tn = tsg_cdiv(a.rows, TN);
-  if (d->dtype == TSG_BF16) launch_stat<TsgBf16>(a, tm, tn, s);
-  else launch_stat<TsgF16>(a, tm, tn, s);
+  const int tm = d->dtype == TSG_BF16  ? launch_stat<TsgBf16, false>(a, s)
+                 : d->dtype == TSG_F16 ? launch_stat<TsgF16, false>(a, s)
+                                       : launch_stat<TsgF16, true>(a, s);
   hipLaunchKernelGGL(xent_join_kernel, dim3(tsg_cdiv(a.rows, 32)), dim3(256), 0, s, a, tm, d->row_loss);
   if (d->reduction) hipLaunchKernelGGL(xent_reduce_kernel, dim3(1), dim3(1024), 0, s, a, (const float*)d->row_loss, d->loss, d->reduction == 2);
   TSG_LAUNCH_CHECK();
