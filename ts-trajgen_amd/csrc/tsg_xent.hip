@@ -19,8 +19,6 @@
 // All sums, maxima and logarithms are f32.  Nothing depends on the order of workgroups: no floating-point atomics.
 #include "tsg_mma.h"
 
-#include <type_traits>
-
 namespace {
 
 constexpr int TK = 64;  // k of one step
@@ -94,6 +92,7 @@ __device__ __forceinline__ void product(Acc<T>& acc, char* lds, const Operand& a
   const unsigned at0 = tsg_lds_addr(lds), bt0 = tsg_lds_addr(lds) + T::A;
   al.init(a.row, AC ? a.cols / 8 : TK / 8, at0, wave, lane);
   bl.init(b.row, BC ? b.cols / 8 : TK / 8, bt0, wave, lane);
+  unsigned long long used = MASKED ? b.used[0] : 0ull;
   auto fetch = [&](int pass, int k0, int buf) {
     const char* ap = a.p + (pass == 2 ? a.plane : 0);
     const char* bp = b.p + (pass == 1 ? b.plane : 0);
@@ -104,7 +103,7 @@ __device__ __forceinline__ void product(Acc<T>& acc, char* lds, const Operand& a
     }
     if (AC) al.load(ap + (long)k0 * a.row, a.rows - k0, a.cols * 2, buf * T::STAGE);
     else al.load(ap + k0 * 2, a.rows, min(a.cols - k0, TK) * 2, buf * T::STAGE);
-    if (BC && MASKED) bl.load(bp + (long)k0 * b.row, b.rows - k0, b.cols * 2, buf * T::STAGE, b.used[k0 / 64]);
+    if (BC && MASKED) bl.load(bp + (long)k0 * b.row, b.rows - k0, b.cols * 2, buf * T::STAGE, used);
     else if (BC) bl.load(bp + (long)k0 * b.row, b.rows - k0, b.cols * 2, buf * T::STAGE);
     else bl.load(bp + k0 * 2, b.rows, min(b.cols - k0, TK) * 2, buf * T::STAGE);
     if (narrow) {
@@ -113,7 +112,10 @@ __device__ __forceinline__ void product(Acc<T>& acc, char* lds, const Operand& a
     }
   };
   int pass = 0, k0 = 0;
-  if (steps) fetch(0, 0, 0);
+  if (steps) {
+    fetch(0, 0, 0);
+    if (MASKED) used = b.used[(TK < K ? TK : 0) / 64];
+  }
   for (int step = 0, buf = 0; step < steps; ++step, buf ^= 1) {
     tsg_dma_wait();
     __syncthreads();
@@ -121,6 +123,7 @@ __device__ __forceinline__ void product(Acc<T>& acc, char* lds, const Operand& a
       k0 += TK;
       if (k0 >= K) k0 = 0, ++pass;
       fetch(pass, k0, buf ^ 1);
+      if (MASKED) used = b.used[(k0 + TK < K ? k0 + TK : 0) / 64];  // for the step after: a scalar load under this one's products
     }
     const unsigned at = tsg_opaque(a0) + buf * T::STAGE, bt = tsg_opaque(b0) + buf * T::STAGE;
 #pragma unroll
@@ -135,6 +138,8 @@ __device__ __forceinline__ void product(Acc<T>& acc, char* lds, const Operand& a
 #pragma unroll
         for (int y = 0; y < T::XN; ++y) tsg_mma<D>(fa[x], fb[y], acc[x][y]);
     }
+    constexpr int READS = T::XM * (AC ? 2 : 1) + T::XN * (BC ? 2 : 1), PRODUCTS = T::XM * T::XN;  // of 16 k
+    tsg_interleave<READS * TK / 16, PRODUCTS * TK / 16, READS, (READS + PRODUCTS - 1) / PRODUCTS>();
   }
   __syncthreads();  // the epilogue may use the tiles' memory
 }
@@ -176,6 +181,7 @@ template <typename D, typename T, bool SPLIT> __device__ __forceinline__ void lo
       if (a.bias && v < a.vocab) b = SPLIT ? reinterpret_cast<const float*>(a.bias)[v] : (float)reinterpret_cast<const typename D::type*>(a.bias)[v];
 #pragma unroll
       for (int y = 0; y < T::XN; ++y) acc[x][y][i] = v < a.vocab ? (SPLIT ? acc[x][y][i] * by : acc[x][y][i]) + b : -INFINITY;
+      if (i == 15) __builtin_amdgcn_sched_barrier(0);  // or the biases of all 32 XM rows are fetched at once, into registers that are not there
     }
 }
 
@@ -736,10 +742,8 @@ template <typename D, typename OUT> void backward_piece(XentArgs a, const tsg_xe
   constexpr bool SPLIT = __is_same(OUT, float);
   const int scaled = !__is_same(D, TsgBf16);
   int tt = 0;
-  int shape = shape_of(a.vc, a.rows);
-  if (SPLIT && shape == BIG) shape = MID;  // 256 x 256 and the two planes of dz do not fit the registers
-  with_tile(shape, [&](auto t) {
-    typedef std::conditional_t<SPLIT && __is_same(decltype(t), Big), Mid, decltype(t)> T;
+  with_tile(shape_of(a.vc, a.rows), [&](auto t) {
+    typedef decltype(t) T;
     tt = tsg_cdiv(a.rows, T::TN);
     const int tv = tsg_cdiv(a.vc, T::TM);
     hipLaunchKernelGGL((xent_dz_kernel<D, T, SPLIT>), dim3((unsigned)(tv * tt)), dim3(64 * T::WAVES), 0, s, a, tv, tt);
