@@ -574,7 +574,7 @@ int tsg_attn_backward(const tsg_attn_desc* d, void* stream);
  * have the type of h and w.  The backward takes d_loss (one number, or one per row for reduction 0) and the stats that
  * the forward left, takes the vocabulary in pieces and writes dh, dw and dbias whole.
  * Base addresses of h and w are 16-byte aligned, rows a multiple of 16 and less than 2^23 bytes apart, hidden a multiple of 8 (pad with
- * zeros), dh 16-byte aligned with rows a multiple of 4 elements apart, the workspace 256-byte aligned; tsg_xent_workspace says how much.  n_rows >= 1. */
+ * zeros), dh and dw 16-byte aligned with rows a multiple of 4 elements apart, the workspace 256-byte aligned; tsg_xent_workspace says how much.  n_rows >= 1. */
 typedef struct tsg_xent_desc {
   int32_t dtype, hidden, reduction, reserved;
   int64_t n_rows, n_vocab, ignore_index;

@@ -375,7 +375,8 @@ def check_entropy(dt, h, w, b, target, reduction='mean'):
 
 @pytest.mark.parametrize('dt', TYPES)
 @pytest.mark.parametrize('t,v,k', [(1, 1, 8), (1, 300, 64), (61, 1000, 256), (129, 129, 72), (300, 5003, 100), (128, 128, 128),
-                                   (257, 4097, 320), (5, 11096, 256), (700, 640, 1000), (64, 2048, 3)])
+                                   (257, 4097, 320), (5, 11096, 256), (700, 640, 1000), (64, 2048, 3),
+                                   (2500, 9001, 64), (4100, 8200, 260)])
 def test_cross_entropy_sizes(dt, t, v, k):
     check_entropy(dt, *entropy_case(dt, t, v, k, seed=t + v))
 

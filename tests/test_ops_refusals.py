@@ -92,7 +92,7 @@ def test_cross_entropy_descriptor(kw, rc):
 
 
 def test_cross_entropy_backward_descriptor():
-    for kw in (dict(d_loss=None), dict(dh=None), dict(dw=None), dict(dbias=None), dict(dh_row=8), dict(dh_row=66), dict(dh=4100), dict(dw_row=8)):
+    for kw in (dict(d_loss=None), dict(dh=None), dict(dw=None), dict(dbias=None), dict(dh_row=8), dict(dh_row=66), dict(dh=4100), dict(dw_row=8), dict(dw_row=66), dict(dw=4100)):
         assert _xent('tsg_xent_backward', **kw) == -1
     assert _xent('tsg_xent_backward', workspace_bytes=100) == -2
 

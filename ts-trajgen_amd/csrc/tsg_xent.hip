@@ -65,6 +65,8 @@ struct XentArgs {
   float* db_part;               // [row tiles][vc]
   float* dh_part;               // [splits][rows][hidden]
   int splits, split_len, first;
+  float* dw_part;               // [dw_splits][vc][hidden], or null: whole sums go to dw
+  int dw_len;                   // rows of a stretch
   char* dw;
   long dw_row;
 };
@@ -184,6 +186,9 @@ template <typename D, typename T, bool SPLIT> __device__ __forceinline__ void lo
       if (i == 15) __builtin_amdgcn_sched_barrier(0);  // or the biases of all 32 XM rows are fetched at once, into registers that are not there
     }
 }
+
+// orders LDS alone: __syncthreads would wait for the stores to memory as well
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
 
@@ -343,6 +348,41 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dz_kernel(XentArgs a, i
         z[x][y][i] = g == 0.0f ? 0.0f : (at == 32 * x + (i & 3) + 8 * (i >> 2) ? p - 1.0f : p) * g;
       }
   }
+  if (a.db_part) {
+    // sums over the states: 16 registers x 32 lanes, halving the registers with four bits of the lane
+    float* join = reinterpret_cast<float*>(lds);  // [WN][TM]
+#pragma unroll
+    for (int x = 0; x < T::XM; ++x) {
+      float sums[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        sums[i] = z[x][0][i];
+#pragma unroll
+        for (int y = 1; y < T::XN; ++y) sums[i] += z[x][y][i];
+      }
+#pragma unroll
+      for (int n = 8; n > 0; n >>= 1) {
+        const bool up = lane & (2 * n);
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+          const float keep = up ? sums[i + n] : sums[i], send = up ? sums[i] : sums[i + n];
+          sums[i] = keep + __shfl_xor(send, 2 * n, 64);
+        }
+      }
+      sums[0] += __shfl_xor(sums[0], 1, 64);
+      const int i = (lane & 31) >> 1;
+      join[wave % T::WN * T::TM + wm + 32 * x + (i & 3) + 8 * (i >> 2) + 4 * h] = sums[0];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    lds_barrier();
+    for (int m = threadIdx.x; m < T::TM && tm * T::TM + m < a.vc; m += 64 * T::WAVES) {
+      float v = join[m];
+#pragma unroll
+      for (int w = 1; w < T::WN; ++w) v += join[w * T::TM + m];
+      a.db_part[(long)tn * a.vc + tm * T::TM + m] = v;
+    }
+    lds_barrier();
+  }
 #pragma unroll 1
   for (int plane = 0; plane < (SPLIT ? 2 : 1); ++plane) {
 #pragma unroll
@@ -352,18 +392,16 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dz_kernel(XentArgs a, i
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           typedef typename D::type E;
-          float d[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            d[r] = z[x][y][4 * q + r];
-            if (SPLIT && plane) d[r] -= (float)(E)d[r];
-          }
           uint2 v;
-          v.x = tsg_pack2<D>(d[0], d[1]);
-          v.y = tsg_pack2<D>(d[2], d[3]);
+          v.x = tsg_pack2<D>(z[x][y][4 * q], z[x][y][4 * q + 1]);
+          v.y = tsg_pack2<D>(z[x][y][4 * q + 2], z[x][y][4 * q + 3]);
+          if (SPLIT) {  // what is left over is the second plane
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[x][y][4 * q + r] -= (float)(E)z[x][y][4 * q + r];
+          }
           *reinterpret_cast<uint2*>(lds + (wn + 32 * y + (lane & 31)) * ROW + (wm + 32 * x + 8 * q + 4 * h) * 2) = v;
         }
-    __syncthreads();
+    lds_barrier();
     constexpr int CH = T::TM / 8;
 #pragma unroll
     for (int k = 0; k < T::TN * CH / (64 * T::WAVES); ++k) {
@@ -371,48 +409,7 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dz_kernel(XentArgs a, i
       if (t < a.rows && tm * T::TM + c * 8 < a.ldz)
         *reinterpret_cast<tsg_u4*>(a.dz + plane * a.dz_plane + ((long)t * a.ldz + tm * T::TM + c * 8) * 2) = *reinterpret_cast<const tsg_u4*>(lds + n * ROW + c * 16);
     }
-    __syncthreads();
-  }
-  if (!a.db_part) return;
-  // sums over the states: 16 XM registers x 32 lanes, halving the registers with every bit of the lane while there are two left
-  float sums[16 * T::XM];
-#pragma unroll
-  for (int x = 0; x < T::XM; ++x)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float v = z[x][0][i];
-#pragma unroll
-      for (int y = 1; y < T::XN; ++y) v += z[x][y][i];
-      sums[16 * x + i] = v;
-    }
-  int n = 16 * T::XM;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    if (n > 1) {
-      n /= 2;
-      const bool up = lane & o;
-#pragma unroll
-      for (int i = 0; i < 8 * T::XM; ++i)
-        if (i < n) {
-          const float keep = up ? sums[i + n] : sums[i], send = up ? sums[i] : sums[i + n];
-          sums[i] = keep + __shfl_xor(send, o, 64);
-        }
-    } else {
-      sums[0] += __shfl_xor(sums[0], o, 64);
-    }
-  }
-  float* join = reinterpret_cast<float*>(lds);  // [WN][TM]
-#pragma unroll
-  for (int k = 0; k < (T::XM > 2 ? T::XM / 2 : 1); ++k) {
-    const int id = T::XM == 1 ? (lane & 31) >> 1 : (lane & 31) * (T::XM / 2) + k, x = id >> 4, i = id & 15;
-    join[wave % T::WN * T::TM + wm + 32 * x + (i & 3) + 8 * (i >> 2) + 4 * h] = sums[k];
-  }
-  __syncthreads();
-  for (int m = threadIdx.x; m < T::TM && tm * T::TM + m < a.vc; m += 64 * T::WAVES) {
-    float v = join[m];
-#pragma unroll
-    for (int w = 1; w < T::WN; ++w) v += join[w * T::TM + m];
-    a.db_part[(long)tn * a.vc + tm * T::TM + m] = v;
+    lds_barrier();
   }
 }
 
@@ -423,12 +420,13 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dw_kernel(XentArgs a, i
   __shared__ __attribute__((aligned(1024))) char lds[2 * T::STAGE];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
   int tm, tn;
-  tile_of(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
+  tile_of(blockIdx.x % (tiles_m * tiles_n), tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
+  const int split_id = blockIdx.x / (tiles_m * tiles_n), t0 = split_id * a.dw_len, len = min(a.dw_len, a.rows - t0);
   Acc<T> acc;
   zero_acc<T>(acc);
-  const Operand A = {a.dz + (long)tm * T::TM * 2, a.ldz * 2, a.dz_plane, a.rows, (int)a.ldz - tm * T::TM, nullptr};
-  const Operand B = {a.h + (long)tn * T::TN * 2, a.h_row, a.h_plane, a.rows, a.hidden - tn * T::TN, a.used};
-  product<D, T, true, true, true>(acc, lds, A, B, a.rows, SPLIT ? 3 : 1, wave, lane);
+  const Operand A = {a.dz + (t0 * a.ldz + tm * T::TM) * 2, a.ldz * 2, a.dz_plane, len, (int)a.ldz - tm * T::TM, nullptr};
+  const Operand B = {a.h + t0 * a.h_row + (long)tn * T::TN * 2, a.h_row, a.h_plane, len, a.hidden - tn * T::TN, a.used + t0 / 64};
+  if (len > 0) product<D, T, true, true, true>(acc, lds, A, B, len, SPLIT ? 3 : 1, wave, lane);
   float by = __is_same(D, TsgBf16) ? 1.0f : 1.0f / scale_of(*a.gmax);
   if (SPLIT) by /= a.scales[0];
   const int wm = wave / T::WN * 32 * T::XM, wn = wave % T::WN * 32 * T::XN;
@@ -439,7 +437,10 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dw_kernel(XentArgs a, i
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int m = tm * T::TM + wm + 32 * x + (i & 3) + 8 * (i >> 2) + 4 * h, k = tn * T::TN + wn + 32 * y + (lane & 31);
-        if (m < a.vc && k < a.hidden) reinterpret_cast<OUT*>(a.dw + (long)(a.v0 + m) * a.dw_row)[k] = (OUT)(acc[x][y][i] * by);
+        if (m < a.vc && k < a.hidden) {
+          if (a.dw_part) a.dw_part[((long)split_id * a.vc + m) * a.hidden + k] = acc[x][y][i];
+          else reinterpret_cast<OUT*>(a.dw + (long)(a.v0 + m) * a.dw_row)[k] = (OUT)(acc[x][y][i] * by);
+        }
       }
 }
 
@@ -476,18 +477,20 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dh_kernel(XentArgs a, i
       }
 }
 
-// Four elements per thread; PARTS of the workgroup's waves share the stretches (1 or 4)
+// A gradient from its stretches' sums: [splits][n / hidden][hidden] f32 -> rows of OUT, by 1 / (scale of dz) (scaled) and 1 / *other.
+// Four elements per thread; PARTS of the workgroup's waves share the stretches (1 or 4).
 template <typename OUT, int PARTS>
-__global__ __launch_bounds__(256) void xent_dh_out_kernel(XentArgs a, OUT* dh, long dh_row, int scaled) {
+__global__ __launch_bounds__(256) void xent_join_grad_kernel(const float* from, int splits, long n, int hidden, OUT* out, long out_row, const unsigned* gmax, int scaled,
+                                                             const float* other) {
   constexpr int WIDE = 256 / PARTS;
   __shared__ float4 join[PARTS][WIDE];
   const int part = threadIdx.x / WIDE, lane = threadIdx.x % WIDE;
-  const long i = ((long)blockIdx.x * WIDE + lane) * 4, n = (long)a.rows * a.hidden;
+  const long i = ((long)blockIdx.x * WIDE + lane) * 4;
   float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (i < n)
 #pragma unroll 4
-    for (int p = part; p < a.splits; p += PARTS) {
-      const float4 v = *reinterpret_cast<const float4*>(a.dh_part + p * n + i);
+    for (int p = part; p < splits; p += PARTS) {
+      const float4 v = *reinterpret_cast<const float4*>(from + p * n + i);
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
   if (PARTS > 1) {
@@ -501,9 +504,9 @@ __global__ __launch_bounds__(256) void xent_dh_out_kernel(XentArgs a, OUT* dh, l
     }
   }
   if (i >= n) return;
-  float by = scaled ? 1.0f / scale_of(*a.gmax) : 1.0f;
-  if (__is_same(OUT, float)) by /= a.scales[1];
-  OUT* to = dh + (i / a.hidden) * dh_row + i % a.hidden;
+  float by = scaled ? 1.0f / scale_of(*gmax) : 1.0f;
+  if (__is_same(OUT, float)) by /= *other;
+  OUT* to = out + (i / hidden) * out_row + i % hidden;
   OUT v[4] = {(OUT)(s.x * by), (OUT)(s.y * by), (OUT)(s.z * by), (OUT)(s.w * by)};
   if (sizeof(OUT) == 4) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(v);
   else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(v);
@@ -597,7 +600,8 @@ __global__ __launch_bounds__(256) void xent_planes_kernel(Planes a) {
 // ------------------------------------------------------------------------------------------------------ host side
 struct Layout {
   size_t gmax, amax, planes, h_plane, w_plane, part, zt, g, used, dz, dz_plane, db, dh, total;
-  int vc, splits, split_len, dh_shape;
+  size_t dw;
+  int vc, splits, split_len, dh_shape, dw_shape, dw_splits, dw_len;
 };
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -657,6 +661,21 @@ Layout layout_of(const tsg_xent_desc* d, bool backward) {
     l.split_len = (int)(((vc + s - 1) / s + TK - 1) / TK * TK);
     l.splits = (int)((vc + l.split_len - 1) / l.split_len);
     l.dh = take((size_t)l.splits * T * K * 4);
+    // dW of a narrow state has few tiles too (40307 x 256: 158 of 256 x 256): cut the rows where that leaves the CUs less idle, each
+    // cut priced at 2 % for the sums it writes and reads again
+    l.dw_shape = shape_of((int64_t)vc, (int64_t)K);
+    l.dw_splits = 1;
+    const int64_t big = (int64_t)tsg_cdiv(vc, Big::TM) * tsg_cdiv(K, Big::TN);
+    if (big < 768 && big >= 32 && T >= 2048) {
+      double best = 1e9;
+      for (int c = 1; c <= 8 && T / c >= 1024; ++c) {
+        const double cost = (double)((big * c + 255) / 256) / c + 0.02 * c;
+        if (cost < best) best = cost, l.dw_splits = c;
+      }
+      l.dw_shape = BIG;
+    }
+    l.dw_len = (int)(((T + l.dw_splits - 1) / l.dw_splits + 63) / 64 * 64);
+    l.dw = l.dw_splits > 1 ? take((size_t)l.dw_splits * vc * K * 4) : 0;
   }
   l.total = at;
   return l;
@@ -678,7 +697,7 @@ int check_xent(const tsg_xent_desc* d, bool backward) {
   if (!backward && d->reduction && !d->loss) return TSG_E_INVALID;
   if (d->dtype == TSG_F32 && !d->scales) return TSG_E_INVALID;
   if (backward && (!d->d_loss || !d->dh || !d->dw || (d->bias && !d->dbias))) return TSG_E_INVALID;
-  if (backward && (d->dh_row < d->hidden || d->dw_row < d->hidden || d->dh_row % 4 || (uintptr_t)d->dh % 16)) return TSG_E_INVALID;
+  if (backward && (d->dh_row < d->hidden || d->dw_row < d->hidden || d->dh_row % 4 || d->dw_row % 4 || (uintptr_t)d->dh % 16 || (uintptr_t)d->dw % 16)) return TSG_E_INVALID;
   return 0;
 }
 
@@ -748,10 +767,10 @@ template <typename D, typename OUT> void backward_piece(XentArgs a, const tsg_xe
     const int tv = tsg_cdiv(a.vc, T::TM);
     hipLaunchKernelGGL((xent_dz_kernel<D, T, SPLIT>), dim3((unsigned)(tv * tt)), dim3(64 * T::WAVES), 0, s, a, tv, tt);
   });
-  with_tile(shape_of(a.vc, a.hidden), [&](auto t) {
+  with_tile(l.dw_shape, [&](auto t) {
     typedef decltype(t) T;
     const int tv = tsg_cdiv(a.vc, T::TM), tk = tsg_cdiv(a.hidden, T::TN);
-    hipLaunchKernelGGL((xent_dw_kernel<D, T, OUT>), dim3((unsigned)(tv * tk)), dim3(64 * T::WAVES), 0, s, a, tv, tk);
+    hipLaunchKernelGGL((xent_dw_kernel<D, T, OUT>), dim3((unsigned)(tv * tk * l.dw_splits)), dim3(64 * T::WAVES), 0, s, a, tv, tk);
   });
   with_tile(l.dh_shape, [&](auto t) {
     typedef decltype(t) T;
@@ -759,12 +778,14 @@ template <typename D, typename OUT> void backward_piece(XentArgs a, const tsg_xe
     hipLaunchKernelGGL((xent_dh_kernel<D, T, SPLIT>), dim3((unsigned)(tr * tk * l.splits)), dim3(64 * T::WAVES), 0, s, a, tr, tk);
   });
   if (d->bias) hipLaunchKernelGGL(xent_db_out_kernel<OUT>, dim3(tsg_cdiv(a.vc, 64)), dim3(256), 0, s, a, (OUT*)d->dbias, tt, scaled);
-  if (a.v0 + a.vc >= a.vocab)
-  {
-    const long quads = (long)a.rows * a.hidden / 4;
-    if (l.splits >= 16) hipLaunchKernelGGL((xent_dh_out_kernel<OUT, 4>), dim3((unsigned)((quads + 63) / 64)), dim3(256), 0, s, a, (OUT*)d->dh, (long)d->dh_row, scaled);
-    else hipLaunchKernelGGL((xent_dh_out_kernel<OUT, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, a, (OUT*)d->dh, (long)d->dh_row, scaled);
-  }
+  auto join = [&](const float* from, int splits, long n, OUT* out, long out_row, const float* other) {
+    if (splits >= 16)
+      hipLaunchKernelGGL((xent_join_grad_kernel<OUT, 4>), dim3((unsigned)((n / 4 + 63) / 64)), dim3(256), 0, s, from, splits, n, a.hidden, out, out_row, a.gmax, scaled, other);
+    else
+      hipLaunchKernelGGL((xent_join_grad_kernel<OUT, 1>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, from, splits, n, a.hidden, out, out_row, a.gmax, scaled, other);
+  };
+  if (a.dw_part) join(a.dw_part, l.dw_splits, (long)a.vc * a.hidden, (OUT*)d->dw + (long)a.v0 * d->dw_row, d->dw_row, a.scales);
+  if (a.v0 + a.vc >= a.vocab) join(a.dh_part, l.splits, (long)a.rows * a.hidden, (OUT*)d->dh, d->dh_row, SPLIT ? a.scales + 1 : nullptr);
 }
 
 }  // namespace
@@ -811,6 +832,8 @@ extern "C" int tsg_xent_backward(const tsg_xent_desc* d, void* stream) {
   a.db_part = d->bias ? (float*)(ws + l.db) : nullptr;
   a.dh_part = (float*)(ws + l.dh);
   a.splits = l.splits, a.split_len = l.split_len;
+  a.dw_part = l.dw_splits > 1 ? (float*)(ws + l.dw) : nullptr;
+  a.dw_len = l.dw_len;
   a.dw = (char*)d->dw, a.dw_row = d->dw_row * (d->dtype == TSG_F32 ? 4 : 2);
   a.ldz = l.vc;
   if (d->dtype == TSG_F32) make_planes(d, a, l, true, s);
