@@ -12,6 +12,7 @@ first order: differentiating a gradient raises.
 """
 import ctypes as C
 import math
+import weakref
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -46,48 +47,67 @@ def _dtype(what, *tensors):
     return DTYPES[dt]
 
 
-def _hold_leaves(*leaves):
-    """The gradient accumulators of the leaves, to be held over the call that uses them.
+def _stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev.index)     # torch.cuda.current_stream(dev).cuda_stream without the object
 
-    Capturing a backward while an eager autograd graph of the same leaf is alive ends the process: the accumulator that graph
-    keeps is tied to the stream it was made on, and joining that stream breaks the capture.  So every eager call leaves its
-    stream on the accumulators, and a call under capture that finds another one refuses."""
-    held = []
-    if not torch.is_grad_enabled():
-        return held
-    here = torch.cuda.current_stream().cuda_stream
-    capturing = torch.cuda.is_current_stream_capturing()
-    for t in leaves:
-        if t is None or not t.requires_grad or not t.is_leaf:
-            continue
-        node = torch.autograd.graph.get_gradient_edge(t).node
-        if capturing and node.metadata.get('ts_trajgen_amd.stream', here) != here:
-            raise RuntimeError('capture of a backward while an eager autograd graph of the same leaf is alive: drop the '
-                               'eager results (del, or .detach() what is kept) before capturing')
-        node.metadata['ts_trajgen_amd.stream'] = here
-        held.append(node)
-    return held
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(entry, d, dev):
+    """entry(d, the current stream of dev) of libtsg, with dev current: a call is a few microseconds of host time all told."""
+    fn = getattr(_lib.lib(), entry)
+    if torch._C._cuda_getDevice() == dev.index:
+        rc = fn(C.byref(d), _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(C.byref(d), _stream(dev))
+    if rc:
+        _lib.check(rc, entry)
+
+
+_LIVE = weakref.WeakSet()     # the operators' own nodes in autograd graphs that are alive
+
+
+def _enter(ctx, *inputs):
+    """Notes a node, its leaves and the stream it was made on.
+
+    Capturing a backward while an eager autograd graph of the same leaf is alive ends the process: the leaf's gradient
+    accumulator is tied to the stream that graph was made on, and joining that stream breaks the capture.  So a call under
+    capture that finds a living node of another stream over one of its leaves refuses."""
+    leaves = {id(t) for t in inputs if t is not None and t.requires_grad and t.is_leaf}
+    if not leaves:
+        return
+    here = _stream(inputs[0].device)
+    if torch.cuda.is_current_stream_capturing():
+        for node in list(_LIVE):
+            if node.stream != here and not leaves.isdisjoint(node.leaves):
+                raise RuntimeError('capture of a backward while an eager autograd graph of the same leaf is alive: drop the '
+                                   'eager results (del, or .detach() what is kept) before capturing')
+    ctx.leaves, ctx.stream = leaves, here
+    _LIVE.add(ctx)
 
 
 # ---------------------------------------------------------------------------------------------------------- dropout
 def _drop(x, p, seed, site, step):
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     x = x.contiguous()
+    y = torch.empty_like(x)
     d = _lib.DropoutDesc()
     d.n, d.dtype, d.site, d.seed, d.p = x.numel(), DTYPES[x.dtype], site, seed, p
     if torch.is_tensor(step):
-        d.step_dev = _lib.ptr(step)
+        d.step_dev = _ptr(step)
     else:
         d.step = step
-    d.x, d.y = _lib.ptr(x), _lib.ptr(y)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().tsg_dropout(C.byref(d), _lib.current_stream()), 'tsg_dropout')
+    d.x, d.y = _ptr(x), _ptr(y)
+    _call('tsg_dropout', d, x.device)
     return y
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, site, step):
+        _enter(ctx, x)
         ctx.cfg = (p, seed, site)
         if torch.is_tensor(step):
             ctx.save_for_backward(step)     # advancing it before the backward is an error that autograd reports
@@ -129,10 +149,7 @@ def dropout(x, p, seed, site=0, step=0):
     p, seed, site = float(p), int(seed), int(site)
     step = step if torch.is_tensor(step) else int(step)
     check_rng('dropout', p, seed, site, step, dev)
-    held = _hold_leaves(x)
-    y = _Dropout.apply(x, p, seed, site, step)
-    del held
-    return y
+    return _Dropout.apply(x, p, seed, site, step)
 
 
 # -------------------------------------------------------------------------------------------------------- attention
@@ -156,12 +173,12 @@ def _attn_desc(q, k, v, q_ptr, k_ptr, scale, out, stats):
     d.dtype, d.n_seq = DTYPES[q.dtype], q_ptr.numel() - 1
     d.heads, d.kv_heads, d.dim, d.scale = q.shape[1], k.shape[1], q.shape[2], scale
     d.n_q, d.n_k = q.shape[0], k.shape[0]
-    d.q_ptr, d.k_ptr = _lib.ptr(q_ptr), _lib.ptr(k_ptr)
+    d.q_ptr, d.k_ptr = _ptr(q_ptr), _ptr(k_ptr)
     for name, t in (('q', q), ('k', k), ('v', v), ('out', out)):
-        setattr(d, name, _lib.ptr(t))
+        setattr(d, name, _ptr(t))
         setattr(d, name + '_row', t.stride(0))
         setattr(d, name + '_head', t.stride(1))
-    d.stats = _lib.ptr(stats)
+    d.stats = _ptr(stats)
     return d
 
 
@@ -170,14 +187,14 @@ def _attn_workspace(d, dev, backward):
     _lib.check(_lib.lib().tsg_attn_workspace(C.byref(d), C.byref(sizes[0]), C.byref(sizes[1])), 'tsg_attn_workspace')
     need = sizes[backward].value
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    d.workspace, d.workspace_bytes = _lib.ptr(ws), need
+    d.workspace, d.workspace_bytes = _ptr(ws), need
     return ws
 
 
 class _CausalAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_ptr, k_ptr, scale):
-        L = _lib.lib()
+        _enter(ctx, q, k, v)
         dim, per = q.shape[2], 4 if q.dtype == torch.float32 else 8
         wide = -(-dim // per) * per
         ql, kl, vl = (_laid_out(t.detach(), per, wide) for t in (q, k, v))
@@ -187,11 +204,10 @@ class _CausalAttention(torch.autograd.Function):
         rest = None
         if q.dtype != torch.float32 and any(ctx.needs_input_grad[:3]):
             rest = torch.empty(out.shape, dtype=q.dtype, device=q.device)
-            d.out_rest = _lib.ptr(rest)
+            d.out_rest = _ptr(rest)
         ws = _attn_workspace(d, q.device, 0)  # noqa: F841  (held until the launches are on the stream)
         if q.shape[0] and k.shape[0]:
-            with torch.cuda.device(q.device):
-                _lib.check(L.tsg_attn_forward(C.byref(d), _lib.current_stream()), 'tsg_attn_forward')
+            _call('tsg_attn_forward', d, q.device)
         else:
             out.zero_()
         if any(ctx.needs_input_grad[:3]):
@@ -211,17 +227,16 @@ class _CausalAttention(torch.autograd.Function):
         dq, dk, dv = (torch.empty(t.shape[:2] + (wide,), dtype=t.dtype, device=t.device) for t in (q, k, v))
         if q.shape[0] and k.shape[0]:
             d = _attn_desc(ql, kl, vl, q_ptr, k_ptr, ctx.scale, ol, stats)
-            d.out_rest = _lib.ptr(rest)
+            d.out_rest = _ptr(rest)
             delta = torch.empty(stats.shape[:2], dtype=torch.float32, device=q.device)
-            d.d_out, d.d_out_row, d.d_out_head = _lib.ptr(gl), gl.stride(0), gl.stride(1)
+            d.d_out, d.d_out_row, d.d_out_head = _ptr(gl), gl.stride(0), gl.stride(1)
             for name, t in (('dq', dq), ('dk', dk), ('dv', dv)):
-                setattr(d, name, _lib.ptr(t))
+                setattr(d, name, _ptr(t))
                 setattr(d, name + '_row', t.stride(0))
                 setattr(d, name + '_head', t.stride(1))
-            d.delta = _lib.ptr(delta)
+            d.delta = _ptr(delta)
             ws = _attn_workspace(d, q.device, 1)  # noqa: F841
-            with torch.cuda.device(q.device):
-                _lib.check(_lib.lib().tsg_attn_backward(C.byref(d), _lib.current_stream()), 'tsg_attn_backward')
+            _call('tsg_attn_backward', d, q.device)
         else:
             for t in (dq, dk, dv):
                 t.zero_()
@@ -263,10 +278,7 @@ def causal_attention(q, k, v, seq_ptr, kv_ptr=None, scale=None):
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError('causal_attention: scale is positive, got %r' % scale)
-    held = _hold_leaves(q, k, v)
-    out = _CausalAttention.apply(q, k, v, seq_ptr, kv_ptr, scale)
-    del held
-    return out
+    return _CausalAttention.apply(q, k, v, seq_ptr, kv_ptr, scale)
 
 
 # ---------------------------------------------------------------------------------------------------- cross entropy
@@ -287,9 +299,9 @@ def _xent_desc(h, w, bias, target, ignore, reduction, stats, scales):
     d = _lib.XentDesc()
     d.dtype, d.hidden, d.reduction = DTYPES[h.dtype], h.shape[1], reduction
     d.n_rows, d.n_vocab, d.ignore_index = h.shape[0], w.shape[0], ignore
-    d.h, d.w, d.bias = _lib.ptr(h), _lib.ptr(w), _lib.ptr(bias)
+    d.h, d.w, d.bias = _ptr(h), _ptr(w), _ptr(bias)
     d.h_row, d.w_row = max(h.stride(0), h.shape[1]), max(w.stride(0), w.shape[1])
-    d.target, d.stats, d.scales = _lib.ptr(target), _lib.ptr(stats), _lib.ptr(scales)
+    d.target, d.stats, d.scales = _ptr(target), _ptr(stats), _ptr(scales)
     return d
 
 
@@ -297,13 +309,14 @@ def _xent_workspace(d, dev, backward):
     sizes = C.c_size_t(), C.c_size_t()
     _lib.check(_lib.lib().tsg_xent_workspace(C.byref(d), C.byref(sizes[0]), C.byref(sizes[1])), 'tsg_xent_workspace')
     ws = torch.empty(sizes[backward].value, dtype=torch.uint8, device=dev)
-    d.workspace, d.workspace_bytes = _lib.ptr(ws), ws.numel()
+    d.workspace, d.workspace_bytes = _ptr(ws), ws.numel()
     return ws
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, w, bias, target, ignore, reduction):
+        _enter(ctx, h, w, bias)
         wide = -(-h.shape[1] // 8) * 8
         hl, wl = _rows_for(h.detach(), wide), _rows_for(w.detach(), wide)
         bl = None if bias is None else bias.detach().contiguous()
@@ -313,10 +326,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         loss = rows if reduction == 0 else torch.empty((), dtype=torch.float32, device=h.device)
         scales = torch.empty(2, dtype=torch.float32, device=h.device) if h.dtype == torch.float32 else None
         d = _xent_desc(hl, wl, bl, target, ignore, reduction, stats, scales)
-        d.row_loss, d.loss = _lib.ptr(rows), _lib.ptr(loss)
+        d.row_loss, d.loss = _ptr(rows), _ptr(loss)
         ws = _xent_workspace(d, h.device, 0)
-        with torch.cuda.device(h.device):
-            _lib.check(_lib.lib().tsg_xent_forward(C.byref(d), _lib.current_stream()), 'tsg_xent_forward')
+        _call('tsg_xent_forward', d, h.device)
         del ws
         if any(ctx.needs_input_grad[:3]):
             ctx.save_for_backward(h, w, bias, target, stats, scales)
@@ -335,11 +347,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
         dh = torch.empty((h.shape[0], wide), dtype=h.dtype, device=h.device)
         dw = torch.empty((w.shape[0], wide), dtype=h.dtype, device=h.device)
         db = None if bias is None else torch.empty_like(bl)
-        d.d_loss, d.dh, d.dw, d.dbias = _lib.ptr(d_loss), _lib.ptr(dh), _lib.ptr(dw), _lib.ptr(db)
+        d.d_loss, d.dh, d.dw, d.dbias = _ptr(d_loss), _ptr(dh), _ptr(dw), _ptr(db)
         d.dh_row = d.dw_row = wide
         ws = _xent_workspace(d, h.device, 1)
-        with torch.cuda.device(h.device):
-            _lib.check(_lib.lib().tsg_xent_backward(C.byref(d), _lib.current_stream()), 'tsg_xent_backward')
+        _call('tsg_xent_backward', d, h.device)
         del ws
         if wide != width:
             dh, dw = dh[:, :width].contiguous(), dw[:, :width].contiguous()
@@ -368,7 +379,4 @@ def linear_cross_entropy(h, weight, target, bias=None, ignore_index=-100, reduct
         raise ValueError('linear_cross_entropy: target is int64 [rows], got %s %s' % (target.dtype, tuple(target.shape)))
     if reduction not in REDUCTIONS:
         raise ValueError("linear_cross_entropy: reduction is 'none', 'sum' or 'mean', got %r" % (reduction,))
-    held = _hold_leaves(h, weight, bias)
-    loss = _LinearCrossEntropy.apply(h, weight, bias, target, int(ignore_index), REDUCTIONS[reduction])
-    del held
-    return loss
+    return _LinearCrossEntropy.apply(h, weight, bias, target, int(ignore_index), REDUCTIONS[reduction])
