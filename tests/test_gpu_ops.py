@@ -237,6 +237,19 @@ def test_attention_views_are_read_by_their_strides():
         assert y.grad.shape == y.shape and torch.isfinite(y.grad.float()).all()
 
 
+def test_attention_single_rows_read_subnormal_keys():
+    # keys below f16's smallest normal number still have their products
+    from ts_trajgen_amd import ops
+    g = torch.Generator().manual_seed(4)
+    q = (torch.randn(1, 4, 64, generator=g) * 1e4).half()      # inside f16: its largest is 65504
+    k = (torch.randn(300, 1, 64, generator=g) * 1e-5).half()
+    v = torch.randn(300, 1, 64, generator=g).half()
+    want = plain_attention(q, k, v, [0, 1], [0, 300], 1.0)[0]
+    out = ops.causal_attention(q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor([0, 1], dtype=torch.int32, device=DEV),
+                               torch.tensor([0, 300], dtype=torch.int32, device=DEV), 1.0)
+    assert rel(out, want) < bound(torch.float16)
+
+
 def test_attention_extreme_scores():
     # one key dominates by more than f32's exponent range, and scores of the lowest finite size
     from ts_trajgen_amd import ops

@@ -10,7 +10,7 @@
 // Trajectories of a few dozen positions fill a tile that way.  The same holds for a tile of keys and the query
 // rows that see them.  No lengths are needed on the host.  Rows of no sequence give zeros.
 //
-// Tile kernels (dim <= 256): a workgroup of four waves owns 128 rows, 32 per wave (f32: 64 and 16); the wave computes the TRANSPOSED
+// Tile kernels (16-bit types, dim <= 256): a workgroup of four waves owns 128 rows, 32 per wave; the wave computes the TRANSPOSED
 // score tile (A = keys, B = its rows), so that a lane holds one row: the softmax statistics are one register per
 // lane, and the probabilities feed the next product as they stand (tsg_mma.h).  Scores, statistics and outputs are held
 // in f32; p and ds are rounded to the operand type for the matrix cores (nearest even, 2^-9 relative for bf16, which is
@@ -215,10 +215,9 @@ template <typename D> constexpr int rows_per_wg() { return TsgElem<D>::BYTES == 
 
 // ------------------------------------------------------------------------------------------------- forward, tiles
 template <typename D, int DP, int BK>
-__global__ __launch_bounds__(256, (DP > 128 && TsgElem<D>::BYTES == 2) ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
   typedef TsgElem<D> E;
   typedef typename E::Acc Acc;
-  constexpr bool F32 = E::BYTES == 4;
   constexpr int W = E::W, PARTS = 64 / W, CH = DP / E::EPC, NF = CH / PARTS, ND = DP / W, NB = BK / W, TILE = BK * CH * 16;
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
   __shared__ int edge[8];
@@ -242,7 +241,7 @@ __global__ __launch_bounds__(256, (DP > 128 && TsgElem<D>::BYTES == 2) ? 1 : 2) 
   float m = -INFINITY, l = 0.0f;
   const char* kbase = a.k + kvh * a.k_head;
   const char* vbase = a.v + kvh * a.v_head;
-  TsgLoader<BK, CH, 4, F32> kl, vl;
+  TsgLoader<BK, CH, 4> kl, vl;
   kl.init(a.k_row, a.chunks, tsg_lds_addr(lds), wave, lane);
   vl.init(a.v_row, a.chunks, tsg_lds_addr(lds) + TILE, wave, lane);
   auto fetch = [&](int k0, int buf) {
@@ -266,7 +265,7 @@ __global__ __launch_bounds__(256, (DP > 128 && TsgElem<D>::BYTES == 2) ? 1 : 2) 
 #pragma unroll
       for (int s = 0; s < NF; ++s) tsg_mma<D>(tsg_row_frag<D>(row, s, W * n * CH * 16), qf[s], z[n]);
     }
-    if constexpr (!F32) tsg_interleave<NB * NF, NB * NF, 6, 1>();
+    tsg_interleave<NB * NF, NB * NF, 6, 1>();
     __builtin_amdgcn_s_setprio(0);
     if (k0 < b.in_lo || k0 + BK > b.in_hi) {
       keep_branch();
@@ -298,10 +297,9 @@ __global__ __launch_bounds__(256, (DP > 128 && TsgElem<D>::BYTES == 2) ? 1 : 2) 
       m = top;
     }
     const float off = m == -INFINITY ? 0.0f : m;  // nothing seen yet: exp2(-inf) = 0, not NaN
-    // f32 takes the reference off before the scaling (all of z - m's bits; products of the type's lowest value stay finite); for
-    // the 16-bit types one fused operation does, where the scaling cannot overflow, and what rounding m scale2 leaves over goes
-    // into the row's logarithm at the end.
-    if (!F32 && a.scale2 <= 1.0f) {
+    // One fused operation takes the reference off, where the scaling cannot overflow, and what rounding m scale2 leaves over goes
+    // into the row's logarithm at the end; else it comes off before the scaling (products of the type's lowest value stay finite).
+    if (a.scale2 <= 1.0f) {
       const float off2 = off * a.scale2;
 #pragma unroll
       for (int n = 0; n < NB; ++n)
@@ -327,25 +325,24 @@ __global__ __launch_bounds__(256, (DP > 128 && TsgElem<D>::BYTES == 2) ? 1 : 2) 
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) p.template mma<CH>(col, dt, TILE + W * n * CH * 16, acc[dt]);
     }
-    if constexpr (!F32) tsg_interleave<NB * ND * 4, NB * ND * 2, 8, 2>();
+    tsg_interleave<NB * ND * 4, NB * ND * 2, 8, 2>();
     __builtin_amdgcn_s_setprio(0);
   }
   l = parts_sum<W>(l);
   if (t < a.n_q) {
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
     store_rows<D, ND>(acc, a.out + (long)t * a.o_row + head * a.o_head, by, a.dim, h);
-    if (!F32 && a.rest) store_rows<D, ND, true>(acc, a.rest + ((long)t * a.heads + head) * a.dim * E::BYTES, by, a.dim, h);
-    const float left = !F32 && a.scale2 <= 1.0f ? __builtin_fmaf(m, a.scale2, -(m * a.scale2)) : 0.0f;
+    if (a.rest) store_rows<D, ND, true>(acc, a.rest + ((long)t * a.heads + head) * a.dim * E::BYTES, by, a.dim, h);
+    const float left = a.scale2 <= 1.0f ? __builtin_fmaf(m, a.scale2, -(m * a.scale2)) : 0.0f;
     if (h == 0) a.stat[(long)head * a.n_q + t] = l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l) - left);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ backward, tiles: dq
 template <typename D, int DP, int BK>
-__global__ __launch_bounds__(256, (DP > 128 && TsgElem<D>::BYTES == 2) ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
   typedef TsgElem<D> E;
   typedef typename E::Acc Acc;
-  constexpr bool F32 = E::BYTES == 4;
   constexpr int W = E::W, PARTS = 64 / W, CH = DP / E::EPC, NF = CH / PARTS, ND = DP / W, NB = BK / W, TILE = BK * CH * 16;
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
   __shared__ int edge[8];
@@ -367,7 +364,7 @@ __global__ __launch_bounds__(256, (DP > 128 && TsgElem<D>::BYTES == 2) ? 1 : 2) 
       const int c = PARTS * s + h;
       const bool ok = t < a.n_q && c < a.chunks;
       delta += frag_dot<D>(chunk_of(orow, c, ok), gf[s]);
-      if (!F32 && a.rest) delta += frag_dot<D>(chunk_of(a.rest + ((long)t * a.heads + head) * a.dim * E::BYTES, c, ok), gf[s]);
+      if (a.rest) delta += frag_dot<D>(chunk_of(a.rest + ((long)t * a.heads + head) * a.dim * E::BYTES, c, ok), gf[s]);
     }
     delta = parts_sum<W>(delta);
     if (t < a.n_q) {
@@ -385,7 +382,7 @@ __global__ __launch_bounds__(256, (DP > 128 && TsgElem<D>::BYTES == 2) ? 1 : 2) 
     for (int i = 0; i < E::REGS; ++i) acc[dt][i] = 0.0f;
   const char* kbase = a.k + kvh * a.k_head;
   const char* vbase = a.v + kvh * a.v_head;
-  TsgLoader<BK, CH, 4, F32> kl, vl;
+  TsgLoader<BK, CH, 4> kl, vl;
   kl.init(a.k_row, a.chunks, tsg_lds_addr(lds), wave, lane);
   vl.init(a.v_row, a.chunks, tsg_lds_addr(lds) + TILE, wave, lane);
   auto fetch = [&](int k0, int buf) {
@@ -413,7 +410,7 @@ __global__ __launch_bounds__(256, (DP > 128 && TsgElem<D>::BYTES == 2) ? 1 : 2) 
         tsg_mma<D>(tsg_row_frag<D>(row, s, W * n * CH * 16), qf[s], z);
         tsg_mma<D>(tsg_row_frag<D>(row, s, TILE + W * n * CH * 16), gf[s], dp);
       }
-      if constexpr (!F32) tsg_interleave<2 * NF, 2 * NF, 6, 1>();
+      tsg_interleave<2 * NF, 2 * NF, 6, 1>();
 #pragma unroll
       for (int i = 0; i < E::REGS; ++i) z[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i] - st.x, a.scale2, -st.y)) * dp[i];
       if (edge_tile) {
@@ -429,21 +426,20 @@ __global__ __launch_bounds__(256, (DP > 128 && TsgElem<D>::BYTES == 2) ? 1 : 2) 
       ds.set(z);
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) ds.template mma<CH>(col, dt, W * n * CH * 16, acc[dt]);
-      if constexpr (!F32) tsg_interleave<ND * 4, ND * 2, 8, 2>();
+      tsg_interleave<ND * 4, ND * 2, 8, 2>();
     }
   }
   if (t < a.n_q) store_rows<D, ND>(acc, a.dq + (long)t * a.dq_row + head * a.dq_head, a.scale, a.dim, h);
 }
 
 // ------------------------------------------------------------------------------------------ backward, tiles: dk and dv
-// PART 0: both; 1: dv only; 2: dk only (16-bit types at 256 wide: keys, values and both sums do not fit the registers at once)
+// PART 0: both; 1: dv only; 2: dk only (256 wide: keys, values and both sums do not fit the registers at once)
 // VL: the values' fragments are read from LDS in every step instead of held in registers, which then suffice without spills
-// (16-bit types 128 wide at two waves a SIMD, 256 wide at one; f32 256 wide).
+// (128 wide at two waves a SIMD, 256 wide at one).
 template <typename D, int DP, int BQ, int PART, bool VL>
-__global__ __launch_bounds__(256, DP * TsgElem<D>::BYTES > 256 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
   typedef TsgElem<D> E;
   typedef typename E::Acc Acc;
-  constexpr bool F32 = E::BYTES == 4;
   constexpr int W = E::W, PARTS = 64 / W, CH = DP / E::EPC, NF = CH / PARTS, ND = DP / W, NB = BQ / W, TILE = BQ * CH * 16;
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + (VL ? 4 * W * CH * 16 : 0)];
   __shared__ __attribute__((aligned(16))) float stat[2][3][BQ];  // maximum, log2 of the sum, delta
@@ -457,7 +453,7 @@ __global__ __launch_bounds__(256, DP * TsgElem<D>::BYTES > 256 ? 1 : 2) void att
   load_frags<PARTS>(kf, a.k + (long)j * a.k_row + kvh * a.k_head, j < a.n_k, a.chunks, h);
   if constexpr (PART != 1 && VL) {
     // the wave's own rows: no other wave reads them, and the first step waits for them
-    TsgLoader<W, CH, 1, F32> vl;
+    TsgLoader<W, CH, 1> vl;
     vl.init(a.v_row, a.chunks, tsg_lds_addr(lds) + 4 * TILE + wave * W * CH * 16, 0, lane);
     const int j0 = tile * (4 * W) + wave * W;
     vl.load(a.v + (long)j0 * a.v_row + kvh * a.v_head, a.n_k - j0, a.chunks * 16, 0);
@@ -484,7 +480,7 @@ __global__ __launch_bounds__(256, DP * TsgElem<D>::BYTES > 256 ? 1 : 2) void att
     if (p.t0 >= b.hi) p.t0 = b.lo, ++p.head;
     return p;
   };
-  TsgLoader<BQ, CH, 4, F32> ql, gl;
+  TsgLoader<BQ, CH, 4> ql, gl;
   ql.init(a.q_row, a.chunks, tsg_lds_addr(lds), wave, lane);
   gl.init(a.do_row, a.chunks, tsg_lds_addr(lds) + TILE, wave, lane);
   auto fetch = [&](Step p, int buf) {
@@ -542,7 +538,7 @@ __global__ __launch_bounds__(256, DP * TsgElem<D>::BYTES > 256 ? 1 : 2) void att
           tsg_mma<D>(tsg_row_frag<D>(row, s, TILE + W * n * CH * 16),
                      VL ? tsg_row_frag<D>(vrow, s, 0) : vf[VL ? 0 : s], dp);
       }
-      if constexpr (!F32) tsg_interleave<(PART == 1 ? 1 : VL ? 3 : 2) * NF, (PART == 1 ? 1 : 2) * NF, 6, PART != 1 && VL ? 2 : 1>();
+      tsg_interleave<(PART == 1 ? 1 : VL ? 3 : 2) * NF, (PART == 1 ? 1 : 2) * NF, 6, PART != 1 && VL ? 2 : 1>();
 #pragma unroll
       for (int g = 0; g < E::REGS / 4; ++g) {
         const float4 ms = *reinterpret_cast<const float4*>(&stat[buf][0][W * n + 8 * g + 4 * h]);
@@ -870,27 +866,47 @@ template <typename D> __global__ __launch_bounds__(256) void attn_dkv_join_kerne
 // each, NC of them), so a wave reads 64 / LPR keys at once; every such lane group keeps its own running maximum, sum and
 // weighted values for the G heads that share the key, joined at the end through LDS, and over the splits by
 // attn_join_kernel.  Bound by reading the keys and values once.
-template <typename D> struct Chunk {
-  float v[TsgElem<D>::EPC];
-  __device__ __forceinline__ void set(tsg_u4 u) {
-    typedef typename D::type T;
-    typedef T T2 __attribute__((ext_vector_type(2)));
+template <typename D> __device__ __forceinline__ float chunk_dot(tsg_u4 a, tsg_u4 b, float s) {  // two products an instruction
+  typedef typename D::type T;
+  typedef T T2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const unsigned x = u[w];
+  for (int w = 0; w < 4; ++w) {
+    const unsigned x = a[w], y = b[w];
+    if constexpr (__is_same(D, TsgBf16)) s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(T2, x), __builtin_bit_cast(T2, y), s, false);
+    else s = __builtin_amdgcn_fdot2(__builtin_bit_cast(T2, x), __builtin_bit_cast(T2, y), s, false);
+  }
+  return s;
+}
+template <> __device__ __forceinline__ float chunk_dot<TsgF32>(tsg_u4 a, tsg_u4 b, float s) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) s = __builtin_fmaf(__uint_as_float(a[w]), __uint_as_float(b[w]), s);
+  return s;
+}
+template <typename D> __device__ __forceinline__ void chunk_to_f32(tsg_u4 u, float (&v)[TsgElem<D>::EPC]) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const unsigned x = u[w];
+    if constexpr (TsgElem<D>::BYTES == 4) {
+      v[w] = __uint_as_float(x);
+    } else {
+      typedef typename D::type T;
+      typedef T T2 __attribute__((ext_vector_type(2)));
       const T2 p = __builtin_bit_cast(T2, x);
       v[2 * w] = (float)p.x;
       v[2 * w + 1] = (float)p.y;
     }
   }
-};
-template <> struct Chunk<TsgF32> {
-  float v[4];
-  __device__ __forceinline__ void set(tsg_u4 u) {
+}
+// sum over the LPR lanes of a key: inside a row of 16 lanes by DPP (no trip through LDS), beyond it by shuffles
+template <int LPR> __device__ __forceinline__ float over_lanes(float v) {
+  v += tsg_dpp<0xB1>(v);
+  v += tsg_dpp<0x4E>(v);
+  v += tsg_dpp<0x141>(v);
+  if (LPR > 8) v += tsg_dpp<0x140>(v);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) v[w] = __uint_as_float(u[w]);
-  }
-};
+  for (int w = 16; w < LPR; w <<= 1) v += __shfl_xor(v, w, 64);
+  return v;
+}
 
 template <typename D, int LPR, int NC, int G>
 __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
@@ -910,7 +926,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
   keys_of_row(a, t, t, lo, hi);
   const long span = hi - lo;
   const int j0 = lo + (int)(span * split / a.n_split), j1 = lo + (int)(span * (split + 1) / a.n_split);
-  Chunk<D> qv[G][NC];
+  tsg_u4 qv[G][NC];
   float o[G][NE], m[G], l[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
@@ -921,7 +937,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
       const int ch = part + c * LPR;
       tsg_u4 u = {0u, 0u, 0u, 0u};
       if (g < n_heads && ch < a.chunks) u = *reinterpret_cast<const tsg_u4*>(row + ch * 16);
-      qv[g][c].set(u);
+      qv[g][c] = u;
     }
 #pragma unroll
     for (int e = 0; e < NE; ++e) o[g][e] = 0.0f;
@@ -949,29 +965,25 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
           for (int u = 0; u < U; ++u) kr[u][c] = vr[u][c] = tsg_u4{0u, 0u, 0u, 0u};
         }
     }
+    if (j + (U - 1) * GROUPS >= j1) {  // a key behind the end was read again: its value must not enter, not even times 0
+      keep_branch();
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j + u * GROUPS >= j1) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) vr[u][c] = tsg_u4{0u, 0u, 0u, 0u};
+        }
+    }
     float z[G][U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      Chunk<D> kc[NC];
-#pragma unroll
-      for (int c = 0; c < NC; ++c) kc[c].set(kr[u][c]);
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         float s = 0.0f;
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int e = 0; e < EPC; ++e) s += kc[c].v[e] * qv[g][c].v[e];
-        z[g][u] = s;
-      }
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-#pragma unroll
-        for (int w = LPR / 2; w > 0; w >>= 1) z[g][u] += __shfl_xor(z[g][u], w, 64);
-        if (j + u * GROUPS >= j1) z[g][u] = -INFINITY;
+        for (int c = 0; c < NC; ++c) s = chunk_dot<D>(kr[u][c], qv[g][c], s);
+        s = over_lanes<LPR>(s);
+        z[g][u] = j + u * GROUPS >= j1 ? -INFINITY : s;
       }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -991,18 +1003,16 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      Chunk<D> vc[NC];
-      const bool in = j + u * GROUPS < j1;  // a key behind the end was read again: its value must not enter, not even times 0
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int c = 0; c < NC; ++c) vc[c].set(vr[u][c]);
+      for (int c = 0; c < NC; ++c) {
+        float v[EPC];
+        chunk_to_f32<D>(vr[u][c], v);
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int e = 0; e < EPC; ++e) o[g][c * EPC + e] += in ? z[g][u] * vc[c].v[e] : 0.0f;
-    }
+          for (int e = 0; e < EPC; ++e) o[g][c * EPC + e] = __builtin_fmaf(z[g][u], v[e], o[g][c * EPC + e]);
+      }
   }
   // join the lane groups: common maximum, then sums over the groups of a wave (shuffles) and over the waves (LDS)
   if (part == 0)
@@ -1013,10 +1023,12 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     float v = -INFINITY;
+#pragma unroll 4
     for (int x = 0; x < GROUPS; ++x) v = fmaxf(v, st_m[x][g]);
     top[g] = v;
     const float off = v == -INFINITY ? 0.0f : v;
     float s = 0.0f;
+#pragma unroll 4
     for (int x = 0; x < GROUPS; ++x) s += st_l[x][g] * __builtin_amdgcn_exp2f((st_m[x][g] - off) * a.scale2);
     sum[g] = s;
     const float by = __builtin_amdgcn_exp2f((m[g] - off) * a.scale2);
@@ -1261,15 +1273,15 @@ template <typename D> int forward_of(const tsg_attn_desc* d, hipStream_t s) {
     if (a.n_split > 1) hipLaunchKernelGGL(attn_join_kernel<D>, dim3((unsigned)((long)a.n_q * a.heads)), dim3(64), 0, s, a);
   } else {
     const dim3 grid((unsigned)(tsg_cdiv(a.n_q, rows_per_wg<D>()) * a.heads)), block(256);
-    constexpr int BK = TsgElem<D>::BYTES == 4 ? 32 : 64;
     if constexpr (__is_same(D, TsgF32)) {
       if (a.dim <= 64) hipLaunchKernelGGL(attn_f32_fwd_kernel<1>, grid, dim3(64), 0, s, a);
       else if (a.dim <= 128) hipLaunchKernelGGL(attn_f32_fwd_kernel<2>, grid, dim3(128), 0, s, a);
-      else hipLaunchKernelGGL(attn_f32_fwd_kernel<4>, grid, dim3(256), 0, s, a);
-    } else
-    if (a.dim <= 64) hipLaunchKernelGGL((attn_fwd_kernel<D, 64, 64>), grid, block, 0, s, a);
-    else if (a.dim <= 128) hipLaunchKernelGGL((attn_fwd_kernel<D, 128, BK>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((attn_fwd_kernel<D, 256, BK / 2>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL(attn_f32_fwd_kernel<4>, grid, block, 0, s, a);
+    } else {
+      if (a.dim <= 64) hipLaunchKernelGGL((attn_fwd_kernel<D, 64, 64>), grid, block, 0, s, a);
+      else if (a.dim <= 128) hipLaunchKernelGGL((attn_fwd_kernel<D, 128, 64>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((attn_fwd_kernel<D, 256, 32>), grid, block, 0, s, a);
+    }
   }
   TSG_LAUNCH_CHECK();
   return 0;
@@ -1287,34 +1299,34 @@ template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
   }
   constexpr int R = rows_per_wg<D>();
   const dim3 gq((unsigned)(tsg_cdiv(a.n_q, R) * a.heads)), gk((unsigned)(tsg_cdiv(a.n_k, R) * a.kv_heads * a.n_split));
-  constexpr bool F32 = __is_same(D, TsgF32);
-  if (a.n_q) {
-    if constexpr (F32) {
+  if constexpr (__is_same(D, TsgF32)) {
+    if (a.n_q) {
       if (a.dim <= 64) hipLaunchKernelGGL(attn_f32_dq_kernel<1>, gq, dim3(64), 0, s, a);
       else if (a.dim <= 128) hipLaunchKernelGGL(attn_f32_dq_kernel<2>, gq, dim3(128), 0, s, a);
-      else hipLaunchKernelGGL(attn_f32_dq_kernel<4>, gq, dim3(256), 0, s, a);
-    } else
-    if (a.dim <= 64) hipLaunchKernelGGL((attn_dq_kernel<D, 64, 64>), gq, block, 0, s, a);
-    else if (a.dim <= 128) hipLaunchKernelGGL((attn_dq_kernel<D, 128, F32 ? 32 : 64>), gq, block, 0, s, a);
-    else hipLaunchKernelGGL((attn_dq_kernel<D, 256, F32 ? 16 : 32>), gq, block, 0, s, a);
-  }
-  if (a.n_k) {
-    if constexpr (F32) {
+      else hipLaunchKernelGGL(attn_f32_dq_kernel<4>, gq, block, 0, s, a);
+    }
+    if (a.n_k) {
       if (a.dim <= 64) hipLaunchKernelGGL(attn_f32_dkv_kernel<1>, gk, dim3(64), 0, s, a);
       else if (a.dim <= 128) hipLaunchKernelGGL(attn_f32_dkv_kernel<2>, gk, dim3(128), 0, s, a);
-      else hipLaunchKernelGGL(attn_f32_dkv_kernel<4>, gk, dim3(256), 0, s, a);
-    } else
-    if (a.dim <= 64) hipLaunchKernelGGL((attn_dkv_kernel<D, 64, 32, 0, false>), gk, block, 0, s, a);
-    else if (a.dim <= 128)
-      hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0, !F32>), gk, block, 0, s, a);
-    else if constexpr (F32) hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 16, 0, true>), gk, block, 0, s, a);
-    else {
-      hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 1, false>), gk, block, 0, s, a);
-      hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 2, true>), gk, block, 0, s, a);
+      else hipLaunchKernelGGL(attn_f32_dkv_kernel<4>, gk, block, 0, s, a);
     }
-    if (a.n_split > 1)
-      hipLaunchKernelGGL(attn_dkv_join_kernel<D>, dim3((unsigned)(((long)a.n_k * a.kv_heads * a.dim / 4 + 255) / 256), 2), block, 0, s, a);
+  } else {
+    if (a.n_q) {
+      if (a.dim <= 64) hipLaunchKernelGGL((attn_dq_kernel<D, 64, 64>), gq, block, 0, s, a);
+      else if (a.dim <= 128) hipLaunchKernelGGL((attn_dq_kernel<D, 128, 64>), gq, block, 0, s, a);
+      else hipLaunchKernelGGL((attn_dq_kernel<D, 256, 32>), gq, block, 0, s, a);
+    }
+    if (a.n_k) {
+      if (a.dim <= 64) hipLaunchKernelGGL((attn_dkv_kernel<D, 64, 32, 0, false>), gk, block, 0, s, a);
+      else if (a.dim <= 128) hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0, true>), gk, block, 0, s, a);
+      else {
+        hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 1, false>), gk, block, 0, s, a);
+        hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 2, true>), gk, block, 0, s, a);
+      }
+    }
   }
+  if (a.n_k && a.n_split > 1)
+    hipLaunchKernelGGL(attn_dkv_join_kernel<D>, dim3((unsigned)(((long)a.n_k * a.kv_heads * a.dim / 4 + 255) / 256), 2), block, 0, s, a);
   TSG_LAUNCH_CHECK();
   return 0;
 }

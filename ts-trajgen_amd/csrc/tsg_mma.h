@@ -3,10 +3,10 @@
 //
 // A product covers W x W results: W = 32 for the 16-bit types, 16 for f32 (where an operand takes twice the registers).
 // Lane l has column l % W of it and is part h = l / W of 64 / W; the accumulator's register i is row (i & 3) + 8 (i >> 2) + 4 h.
-// A tile in LDS is [rows][CH] chunks of 16 bytes (8 elements of 16 bits or 4 of 32).  Chunk c of row r lies at
-// position c ^ swz(r) of its row, which spreads both kinds of read over the banks:
-//   row fragment  lane l takes chunk (64 / W) s + h of row l % W: the k index of the product runs along the row
+//   row fragment  lane l takes chunk (64 / W) s + h (16 bytes) of row l % W: the k index of the product runs along the row
 //   col fragment  lane l takes column l % W of eight (f32: one) rows: the k index runs down the rows
+// A tile of 16-bit elements in LDS is [rows][CH] chunks of 16 bytes; chunk c of row r lies at position c ^ swz(r) of its row,
+// which spreads both kinds of read over the banks (the col fragment is a transposing load, ds_read_b64_tr_b16).
 // A sum does not care how its k index is numbered as long as both operands agree, so an accumulator is
 // fed back as the B operand of the next product without moving data between lanes: the col fragment of the A operand
 // is read from exactly the rows that the lane's accumulator registers stand for.
@@ -64,12 +64,9 @@ template <> __device__ __forceinline__ void tsg_mma<TsgF32>(tsg_u4 a, tsg_u4 b, 
 }
 
 // swz(r) for rows of CH chunks (see the top): a bijection of 16 neighbouring rows (CH < 16: eight pairs of them) onto the bank
-// groups.  The transposing loads of the 16-bit types take four neighbouring rows at once, the f32 ones rows four apart:
-// those get the positions that lie furthest from each other.
-template <int CH, bool F32 = false> __device__ __forceinline__ int tsg_swz(int r) {
-  if (F32) return r & 15;
+// groups, with four neighbouring rows, which the transposing loads take at once, as far apart as can be.
+template <int CH> __device__ __forceinline__ int tsg_swz(int r) {
   if (CH >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
-  if (CH == 4) return (r >> 2) & 3;
   return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
 }
 
@@ -85,27 +82,24 @@ __device__ __forceinline__ unsigned tsg_opaque(unsigned v) {
   return v;
 }
 template <typename D, int CH> struct TsgLane {
-  static constexpr bool F32 = TsgElem<D>::BYTES == 4;
   static constexpr int W = TsgElem<D>::W, PARTS = 64 / W, ROW = CH * 16;
   // first row fragment of row l % W of the tile
   static __device__ __forceinline__ unsigned row(int lane) {
     const int r = lane % W, h = lane / W;
-    return r * ROW + ((h ^ tsg_swz<CH, F32>(r)) << 4);
+    return r * ROW + ((h ^ tsg_swz<CH>(r)) << 4);
   }
   // first column fragment of the W rows from the tile's start, numbered as an accumulator's registers number them
   static __device__ __forceinline__ unsigned col(int lane) {
-    if (F32) return 4 * (lane >> 4) * ROW + (((((lane & 15) >> 2) ^ tsg_swz<CH, true>(4 * (lane >> 4))) << 4) | ((lane & 3) << 2));
     const int i = lane & 15, r = 4 * (lane >> 5) + (i >> 2);  // ds_read_b64_tr_b16: 16 lanes hand in 4 rows x 16 columns
     return r * ROW + (((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ tsg_swz<CH>(r)) << 4) + 8 * (i & 1);
   }
-  // the same with k = 8 (l / 32) + 0..7 (16-bit types): the order that a row fragment has
+  // the same with k = 8 (l / 32) + 0..7: the order that a row fragment has
   static __device__ __forceinline__ unsigned col_in_order(int lane) {
     const int i = lane & 15, r = 8 * (lane >> 5) + (i >> 2);
     return r * ROW + (((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ tsg_swz<CH>(r)) << 4) + 8 * (i & 1);
   }
 };
 typedef __attribute__((address_space(3))) const tsg_u4 tsg_lds_u4;
-typedef __attribute__((address_space(3))) const float tsg_lds_f32;
 typedef __attribute__((address_space(3))) tsg_s4 tsg_lds_s4;
 // row fragment of k step s; offset: of the tile and the row block
 template <typename D> __device__ __forceinline__ tsg_u4 tsg_row_frag(unsigned row, int s, int offset) {
@@ -144,18 +138,6 @@ template <typename D> struct TsgAccB {
     }
   }
 };
-template <> struct TsgAccB<TsgF32> {
-  tsg_f4 v;
-  __device__ __forceinline__ void set(const tsg_f4& p) { v = p; }
-  template <int CH> __device__ __forceinline__ void mma(unsigned col, int block, int offset, tsg_f4& acc) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = *reinterpret_cast<tsg_lds_f32*>((uintptr_t)((col ^ (block * 64) ^ (i * 16)) + offset + i * CH * 16));
-      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a, v[i], acc, 0, 0, 0);
-    }
-  }
-};
-
 // ---- tiles from memory straight into LDS (buffer_load_dwordx4 ... lds: lane l's 16 bytes go to m0 + 16 l).
 // The compiler does not see these loads: tsg_dma_wait() before the barrier that hands the tile over, and no load of its
 // own left in flight across a tile loop (tsg_settle), or its waits would drain these too.
@@ -203,7 +185,7 @@ template <int STEP> __device__ __forceinline__ void tsg_dma4(tsg_u4 d, unsigned 
 
 // The loads of a [ROWS][CH] tile by WAVES waves: a lane's byte offsets within the operand's rows, kept over the tile loop.
 // ROWS * stride must stay below 2^31 bytes.
-template <int ROWS, int CH, int WAVES, bool F32 = false> struct TsgLoader {
+template <int ROWS, int CH, int WAVES> struct TsgLoader {
   static constexpr int N = ROWS * CH / 64 / WAVES, DOWN = 64 * WAVES / CH;  // loads per wave; rows from one to the next
   static constexpr bool EVEN = DOWN % 16 == 0;  // the swizzle repeats: one offset serves all
   static_assert(N >= 1 && ROWS * CH % (64 * WAVES) == 0, "whole wave loads");
@@ -215,7 +197,7 @@ template <int ROWS, int CH, int WAVES, bool F32 = false> struct TsgLoader {
     row = (wave * 64 + lane) / CH;
 #pragma unroll
     for (int n = 0; n < (EVEN ? 1 : N); ++n) {
-      const int r = row + n * DOWN, c = ((wave * 64 + lane) % CH) ^ tsg_swz<CH, F32>(r);
+      const int r = row + n * DOWN, c = ((wave * 64 + lane) % CH) ^ tsg_swz<CH>(r);
       off[n] = c < chunks ? r * stride + c * 16 : 0x80000000u;  // behind every bound
     }
   }
