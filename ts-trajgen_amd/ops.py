@@ -153,94 +153,93 @@ def dropout(x, p, seed, site=0, step=0):
 
 
 # -------------------------------------------------------------------------------------------------------- attention
-def _fits(x, per):
-    """Whether the kernels can read x [rows][heads][dim] where it lies."""
-    return (x.stride(2) == 1 and x.shape[2] % per == 0 and x.stride(0) % per == 0 and x.stride(1) % per == 0
-            and x.stride(0) * x.element_size() < 1 << 24 and x.data_ptr() % 16 == 0)
-
-
 def _laid_out(x, per, dim):
-    """x as the kernels read it: 16-byte aligned rows, width padded with zeros to `dim`."""
-    if x.shape[2] == dim and _fits(x, per):
+    """x [rows][heads][width] as the kernels read it: 16-byte aligned rows, width padded with zeros to `dim`."""
+    if x.shape[2] != dim:
+        return torch.nn.functional.pad(x, (0, dim - x.shape[2]))
+    row, head, one = x.stride()
+    if (one == 1 and row % per == 0 and head % per == 0 and row * x.element_size() < 1 << 24 and x.data_ptr() % 16 == 0):
         return x
-    if x.shape[2] == dim:
-        return x.contiguous() if x.contiguous().data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
-    return torch.nn.functional.pad(x, (0, dim - x.shape[2]))
+    return x.clone(memory_format=torch.contiguous_format)
 
 
-def _attn_desc(q, k, v, q_ptr, k_ptr, scale, out, stats):
-    d = _lib.AttnDesc()
-    d.dtype, d.n_seq = DTYPES[q.dtype], q_ptr.numel() - 1
-    d.heads, d.kv_heads, d.dim, d.scale = q.shape[1], k.shape[1], q.shape[2], scale
-    d.n_q, d.n_k = q.shape[0], k.shape[0]
-    d.q_ptr, d.k_ptr = _ptr(q_ptr), _ptr(k_ptr)
-    for name, t in (('q', q), ('k', k), ('v', v), ('out', out)):
-        setattr(d, name, _ptr(t))
-        setattr(d, name + '_row', t.stride(0))
-        setattr(d, name + '_head', t.stride(1))
-    d.stats = _ptr(stats)
-    return d
+def _attn_desc(q, k, v, q_ptr, k_ptr, scale, out, stats, rest):
+    a, b, c, e = q.stride(), k.stride(), v.stride(), out.stride()
+    return _lib.AttnDesc(DTYPES[q.dtype], q_ptr.numel() - 1, q.shape[1], k.shape[1], q.shape[2], scale, q.shape[0], k.shape[0],
+                         q_ptr.data_ptr(), k_ptr.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                         a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1], stats.data_ptr(), _ptr(rest))
 
 
-def _attn_workspace(d, dev, backward):
+def _sizes(entry, d):
+    """Workspace bytes of the forward and of the backward."""
     sizes = C.c_size_t(), C.c_size_t()
-    _lib.check(_lib.lib().tsg_attn_workspace(C.byref(d), C.byref(sizes[0]), C.byref(sizes[1])), 'tsg_attn_workspace')
-    need = sizes[backward].value
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    d.workspace, d.workspace_bytes = _ptr(ws), need
+    _lib.check(getattr(_lib.lib(), entry)(C.byref(d), C.byref(sizes[0]), C.byref(sizes[1])), entry)
+    return sizes[0].value, sizes[1].value
+
+
+def _workspace(d, need, dev):
+    if not need:
+        return None
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), need
     return ws
+
+
+# The descriptor that a forward filled, and what it points to beside the saved tensors, stay on its node: the backward runs on
+# autograd's own thread, where every line of Python costs twice as much.
 
 
 class _CausalAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_ptr, k_ptr, scale):
         _enter(ctx, q, k, v)
-        dim, per = q.shape[2], 4 if q.dtype == torch.float32 else 8
+        dev, dim, per = q.device, q.shape[2], 4 if q.dtype == torch.float32 else 8
         wide = -(-dim // per) * per
-        ql, kl, vl = (_laid_out(t.detach(), per, wide) for t in (q, k, v))
-        out = torch.empty((q.shape[0], q.shape[1], wide), dtype=q.dtype, device=q.device)
-        stats = torch.empty((q.shape[1], q.shape[0], 2), dtype=torch.float32, device=q.device)
-        d = _attn_desc(ql, kl, vl, q_ptr, k_ptr, scale, out, stats)
-        rest = None
-        if q.dtype != torch.float32 and any(ctx.needs_input_grad[:3]):
-            rest = torch.empty(out.shape, dtype=q.dtype, device=q.device)
-            d.out_rest = _ptr(rest)
-        ws = _attn_workspace(d, q.device, 0)  # noqa: F841  (held until the launches are on the stream)
-        if q.shape[0] and k.shape[0]:
-            _call('tsg_attn_forward', d, q.device)
+        n_q, heads = q.shape[0], q.shape[1]
+        train = any(ctx.needs_input_grad[:3])
+        out = torch.empty((n_q, heads, wide), dtype=q.dtype, device=dev)
+        stats = torch.empty(3 * heads * n_q, dtype=torch.float32, device=dev)      # [heads][n_q][2], then delta [heads][n_q]
+        rest = torch.empty_like(out) if train and per == 8 else None
+        if n_q and k.shape[0]:
+            ql, kl, vl = _laid_out(q, per, wide), _laid_out(k, per, wide), _laid_out(v, per, wide)
+            d = _attn_desc(ql, kl, vl, q_ptr, k_ptr, scale, out, stats, rest)
+            sizes = _sizes('tsg_attn_workspace', d)
+            ws = _workspace(d, sizes[0], dev)  # noqa: F841  (held until the launches are on the stream)
+            _call('tsg_attn_forward', d, dev)
+            if train:
+                d.delta = stats.data_ptr() + 8 * heads * n_q
+                ctx.desc, ctx.need, ctx.keep = d, sizes[1], (ql, kl, vl)
         else:
             out.zero_()
-        if any(ctx.needs_input_grad[:3]):
-            ctx.scale, ctx.dim = scale, dim
-            res = out if wide == dim else out[..., :dim].contiguous()
+        res = out if wide == dim else out[..., :dim].contiguous()
+        if train:
             ctx.save_for_backward(q, k, v, q_ptr, k_ptr, res, stats, rest)
-            return res
-        return out if wide == dim else out[..., :dim].contiguous()
+        return res
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        q, k, v, q_ptr, k_ptr, out, stats, rest = ctx.saved_tensors
-        dim, per = ctx.dim, 4 if q.dtype == torch.float32 else 8
+        q, k, v, _, _, out, _, _ = ctx.saved_tensors        # also the check that none of them was written since
+        dev, dim, per = q.device, q.shape[2], 4 if q.dtype == torch.float32 else 8
         wide = -(-dim // per) * per
-        ql, kl, vl, ol, gl = (_laid_out(t.detach(), per, wide) for t in (q, k, v, out, d_out))
-        dq, dk, dv = (torch.empty(t.shape[:2] + (wide,), dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq = torch.empty((q.shape[0], q.shape[1], wide), dtype=q.dtype, device=dev)
+        dk = torch.empty((k.shape[0], k.shape[1], wide), dtype=q.dtype, device=dev)
+        dv = torch.empty_like(dk)
         if q.shape[0] and k.shape[0]:
-            d = _attn_desc(ql, kl, vl, q_ptr, k_ptr, ctx.scale, ol, stats)
-            d.out_rest = _ptr(rest)
-            delta = torch.empty(stats.shape[:2], dtype=torch.float32, device=q.device)
-            d.d_out, d.d_out_row, d.d_out_head = _ptr(gl), gl.stride(0), gl.stride(1)
-            for name, t in (('dq', dq), ('dk', dk), ('dv', dv)):
-                setattr(d, name, _ptr(t))
-                setattr(d, name + '_row', t.stride(0))
-                setattr(d, name + '_head', t.stride(1))
-            d.delta = _ptr(delta)
-            ws = _attn_workspace(d, q.device, 1)  # noqa: F841
-            _call('tsg_attn_backward', d, q.device)
+            d, gl = ctx.desc, _laid_out(d_out, per, wide)
+            ol = out if wide == dim else _laid_out(out, per, wide)
+            d.out, d.d_out, d.dq, d.dk, d.dv = ol.data_ptr(), gl.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+            d.d_out_row, d.d_out_head = gl.stride(0), gl.stride(1)
+            d.dq_row, d.dk_row, d.dv_row = q.shape[1] * wide, k.shape[1] * wide, k.shape[1] * wide
+            d.dq_head = d.dk_head = d.dv_head = wide
+            ws = _workspace(d, ctx.need, dev)  # noqa: F841
+            _call('tsg_attn_backward', d, dev)
         else:
             for t in (dq, dk, dv):
                 t.zero_()
-        return tuple(t if wide == dim else t[..., :dim].contiguous() for t in (dq, dk, dv)) + (None, None, None)
+        if wide != dim:
+            dq, dk, dv = (t[..., :dim].contiguous() for t in (dq, dk, dv))
+        return dq, dk, dv, None, None, None
 
 
 def _check_ptr(name, p):
@@ -295,63 +294,45 @@ def _rows_for(x, wide):
     return x.clone(memory_format=torch.contiguous_format)
 
 
-def _xent_desc(h, w, bias, target, ignore, reduction, stats, scales):
-    d = _lib.XentDesc()
-    d.dtype, d.hidden, d.reduction = DTYPES[h.dtype], h.shape[1], reduction
-    d.n_rows, d.n_vocab, d.ignore_index = h.shape[0], w.shape[0], ignore
-    d.h, d.w, d.bias = _ptr(h), _ptr(w), _ptr(bias)
-    d.h_row, d.w_row = max(h.stride(0), h.shape[1]), max(w.stride(0), w.shape[1])
-    d.target, d.stats, d.scales = _ptr(target), _ptr(stats), _ptr(scales)
-    return d
-
-
-def _xent_workspace(d, dev, backward):
-    sizes = C.c_size_t(), C.c_size_t()
-    _lib.check(_lib.lib().tsg_xent_workspace(C.byref(d), C.byref(sizes[0]), C.byref(sizes[1])), 'tsg_xent_workspace')
-    ws = torch.empty(sizes[backward].value, dtype=torch.uint8, device=dev)
-    d.workspace, d.workspace_bytes = _ptr(ws), ws.numel()
-    return ws
-
-
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, w, bias, target, ignore, reduction):
         _enter(ctx, h, w, bias)
-        wide = -(-h.shape[1] // 8) * 8
-        hl, wl = _rows_for(h.detach(), wide), _rows_for(w.detach(), wide)
-        bl = None if bias is None else bias.detach().contiguous()
-        target = target.contiguous()
-        stats = torch.empty((h.shape[0], 2), dtype=torch.float32, device=h.device)
-        rows = torch.empty(h.shape[0], dtype=torch.float32, device=h.device)
-        loss = rows if reduction == 0 else torch.empty((), dtype=torch.float32, device=h.device)
-        scales = torch.empty(2, dtype=torch.float32, device=h.device) if h.dtype == torch.float32 else None
-        d = _xent_desc(hl, wl, bl, target, ignore, reduction, stats, scales)
-        d.row_loss, d.loss = _ptr(rows), _ptr(loss)
-        ws = _xent_workspace(d, h.device, 0)
-        _call('tsg_xent_forward', d, h.device)
-        del ws
+        dev, rows, wide = h.device, h.shape[0], -(-h.shape[1] // 8) * 8
+        hl, wl = _rows_for(h, wide), _rows_for(w, wide)
+        bl = None if bias is None else bias.contiguous()
+        tl = target.contiguous()
+        # [rows][2] stats, [rows] losses, [2] scales of f32 operands
+        store = torch.empty(3 * rows + 2, dtype=torch.float32, device=dev)
+        at = store.data_ptr()
+        loss = torch.empty(rows if reduction == 0 else (), dtype=torch.float32, device=dev)
+        d = _lib.XentDesc(DTYPES[h.dtype], wide, reduction, 0, rows, w.shape[0], ignore, hl.data_ptr(), wl.data_ptr(), _ptr(bl),
+                          max(hl.stride(0), wide), max(wl.stride(0), wide), tl.data_ptr(),
+                          loss.data_ptr() if reduction == 0 else at + 8 * rows, loss.data_ptr(), at,
+                          at + 12 * rows if h.dtype == torch.float32 else None)
+        sizes = _sizes('tsg_xent_workspace', d)
+        ws = _workspace(d, sizes[0], dev)  # noqa: F841
+        _call('tsg_xent_forward', d, dev)
         if any(ctx.needs_input_grad[:3]):
-            ctx.save_for_backward(h, w, bias, target, stats, scales)
-            ctx.cfg = (ignore, reduction)
+            ctx.save_for_backward(h, w, bias, target, store)
+            ctx.desc, ctx.need, ctx.keep = d, sizes[1], (hl, wl, bl, tl)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss):
-        h, w, bias, target, stats, scales = ctx.saved_tensors
-        width, wide = h.shape[1], -(-h.shape[1] // 8) * 8
-        hl, wl = _rows_for(h.detach(), wide), _rows_for(w.detach(), wide)
-        bl = None if bias is None else bias.detach().contiguous()
-        d_loss = d_loss.contiguous().float()
-        d = _xent_desc(hl, wl, bl, target, ctx.cfg[0], ctx.cfg[1], stats, scales)
-        dh = torch.empty((h.shape[0], wide), dtype=h.dtype, device=h.device)
-        dw = torch.empty((w.shape[0], wide), dtype=h.dtype, device=h.device)
-        db = None if bias is None else torch.empty_like(bl)
-        d.d_loss, d.dh, d.dw, d.dbias = _ptr(d_loss), _ptr(dh), _ptr(dw), _ptr(db)
+        h, w, bias, _, _ = ctx.saved_tensors                # also the check that none of them was written since
+        dev, width, wide = h.device, h.shape[1], ctx.desc.hidden
+        if not d_loss.is_contiguous():
+            d_loss = d_loss.contiguous()
+        dh = torch.empty((h.shape[0], wide), dtype=h.dtype, device=dev)
+        dw = torch.empty((w.shape[0], wide), dtype=h.dtype, device=dev)
+        db = None if bias is None else torch.empty(w.shape[0], dtype=h.dtype, device=dev)
+        d = ctx.desc
+        d.d_loss, d.dh, d.dw, d.dbias = d_loss.data_ptr(), dh.data_ptr(), dw.data_ptr(), _ptr(db)
         d.dh_row = d.dw_row = wide
-        ws = _xent_workspace(d, h.device, 1)
-        _call('tsg_xent_backward', d, h.device)
-        del ws
+        ws = _workspace(d, ctx.need, dev)  # noqa: F841
+        _call('tsg_xent_backward', d, dev)
         if wide != width:
             dh, dw = dh[:, :width].contiguous(), dw[:, :width].contiguous()
         return dh, dw, db, None, None, None
