@@ -531,6 +531,19 @@ typedef struct tsg_dropout_desc {
 
 int tsg_dropout(const tsg_dropout_desc* d, void* stream);
 
+/* tsg_gat_train_forward / _backward with the three masks drawn from that generator where they multiply, instead of read (m_in,
+ * m_proj and m_att must be NULL): site + 0 for x, by element of [N][FIN]; + 1 for the projection, by element of [N][NH*F]; + 2 for the
+ * attention, by element of [E][NH] over edge slots.  Forward and backward take the same p, seed, site and step. */
+typedef struct tsg_gat_dropout {
+  double p;
+  uint64_t seed;
+  uint32_t site, step;
+  const int64_t* step_dev; /* or NULL, as in tsg_dropout_desc */
+} tsg_gat_dropout;
+
+int tsg_gat_train_forward_rng(const tsg_gat_train* d, const tsg_gat_dropout* r, void* stream);
+int tsg_gat_train_backward_rng(const tsg_gat_train* d, const tsg_gat_dropout* r, void* stream);
+
 /* Causal attention over packed sequences.  Sequence s has the query rows [q_ptr[s], q_ptr[s+1]) and the keys
  * [k_ptr[s], k_ptr[s+1]) (device int32, non-decreasing; the two may be one array); its last row sees its last key, a row i
  * places before it one key fewer for each place (so one row per sequence over a kept cache is the single-token form).

@@ -20,7 +20,7 @@ EXPORTS = ('tsg_version', 'tsg_gemm_f32', 'tsg_gat_forward', 'tsg_gat_forward_st
            'tsg_score_candidates', 'tsg_engine_reset', 'tsg_engine_run', 'tsg_engine_run_profiled', 'tsg_engine_graph_create', 'tsg_engine_graph_launch',
            'tsg_engine_graph_destroy', 'tsg_frontier_expand_select',
            'tsg_score_frontier', 'tsg_rollout_run', 'tsg_reconstruct_paths', 'tsg_h_pair_scores', 'tsg_geodesic_pairs',
-           'tsg_dropout', 'tsg_attn_workspace', 'tsg_attn_forward', 'tsg_attn_backward', 'tsg_xent_workspace',
+           'tsg_dropout', 'tsg_gat_train_forward_rng', 'tsg_gat_train_backward_rng', 'tsg_attn_workspace', 'tsg_attn_forward', 'tsg_attn_backward', 'tsg_xent_workspace',
            'tsg_xent_forward', 'tsg_xent_backward')
 
 _p = C.c_void_p
@@ -110,6 +110,10 @@ class DropoutDesc(C.Structure):
                 ('seed', C.c_uint64), ('p', C.c_double), ('step_dev', _p), ('x', _p), ('y', _p)]
 
 
+class GatDropout(C.Structure):
+    _fields_ = [('p', C.c_double), ('seed', C.c_uint64), ('site', C.c_uint32), ('step', C.c_uint32), ('step_dev', _p)]
+
+
 class AttnDesc(C.Structure):
     _fields_ = [('dtype', _i32), ('n_seq', _i32), ('heads', _i32), ('kv_heads', _i32), ('dim', _i32), ('scale', C.c_float),
                 ('n_q', C.c_int64), ('n_k', C.c_int64), ('q_ptr', _p), ('k_ptr', _p),
@@ -176,6 +180,8 @@ def lib():
     L.tsg_geodesic_pairs.argtypes = [_p, _i32, _i32, _p, _p, _p, _p]
     L.tsg_rollout_run.argtypes = [C.POINTER(Model), C.POINTER(Graph), C.POINTER(Rollout), _i32, _p]
     L.tsg_dropout.argtypes = [C.POINTER(DropoutDesc), _p]
+    for name in ('tsg_gat_train_forward_rng', 'tsg_gat_train_backward_rng'):
+        getattr(L, name).argtypes = [C.POINTER(GatTrain), C.POINTER(GatDropout), _p]
     for name in ('tsg_attn_forward', 'tsg_attn_backward'):
         getattr(L, name).argtypes = [C.POINTER(AttnDesc), _p]
     L.tsg_attn_workspace.argtypes = [C.POINTER(AttnDesc), C.POINTER(_sz), C.POINTER(_sz)]

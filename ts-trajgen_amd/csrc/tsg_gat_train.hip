@@ -4,7 +4,12 @@
 // The dense products around it (projection, skip projection and their weight / input gradients) are tsg_gemm_f32
 // calls made by the host wrapper (ts-trajgen_amd/generator/gat.py).  One wave per node, lanes over the F features
 // of a head, edges of a node visited in COO order (the order of the reference's scatter_add_).
-#include "tsg_common.h"
+//
+// The masks are either read (tsg_gat_train_forward / _backward) or recomputed from a counter wherever they multiply
+// (_rng, template RNG = true: tsg_philox.h; site + 0 for the input features, + 1 for the projection, + 2 for the attention by edge
+// slot), which for the projection of 40306 nodes x 5 x 256 saves 206 MB of mask and its making.  A wave then takes four
+// neighbouring features a lane, so that one draw of four words serves all of them.
+#include "tsg_philox.h"
 
 extern "C" int tsg_gemm_f32(const float* A, int lda, const float* Bt, int ldb, const float* bias, float* C, int ldc,
                             int M, int N, int K, void* stream);
@@ -26,7 +31,17 @@ __global__ void gt_mask_mul_kernel(const float* __restrict__ x, const float* __r
 __global__ void gt_init_kernel(float* gmax) { *gmax = -INFINITY; }
 
 // p_d = proj * m_proj (in place), s_src / s_trg = <p_d[n,h,:], a[h,:]>            (gat.py:155,164-165)
-__global__ __launch_bounds__(256) void gt_scores_kernel(tsg_gat_train d) {
+// factors of the features f0 + 4 lane .. + 3 of row w (F a multiple of 4: one draw)
+__device__ __forceinline__ void gt_factors(const TsgRng& r, unsigned step, unsigned long long i, float (&m)[4]) {
+  const uint4 u = tsg_philox(i >> 2, r.site, step, r.k0, r.k1);
+  m[0] = u.x >= r.threshold ? r.scale : 0.0f;
+  m[1] = u.y >= r.threshold ? r.scale : 0.0f;
+  m[2] = u.z >= r.threshold ? r.scale : 0.0f;
+  m[3] = u.w >= r.threshold ? r.scale : 0.0f;
+}
+
+template <bool RNG>
+__global__ __launch_bounds__(256) void gt_scores_kernel(tsg_gat_train d, TsgRng r) {
   const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (w >= (long)d.n_nodes * d.heads) return;
@@ -34,6 +49,29 @@ __global__ __launch_bounds__(256) void gt_scores_kernel(tsg_gat_train d) {
   float* p = d.p_d + (size_t)w * d.fout;
   const float* mk = d.m_proj ? d.m_proj + (size_t)w * d.fout : nullptr;
   float ps = 0.0f, pt = 0.0f;
+  if constexpr (RNG) {
+    const unsigned step = tsg_rng_step(r);
+    if (d.fout % 4 == 0) {
+      for (int f = lane * 4; f < d.fout; f += 256) {
+        float m[4];
+        gt_factors(r, step, (unsigned long long)w * d.fout + f, m);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = m[e] > 0.0f ? p[f + e] * m[e] : 0.0f;
+          p[f + e] = v;
+          ps += v * d.a_src[h * d.fout + f + e];
+          pt += v * d.a_trg[h * d.fout + f + e];
+        }
+      }
+    } else {
+      for (int f = lane; f < d.fout; f += 64) {
+        const float m = tsg_drop_factor(r, step, (unsigned long long)w * d.fout + f), v = m > 0.0f ? p[f] * m : 0.0f;
+        p[f] = v;
+        ps += v * d.a_src[h * d.fout + f];
+        pt += v * d.a_trg[h * d.fout + f];
+      }
+    }
+  } else
   for (int f = lane; f < d.fout; f += 64) {
     float v = p[f];
     if (mk) {
@@ -69,13 +107,15 @@ __global__ __launch_bounds__(256) void gt_edge_max_kernel(tsg_gat_train d) {
 
 // One wave per target node: edge softmax over its incoming edges, attention dropout, aggregation, skip term,
 // head mean / concat, bias, ELU                                             (gat.py:177-199, 93-114)
-__global__ __launch_bounds__(256) void gt_aggregate_kernel(tsg_gat_train d) {
+template <bool RNG>
+__global__ __launch_bounds__(256) void gt_aggregate_kernel(tsg_gat_train d, TsgRng r) {
   const int n = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (n >= d.n_nodes) return;
   const int j0 = d.in_ptr[n], j1 = d.in_ptr[n + 1];
   const int nh = d.heads, F = d.fout;
   const float gmax = *d.gmax;
+  const unsigned step = RNG ? tsg_rng_step(r) : 0u;
   const int outw = d.concat ? nh * F : F;
   for (int f0 = 0; f0 < F; f0 += 64) {
     const int f = f0 + lane;
@@ -93,7 +133,8 @@ __global__ __launch_bounds__(256) void gt_aggregate_kernel(tsg_gat_train d) {
         const int s = d.in_src[j];
         const float v = d.s_src[(size_t)s * nh + h] + st;
         const float att = __expf((v > 0.0f ? v : 0.2f * v) - gmax) / (denom + 1e-16f);  // gat.py:230
-        const float att_d = d.m_att ? att * d.m_att[(size_t)j * nh + h] : att;           // gat.py:180
+        const float att_d = RNG ? att * tsg_drop_factor(r, step, (unsigned long long)j * nh + h)
+                                : d.m_att ? att * d.m_att[(size_t)j * nh + h] : att;     // gat.py:180
         if (f0 == 0 && lane == 0) {
           d.att[(size_t)j * nh + h] = att;
           d.att_d[(size_t)j * nh + h] = att_d;
@@ -148,7 +189,8 @@ __global__ __launch_bounds__(256) void gt_bwd_bias_kernel(tsg_gat_train d) {
 
 // One wave per TARGET node and head: d_att_d[j] = <d_o[n,h,:], p_d[src_j,h,:]> (SDDMM), attention dropout,
 // softmax backward over the neighbourhood, LeakyReLU backward; writes d_pre[j,h] and ds_trg[n,h]
-__global__ __launch_bounds__(256) void gt_bwd_target_kernel(tsg_gat_train d) {
+template <bool RNG>
+__global__ __launch_bounds__(256) void gt_bwd_target_kernel(tsg_gat_train d, TsgRng r) {
   const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int nh = d.heads, F = d.fout;
@@ -156,13 +198,14 @@ __global__ __launch_bounds__(256) void gt_bwd_target_kernel(tsg_gat_train d) {
   const int n = (int)(w / nh), h = (int)(w % nh);
   const int j0 = d.in_ptr[n], j1 = d.in_ptr[n + 1];
   const float* go = d.d_o + (size_t)w * F;
+  const unsigned step = RNG ? tsg_rng_step(r) : 0u;
   float dot = 0.0f;  // sum_j att_j * d_att_j
   for (int j = j0; j < j1; ++j) {
     const float* p = d.p_d + ((size_t)d.in_src[j] * nh + h) * F;
     float s = 0.0f;
     for (int f = lane; f < F; f += 64) s += go[f] * p[f];
     s = tsg_wave_sum(s);
-    const float datt = d.m_att ? s * d.m_att[(size_t)j * nh + h] : s;
+    const float datt = RNG ? s * tsg_drop_factor(r, step, (unsigned long long)j * nh + h) : d.m_att ? s * d.m_att[(size_t)j * nh + h] : s;
     if (lane == 0) d.d_pre[(size_t)j * nh + h] = datt;  // parked until the neighbourhood's sum is known
     dot += d.att[(size_t)j * nh + h] * datt;
   }
@@ -186,7 +229,8 @@ __global__ __launch_bounds__(256) void gt_bwd_target_kernel(tsg_gat_train d) {
 
 // One wave per SOURCE node and head: ds_src[m,h] = sum of d_pre over its outgoing edges;
 // d_p[m,h,:] = (sum_j att_d[j,h] d_o[trg_j,h,:] + ds_src a_src[h,:] + ds_trg[m,h] a_trg[h,:]) * m_proj   (SpMM^T)
-__global__ __launch_bounds__(256) void gt_bwd_source_kernel(tsg_gat_train d) {
+template <bool RNG>
+__global__ __launch_bounds__(256) void gt_bwd_source_kernel(tsg_gat_train d, TsgRng r) {
   const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int nh = d.heads, F = d.fout;
@@ -198,6 +242,28 @@ __global__ __launch_bounds__(256) void gt_bwd_source_kernel(tsg_gat_train d) {
   ds_s = tsg_wave_sum(ds_s);
   if (lane == 0) d.ds_src[w] = ds_s;
   const float ds_t = d.ds_trg[w];
+  if constexpr (RNG) {
+    const unsigned step = tsg_rng_step(r);
+    if (F % 4 == 0) {
+      for (int f = lane * 4; f < F; f += 256) {
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m[4];
+        for (int k = k0; k < k1; ++k) {
+          const int j = d.out_slot[k];
+          const float a = d.att_d[(size_t)j * nh + h];
+          const float* o = d.d_o + ((size_t)d.slot_trg[j] * nh + h) * F + f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += a * o[e];
+        }
+        gt_factors(r, step, (unsigned long long)w * F + f, m);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[e] += ds_s * d.a_src[h * F + f + e] + ds_t * d.a_trg[h * F + f + e];
+          d.d_p[(size_t)w * F + f + e] = m[e] > 0.0f ? acc[e] * m[e] : 0.0f;
+        }
+      }
+      return;
+    }
+  }
   for (int f = lane; f < F; f += 64) {
     float acc = 0.0f;
     for (int k = k0; k < k1; ++k) {
@@ -205,7 +271,12 @@ __global__ __launch_bounds__(256) void gt_bwd_source_kernel(tsg_gat_train d) {
       acc += d.att_d[(size_t)j * nh + h] * d.d_o[((size_t)d.slot_trg[j] * nh + h) * F + f];
     }
     acc += ds_s * d.a_src[h * F + f] + ds_t * d.a_trg[h * F + f];
-    d.d_p[(size_t)w * F + f] = d.m_proj ? acc * d.m_proj[(size_t)w * F + f] : acc;
+    if constexpr (RNG) {
+      const float m = tsg_drop_factor(r, tsg_rng_step(r), (unsigned long long)w * F + f);
+      d.d_p[(size_t)w * F + f] = m > 0.0f ? acc * m : 0.0f;
+    } else {
+      d.d_p[(size_t)w * F + f] = d.m_proj ? acc * d.m_proj[(size_t)w * F + f] : acc;
+    }
   }
 }
 
@@ -245,15 +316,27 @@ int check_train(const tsg_gat_train* d, bool backward) {
   return 0;
 }
 
-}  // namespace
+TsgRng site_of(const tsg_gat_dropout* r, int site) { return tsg_make_rng(r->p, r->seed, r->site + site, r->step, r->step_dev); }
 
-extern "C" int tsg_gat_train_forward(const tsg_gat_train* d, void* stream) {
+int check_rng(const tsg_gat_train* d, const tsg_gat_dropout* r) {
+  if (!r || !(r->p >= 0.0 && r->p <= 1.0) || r->site > 0xffffffffu - 2) return TSG_E_INVALID;
+  return d && (d->m_in || d->m_proj || d->m_att) ? TSG_E_INVALID : 0;  // masks, or a generator
+}
+
+template <bool RNG> int train_forward(const tsg_gat_train* d, const tsg_gat_dropout* g, void* stream) {
   int rc = check_train(d, false);
   if (rc) return rc;
   hipStream_t s = (hipStream_t)stream;
   const long nin = (long)d->n_nodes * d->fin;
   const int NHF = d->heads * d->fout;
-  hipLaunchKernelGGL(gt_mask_mul_kernel, dim3(tsg_cdiv(nin, 256)), dim3(256), 0, s, d->x, d->m_in, d->x_d, nin);
+  if (RNG) {
+    tsg_dropout_desc x = {};
+    x.n = nin, x.dtype = TSG_F32, x.site = g->site, x.step = g->step, x.seed = g->seed, x.p = g->p, x.step_dev = g->step_dev, x.x = d->x, x.y = d->x_d;
+    rc = tsg_dropout(&x, stream);
+    if (rc) return rc;
+  } else {
+    hipLaunchKernelGGL(gt_mask_mul_kernel, dim3(tsg_cdiv(nin, 256)), dim3(256), 0, s, d->x, d->m_in, d->x_d, nin);
+  }
   TSG_LAUNCH_CHECK();
   rc = tsg_gemm_f32(d->x_d, d->fin, d->w_proj_t, NHF, nullptr, d->p_d, NHF, d->n_nodes, NHF, d->fin, stream);
   if (rc) return rc;
@@ -261,26 +344,42 @@ extern "C" int tsg_gat_train_forward(const tsg_gat_train* d, void* stream) {
     rc = tsg_gemm_f32(d->x_d, d->fin, d->w_skip_t, NHF, nullptr, d->skip, NHF, d->n_nodes, NHF, d->fin, stream);
     if (rc) return rc;
   }
-  hipLaunchKernelGGL(gt_scores_kernel, dim3(tsg_cdiv((long)d->n_nodes * d->heads, 4)), dim3(256), 0, s, *d);
+  const TsgRng proj = RNG ? site_of(g, 1) : TsgRng(), att = RNG ? site_of(g, 2) : TsgRng();
+  hipLaunchKernelGGL(gt_scores_kernel<RNG>, dim3(tsg_cdiv((long)d->n_nodes * d->heads, 4)), dim3(256), 0, s, *d, proj);
   hipLaunchKernelGGL(gt_init_kernel, dim3(1), dim3(1), 0, s, d->gmax);
   hipLaunchKernelGGL(gt_edge_max_kernel, dim3(tsg_cdiv(d->n_nodes, 256) < 1024 ? tsg_cdiv(d->n_nodes, 256) : 1024),
                      dim3(256), 0, s, *d);
-  hipLaunchKernelGGL(gt_aggregate_kernel, dim3(tsg_cdiv(d->n_nodes, 4)), dim3(256), 0, s, *d);
+  hipLaunchKernelGGL(gt_aggregate_kernel<RNG>, dim3(tsg_cdiv(d->n_nodes, 4)), dim3(256), 0, s, *d, att);
   TSG_LAUNCH_CHECK();
   return 0;
 }
 
-extern "C" int tsg_gat_train_backward(const tsg_gat_train* d, void* stream) {
+template <bool RNG> int train_backward(const tsg_gat_train* d, const tsg_gat_dropout* g, void* stream) {
   int rc = check_train(d, true);
   if (rc) return rc;
   hipStream_t s = (hipStream_t)stream;
   const long nhf = (long)d->n_nodes * d->heads * d->fout;
   const int outw = d->concat ? d->heads * d->fout : d->fout;
+  const TsgRng proj = RNG ? site_of(g, 1) : TsgRng(), att = RNG ? site_of(g, 2) : TsgRng();
   hipLaunchKernelGGL(gt_bwd_out_kernel, dim3(tsg_cdiv(nhf, 256)), dim3(256), 0, s, *d);
   if (d->bias) hipLaunchKernelGGL(gt_bwd_bias_kernel, dim3(tsg_cdiv(outw, 256)), dim3(256), 0, s, *d);
-  hipLaunchKernelGGL(gt_bwd_target_kernel, dim3(tsg_cdiv((long)d->n_nodes * d->heads, 4)), dim3(256), 0, s, *d);
-  hipLaunchKernelGGL(gt_bwd_source_kernel, dim3(tsg_cdiv((long)d->n_nodes * d->heads, 4)), dim3(256), 0, s, *d);
+  hipLaunchKernelGGL(gt_bwd_target_kernel<RNG>, dim3(tsg_cdiv((long)d->n_nodes * d->heads, 4)), dim3(256), 0, s, *d, att);
+  hipLaunchKernelGGL(gt_bwd_source_kernel<RNG>, dim3(tsg_cdiv((long)d->n_nodes * d->heads, 4)), dim3(256), 0, s, *d, proj);
   hipLaunchKernelGGL(gt_bwd_scoring_kernel, dim3(tsg_cdiv(d->heads * d->fout, 256)), dim3(256), 0, s, *d);
   TSG_LAUNCH_CHECK();
   return 0;
+}
+
+}  // namespace
+
+extern "C" int tsg_gat_train_forward(const tsg_gat_train* d, void* stream) { return train_forward<false>(d, nullptr, stream); }
+extern "C" int tsg_gat_train_backward(const tsg_gat_train* d, void* stream) { return train_backward<false>(d, nullptr, stream); }
+
+extern "C" int tsg_gat_train_forward_rng(const tsg_gat_train* d, const tsg_gat_dropout* r, void* stream) {
+  const int rc = check_rng(d, r);
+  return rc ? rc : train_forward<true>(d, r, stream);
+}
+extern "C" int tsg_gat_train_backward_rng(const tsg_gat_train* d, const tsg_gat_dropout* r, void* stream) {
+  const int rc = check_rng(d, r);
+  return rc ? rc : train_backward<true>(d, r, stream);
 }

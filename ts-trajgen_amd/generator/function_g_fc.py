@@ -4,8 +4,12 @@ Holds the reference's parameters under the reference's names (`road_emb`, `time_
 `intra_attn.w1/w2/w3` -- unused by the reference too, function_g_fc.py:17-19 -- and `out_fc`).  The
 arithmetic (incremental LSTM cell on MFMA, attention over the prefix, gathered out_fc rows) lives in
 libtsg.so and is driven by GeneratorV4 / the engine, which need G and H together; `forward` / `predict` /
-`predict_g` (function_g_fc.py:138-221) return G's share of that evaluation."""
+`predict_g` (function_g_fc.py:138-221) return G's share of that evaluation.  `trajectory_loss` fits function G on whole
+trajectories: the next road at every position, over all roads, differentiable (ts_trajgen_amd.ops)."""
+import torch
 import torch.nn as nn
+
+from .. import ops
 
 
 class IntraAttention(nn.Module):
@@ -65,3 +69,51 @@ class FunctionGFC(nn.Module):
     def predict(self, trace_loc, trace_time, des, candidate_set, candidate_dis, trace_mask=None):
         """softmax of forward() over the candidates (function_g_fc.py:189-204)."""
         return self.predict_g(trace_loc, trace_time, des, candidate_set, candidate_dis, trace_mask)
+
+    def trajectory_loss(self, trace_loc, trace_time, seq_ptr, target=None, reduction='mean', seed=0, step=0):
+        """Cross entropy of the next road at every position of packed trajectories, over all roads (the score of
+        function_g_fc.py:155-184 before its gather, at every prefix at once).
+
+        trace_loc and trace_time hold the trajectories one behind the other ([n] integers), seq_ptr ([n_seq + 1] int32)
+        their starts.  target ([n] int64, -100 = not counted) defaults to the next road of the same trajectory; positions of
+        no trajectory never count.  In training mode the dropouts of function_g_fc.py:160,182 are live, drawn from the
+        counter (seed, site 0 and 1, step): give every training step its own step.  hidden_size is at most 512 and a
+        multiple of 4 (ops.causal_attention).  The call waits for the device once: it looks at the lengths and ids."""
+        dev = self.out_fc.weight.device
+        if dev.type != 'cuda':
+            raise RuntimeError('FunctionGFC.trajectory_loss needs its parameters on a HIP device (no CPU fallback)')
+        loc, tim, ptr = trace_loc.to(dev).long(), trace_time.to(dev).long(), seq_ptr.to(dev)
+        if loc.dim() != 1 or loc.shape != tim.shape or not loc.numel():
+            raise ValueError('trajectory_loss: trace_loc and trace_time are [n], n >= 1, got %s and %s'
+                             % (tuple(loc.shape), tuple(tim.shape)))
+        if ptr.dim() != 1 or ptr.dtype != torch.int32 or ptr.numel() < 2:
+            raise ValueError('trajectory_loss: seq_ptr is int32 [n_seq + 1], n_seq >= 1')
+        if target is not None and (target.shape != loc.shape or target.dtype != torch.int64):
+            raise ValueError('trajectory_loss: target is int64 [n]')
+        n = loc.shape[0]
+        lens = ptr[1:] - ptr[:-1]
+        first, end, least, longest, loc0, loc1, tim0, tim1 = torch.stack(
+            [v.long() for v in (ptr[0], ptr[-1], lens.min(), lens.max(), loc.min(), loc.max(), tim.min(), tim.max())]).tolist()
+        if first < 0 or end > n or least < 0:
+            raise ValueError('trajectory_loss: seq_ptr does not grow inside [0, %d]' % n)
+        if loc0 < 0 or loc1 >= self.road_emb.num_embeddings or tim0 < 0 or tim1 >= self.time_emb.num_embeddings:
+            raise ValueError('trajectory_loss: an id is outside its embedding')
+        at = torch.arange(n, device=dev, dtype=torch.int32)
+        inside = (at >= first) & (at < end)
+        seq = (torch.searchsorted(ptr, at, right=True) - 1).clamp_(0, ptr.numel() - 2)
+        pos = torch.where(inside, at - ptr[seq], torch.zeros_like(at)).long()
+        if target is None:
+            target = torch.where(pos == lens[seq] - 1, torch.full_like(loc, -100), torch.roll(loc, -1))
+        target = torch.where(inside, target.to(dev), torch.full_like(loc, -100))
+        drop = self.dropout_p if self.training else 0.0
+        x = torch.cat([self.road_emb(loc), self.time_emb(tim)], dim=1)
+        if drop:
+            x = ops.dropout(x, drop, seed, site=0, step=step)
+        # the recurrence runs over the padded batch; what it computes behind a trajectory's end is never looked at
+        grid = (ptr[:-1].long().unsqueeze(1) + torch.arange(max(longest, 1), device=dev)).clamp_(max=n - 1)
+        h = self.lstm(x[grid])[0][seq, pos]
+        q = h.unsqueeze(1)
+        a = ops.causal_attention(q, q, q, ptr, scale=1.0).squeeze(1)
+        if drop:
+            a = ops.dropout(a, drop, seed, site=1, step=step)
+        return ops.linear_cross_entropy(a, self.out_fc.weight, target, bias=self.out_fc.bias, reduction=reduction)

@@ -5,7 +5,8 @@ Parameters keep the reference's names and shapes (`linear_proj.weight`, `skip_pr
 same `torch.manual_seed` reproduces the same initial weights.  After `.train(False)` (the generation path: the
 reference's dropouts are the identity) `forward` runs `tsg_gat_forward`; in training mode it runs
 `tsg_gat_train_forward` under autograd (`tsg_gat_train_backward` + `tsg_gemm_f32` for the dense gradients), the three
-dropouts of gat.py:149,155,180 drawn on the device from torch's generator (or taken from `dropout_masks`).
+dropouts of gat.py:149,155,180 drawn on the device from torch's generator (or taken from `dropout_masks`, or, with `dropout_rng`,
+recomputed from a counter inside the kernels: nothing of their size is stored).
 """
 import ctypes as C
 
@@ -85,13 +86,25 @@ class _GATTrainFn(torch.autograd.Function):
         d.score_bytes = n * nh * 4
         d.edge_bytes = max(e, 1) * nh * 4
         d.out_bytes = bufs['out'].numel() * 4
+        rng = None
+        if cfg.get('rng') is not None:
+            from ..ops import _enter
+            _enter(ctx, x, w_proj, w_skip, a_src, a_trg, bias)
+            p, seed, site, step = cfg['rng']
+            rng = _lib.GatDropout(p, seed, site, 0 if torch.is_tensor(step) else step, step.data_ptr() if torch.is_tensor(step) else None)
+            # the output is saved as such, not held by its own node; advancing the step before the backward is an error
+            ctx.save_for_backward(bufs['out'], *([step] if torch.is_tensor(step) else []))
         with torch.cuda.device(dev):
-            _lib.check(L.tsg_gat_train_forward(C.byref(d), _lib.current_stream()), 'tsg_gat_train_forward')
+            if rng is None:
+                _lib.check(L.tsg_gat_train_forward(C.byref(d), _lib.current_stream()), 'tsg_gat_train_forward')
+            else:
+                _lib.check(L.tsg_gat_train_forward_rng(C.byref(d), C.byref(rng), _lib.current_stream()), 'tsg_gat_train_forward_rng')
+        ctx.rng = rng
         ctx.cfg, ctx.bufs, ctx.x, ctx.w = cfg, bufs, x, (w_proj.detach().contiguous().float(),
                                                       None if identity else w_skip.detach().contiguous().float())
         ctx.desc = d
         ctx.has_bias = bias is not None
-        return bufs['out']
+        return bufs['out'] if rng is None else bufs.pop('out')
 
     @staticmethod
     def backward(ctx, d_out):
@@ -112,8 +125,13 @@ class _GATTrainFn(torch.autograd.Function):
         d.d_out = _lib.ptr(d_out)
         for k, v in g.items():
             setattr(d, k, _lib.ptr(v))
+        if ctx.rng is not None:
+            ctx.saved_tensors   # raises if the step was advanced or the output overwritten since the forward
         with torch.cuda.device(dev):
-            _lib.check(L.tsg_gat_train_backward(C.byref(d), _lib.current_stream()), 'tsg_gat_train_backward')
+            if ctx.rng is None:
+                _lib.check(L.tsg_gat_train_backward(C.byref(d), _lib.current_stream()), 'tsg_gat_train_backward')
+            else:
+                _lib.check(L.tsg_gat_train_backward_rng(C.byref(d), C.byref(ctx.rng), _lib.current_stream()), 'tsg_gat_train_backward_rng')
         w_proj, w_skip = ctx.w
         x_d = b['x_d']
         d_w_proj = gemm(g['d_p'].t().contiguous(), x_d)             # [NH*F, N] . [N, FIN]
@@ -124,7 +142,12 @@ class _GATTrainFn(torch.autograd.Function):
         else:
             d_w_skip = gemm(g['d_o'].t().contiguous(), x_d)
             d_x_d = d_x_d + gemm(g['d_o'], w_skip)
-        d_x = d_x_d * cfg['m_in'] if cfg['m_in'] is not None else d_x_d
+        if ctx.rng is not None:
+            from ..ops import _drop
+            p, seed, site, step = cfg['rng']
+            d_x = _drop(d_x_d, p, seed, site, step)
+        else:
+            d_x = d_x_d * cfg['m_in'] if cfg['m_in'] is not None else d_x_d
         return (d_x, d_w_proj, d_w_skip, g['d_a_src'].view(1, nh, fo), g['d_a_trg'].view(1, nh, fo),
                 g.get('d_bias'), None)
 
@@ -156,6 +179,8 @@ class GATLayerImp3(nn.Module):
         self._tg = None
         self.dropout_masks = None   # training mode: (m_in (N, FIN), m_proj (N, NH*F), m_att (E, NH) in COO edge order),
         #                             each scaled by 1 / (1 - p); None = drawn from torch's generator on the device
+        self.dropout_rng = None     # training mode: (seed, site, step) of ops.dropout, sites site .. site + 2 are this layer's: the
+        #                             masks come from that counter inside the kernels instead; step may be a device int64
         nn.init.xavier_uniform_(self.linear_proj.weight)
         nn.init.xavier_uniform_(self.scoring_fn_target)
         nn.init.xavier_uniform_(self.scoring_fn_source)
@@ -200,7 +225,17 @@ class GATLayerImp3(nn.Module):
         nh, fo = self.num_of_heads, self.num_out_features
         in_ptr, in_src, out_ptr, out_slot, slot_trg, order = self._train_graph(edge_index, n, dev)
         e = int(in_src.numel())
-        if self.dropout_masks is not None:
+        rng = None
+        if self.dropout_rng is not None:
+            if self.dropout_masks is not None:
+                raise ValueError('dropout_masks and dropout_rng are set: one of them decides what is dropped')
+            from ..ops import check_rng
+            seed, site, step = self.dropout_rng
+            for at in (site, site + 2):
+                check_rng('GATLayerImp3', self.dropout_prob, seed, at, step, dev)
+            rng = (float(self.dropout_prob), int(seed), int(site), step if torch.is_tensor(step) else int(step))
+            m_in = m_proj = m_att = None
+        elif self.dropout_masks is not None:
             m_in, m_proj, m_att = [m.to(dev).float().contiguous() for m in self.dropout_masks]
         else:
             keep = 1.0 - self.dropout_prob
@@ -209,8 +244,10 @@ class GATLayerImp3(nn.Module):
             m_att = (torch.rand((e, nh), device=dev) < keep).float() / keep
         cfg = {'heads': nh, 'fout': fo, 'concat': bool(self.concat), 'in_ptr': in_ptr, 'in_src': in_src,
                'out_ptr': out_ptr, 'out_slot': out_slot, 'slot_trg': slot_trg,
-               'm_in': m_in.reshape(n, fin), 'm_proj': m_proj.reshape(n, nh * fo),
-               'm_att': m_att.reshape(e, nh)[order].contiguous()}
+               'rng': rng}
+        cfg.update({'m_in': None, 'm_proj': None, 'm_att': None} if rng is not None else
+                   {'m_in': m_in.reshape(n, fin), 'm_proj': m_proj.reshape(n, nh * fo),
+                    'm_att': m_att.reshape(e, nh)[order].contiguous()})
         out = _GATTrainFn.apply(x, self.linear_proj.weight, self.skip_proj.weight, self.scoring_fn_source,
                                 self.scoring_fn_target, self.bias, cfg)
         return out, edge_index
