@@ -265,6 +265,52 @@ def test_attention_extreme_scores():
     assert torch.allclose(out[5:, 0], v[5, 0].expand(59, 64), atol=1e-6)
 
 
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('lens,broken,heads,kv_heads,dim', [
+    ([5, 9, 3, 20], 1, 2, 1, 32), ([5, 9, 3, 20], 1, 4, 2, 128), ([40, 1, 0, 70, 33], 3, 2, 2, 256),
+    ([30, 300, 40, 200], 1, 4, 2, 128), ([1000, 900, 1100], 1, 4, 1, 64), ([2500, 2700], 0, 8, 1, 128)])
+def test_attention_values_that_are_not_finite_stay_in_their_sequence(dt, lens, broken, heads, kv_heads, dim):
+    """Infinities and NaN in one sequence's operands: every other sequence gives what it gives without them, rows before
+    the first broken key do too, and rows that see one say so.  What it gives: a row's running reference moves when that of
+    any row of its wave has to, so a neighbour's scores decide between references and hence between roundings; both
+    results are within bound() of the true one, and so within twice that of each other."""
+    from ts_trajgen_amd import ops
+    g = torch.Generator().manual_seed(3)
+    n, p = sum(lens), ptr(lens)
+    q, k, v, do = [torch.randn(n, x, dim, generator=g).to(dt) for x in (heads, kv_heads, kv_heads, heads)]
+    i, j = int(p[broken]), int(p[broken + 1])
+    q[int(p[broken + 1]) - 1, :, 0] = 1.0      # an infinite key is then a score of +inf
+    others = torch.ones(n, dtype=torch.bool)
+    others[i:j] = False
+
+    def run(q, k, v, do):
+        q, k, v = [x.to(DEV).requires_grad_(True) for x in (q, k, v)]
+        o = ops.causal_attention(q, k, v, torch.tensor(p, dtype=torch.int32, device=DEV))
+        return [x.cpu() for x in [o.detach()] + list(torch.autograd.grad(o, (q, k, v), do.to(DEV)))]
+    want = run(q, k, v, do)
+    # the sequence's last row is broken in each operand in turn
+    for at, value in [(0, float('nan')), (1, float('inf')), (2, float('nan')), (2, float('-inf')), (3, float('inf'))]:
+        ops_ = [x.clone() for x in (q, k, v, do)]
+        ops_[at][j - 1, 0, dim // 2 if at == 2 else 0] = value
+        got = run(*ops_)
+        for what, a, b in zip(('out', 'dq', 'dk', 'dv'), got, want):
+            assert rel(a[others], b[others]) <= 2 * bound_of(dt, b[others]), (at, value, what)
+            if what in ('out', 'dq'):       # rows before the broken one do not see it
+                assert rel(a[i:j - 1], b[i:j - 1]) <= 2 * bound_of(dt, b[i:j - 1]), (at, value, what)
+        if at < 3:
+            assert not torch.isfinite(got[0][j - 1, 0]).all()
+        if at == 2:     # only that column, and only the heads over that key
+            bad = ~torch.isfinite(got[0][j - 1])
+            group = heads // kv_heads
+            assert bad[:group, dim // 2].all() and int(bad.sum()) == group
+    # a whole sequence of them
+    ops_ = [x.clone() for x in (q, k, v, do)]
+    for x in ops_:
+        x[i:j] = float('nan')
+    for a, b in zip(run(*ops_), want):
+        assert rel(a[others], b[others]) <= 2 * bound_of(dt, b[others]) and torch.isnan(a[i:j]).all()
+
+
 def test_attention_gradient_against_differences():
     from ts_trajgen_amd import ops
     torch.manual_seed(0)

@@ -209,19 +209,87 @@ template <int W> __device__ __forceinline__ float parts_sum(float v) {
   for (int o = W; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
+// The second product of a tile multiplies p = 0 (ds = 0) with the operand rows that a row must not see, and 0 times an infinity or NaN
+// is NaN: one broken trajectory would spoil its neighbours in the tile.  Only tiles that mask have such pairs.  So a kernel
+// whose sums are not all finite walks its tiles once more (SEEN): in tiles that mask, elements that are not finite then
+// reach exactly the rows that see them (a count of them per sum, a third product), and all other sums are formed with zeros in
+// their place.  Finite operands pay one look at the sums; rows that see such an element hold NaN or infinities as they should.
+// The second walk starts from the arguments and an index that the compiler cannot connect with the first one's: nothing is held for it.
+__device__ __forceinline__ void tsg_again(int& tid) { asm volatile("" : "+v"(tid)); }
+template <int NW> __device__ __forceinline__ bool any_wave(float zero, int wave, int* slot /* [NW], used once */) {
+  const bool bad = __any(!(zero == 0.0f));
+  if (NW == 1) return bad;
+  if ((threadIdx.x & 63) == 0) slot[wave] = bad;
+  __syncthreads();  // and all waves are done with the tiles
+  int n = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) n |= slot[w];
+  return __builtin_amdgcn_readfirstlane(n) != 0;
+}
+template <typename A, int N> __device__ __forceinline__ float zero_of(const A (&acc)[N], float z = 0.0f) {  // NaN if any is not finite
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(A) / 4); ++i) z = __builtin_fmaf(acc[n][i], 0.0f, z);
+  return z;
+}
+// the word's elements that are not finite: ones; the others: as they are
+template <typename D> __device__ __forceinline__ void split_bad(unsigned w, unsigned& good, unsigned& bad) {
+  constexpr bool BF = __is_same(D, TsgBf16);
+  constexpr unsigned E = BF ? 0x7f80u : 0x7c00u, ONE = BF ? 0x3f80u : 0x3c00u;
+  const bool lo = (w & E) == E, hi = (w & (E << 16)) == E << 16;
+  good = (lo ? 0u : w & 0xffffu) | (hi ? 0u : w & 0xffff0000u);
+  bad = (lo ? ONE : 0u) | (hi ? ONE << 16 : 0u);
+}
+template <typename D, int CH>
+__device__ __forceinline__ void mma_seen(const TsgAccB<D>& p, const TsgAccB<D>& sees, unsigned col, int block, int offset, tsg_f32x16& acc) {
+  const unsigned at = col ^ (block * 64);
+  __builtin_amdgcn_sched_barrier(0);  // one block at a time: this walk must not cost the other one registers
+  tsg_f32x16 extra, count;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) extra[i] = count[i] = 0.0f;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const tsg_u4 x = TsgAccB<D>::template frag<CH>(at, offset, t);
+    tsg_u4 good, lost, ones;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      unsigned g, b;
+      split_bad<D>(x[w], g, b);
+      good[w] = g, lost[w] = x[w] & ~g, ones[w] = b;
+    }
+    tsg_mma<D>(good, p.v[t], acc);
+    tsg_mma<D>(lost, p.v[t], extra);
+    tsg_mma<D>(ones, sees.v[t], count);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] += count[i] > 0.0f ? extra[i] : 0.0f;
+  __builtin_amdgcn_sched_barrier(0);
+}
+// which of the accumulator's rows, 8 (i / 4) + 4 h + i % 4 from a tile's start, lie in [first, last); first and last: less 4 h
+template <typename D> __device__ __forceinline__ TsgAccB<D> sees_of(int first, int last) {
+  tsg_f32x16 s;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int at = (i & 3) + 8 * (i >> 2);
+    s[i] = at >= first && at < last ? 1.0f : 0.0f;
+  }
+  TsgAccB<D> b;
+  b.set(s);
+  return b;
+}
 // in a branch that is seldom taken: keeps the compiler from running both sides and selecting
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 template <typename D> constexpr int rows_per_wg() { return TsgElem<D>::BYTES == 4 ? 16 : 128; }
 
 // ------------------------------------------------------------------------------------------------- forward, tiles
-template <typename D, int DP, int BK>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
+template <typename D, int DP, int BK, bool SEEN>
+__device__ __forceinline__ float attn_fwd_tiles(const AttnArgs& a, int tid, char* lds, int* edge) {
   typedef TsgElem<D> E;
   typedef typename E::Acc Acc;
   constexpr int W = E::W, PARTS = 64 / W, CH = DP / E::EPC, NF = CH / PARTS, ND = DP / W, NB = BK / W, TILE = BK * CH * 16;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
-  __shared__ int edge[8];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane / W;
+  const int wave = tid >> 6, lane = tid & 63, h = lane / W;
   const unsigned row0 = tsg_lds_addr(lds) + TsgLane<D, CH>::row(lane), col0 = tsg_lds_addr(lds) + TsgLane<D, CH>::col(lane);
   const int tiles = gridDim.x / a.heads;
   const int tile = tiles - 1 - (int)(blockIdx.x / a.heads), head = blockIdx.x % a.heads;  // late rows see most keys: first
@@ -234,11 +302,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_fwd_kernel(AttnArg
   keys_of_row(a, w0, t, lo, hi);
   const Bounds b = bounds_of<W>(lo, hi, wave, edge);
   Acc acc[ND];
-#pragma unroll
-  for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-    for (int i = 0; i < E::REGS; ++i) acc[dt][i] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
+  float m, l;
   const char* kbase = a.k + kvh * a.k_head;
   const char* vbase = a.v + kvh * a.v_head;
   TsgLoader<BK, CH, 4> kl, vl;
@@ -248,6 +312,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_fwd_kernel(AttnArg
     kl.load(kbase + (long)k0 * a.k_row, b.hi - k0, a.chunks * 16, buf * 2 * TILE);
     vl.load(vbase + (long)k0 * a.v_row, b.hi - k0, a.chunks * 16, buf * 2 * TILE);
   };
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int i = 0; i < E::REGS; ++i) acc[dt][i] = 0.0f;
+  m = -INFINITY, l = 0.0f;
   if (b.lo < b.hi) fetch(b.lo, 0);
   tsg_settle(qf);
   for (int k0 = b.lo, buf = 0; k0 < b.hi; k0 += BK, buf ^= 1) {
@@ -322,12 +391,19 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_fwd_kernel(AttnArg
       __builtin_amdgcn_s_setprio(1);
       TsgAccB<D> p;
       p.set(z[n]);
+      if constexpr (SEEN) {
+        const TsgAccB<D> sees = sees_of<D>(lo - k0 - W * n - 4 * h, hi - k0 - W * n - 4 * h);
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt) p.template mma<CH>(col, dt, TILE + W * n * CH * 16, acc[dt]);
+        for (int dt = 0; dt < ND; ++dt) mma_seen<D, CH>(p, sees, col, dt, TILE + W * n * CH * 16, acc[dt]);
+      } else {
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) p.template mma<CH>(col, dt, TILE + W * n * CH * 16, acc[dt]);
+      }
     }
-    tsg_interleave<NB * ND * 4, NB * ND * 2, 8, 2>();
+    if constexpr (!SEEN) tsg_interleave<NB * ND * 4, NB * ND * 2, 8, 2>();
     __builtin_amdgcn_s_setprio(0);
   }
+  const float zero = zero_of(acc);
   l = parts_sum<W>(l);
   if (t < a.n_q) {
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
@@ -336,17 +412,27 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_fwd_kernel(AttnArg
     const float left = a.scale2 <= 1.0f ? __builtin_fmaf(m, a.scale2, -(m * a.scale2)) : 0.0f;
     if (h == 0) a.stat[(long)head * a.n_q + t] = l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l) - left);
   }
+  return zero;
+}
+template <typename D, int DP, int BK>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void attn_fwd_kernel(AttnArgs a) {
+  constexpr int CH = DP / TsgElem<D>::EPC, TILE = BK * CH * 16;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
+  __shared__ int edge[8], redo[4];
+  int tid = threadIdx.x;
+  if (any_wave<4>(attn_fwd_tiles<D, DP, BK, false>(a, tid, lds, edge), tid >> 6, redo)) {
+    tsg_again(tid);
+    attn_fwd_tiles<D, DP, BK, true>(a, tid, lds, edge);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ backward, tiles: dq
-template <typename D, int DP, int BK>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
+template <typename D, int DP, int BK, bool SEEN>
+__device__ __forceinline__ float attn_dq_tiles(const AttnArgs& a, int tid, char* lds, int* edge) {
   typedef TsgElem<D> E;
   typedef typename E::Acc Acc;
   constexpr int W = E::W, PARTS = 64 / W, CH = DP / E::EPC, NF = CH / PARTS, ND = DP / W, NB = BK / W, TILE = BK * CH * 16;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
-  __shared__ int edge[8];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane / W;
+  const int wave = tid >> 6, lane = tid & 63, h = lane / W;
   const unsigned row0 = tsg_lds_addr(lds) + TsgLane<D, CH>::row(lane), col0 = tsg_lds_addr(lds) + TsgLane<D, CH>::col(lane);
   const int tiles = gridDim.x / a.heads;
   const int tile = tiles - 1 - (int)(blockIdx.x / a.heads), head = blockIdx.x % a.heads;
@@ -376,10 +462,6 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dq_kernel(AttnArgs
   keys_of_row(a, w0, t, lo, hi);
   const Bounds b = bounds_of<W>(lo, hi, wave, edge);
   Acc acc[ND];
-#pragma unroll
-  for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-    for (int i = 0; i < E::REGS; ++i) acc[dt][i] = 0.0f;
   const char* kbase = a.k + kvh * a.k_head;
   const char* vbase = a.v + kvh * a.v_head;
   TsgLoader<BK, CH, 4> kl, vl;
@@ -389,6 +471,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dq_kernel(AttnArgs
     kl.load(kbase + (long)k0 * a.k_row, b.hi - k0, a.chunks * 16, buf * 2 * TILE);
     vl.load(vbase + (long)k0 * a.v_row, b.hi - k0, a.chunks * 16, buf * 2 * TILE);
   };
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int i = 0; i < E::REGS; ++i) acc[dt][i] = 0.0f;
   if (b.lo < b.hi) fetch(b.lo, 0);
   tsg_settle(qf);
   tsg_settle(gf);
@@ -399,8 +485,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dq_kernel(AttnArgs
     if (k0 + BK < b.hi) fetch(k0 + BK, buf ^ 1);
     if (k0 >= b.wave_hi || k0 + BK <= b.wave_lo) continue;
     const unsigned row = tsg_opaque(row0) + buf * 2 * TILE, col = tsg_opaque(col0) + buf * 2 * TILE;
+    constexpr int UNROLL = SEEN ? 1 : NB;
     const bool edge_tile = k0 < b.in_lo || k0 + BK > b.in_hi;
-#pragma unroll
+#pragma unroll UNROLL
     for (int n = 0; n < NB; ++n) {
       Acc z, dp;
 #pragma unroll
@@ -424,27 +511,43 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dq_kernel(AttnArgs
       }
       TsgAccB<D> ds;
       ds.set(z);
+      if constexpr (SEEN) {
+        const TsgAccB<D> sees = sees_of<D>(lo - k0 - W * n - 4 * h, hi - k0 - W * n - 4 * h);
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt) ds.template mma<CH>(col, dt, W * n * CH * 16, acc[dt]);
-      tsg_interleave<ND * 4, ND * 2, 8, 2>();
+        for (int dt = 0; dt < ND; ++dt) mma_seen<D, CH>(ds, sees, col, dt, W * n * CH * 16, acc[dt]);
+      } else {
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) ds.template mma<CH>(col, dt, W * n * CH * 16, acc[dt]);
+        tsg_interleave<ND * 4, ND * 2, 8, 2>();
+      }
     }
   }
+  const float zero = zero_of(acc);
   if (t < a.n_q) store_rows<D, ND>(acc, a.dq + (long)t * a.dq_row + head * a.dq_head, a.scale, a.dim, h);
+  return zero;
+}
+template <typename D, int DP, int BK>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void attn_dq_kernel(AttnArgs a) {
+  constexpr int CH = DP / TsgElem<D>::EPC, TILE = BK * CH * 16;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
+  __shared__ int edge[8], redo[4];
+  int tid = threadIdx.x;
+  if (any_wave<4>(attn_dq_tiles<D, DP, BK, false>(a, tid, lds, edge), tid >> 6, redo)) {
+    tsg_again(tid);
+    attn_dq_tiles<D, DP, BK, true>(a, tid, lds, edge);
+  }
 }
 
 // ------------------------------------------------------------------------------------------ backward, tiles: dk and dv
 // PART 0: both; 1: dv only; 2: dk only (256 wide: keys, values and both sums do not fit the registers at once)
 // VL: the values' fragments are read from LDS in every step instead of held in registers, which then suffice without spills
 // (128 wide at two waves a SIMD, 256 wide at one).
-template <typename D, int DP, int BQ, int PART, bool VL>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
+template <typename D, int DP, int BQ, int PART, bool VL, bool SEEN>
+__device__ __forceinline__ float attn_dkv_tiles(const AttnArgs& a, int tid, char* lds, int* edge, float (*stat)[3][BQ]) {
   typedef TsgElem<D> E;
   typedef typename E::Acc Acc;
   constexpr int W = E::W, PARTS = 64 / W, CH = DP / E::EPC, NF = CH / PARTS, ND = DP / W, NB = BQ / W, TILE = BQ * CH * 16;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + (VL ? 4 * W * CH * 16 : 0)];
-  __shared__ __attribute__((aligned(16))) float stat[2][3][BQ];  // maximum, log2 of the sum, delta
-  __shared__ int edge[8];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = lane / W;
+  const int wave = tid >> 6, lane = tid & 63, h = lane / W;
   const unsigned row0 = tsg_lds_addr(lds) + TsgLane<D, CH>::row(lane), col0 = tsg_lds_addr(lds) + TsgLane<D, CH>::col(lane);
   // early keys are seen by most rows: first.  With n_split > 1 the walk over the rows is cut into that many stretches.
   const int split = blockIdx.x / a.kv_heads % a.n_split, tile = blockIdx.x / a.kv_heads / a.n_split, kvh = blockIdx.x % a.kv_heads;
@@ -462,13 +565,6 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dkv_kernel(AttnArg
   rows_of_key(a, w0, j, lo, hi);
   const Bounds b = bounds_of<W>(lo, hi, wave, edge);
   Acc dk[PART == 1 ? 1 : ND], dv[PART == 2 ? 1 : ND];
-#pragma unroll
-  for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-    for (int i = 0; i < E::REGS; ++i) {
-      if constexpr (PART != 1) dk[dt][i] = 0.0f;
-      if constexpr (PART != 2) dv[dt][i] = 0.0f;
-    }
   // the walk: for every head of the group the row tiles [b.lo, b.hi), as one sequence of steps
   const int per = b.lo < b.hi ? (b.hi - b.lo + BQ - 1) / BQ : 0, all = per * a.group;
   const int first = (int)((long)all * split / a.n_split), steps = (int)((long)all * (split + 1) / a.n_split) - first;
@@ -495,6 +591,13 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dkv_kernel(AttnArg
   auto stat_to = [&](int buf, float2 st, float delta) {
     if (tid < BQ) stat[buf][0][tid] = st.x, stat[buf][1][tid] = st.y, stat[buf][2][tid] = delta;
   };
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int i = 0; i < E::REGS; ++i) {
+      if constexpr (PART != 1) dk[dt][i] = 0.0f;
+      if constexpr (PART != 2) dv[dt][i] = 0.0f;
+    }
   float2 st = make_float2(0.0f, INFINITY);
   float delta = 0.0f;
   Step now = {kvh * a.group + (steps ? first / per : 0), b.lo + (steps ? first % per : 0) * BQ};
@@ -519,8 +622,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dkv_kernel(AttnArg
     if (t0 >= b.wave_hi || t0 + BQ <= b.wave_lo) continue;
     const unsigned row = tsg_opaque(row0) + buf * 2 * TILE, col = tsg_opaque(col0) + buf * 2 * TILE;
     const unsigned vrow = tsg_opaque(row0) + 4 * TILE + wave * W * CH * 16;
+    constexpr int UNROLL = SEEN ? 1 : NB;
     const bool edge_tile = t0 < b.in_lo || t0 + BQ > b.in_hi;
-#pragma unroll
+#pragma unroll UNROLL
     for (int n = 0; n < NB; ++n) {
       Acc z, dp;
 #pragma unroll
@@ -559,6 +663,22 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dkv_kernel(AttnArg
           }
         }
       }
+      if constexpr (SEEN) {
+        TsgAccB<D> pb, sb;
+        pb.set(z);
+        if constexpr (PART != 1) {
+#pragma unroll
+          for (int i = 0; i < E::REGS; ++i) dp[i] *= z[i];
+          sb.set(dp);
+        }
+        const TsgAccB<D> sees = sees_of<D>(lo - t0 - W * n - 4 * h, hi - t0 - W * n - 4 * h);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+          if constexpr (PART != 2) mma_seen<D, CH>(pb, sees, col, dt, TILE + W * n * CH * 16, dv[dt]);
+          if constexpr (PART != 1) mma_seen<D, CH>(sb, sees, col, dt, W * n * CH * 16, dk[dt]);
+        }
+        continue;
+      }
       if constexpr (PART != 2) {
         TsgAccB<D> pb;
         pb.set(z);
@@ -575,6 +695,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dkv_kernel(AttnArg
       }
     }
   }
+  float zero = 0.0f;
+  if constexpr (PART != 1) zero = zero_of(dk, zero);
+  if constexpr (PART != 2) zero = zero_of(dv, zero);
   if (j < a.n_k && a.n_split > 1) {
     float* p = a.part + (((long)split * a.n_k + j) * a.kv_heads + kvh) * a.dim;
     if constexpr (PART != 1) store_sums<D, ND>(dk, p, a.dim, h);
@@ -582,6 +705,27 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_dkv_kernel(AttnArg
   } else if (j < a.n_k) {
     if constexpr (PART != 1) store_rows<D, ND>(dk, a.dk + (long)j * a.dk_row + kvh * a.dk_head, a.scale, a.dim, h);
     if constexpr (PART != 2) store_rows<D, ND>(dv, a.dv + (long)j * a.dv_row + kvh * a.dv_head, 1.0f, a.dim, h);
+  }
+  return zero;
+}
+template <typename D, int DP, int BQ, int PART, bool VL>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void attn_dkv_kernel(AttnArgs a) {
+  constexpr int W = TsgElem<D>::W, CH = DP / TsgElem<D>::EPC, TILE = BQ * CH * 16;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + (VL ? 4 * W * CH * 16 : 0)];
+  __shared__ __attribute__((aligned(16))) float stat[2][3][BQ];  // maximum, log2 of the sum, delta
+  __shared__ int edge[8], redo[4];
+  int tid = threadIdx.x;
+  if (any_wave<4>(attn_dkv_tiles<D, DP, BQ, PART, VL, false>(a, tid, lds, edge, stat), tid >> 6, redo)) {
+    // one after the other: with both it would need more registers than the first walk
+    if constexpr (PART != 2) {
+      tsg_again(tid);
+      attn_dkv_tiles<D, DP, BQ, 1, false, true>(a, tid, lds, edge, stat);
+    }
+    if constexpr (PART == 0) __syncthreads();
+    if constexpr (PART != 1) {
+      tsg_again(tid);
+      attn_dkv_tiles<D, DP, BQ, 2, VL, true>(a, tid, lds, edge, stat);
+    }
   }
 }
 
@@ -630,6 +774,25 @@ __device__ __forceinline__ void add16(Sum16& acc, const tsg_f4 (&v)[4], const ts
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][e], p[i], acc[e], 0, 0, 0);
 }
+// the same, and elements that are not finite reach only the sums of rows that see them (mma_seen)
+__device__ __forceinline__ void add16_seen(Sum16& acc, const tsg_f4 (&v)[4], const tsg_f4& p, int first, int last) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    tsg_f4 extra = {0.0f, 0.0f, 0.0f, 0.0f}, count = extra;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x = v[i][e];
+      asm volatile("" : "+v"(x));  // here and not earlier: registers
+      const bool bad = (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
+      acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(bad ? 0.0f : x, p[i], acc[e], 0, 0, 0);
+      extra = __builtin_amdgcn_mfma_f32_16x16x4f32(bad ? x : 0.0f, p[i], extra, 0, 0, 0);
+      count = __builtin_amdgcn_mfma_f32_16x16x4f32(bad ? 1.0f : 0.0f, i >= first && i < last ? 1.0f : 0.0f, count, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[e][i] += count[i] > 0.0f ? extra[i] : 0.0f;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
 __device__ __forceinline__ void zero16(Sum16& acc) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) acc[e] = tsg_f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -652,9 +815,8 @@ template <int NW, typename V> __device__ __forceinline__ V over_waves(V (*slot)[
   return sum;
 }
 
-template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_fwd_kernel(AttnArgs a) {
-  __shared__ tsg_f4 meet[2][NW][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 4;
+template <int NW, bool SEEN> __device__ __forceinline__ float attn_f32_fwd_tiles(const AttnArgs& a, int tid, tsg_f4 (*meet)[NW][64]) {
+  const int wave = tid >> 6, lane = tid & 63, h = lane >> 4;
   const int tiles = gridDim.x / a.heads;
   const int t0 = (tiles - 1 - (int)(blockIdx.x / a.heads)) * 16, head = blockIdx.x % a.heads, kvh = head / a.group;
   const int t = t0 + (lane & 15);
@@ -666,8 +828,9 @@ template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_fwd_kernel
   keys_of_row(a, t0, t, lo, hi);
   const Bounds b = wave_bounds<16>(lo, hi);
   Sum16 acc;
+  float m, l;
   zero16(acc);
-  float m = -INFINITY, l = 0.0f;
+  m = -INFINITY, l = 0.0f;
   for (int k0 = b.wave_lo, buf = 0; k0 < b.wave_hi; k0 += 16, buf ^= 1) {
     tsg_u4 kf[4];
     tsg_f4 vf[4];
@@ -698,19 +861,29 @@ template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_fwd_kernel
       z[i] = __builtin_amdgcn_exp2f((z[i] - off) * a.scale2);
       l += z[i];
     }
-    add16(acc, vf, z);
+    if constexpr (SEEN) add16_seen(acc, vf, z, lo - k0 - 4 * h, hi - k0 - 4 * h);
+    else add16(acc, vf, z);
   }
+  const float zero = zero_of(acc);
   l = parts_sum<16>(l);
   if (t < a.n_q) {
     store16(acc, a.out + (long)t * a.o_row + head * a.o_head, l == 0.0f ? 0.0f : 1.0f / l, a.dim, wave, h);
-    if (threadIdx.x < 16) a.stat[(long)head * a.n_q + t] = l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l));
+    if (tid < 16) a.stat[(long)head * a.n_q + t] = l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l));
+  }
+  return zero;
+}
+template <int NW> __global__ __launch_bounds__(64 * NW, 4) void attn_f32_fwd_kernel(AttnArgs a) {
+  __shared__ tsg_f4 meet[2][NW][64];
+  __shared__ int redo[NW];
+  int tid = threadIdx.x;
+  if (any_wave<NW>(attn_f32_fwd_tiles<NW, false>(a, tid, meet), tid >> 6, redo)) {
+    tsg_again(tid);
+    attn_f32_fwd_tiles<NW, true>(a, tid, meet);
   }
 }
 
-template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_dq_kernel(AttnArgs a) {
-  __shared__ tsg_f4 meet[4][NW][64];
-  __shared__ float meet_delta[NW][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 4;
+template <int NW, bool SEEN> __device__ __forceinline__ float attn_f32_dq_tiles(const AttnArgs& a, int tid, tsg_f4 (*meet)[NW][64], float (*meet_delta)[64]) {
+  const int wave = tid >> 6, lane = tid & 63, h = lane >> 4;
   const int tiles = gridDim.x / a.heads;
   const int t0 = (tiles - 1 - (int)(blockIdx.x / a.heads)) * 16, head = blockIdx.x % a.heads, kvh = head / a.group;
   const int t = t0 + (lane & 15);
@@ -735,11 +908,11 @@ template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_dq_kernel(
   float2 st = make_float2(0.0f, INFINITY);
   if (t < a.n_q) {
     st = a.stat[(long)head * a.n_q + t];
-    if (threadIdx.x < 16) a.delta[(long)head * a.n_q + t] = delta;  // the dk / dv kernel, next on the stream, reads it
+    if (tid < 16) a.delta[(long)head * a.n_q + t] = delta;  // the dk / dv kernel, next on the stream, reads it
   }
   Sum16 acc;
-  zero16(acc);
   Rows16 k(a.k_row, a.chunks, wave, lane), v(a.v_row, a.chunks, wave, lane);
+  zero16(acc);
   for (int k0 = b.wave_lo, buf = 0; k0 < b.wave_hi; k0 += 16, buf ^= 2) {
     tsg_u4 kf[4], vf[4];
     tsg_f4 kc[4];
@@ -747,7 +920,7 @@ template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_dq_kernel(
     v.at(a.v + kvh * a.v_head + (long)k0 * a.v_row, b.wave_hi - k0);
     k.rows(kf);
     v.rows(vf);
-    k.cols(kc);
+    if constexpr (!SEEN) k.cols(kc);
     tsg_f4 z = dot16(kf, qf, tsg_f4{0.0f, 0.0f, 0.0f, 0.0f}), dp = dot16(vf, gf, tsg_f4{0.0f, 0.0f, 0.0f, 0.0f});
     if (NW > 1) meet[buf][wave][lane] = z;
     dp = over_waves<NW>(meet[buf + 1], dp, wave, lane);
@@ -764,14 +937,31 @@ template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_dq_kernel(
       for (int i = 0; i < 4; ++i)
         if (k0 + 4 * h + i < lo || k0 + 4 * h + i >= hi) z[i] = 0.0f;
     }
-    add16(acc, kc, z);
+    if constexpr (SEEN) {
+      __builtin_amdgcn_sched_barrier(0);
+      k.cols(kc);
+      add16_seen(acc, kc, z, lo - k0 - 4 * h, hi - k0 - 4 * h);
+    } else {
+      add16(acc, kc, z);
+    }
   }
+  const float zero = zero_of(acc);
   if (t < a.n_q) store16(acc, a.dq + (long)t * a.dq_row + head * a.dq_head, a.scale, a.dim, wave, h);
+  return zero;
+}
+template <int NW> __global__ __launch_bounds__(64 * NW, 4) void attn_f32_dq_kernel(AttnArgs a) {
+  __shared__ tsg_f4 meet[4][NW][64];
+  __shared__ int redo[NW];
+  __shared__ float meet_delta[NW][64];
+  int tid = threadIdx.x;
+  if (any_wave<NW>(attn_f32_dq_tiles<NW, false>(a, tid, meet, meet_delta), tid >> 6, redo)) {
+    tsg_again(tid);
+    attn_f32_dq_tiles<NW, true>(a, tid, meet, meet_delta);
+  }
 }
 
-template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_dkv_kernel(AttnArgs a) {
-  __shared__ tsg_f4 meet[4][NW][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 4;
+template <int NW, bool SEEN> __device__ __forceinline__ float attn_f32_dkv_tiles(const AttnArgs& a, int tid, tsg_f4 (*meet)[NW][64]) {
+  const int wave = tid >> 6, lane = tid & 63, h = lane >> 4;
   const int split = blockIdx.x / a.kv_heads % a.n_split, j0 = blockIdx.x / a.kv_heads / a.n_split * 16, kvh = blockIdx.x % a.kv_heads;
   const int j = j0 + (lane & 15);
   tsg_u4 kf[4], vf[4];
@@ -786,12 +976,12 @@ template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_dkv_kernel
   rows_of_key(a, j0, j, lo, hi);
   const Bounds b = wave_bounds<16>(lo, hi);
   Sum16 dk, dv;
-  zero16(dk);
-  zero16(dv);
   const int per = b.wave_lo < b.wave_hi ? (b.wave_hi - b.wave_lo + 15) / 16 : 0, all = per * a.group;
   const int first = (int)((long)all * split / a.n_split), last = (int)((long)all * (split + 1) / a.n_split);
-  int head = kvh * a.group + (all ? first / per : 0), t0 = b.wave_lo + (all ? first % per : 0) * 16;
   Rows16 q(a.q_row, a.chunks, wave, lane), g(a.do_row, a.chunks, wave, lane);
+  zero16(dk);
+  zero16(dv);
+  int head = kvh * a.group + (all ? first / per : 0), t0 = b.wave_lo + (all ? first % per : 0) * 16;
   for (int step = first, buf = 0; step < last; ++step, buf ^= 2) {
     tsg_u4 qf[4], gf[4];
     tsg_f4 qc[4], gc[4];
@@ -799,8 +989,7 @@ template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_dkv_kernel
     g.at(a.d_o + head * a.do_head + (long)t0 * a.do_row, b.wave_hi - t0);
     q.rows(qf);
     g.rows(gf);
-    g.cols(gc);
-    q.cols(qc);
+    if constexpr (!SEEN) g.cols(gc), q.cols(qc);
     float2 st[4];
     float delta[4];
 #pragma unroll
@@ -828,12 +1017,21 @@ template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_dkv_kernel
       for (int i = 0; i < 4; ++i)
         if (t0 + 4 * h + i < lo || t0 + 4 * h + i >= hi) z[i] = dp[i] = 0.0f;
     }
-    add16(dv, gc, z);
-    add16(dk, qc, dp);
+    if constexpr (SEEN) {
+      __builtin_amdgcn_sched_barrier(0);
+      g.cols(gc);
+      add16_seen(dv, gc, z, lo - t0 - 4 * h, hi - t0 - 4 * h);
+      q.cols(qc);
+      add16_seen(dk, qc, dp, lo - t0 - 4 * h, hi - t0 - 4 * h);
+    } else {
+      add16(dv, gc, z);
+      add16(dk, qc, dp);
+    }
     t0 += 16;
     if (t0 >= b.wave_hi) t0 = b.wave_lo, ++head;
   }
-  if (j >= a.n_k) return;
+  const float zero = zero_of(dk, zero_of(dv));
+  if (j >= a.n_k) return zero;
   if (a.n_split > 1) {
     char* p = reinterpret_cast<char*>(a.part + (((long)split * a.n_k + j) * a.kv_heads + kvh) * a.dim);
     store16(dk, p, 1.0f, a.dim, wave, h);
@@ -841,6 +1039,16 @@ template <int NW> __global__ __launch_bounds__(64 * NW) void attn_f32_dkv_kernel
   } else {
     store16(dk, a.dk + (long)j * a.dk_row + kvh * a.dk_head, a.scale, a.dim, wave, h);
     store16(dv, a.dv + (long)j * a.dv_row + kvh * a.dv_head, 1.0f, a.dim, wave, h);
+  }
+  return zero;
+}
+template <int NW> __global__ __launch_bounds__(64 * NW, 3) void attn_f32_dkv_kernel(AttnArgs a) {
+  __shared__ tsg_f4 meet[4][NW][64];
+  __shared__ int redo[NW];
+  int tid = threadIdx.x;
+  if (any_wave<NW>(attn_f32_dkv_tiles<NW, false>(a, tid, meet), tid >> 6, redo)) {
+    tsg_again(tid);
+    attn_f32_dkv_tiles<NW, true>(a, tid, meet);
   }
 }
 

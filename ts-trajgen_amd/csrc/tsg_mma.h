@@ -131,11 +131,12 @@ template <typename D> struct TsgAccB {
   template <int CH> __device__ __forceinline__ void mma(unsigned col, int block, int offset, tsg_f32x16& acc) const {
     const unsigned at = col ^ (block * 64);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const tsg_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tsg_lds_s4*>((uintptr_t)(at + offset + 16 * t * CH * 16)));
-      const tsg_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tsg_lds_s4*>((uintptr_t)((at ^ 32) + offset + (16 * t + 8) * CH * 16)));
-      tsg_mma<D>(tsg_join4(x, y), v[t], acc);
-    }
+    for (int t = 0; t < 2; ++t) tsg_mma<D>(frag<CH>(at, offset, t), v[t], acc);
+  }
+  template <int CH> static __device__ __forceinline__ tsg_u4 frag(unsigned at, int offset, int t) {
+    const tsg_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tsg_lds_s4*>((uintptr_t)(at + offset + 16 * t * CH * 16)));
+    const tsg_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tsg_lds_s4*>((uintptr_t)((at ^ 32) + offset + (16 * t + 8) * CH * 16)));
+    return tsg_join4(x, y);
   }
 };
 // ---- tiles from memory straight into LDS (buffer_load_dwordx4 ... lds: lane l's 16 bytes go to m0 + 16 l).
