@@ -495,6 +495,35 @@ def test_cross_entropy_rows_left_out_hold_anything(dt):
     assert float(got[0][target == -100].abs().sum()) == 0.0
 
 
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('value', [float('nan'), float('inf')])
+def test_cross_entropy_rows_that_are_not_finite_spoil_only_themselves(dt, value):
+    """A state, and an upstream gradient, that are not finite: the other rows' losses and dh are what they are without.  All of
+    it is small (2^-20), so that a scale taken from the broken value would lose it."""
+    from ts_trajgen_amd import ops
+    h, w, b, target = entropy_case(dt, 130, 900, 64, seed=12, ignored=0.0, h_by=2.0 ** -6 if dt == torch.float16 else 2.0 ** -20)
+    up = torch.rand(130, generator=torch.Generator().manual_seed(2)).to(DEV) * 2.0 ** -10 + 2.0 ** -12
+    keep = torch.arange(130) != 17
+
+    def run(h, up):
+        h = h.detach().requires_grad_(True)
+        rows = ops.linear_cross_entropy(h, w, target, bias=b, reduction='none')
+        return rows.detach(), torch.autograd.grad(rows, h, up)[0]
+    rows, dh = run(h, up)
+    _, want, _, _ = plain_cross_entropy(h, w, b, target, -100, up)
+    assert rel(dh, want) < bound_of(dt, want)
+    bad = h.detach().clone()
+    bad[17, 3] = value
+    rows2, dh2 = run(bad, up)
+    assert torch.isnan(rows2[17]) and rel(rows2[keep], rows[keep]) < 2e-5
+    assert torch.isnan(dh2[17].float()).all() and rel(dh2[keep], want[keep]) < bound_of(dt, want[keep])
+    up2 = up.clone()
+    up2[17] = value
+    rows2, dh2 = run(h, up2)
+    assert torch.equal(rows2, rows) and rel(dh2[keep], want[keep]) < bound_of(dt, want[keep])
+    assert not torch.isfinite(dh2[17].float()).any()
+
+
 def test_cross_entropy_masked_entries_empty_means_and_bad_targets():
     from ts_trajgen_amd import ops
     for dt in TYPES:

@@ -44,6 +44,9 @@ __device__ __forceinline__ float scale_of(unsigned bits) {
   return ldexpf(1.0f, s);
 }
 
+// what a magnitude says to a common scale: one that is not finite spoils its own row, not the others' precision
+__device__ __forceinline__ float weight_of(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.0f; }
+
 struct XentArgs {
   const char *h, *w;            // operands of the products (f32: their planes in the workspace)
   long h_row, w_row;            // bytes
@@ -309,7 +312,7 @@ __global__ __launch_bounds__(1024) void xent_grad_kernel(XentArgs a, const float
     if (in) a.g[t] = g;
     const unsigned long long used = __ballot(g != 0.0f);
     if ((threadIdx.x & 63) == 0) a.used[t >> 6] = used;
-    m = fmaxf(m, fabsf(g));
+    m = fmaxf(m, weight_of(g));
   }
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
@@ -559,7 +562,7 @@ __global__ __launch_bounds__(256) void xent_amax_kernel(Planes a) {
   for (long i = b * 256 + threadIdx.x; i < n; i += nb * 256) {
     if (first && a.target[i / a.chunks] == a.ignore) continue;
     const float4 v = row4(x, row, i, a.chunks);
-    m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+    m = fmaxf(m, fmaxf(fmaxf(weight_of(v.x), weight_of(v.y)), fmaxf(weight_of(v.z), weight_of(v.w))));
   }
   m = block_max(m, join);
   if (threadIdx.x == 0) a.amax[blockIdx.x] = m;
