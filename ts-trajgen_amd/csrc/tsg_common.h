@@ -60,6 +60,26 @@ __device__ __forceinline__ float tsg_wave_max_u(float v) {
   return fmaxf(fmaxf(tsg_lane_value(v, 0), tsg_lane_value(v, 16)), fmaxf(tsg_lane_value(v, 32), tsg_lane_value(v, 48)));
 }
 
+// a + b * c in two roundings.  Search results are held to recorded orders of nearly equal priorities, so which products round
+// before they are added is part of them and stated, not left to what the compiler happens to fuse.
+__device__ __forceinline__ float tsg_add_product(float a, float b, float c) {
+#pragma clang fp contract(off)
+  const float p = b * c;
+  return a + p;
+}
+__device__ __forceinline__ float tsg_cell(float f, float c, float i, float g) {  // f c + i g, each product rounded
+#pragma clang fp contract(off)
+  const float x = f * c, y = i * g;
+  return x + y;
+}
+// sum of products of a lane's JT elements: one and the first two of eight fused
+template <int JT> __device__ __forceinline__ float tsg_lane_dot(const float (&x)[JT], const float (&y)[JT]) {
+  float p = 0.0f;
+#pragma unroll
+  for (int j = 0; j < JT; ++j) p = JT == 1 || (JT == 8 && j < 2) ? __builtin_fmaf(x[j], y[j], p) : tsg_add_product(p, x[j], y[j]);
+  return p;
+}
+
 // v_exp_f32 / v_rcp_f32 forms (about 1e-7 absolute error, far inside the 1e-4 parity budget)
 #ifndef TSG_PRECISE_GATES
 #define TSG_PRECISE_GATES 0  // 1: libm expf / tanhf and a true division (ablation: do fewer near-ties flip?)

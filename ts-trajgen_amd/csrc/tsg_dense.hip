@@ -344,7 +344,7 @@ __global__ __launch_bounds__(256, 2) void lstm_layer_kernel(LstmArgs a) {
     const float zi = acc[0][i] + tv.x, zf = acc[1][i] + tv.y;
     const float zg = acc[2][i] + tv.z, zo = acc[3][i] + tv.w;
     const float cp = s_prev[r] >= 0 ? cprev[i] : 0.0f;
-    const float cn = tsg_sigmoid(zf) * cp + tsg_sigmoid(zi) * tsg_tanh(zg);
+    const float cn = tsg_cell(tsg_sigmoid(zf), cp, tsg_sigmoid(zi), tsg_tanh(zg));
     const float hn = tsg_sigmoid(zo) * tsg_tanh(cn);
     if (s_out[r] < 0) continue;  // no row at this position of the tile
     const size_t o = (size_t)s_out[r] * hp + u;
@@ -638,7 +638,7 @@ __device__ __forceinline__ void lstm_layer_split_body(const LstmArgs& a) {
     const float zi = acc[0][i] * inv + tv.x, zf = acc[1][i] * inv + tv.y;
     const float zg = acc[2][i] * inv + tv.z, zo = acc[3][i] * inv + tv.w;
     const float cp = s_prev[r] >= 0 ? cprev[i] : 0.0f;
-    const float cn = tsg_sigmoid(zf) * cp + tsg_sigmoid(zi) * tsg_tanh(zg);
+    const float cn = tsg_cell(tsg_sigmoid(zf), cp, tsg_sigmoid(zi), tsg_tanh(zg));
     const float hn = tsg_sigmoid(zo) * tsg_tanh(cn);
     if (s_out[r] < 0) continue;  // no row at this position of the tile
     const size_t o = (size_t)s_out[r] * hp + u;

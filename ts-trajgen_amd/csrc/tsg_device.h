@@ -123,9 +123,10 @@ __device__ __forceinline__ void attn_fold4(AttnAcc<JT>& s, float key[4][JT], uns
   float part[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    part[u] = 0.0f;
+    float x[JT], y[JT];
 #pragma unroll
-    for (int j = 0; j < JT; ++j) part[u] += key[u][j] * q[j];
+    for (int j = 0; j < JT; ++j) x[j] = key[u][j], y[j] = q[j];
+    part[u] = tsg_lane_dot<JT>(x, y);
   }
 #pragma unroll
   for (int u = 0; u < 4; ++u) part[u] = tsg_wave_sum_u(part[u]);
@@ -146,7 +147,7 @@ __device__ __forceinline__ void attn_fold4(AttnAcc<JT>& s, float key[4][JT], uns
   for (int j = 0; j < JT; ++j) {
     float a = s.v[j] * scale;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) a += w[u] * key[u][j];
+    for (int u = 0; u < 4; ++u) a = JT == 1 && u < 3 ? tsg_add_product(a, w[u], key[u][j]) : __builtin_fmaf(w[u], key[u][j], a);
     s.v[j] = a;
   }
   s.m = mn;
@@ -205,10 +206,10 @@ __device__ __forceinline__ void attn_fold_n(AttnAcc<JT>& s, float key[N][JT], un
   float part[N];
 #pragma unroll
   for (int u = 0; u < N; ++u) {
-    float p = 0.0f;
+    float x[JT], y[JT];
 #pragma unroll
-    for (int j = 0; j < JT; ++j) p += key[u][j] * q[j];
-    part[u] = tsg_wave_sum_u(p);
+    for (int j = 0; j < JT; ++j) x[j] = key[u][j], y[j] = q[j];
+    part[u] = tsg_wave_sum_u(tsg_lane_dot<JT>(x, y));
   }
   float mn = s.m;
 #pragma unroll
@@ -227,7 +228,7 @@ __device__ __forceinline__ void attn_fold_n(AttnAcc<JT>& s, float key[N][JT], un
   for (int j = 0; j < JT; ++j) {
     float a = s.v[j] * scale;
 #pragma unroll
-    for (int u = 0; u < N; ++u) a += w[u] * key[u][j];
+    for (int u = 0; u < N; ++u) a = JT == 1 && u < N - 1 ? tsg_add_product(a, w[u], key[u][j]) : __builtin_fmaf(w[u], key[u][j], a);
     s.v[j] = a;
   }
   s.m = mn;
@@ -240,9 +241,13 @@ __device__ __forceinline__ float tsg_h_logit(const tsg_model& m, int cand, int d
   const float* pt = m.pto + (size_t)des * TSG_H_HIDDEN;
   float acc = hpar[40];
 #pragma unroll
-  for (int j = 0; j < TSG_H_HIDDEN; ++j) acc += hpar[20 + j] * fmaxf(pf[j] + pt[j], 0.0f);
+  for (int j = 0; j < TSG_H_HIDDEN; ++j) {
+    const float x = fmaxf(pf[j] + pt[j], 0.0f);
+    acc = j < 8 ? __builtin_fmaf(hpar[20 + j], x, acc) : tsg_add_product(acc, hpar[20 + j], x);
+  }
 #pragma unroll
-  for (int j = 0; j < TSG_H_HIDDEN; ++j) acc += hpar[30 + j] * fmaxf(hpar[j] * dis + hpar[10 + j], 0.0f);
+  for (int j = 0; j < TSG_H_HIDDEN; ++j)
+    acc = tsg_add_product(acc, hpar[30 + j], fmaxf(__builtin_fmaf(hpar[j], dis, hpar[10 + j]), 0.0f));
   return acc;
 }
 

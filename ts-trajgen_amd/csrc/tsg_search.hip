@@ -517,10 +517,10 @@ __global__ __launch_bounds__(256) void score_frontier_kernel(tsg_model m, Engine
     float part[G];
 #pragma unroll
     for (int u = 0; u < G; ++u) {
-      float p = 0.0f;
+      float w[JT];
 #pragma unroll
-      for (int j = 0; j < JT; ++j) p += keyB[u][j] * pooled[j];
-      part[u] = p;
+      for (int j = 0; j < JT; ++j) w[j] = keyB[u][j];
+      part[u] = tsg_lane_dot<JT>(w, pooled);
     }
 #pragma unroll
     for (int u = 0; u < G; ++u) part[u] = tsg_wave_sum_u(part[u]);
@@ -538,7 +538,8 @@ __global__ __launch_bounds__(256) void score_frontier_kernel(tsg_model m, Engine
       load_row<JT>(m.out_w + (size_t)cid * hp, w, J, lane);
       part[u] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < JT; ++j) part[u] += w[j] * pooled[j];
+      for (int j = 0; j < JT; ++j)
+        part[u] = u == 0 && JT > 1 ? tsg_add_product(part[u], w[j], pooled[j]) : __builtin_fmaf(w[j], pooled[j], part[u]);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) part[u] = tsg_wave_sum_u(part[u]);
