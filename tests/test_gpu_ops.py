@@ -634,3 +634,27 @@ def test_the_operators_together_over_packed_trajectories():
     assert rel(loss, want) < 1e-5
     for a, e in zip(got, torch.autograd.grad(want, [xd, wd, bd])):
         assert rel(a, e) < 1e-5
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_saved_tensors_that_hooks_move_elsewhere(dt):
+    """Under save_on_cpu everything saved leaves its memory, which other tensors then take."""
+    from ts_trajgen_amd import ops
+    g = torch.Generator().manual_seed(9)
+    p = torch.tensor(ptr([40, 3, 90]), dtype=torch.int32)
+    x = torch.randn(133, 2, 36, generator=g).to(dt).to(DEV).requires_grad_(True)
+    h, w, b, target = entropy_case(dt, 133, 500, 72, seed=4)
+    step = torch.tensor([6], device=DEV)
+
+    def losses():
+        a = ops.causal_attention(x * 1.0, x * 0.5, x, p.to(DEV))
+        y = ops.dropout(a.reshape(133, 72) * h, 0.3, 5, 2, step.clone())
+        return ops.linear_cross_entropy(y, w, target.clone(), bias=b)
+    want = torch.autograd.grad(losses(), [x, h, w, b])
+    with torch.autograd.graph.save_on_cpu():
+        loss = losses()
+    junk = [torch.full((n,), float('nan'), device=DEV) for n in (50, 133, 400, 5000, 20000, 40000) for _ in range(20)]
+    got = torch.autograd.grad(loss, [x, h, w, b])
+    for a, e in zip(got, want):
+        assert torch.equal(a, e)
+    del junk

@@ -174,3 +174,22 @@ def test_encoder_graph_goes_with_its_output():
         assert len(ops._LIVE) == before
     finally:
         gc.enable()
+
+
+def test_encoder_saved_tensors_that_hooks_move_elsewhere():
+    layer = encoder(8, 8, 2, True)
+    edges = torch.randint(0, 50, (2, 200), generator=torch.Generator().manual_seed(2)).to(DEV)
+    x = torch.randn(50, 8, device=DEV, requires_grad=True)
+
+    def loss():
+        layer.dropout_rng = (1, 0, torch.tensor([3], device=DEV))
+        return (layer((x, edges))[0] ** 2).sum()
+    leaves = [x, layer.linear_proj.weight, layer.bias]
+    want = torch.autograd.grad(loss(), leaves)
+    with torch.autograd.graph.save_on_cpu():
+        value = loss()
+    layer.dropout_rng = None
+    junk = [torch.full((n,), float('nan'), device=DEV) for n in (2, 400, 800) for _ in range(20)]
+    for a, e in zip(torch.autograd.grad(value, leaves), want):
+        assert torch.equal(a, e)
+    del junk

@@ -126,7 +126,10 @@ class _GATTrainFn(torch.autograd.Function):
         for k, v in g.items():
             setattr(d, k, _lib.ptr(v))
         if ctx.rng is not None:
-            ctx.saved_tensors   # raises if the step was advanced or the output overwritten since the forward
+            out, *step = ctx.saved_tensors   # raises if the step was advanced or the output overwritten since the forward
+            d.out = _lib.ptr(out)
+            if step:
+                ctx.rng.step_dev = _lib.ptr(step[0])
         with torch.cuda.device(dev):
             if ctx.rng is None:
                 _lib.check(L.tsg_gat_train_backward(C.byref(d), _lib.current_stream()), 'tsg_gat_train_backward')
@@ -144,8 +147,8 @@ class _GATTrainFn(torch.autograd.Function):
             d_x_d = d_x_d + gemm(g['d_o'], w_skip)
         if ctx.rng is not None:
             from ..ops import _drop
-            p, seed, site, step = cfg['rng']
-            d_x = _drop(d_x_d, p, seed, site, step)
+            p, seed, site, at = cfg['rng']
+            d_x = _drop(d_x_d, p, seed, site, step[0] if step else at)
         else:
             d_x = d_x_d * cfg['m_in'] if cfg['m_in'] is not None else d_x_d
         return (d_x, d_w_proj, d_w_skip, g['d_a_src'].view(1, nh, fo), g['d_a_trg'].view(1, nh, fo),

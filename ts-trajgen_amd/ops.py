@@ -119,7 +119,8 @@ class _Dropout(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         p, seed, site = ctx.cfg
-        step = ctx.saved_tensors[0] if ctx.saved_tensors else ctx.step
+        saved = ctx.saved_tensors
+        step = saved[0] if saved else ctx.step
         return _drop(dy, p, seed, site, step), None, None, None, None
 
 
@@ -185,8 +186,8 @@ def _workspace(d, need, dev):
     return ws
 
 
-# The descriptor that a forward filled, and what it points to beside the saved tensors, stay on its node: the backward runs on
-# autograd's own thread, where every line of Python costs twice as much.
+# The descriptor that a forward filled, and everything it points to, stay on its node: the backward runs on autograd's own
+# thread, where every line of Python costs twice as much, and saved tensors may come back from hooks in other memory.
 
 
 class _CausalAttention(torch.autograd.Function):
@@ -208,18 +209,18 @@ class _CausalAttention(torch.autograd.Function):
             _call('tsg_attn_forward', d, dev)
             if train:
                 d.delta = stats.data_ptr() + 8 * heads * n_q
-                ctx.desc, ctx.need, ctx.keep = d, sizes[1], (ql, kl, vl)
+                ctx.desc, ctx.need, ctx.keep = d, sizes[1], (ql, kl, vl, q_ptr, k_ptr, stats, rest)
         else:
             out.zero_()
         res = out if wide == dim else out[..., :dim].contiguous()
         if train:
-            ctx.save_for_backward(q, k, v, q_ptr, k_ptr, res, stats, rest)
+            ctx.save_for_backward(q, k, v, q_ptr, k_ptr, res)
         return res
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        q, k, v, _, _, out, _, _ = ctx.saved_tensors        # also the check that none of them was written since
+        q, k, v, _, _, out = ctx.saved_tensors        # also the check that none of them was written since
         dev, dim, per = q.device, q.shape[2], 4 if q.dtype == torch.float32 else 8
         wide = -(-dim // per) * per
         dq = torch.empty((q.shape[0], q.shape[1], wide), dtype=q.dtype, device=dev)
@@ -314,14 +315,14 @@ class _LinearCrossEntropy(torch.autograd.Function):
         ws = _workspace(d, sizes[0], dev)  # noqa: F841
         _call('tsg_xent_forward', d, dev)
         if any(ctx.needs_input_grad[:3]):
-            ctx.save_for_backward(h, w, bias, target, store)
-            ctx.desc, ctx.need, ctx.keep = d, sizes[1], (hl, wl, bl, tl)
+            ctx.save_for_backward(h, w, bias, target)
+            ctx.desc, ctx.need, ctx.keep = d, sizes[1], (hl, wl, bl, tl, store)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss):
-        h, w, bias, _, _ = ctx.saved_tensors                # also the check that none of them was written since
+        h, w, bias, _ = ctx.saved_tensors                # also the check that none of them was written since
         dev, width, wide = h.device, h.shape[1], ctx.desc.hidden
         if not d_loss.is_contiguous():
             d_loss = d_loss.contiguous()
