@@ -427,7 +427,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void attn_fwd_
 }
 
 // ------------------------------------------------------------------------------------------------ backward, tiles: dq
-template <typename D, int DP, int BK, bool SEEN>
+template <typename D, int DP, int BK, bool REST, bool SEEN>
 __device__ __forceinline__ float attn_dq_tiles(const AttnArgs& a, int tid, char* lds, int* edge) {
   typedef TsgElem<D> E;
   typedef typename E::Acc Acc;
@@ -519,6 +519,12 @@ __device__ __forceinline__ float attn_dq_tiles(const AttnArgs& a, int tid, char*
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) ds.template mma<CH>(col, dt, W * n * CH * 16, acc[dt]);
         tsg_interleave<ND * 4, ND * 2, 8, 2>();
+        if (REST && edge_tile) {
+          keep_branch();
+          ds.set_rest(z);
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) ds.template mma<CH>(col, dt, W * n * CH * 16, acc[dt]);
+        }
       }
     }
   }
@@ -526,15 +532,19 @@ __device__ __forceinline__ float attn_dq_tiles(const AttnArgs& a, int tid, char*
   if (t < a.n_q) store_rows<D, ND>(acc, a.dq + (long)t * a.dq_row + head * a.dq_head, a.scale, a.dim, h);
   return zero;
 }
-template <typename D, int DP, int BK>
+// REST: a gradient of a short sequence is the sum of few products, and the rounding of ds costs as much there as the output's own (error 1.48
+// to 1.52 times that of sums in 32 bits, rounded once).  In tiles that mask, where short sequences lie, the rest of ds is multiplied as well: 1.05
+// to 1.26 times.  Sequences of 1024 positions and more in the mean do without: 1.44 to 1.46 there, for 16 and 30 us of 303 and 465 (dq, dk and dv
+// of 4 sequences of 2.5-4 k positions, 16 heads over 4, 128 wide), which the branch costs every tile.
+template <typename D, int DP, int BK, bool REST>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void attn_dq_kernel(AttnArgs a) {
   constexpr int CH = DP / TsgElem<D>::EPC, TILE = BK * CH * 16;
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
   __shared__ int edge[8], redo[4];
   int tid = threadIdx.x;
-  if (any_wave<4>(attn_dq_tiles<D, DP, BK, false>(a, tid, lds, edge), tid >> 6, redo)) {
+  if (any_wave<4>(attn_dq_tiles<D, DP, BK, REST, false>(a, tid, lds, edge), tid >> 6, redo)) {
     tsg_again(tid);
-    attn_dq_tiles<D, DP, BK, true>(a, tid, lds, edge);
+    attn_dq_tiles<D, DP, BK, REST, true>(a, tid, lds, edge);
   }
 }
 
@@ -542,7 +552,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void attn_dq_k
 // PART 0: both; 1: dv only; 2: dk only (256 wide: keys, values and both sums do not fit the registers at once)
 // VL: the values' fragments are read from LDS in every step instead of held in registers, which then suffice without spills
 // (128 wide at two waves a SIMD, 256 wide at one).
-template <typename D, int DP, int BQ, int PART, bool VL, bool SEEN>
+template <typename D, int DP, int BQ, int PART, bool VL, bool REST, bool SEEN>
 __device__ __forceinline__ float attn_dkv_tiles(const AttnArgs& a, int tid, char* lds, int* edge, float (*stat)[3][BQ]) {
   typedef TsgElem<D> E;
   typedef typename E::Acc Acc;
@@ -692,6 +702,12 @@ __device__ __forceinline__ float attn_dkv_tiles(const AttnArgs& a, int tid, char
         sb.set(dp);
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) sb.template mma<CH>(col, dt, W * n * CH * 16, dk[dt]);
+        if (REST && edge_tile) {
+          keep_branch();
+          sb.set_rest(dp);
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) sb.template mma<CH>(col, dt, W * n * CH * 16, dk[dt]);
+        }
       }
     }
   }
@@ -708,23 +724,23 @@ __device__ __forceinline__ float attn_dkv_tiles(const AttnArgs& a, int tid, char
   }
   return zero;
 }
-template <typename D, int DP, int BQ, int PART, bool VL>
+template <typename D, int DP, int BQ, int PART, bool VL, bool REST>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void attn_dkv_kernel(AttnArgs a) {
   constexpr int W = TsgElem<D>::W, CH = DP / TsgElem<D>::EPC, TILE = BQ * CH * 16;
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + (VL ? 4 * W * CH * 16 : 0)];
   __shared__ __attribute__((aligned(16))) float stat[2][3][BQ];  // maximum, log2 of the sum, delta
   __shared__ int edge[8], redo[4];
   int tid = threadIdx.x;
-  if (any_wave<4>(attn_dkv_tiles<D, DP, BQ, PART, VL, false>(a, tid, lds, edge, stat), tid >> 6, redo)) {
+  if (any_wave<4>(attn_dkv_tiles<D, DP, BQ, PART, VL, REST, false>(a, tid, lds, edge, stat), tid >> 6, redo)) {
     // one after the other: with both it would need more registers than the first walk
     if constexpr (PART != 2) {
       tsg_again(tid);
-      attn_dkv_tiles<D, DP, BQ, 1, false, true>(a, tid, lds, edge, stat);
+      attn_dkv_tiles<D, DP, BQ, 1, false, false, true>(a, tid, lds, edge, stat);
     }
     if constexpr (PART == 0) __syncthreads();
     if constexpr (PART != 1) {
       tsg_again(tid);
-      attn_dkv_tiles<D, DP, BQ, 2, VL, true>(a, tid, lds, edge, stat);
+      attn_dkv_tiles<D, DP, BQ, 2, VL, false, true>(a, tid, lds, edge, stat);
     }
   }
 }
@@ -1495,6 +1511,23 @@ template <typename D> int forward_of(const tsg_attn_desc* d, hipStream_t s) {
   return 0;
 }
 
+template <typename D, bool REST> void launch_backward(const AttnArgs& a, dim3 gq, dim3 gk, hipStream_t s) {
+  const dim3 block(256);
+  if (a.n_q) {
+    if (a.dim <= 64) hipLaunchKernelGGL((attn_dq_kernel<D, 64, 64, REST>), gq, block, 0, s, a);
+    else if (a.dim <= 128) hipLaunchKernelGGL((attn_dq_kernel<D, 128, 64, REST>), gq, block, 0, s, a);
+    else hipLaunchKernelGGL((attn_dq_kernel<D, 256, 32, REST>), gq, block, 0, s, a);
+  }
+  if (a.n_k) {
+    if (a.dim <= 64) hipLaunchKernelGGL((attn_dkv_kernel<D, 64, 32, 0, REST, REST>), gk, block, 0, s, a);  // the rest takes the values' registers
+    else if (a.dim <= 128) hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0, true, REST>), gk, block, 0, s, a);
+    else {
+      hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 1, false, false>), gk, block, 0, s, a);
+      hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 2, true, REST>), gk, block, 0, s, a);
+    }
+  }
+}
+
 template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
   AttnArgs a = args_of(d);
   a.n_split = dkv_splits_of(d);
@@ -1519,19 +1552,8 @@ template <typename D> int backward_of(const tsg_attn_desc* d, hipStream_t s) {
       else hipLaunchKernelGGL(attn_f32_dkv_kernel<4>, gk, block, 0, s, a);
     }
   } else {
-    if (a.n_q) {
-      if (a.dim <= 64) hipLaunchKernelGGL((attn_dq_kernel<D, 64, 64>), gq, block, 0, s, a);
-      else if (a.dim <= 128) hipLaunchKernelGGL((attn_dq_kernel<D, 128, 64>), gq, block, 0, s, a);
-      else hipLaunchKernelGGL((attn_dq_kernel<D, 256, 32>), gq, block, 0, s, a);
-    }
-    if (a.n_k) {
-      if (a.dim <= 64) hipLaunchKernelGGL((attn_dkv_kernel<D, 64, 32, 0, false>), gk, block, 0, s, a);
-      else if (a.dim <= 128) hipLaunchKernelGGL((attn_dkv_kernel<D, 128, 32, 0, true>), gk, block, 0, s, a);
-      else {
-        hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 1, false>), gk, block, 0, s, a);
-        hipLaunchKernelGGL((attn_dkv_kernel<D, 256, 32, 2, true>), gk, block, 0, s, a);
-      }
-    }
+    if (d->n_q < 1024 * (int64_t)d->n_seq) launch_backward<D, true>(a, gq, gk, s);
+    else launch_backward<D, false>(a, gq, gk, s);
   }
   if (a.n_k && a.n_split > 1)
     hipLaunchKernelGGL(attn_dkv_join_kernel<D>, dim3((unsigned)(((long)a.n_k * a.kv_heads * a.dim / 4 + 255) / 256), 2), block, 0, s, a);

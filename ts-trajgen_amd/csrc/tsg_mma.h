@@ -128,6 +128,12 @@ template <typename D> struct TsgAccB {
 #pragma unroll
       for (int w = 0; w < 4; ++w) v[t][w] = tsg_pack2<D>(p[8 * t + 2 * w], p[8 * t + 2 * w + 1]);
   }
+  // what set() rounded off p
+  __device__ __forceinline__ void set_rest(tsg_f32x16 p) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] -= (float)(typename D::type)p[i];
+    set(p);
+  }
   template <int CH> __device__ __forceinline__ void mma(unsigned col, int block, int offset, tsg_f32x16& acc) const {
     const unsigned at = col ^ (block * 64);
 #pragma unroll
