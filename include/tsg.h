@@ -23,6 +23,8 @@
  *     three f16 matrix-core passes per product with fp32 accumulation, and stores hidden states in that form;
  *     gates use v_exp_f32 / v_rcp_f32.  state_format == 0 is the plain fp32 matrix-core path.  Both forms give the
  *     oracle's trajectories on every golden and full-size test; a near-tie (|df| < 1e-5) may fall differently.
+ *     The operators over sequences (tsg_dropout, tsg_attn_*, tsg_xent_*) take f32, bf16 and f16; their sums, statistics and
+ *     exponentials are f32, and what they round to fewer bits is said where they are declared.
  */
 #ifndef TSG_H_
 #define TSG_H_
@@ -554,6 +556,8 @@ int tsg_gat_train_backward_rng(const tsg_gat_train* d, const tsg_gat_dropout* r,
  * stats [heads][n_q][2] f32 is written by the forward (a row's largest q.k, and the base-2 logarithm of the sum of
  * exp(scale (q.k - largest)); 0 and +inf where a row sees nothing) and read, with out, by the backward, which writes
  * delta [heads][n_q].
+ * 16-bit types: p and the gradients of the scores are rounded to the type where they enter a product, all sums are f32.  Elements
+ * that are not finite reach the rows that see them and no others (where one is infinite, a sum over it may be NaN).
  * workspace: what tsg_attn_workspace says, 16-byte aligned, for the forward with few rows over many keys and for the
  * backward of few long sequences; 0 bytes = none needed. */
 typedef struct tsg_attn_desc {
@@ -586,6 +590,8 @@ int tsg_attn_backward(const tsg_attn_desc* d, void* stream);
  * other target outside [0, n_vocab) makes the row's loss and gradients NaN.  bias (may be NULL) and the gradients
  * have the type of h and w.  The backward takes d_loss (one number, or one per row for reduction 0) and the stats that
  * the forward left, takes the vocabulary in pieces and writes dh, dw and dbias whole.
+ * The gradients of the logits are rounded to the type where they enter a product (f32: h, w and they are two f16 numbers each, 22
+ * bits together); all sums, maxima and logarithms are f32.
  * Base addresses of h and w are 16-byte aligned, rows a multiple of 16 and less than 2^23 bytes apart, hidden a multiple of 8 (pad with
  * zeros), dh and dw 16-byte aligned with rows a multiple of 4 elements apart, the workspace 256-byte aligned; tsg_xent_workspace says how much.  n_rows >= 1. */
 typedef struct tsg_xent_desc {

@@ -105,3 +105,20 @@ def test_cross_entropy_refuses_cpu_tensors():
 def test_attention_backward_of_one_long_sequence_needs_its_workspace():
     assert _attn('tsg_attn_backward', n_q=4096, n_k=4096) == -2
     assert _attn('tsg_attn_backward', n_q=4096, n_k=4096, workspace=4104, workspace_bytes=1 << 40) == -2
+
+
+def test_encoder_entries_with_a_generator_refuse_before_any_launch():
+    import ctypes as C
+    from ts_trajgen_amd import _lib
+    L = _lib.lib()
+    for entry in (L.tsg_gat_train_forward_rng, L.tsg_gat_train_backward_rng):
+        d, ok = _lib.GatTrain(), _lib.GatDropout(0.5, 1, 0, 0, None)
+        assert entry(None, C.byref(ok), None) < 0
+        assert entry(C.byref(d), None, None) < 0
+        assert entry(C.byref(d), C.byref(ok), None) < 0         # an empty description of the layer
+        for bad in [(-0.1, 1, 0), (1.5, 1, 0), (float('nan'), 1, 0), (0.5, 1, (1 << 32) - 2)]:
+            assert entry(C.byref(d), C.byref(_lib.GatDropout(*bad, 0, None)), None) < 0
+        for mask in ('m_in', 'm_proj', 'm_att'):                # masks, or a generator
+            d = _lib.GatTrain()
+            setattr(d, mask, 4096)
+            assert entry(C.byref(d), C.byref(ok), None) < 0

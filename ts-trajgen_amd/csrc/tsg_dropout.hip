@@ -2,7 +2,8 @@
 // the same call on the gradient.  A dropped element is 0 whatever x holds there (a select, not a product).
 //
 // Bound: one read and one write of the tensor (HBM), against ten Philox rounds for four elements (20 32 x 32 -> 64 bit
-// products, quarter rate).
+// products, quarter rate).  40306 x 1280 f32: 74 us, 5.5 TB/s (a large device copy: 5.1); 16384 x 4096 bf16: 54 us, 5.0 TB/s; one
+// pass over 251 x 306 is 3 us, all launch.
 #include "tsg_philox.h"
 
 #include <hip/hip_bf16.h>
