@@ -12,6 +12,7 @@ first order: differentiating a gradient raises.
 """
 import ctypes as C
 import math
+import threading
 import weakref
 
 import torch
@@ -68,6 +69,7 @@ def _call(entry, d, dev):
 
 
 _LIVE = weakref.WeakSet()     # the operators' own nodes in autograd graphs that are alive
+_LIVE_LOCK = threading.Lock()
 
 
 def _enter(ctx, *inputs):
@@ -81,12 +83,15 @@ def _enter(ctx, *inputs):
         return
     here = _stream(inputs[0].device)
     if torch.cuda.is_current_stream_capturing():
-        for node in list(_LIVE):
+        with _LIVE_LOCK:
+            nodes = list(_LIVE)
+        for node in nodes:
             if node.stream != here and not leaves.isdisjoint(node.leaves):
                 raise RuntimeError('capture of a backward while an eager autograd graph of the same leaf is alive: drop the '
                                    'eager results (del, or .detach() what is kept) before capturing')
     ctx.leaves, ctx.stream = leaves, here
-    _LIVE.add(ctx)
+    with _LIVE_LOCK:
+        _LIVE.add(ctx)
 
 
 # ---------------------------------------------------------------------------------------------------------- dropout
