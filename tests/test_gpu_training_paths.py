@@ -193,3 +193,18 @@ def test_encoder_saved_tensors_that_hooks_move_elsewhere():
     for a, e in zip(torch.autograd.grad(value, leaves), want):
         assert torch.equal(a, e)
     del junk
+
+
+@pytest.mark.parametrize('hidden', [50, 320])
+def test_function_g_of_other_widths(hidden):
+    loc, tim, ptr = trajectories([12, 40, 2])
+    ref = function_g(hidden=hidden).double()
+    want = plain_loss(ref, loc, tim, ptr)
+    want.backward()
+    m = function_g(hidden=hidden).to(DEV).train(True)
+    got = m.trajectory_loss(loc, tim, ptr)
+    got.backward()
+    assert abs(float(got.detach()) - float(want.detach())) <= 2e-5 * float(want.detach())
+    for (k, w), r in zip(m.named_parameters(), ref.parameters()):
+        if r.grad is not None:
+            assert float((w.grad.double().cpu() - r.grad).norm() / r.grad.norm()) <= 2e-5, k

@@ -77,8 +77,9 @@ class FunctionGFC(nn.Module):
         trace_loc and trace_time hold the trajectories one behind the other ([n] integers), seq_ptr ([n_seq + 1] int32)
         their starts.  target ([n] int64, -100 = not counted) defaults to the next road of the same trajectory; positions of
         no trajectory never count.  In training mode the dropouts of function_g_fc.py:160,182 are live, drawn from the
-        counter (seed, site 0 and 1, step): give every training step its own step.  hidden_size is at most 512 and a
-        multiple of 4 (ops.causal_attention).  In inference mode torch's recurrence has no backward.  The call waits for the device once: it looks at the lengths and ids."""
+        counter (seed, site 0 and 1, step): give every training step its own step.  hidden_size is at most 512
+        (ops.causal_attention).  In inference mode torch's recurrence has no backward.  The call waits for the
+        device once: it looks at the lengths and ids."""
         dev = self.out_fc.weight.device
         if dev.type != 'cuda':
             raise RuntimeError('FunctionGFC.trajectory_loss needs its parameters on a HIP device (no CPU fallback)')
