@@ -56,9 +56,12 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+_ENTRIES = {}
+
+
 def _call(entry, d, dev):
     """entry(d, the current stream of dev) of libtsg, with dev current: a call is a few microseconds of host time all told."""
-    fn = getattr(_lib.lib(), entry)
+    fn = _ENTRIES.get(entry) or _ENTRIES.setdefault(entry, getattr(_lib.lib(), entry))
     if torch._C._cuda_getDevice() == dev.index:
         rc = fn(C.byref(d), _stream(dev))
     else:
@@ -98,14 +101,9 @@ def _enter(ctx, *inputs):
 def _drop(x, p, seed, site, step):
     x = x.contiguous()
     y = torch.empty_like(x)
-    d = _lib.DropoutDesc()
-    d.n, d.dtype, d.site, d.seed, d.p = x.numel(), DTYPES[x.dtype], site, seed, p
-    if torch.is_tensor(step):
-        d.step_dev = _ptr(step)
-    else:
-        d.step = step
-    d.x, d.y = _ptr(x), _ptr(y)
-    _call('tsg_dropout', d, x.device)
+    on_device = torch.is_tensor(step)
+    _call('tsg_dropout', _lib.DropoutDesc(x.numel(), DTYPES[x.dtype], site, 0 if on_device else step, 0, seed, p,
+                                          step.data_ptr() if on_device else None, x.data_ptr(), y.data_ptr()), x.device)
     return y
 
 
@@ -116,6 +114,7 @@ class _Dropout(torch.autograd.Function):
         ctx.cfg = (p, seed, site)
         if torch.is_tensor(step):
             ctx.save_for_backward(step)     # advancing it before the backward is an error that autograd reports
+            ctx.step = None
         else:
             ctx.step = step
         return _drop(x, p, seed, site, step)
@@ -124,8 +123,7 @@ class _Dropout(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         p, seed, site = ctx.cfg
-        saved = ctx.saved_tensors
-        step = saved[0] if saved else ctx.step
+        step = ctx.saved_tensors[0] if ctx.step is None else ctx.step
         return _drop(dy, p, seed, site, step), None, None, None, None
 
 
