@@ -1,0 +1,158 @@
+"""What the sequence operators keep between forward and backward: only what autograd's saved tensors hold, so that hooks which
+move it (offloading, checkpoints) decide what the backward reads and how long the device holds it."""
+import gc
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+N, VOCAB = 133, 500
+
+
+def attention_inputs(dt, dim):
+    from ts_trajgen_amd import ops
+    g = torch.Generator().manual_seed(dim)
+    p = torch.tensor([0, 40, 43, N], dtype=torch.int32, device=DEV)
+    values = [torch.randn(N, h, dim, generator=g).to(dt).to(DEV) for h in (4, 2, 2)]
+    return values, lambda q, k, v: ops.causal_attention(q, k, v, p)
+
+
+def entropy_inputs(dt, width):
+    from ts_trajgen_amd import ops
+    g = torch.Generator().manual_seed(width)
+    values = [torch.randn(*s, generator=g).to(dt).to(DEV) for s in ((N, width), (VOCAB, width), (VOCAB,))]
+    target = torch.randint(0, VOCAB, (N,), generator=g).to(DEV)
+    return values, lambda h, w, b: ops.linear_cross_entropy(h, w, target, bias=b, reduction='none')
+
+
+CASES = [(attention_inputs, 64), (attention_inputs, 38), (attention_inputs, 320), (entropy_inputs, 64), (entropy_inputs, 36)]
+PADDED = (38, 36)     # read from a copy with wider rows
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('make,width', CASES)
+def test_inputs_written_after_their_saved_copies_moved_away(dt, make, width):
+    """Under save_on_cpu the copies are what was saved, and autograd lets the originals be written: the gradients are those of
+    the values at the forward."""
+    values, op = make(dt, width)
+    leaves = [x.clone().requires_grad_(True) for x in values]
+    want = torch.autograd.grad(op(*leaves), leaves, torch.ones_like(op(*leaves)))
+    mid = [x * 1.0 for x in leaves]
+    with torch.autograd.graph.save_on_cpu():
+        out = op(*mid)
+    with torch.no_grad():
+        for x in mid:
+            x.fill_(0.75)
+    got = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    for a, e in zip(got, want):
+        assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize('make,width', CASES)
+def test_strided_inputs_whose_saved_copies_are_laid_out_anew(make, width):
+    values, op = make(torch.float32, width)
+    leaves = [x.clone().requires_grad_(True) for x in values]
+    want = torch.autograd.grad(op(*leaves), leaves, torch.ones_like(op(*leaves)))
+    for offset in (0, 1, 4):
+        # every row inside a wider one: what a hook brings back has other strides and another address
+        mid = [torch.cat([x.new_zeros(x.shape[:-1] + (offset,)), x, x.new_zeros(x.shape[:-1] + (8,))], dim=-1)[..., offset:-8] for x in leaves]
+        with torch.autograd.graph.save_on_cpu():
+            out = op(*mid)
+        for a, e in zip(torch.autograd.grad(out, leaves, torch.ones_like(out)), want):
+            assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('make,width', CASES)
+def test_what_the_device_holds_goes_with_the_saved_tensors(dt, make, width):
+    values, op = make(dt, width)
+    leaves = [x.requires_grad_(True) for x in values]
+    size = sum(x.numel() * x.element_size() for x in leaves)
+    torch.autograd.grad(op(*leaves).sum(), leaves)               # what libraries allocate once is there
+    ones = torch.ones_like(op(*leaves))
+    for offload in (True, False):
+        gc.collect()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        mid = [x * 1.0 for x in leaves]
+        if offload:
+            with torch.autograd.graph.save_on_cpu():
+                out = op(*mid)
+        else:
+            out = op(*mid)
+        del mid
+        held = out.untyped_storage().nbytes() + 1024             # blocks are multiples of 512 bytes
+        if offload:
+            assert torch.cuda.memory_allocated() - before <= held
+        else:
+            assert torch.cuda.memory_allocated() - before >= size  # the operands, until the backward
+        grads = torch.autograd.grad(out, leaves, ones)
+        del grads
+        assert torch.cuda.memory_allocated() - before <= held    # the result is all that is left of the call
+        del out
+
+
+@pytest.mark.parametrize('make,width', CASES)
+def test_writes_that_autograd_sees_are_errors(make, width):
+    values, op = make(torch.float32, width)
+    leaves = [x.requires_grad_(True) for x in values]
+    for i in range(3):
+        mid = [x * 1.0 for x in leaves]
+        out = op(*mid)
+        with torch.no_grad():
+            mid[i].add_(1.0)
+        if width in PADDED and not (make is entropy_inputs and i == 2):
+            continue                                             # the copy is what counts
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            torch.autograd.grad(out, leaves, torch.ones_like(out))
+
+
+@pytest.mark.parametrize('make,width', CASES)
+def test_backward_twice_over_a_kept_graph(make, width):
+    values, op = make(torch.bfloat16, width)
+    leaves = [x.requires_grad_(True) for x in values]
+    out = op(*leaves)
+    ones = torch.ones_like(out)
+    first = torch.autograd.grad(out, leaves, ones, retain_graph=True)
+    second = torch.autograd.grad(out, leaves, ones)
+    for a, e in zip(first, second):
+        assert torch.equal(a, e)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, leaves, ones)
+
+
+@pytest.mark.parametrize('make,width', CASES)
+def test_hooks_that_bring_back_something_else_are_refused(make, width):
+    """Another type or shape than was saved would be read as what it is not."""
+    values, op = make(torch.float32, width)
+    leaves = [x.requires_grad_(True) for x in values]
+    for back in (lambda x: x.half() if x.is_floating_point() else x, lambda x: x[:1], lambda x: x.cpu()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, back):
+            out = op(*leaves)
+        with pytest.raises(RuntimeError, match='saved tensor'):
+            torch.autograd.grad(out, leaves, torch.ones_like(out))
+
+
+def test_dropout_step_that_a_hook_changed_is_refused():
+    from ts_trajgen_amd import ops
+    x = torch.randn(64, device=DEV, requires_grad=True)
+    step = torch.tensor([3], device=DEV)
+    for back in (lambda s: s.int(), lambda s: s.cpu(), lambda s: s.expand(2)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s, back):
+            y = ops.dropout(x, 0.5, 1, 0, step)
+        with pytest.raises(RuntimeError, match='saved tensor'):
+            y.sum().backward()
+
+
+def test_encoder_tensors_that_a_hook_changed_are_refused():
+    from ts_trajgen_amd.generator.gat import GATLayerImp3
+    layer = GATLayerImp3(8, 8, 2, DEV, concat=True, dropout_prob=0.5).to(DEV).train(True)
+    layer.dropout_rng = (1, 0, torch.tensor([3], device=DEV))
+    edges = torch.arange(9, device=DEV).repeat(2, 1)
+    for back in (lambda s: s.cpu(), lambda s: s[:0]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s, back):
+            out, _ = layer((torch.randn(9, 8, device=DEV, requires_grad=True), edges))
+        with pytest.raises(RuntimeError, match='saved tensor'):
+            out.sum().backward()

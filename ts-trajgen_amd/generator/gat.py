@@ -88,12 +88,12 @@ class _GATTrainFn(torch.autograd.Function):
         d.out_bytes = bufs['out'].numel() * 4
         rng = None
         if cfg.get('rng') is not None:
-            from ..ops import _enter
+            from ..ops import _enter, _save
             _enter(ctx, x, w_proj, w_skip, a_src, a_trg, bias)
             p, seed, site, step = cfg['rng']
             rng = _lib.GatDropout(p, seed, site, 0 if torch.is_tensor(step) else step, step.data_ptr() if torch.is_tensor(step) else None)
             # the output is saved as such, not held by its own node; advancing the step before the backward is an error
-            ctx.save_for_backward(bufs['out'], *([step] if torch.is_tensor(step) else []))
+            _save(ctx, bufs['out'], *([step] if torch.is_tensor(step) else []))
         with torch.cuda.device(dev):
             if rng is None:
                 _lib.check(L.tsg_gat_train_forward(C.byref(d), _lib.current_stream()), 'tsg_gat_train_forward')
@@ -126,7 +126,9 @@ class _GATTrainFn(torch.autograd.Function):
         for k, v in g.items():
             setattr(d, k, _lib.ptr(v))
         if ctx.rng is not None:
-            out, *step = ctx.saved_tensors   # raises if the step was advanced or the output overwritten since the forward
+            from ..ops import _saved
+            out, *step = _saved('GATLayerImp3', ctx)   # raises if the step was advanced or the output overwritten since the forward
+            out = out.contiguous()
             d.out = _lib.ptr(out)
             if step:
                 ctx.rng.step_dev = _lib.ptr(step[0])

@@ -97,6 +97,23 @@ def _enter(ctx, *inputs):
         _LIVE.add(ctx)
 
 
+def _save(ctx, *tensors):
+    """Everything a backward reads goes through autograd's saved tensors: hooks may move it or bring it back from elsewhere (then
+    the operands may be written meanwhile), and a backward that does not keep its graph lets go of it."""
+    ctx.save_for_backward(*tensors)
+    ctx.like = [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+
+
+def _saved(what, ctx):
+    """The saved tensors.  What a hook brings back has other addresses and strides; other shapes, types or devices would be read
+    as what they are not."""
+    tensors = ctx.saved_tensors
+    for t, like in zip(tensors, ctx.like):
+        if like is not None and (t.shape, t.dtype, t.device) != like:
+            raise RuntimeError('%s: a saved tensor %s came back as %s' % (what, like, (t.shape, t.dtype, t.device)))
+    return tensors
+
+
 # ---------------------------------------------------------------------------------------------------------- dropout
 def _drop(x, p, seed, site, step):
     x = x.contiguous()
@@ -113,7 +130,7 @@ class _Dropout(torch.autograd.Function):
         _enter(ctx, x)
         ctx.cfg = (p, seed, site)
         if torch.is_tensor(step):
-            ctx.save_for_backward(step)     # advancing it before the backward is an error that autograd reports
+            _save(ctx, step)                # advancing it before the backward is an error that autograd reports
             ctx.step = None
         else:
             ctx.step = step
@@ -123,7 +140,7 @@ class _Dropout(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         p, seed, site = ctx.cfg
-        step = ctx.saved_tensors[0] if ctx.step is None else ctx.step
+        step = _saved('dropout', ctx)[0] if ctx.step is None else ctx.step
         return _drop(dy, p, seed, site, step), None, None, None, None
 
 
@@ -189,10 +206,6 @@ def _workspace(d, need, dev):
     return ws
 
 
-# The descriptor that a forward filled, and everything it points to, stay on its node: the backward runs on autograd's own
-# thread, where every line of Python costs twice as much, and saved tensors may come back from hooks in other memory.
-
-
 class _CausalAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_ptr, k_ptr, scale):
@@ -204,6 +217,7 @@ class _CausalAttention(torch.autograd.Function):
         out = torch.empty((n_q, heads, wide), dtype=q.dtype, device=dev)
         stats = torch.empty(3 * heads * n_q, dtype=torch.float32, device=dev)      # [heads][n_q][2], then delta [heads][n_q]
         rest = torch.empty_like(out) if train and per == 8 else None
+        ctx.need = None
         if n_q and k.shape[0]:
             ql, kl, vl = _laid_out(q, per, wide), _laid_out(k, per, wide), _laid_out(v, per, wide)
             d = _attn_desc(ql, kl, vl, q_ptr, k_ptr, scale, out, stats, rest)
@@ -211,30 +225,31 @@ class _CausalAttention(torch.autograd.Function):
             ws = _workspace(d, sizes[0], dev)  # noqa: F841  (held until the launches are on the stream)
             _call('tsg_attn_forward', d, dev)
             if train:
-                d.delta = stats.data_ptr() + 8 * heads * n_q
-                ctx.desc, ctx.need, ctx.keep = d, sizes[1], (ql, kl, vl, q_ptr, k_ptr, stats, rest)
+                ctx.need, ctx.scale = sizes[1], scale
+                _save(ctx, ql, kl, vl, q_ptr, k_ptr, out, stats, rest)
         else:
             out.zero_()
-        res = out if wide == dim else out[..., :dim].contiguous()
-        if train:
-            ctx.save_for_backward(q, k, v, q_ptr, k_ptr, res)
-        return res
+        ctx.size = n_q, k.shape[0], heads, k.shape[1], dim, wide, per
+        return out if wide == dim else out[..., :dim].contiguous()
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        q, k, v, _, _, out = ctx.saved_tensors        # also the check that none of them was written since
-        dev, dim, per = q.device, q.shape[2], 4 if q.dtype == torch.float32 else 8
-        wide = -(-dim // per) * per
-        dq = torch.empty((q.shape[0], q.shape[1], wide), dtype=q.dtype, device=dev)
-        dk = torch.empty((k.shape[0], k.shape[1], wide), dtype=q.dtype, device=dev)
+        n_q, n_k, heads, kv_heads, dim, wide, per = ctx.size
+        dev, dt = d_out.device, d_out.dtype
+        dq = torch.empty((n_q, heads, wide), dtype=dt, device=dev)
+        dk = torch.empty((n_k, kv_heads, wide), dtype=dt, device=dev)
         dv = torch.empty_like(dk)
-        if q.shape[0] and k.shape[0]:
-            d, gl = ctx.desc, _laid_out(d_out, per, wide)
-            ol = out if wide == dim else _laid_out(out, per, wide)
-            d.out, d.d_out, d.dq, d.dk, d.dv = ol.data_ptr(), gl.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        if ctx.need is not None:
+            q, k, v, q_ptr, k_ptr, out, stats, rest = _saved('causal_attention', ctx)
+            q, k, v, out, gl = [_laid_out(t, per, wide) for t in (q, k, v, out, d_out)]
+            rest = None if rest is None else rest.contiguous()
+            stats, q_ptr, k_ptr = stats.contiguous(), q_ptr.contiguous(), k_ptr.contiguous()
+            d = _attn_desc(q, k, v, q_ptr, k_ptr, ctx.scale, out, stats, rest)
+            d.d_out, d.dq, d.dk, d.dv = gl.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+            d.delta = stats.data_ptr() + 8 * heads * n_q
             d.d_out_row, d.d_out_head = gl.stride(0), gl.stride(1)
-            d.dq_row, d.dk_row, d.dv_row = q.shape[1] * wide, k.shape[1] * wide, k.shape[1] * wide
+            d.dq_row, d.dk_row, d.dv_row = heads * wide, kv_heads * wide, kv_heads * wide
             d.dq_head = d.dk_head = d.dv_head = wide
             ws = _workspace(d, ctx.need, dev)  # noqa: F841
             _call('tsg_attn_backward', d, dev)
@@ -298,6 +313,15 @@ def _rows_for(x, wide):
     return x.clone(memory_format=torch.contiguous_format)
 
 
+def _xent_desc(h, w, bias, target, ignore, reduction, store, loss):
+    rows, wide = h.shape
+    at = store.data_ptr()        # [rows][2] stats, [rows] losses, [2] scales of f32 operands
+    return _lib.XentDesc(DTYPES[h.dtype], wide, reduction, 0, rows, w.shape[0], ignore, h.data_ptr(), w.data_ptr(), _ptr(bias),
+                         max(h.stride(0), wide), max(w.stride(0), wide), target.data_ptr(),
+                         loss.data_ptr() if loss is not None and reduction == 0 else at + 8 * rows, _ptr(loss), at,
+                         at + 12 * rows if h.dtype == torch.float32 else None)
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, w, bias, target, ignore, reduction):
@@ -306,36 +330,33 @@ class _LinearCrossEntropy(torch.autograd.Function):
         hl, wl = _rows_for(h, wide), _rows_for(w, wide)
         bl = None if bias is None else bias.contiguous()
         tl = target.contiguous()
-        # [rows][2] stats, [rows] losses, [2] scales of f32 operands
         store = torch.empty(3 * rows + 2, dtype=torch.float32, device=dev)
-        at = store.data_ptr()
         loss = torch.empty(rows if reduction == 0 else (), dtype=torch.float32, device=dev)
-        d = _lib.XentDesc(DTYPES[h.dtype], wide, reduction, 0, rows, w.shape[0], ignore, hl.data_ptr(), wl.data_ptr(), _ptr(bl),
-                          max(hl.stride(0), wide), max(wl.stride(0), wide), tl.data_ptr(),
-                          loss.data_ptr() if reduction == 0 else at + 8 * rows, loss.data_ptr(), at,
-                          at + 12 * rows if h.dtype == torch.float32 else None)
+        d = _xent_desc(hl, wl, bl, tl, ignore, reduction, store, loss)
         sizes = _sizes('tsg_xent_workspace', d)
         ws = _workspace(d, sizes[0], dev)  # noqa: F841
         _call('tsg_xent_forward', d, dev)
         if any(ctx.needs_input_grad[:3]):
-            ctx.save_for_backward(h, w, bias, target)
-            ctx.desc, ctx.need, ctx.keep = d, sizes[1], (hl, wl, bl, tl, store)
+            ctx.cfg = h.shape[1], wide, ignore, reduction, sizes[1]
+            _save(ctx, hl, wl, bl, tl, store)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss):
-        h, w, bias, _ = ctx.saved_tensors                # also the check that none of them was written since
-        dev, width, wide = h.device, h.shape[1], ctx.desc.hidden
-        if not d_loss.is_contiguous():
-            d_loss = d_loss.contiguous()
+        width, wide, ignore, reduction, need = ctx.cfg
+        h, w, bias, target, store = _saved('linear_cross_entropy', ctx)
+        dev = h.device
+        h, w, target, store = _rows_for(h, wide), _rows_for(w, wide), target.contiguous(), store.contiguous()
+        bias = None if bias is None else bias.contiguous()
+        d_loss = d_loss.contiguous()
         dh = torch.empty((h.shape[0], wide), dtype=h.dtype, device=dev)
         dw = torch.empty((w.shape[0], wide), dtype=h.dtype, device=dev)
         db = None if bias is None else torch.empty(w.shape[0], dtype=h.dtype, device=dev)
-        d = ctx.desc
+        d = _xent_desc(h, w, bias, target, ignore, reduction, store, None)
         d.d_loss, d.dh, d.dw, d.dbias = d_loss.data_ptr(), dh.data_ptr(), dw.data_ptr(), _ptr(db)
         d.dh_row = d.dw_row = wide
-        ws = _workspace(d, ctx.need, dev)  # noqa: F841
+        ws = _workspace(d, need, dev)  # noqa: F841
         _call('tsg_xent_backward', d, dev)
         if wide != width:
             dh, dw = dh[:, :width].contiguous(), dw[:, :width].contiguous()
