@@ -591,7 +591,10 @@ int tsg_attn_backward(const tsg_attn_desc* d, void* stream);
  * have the type of h and w.  The backward takes d_loss (one number, or one per row for reduction 0) and the stats that
  * the forward left, takes the vocabulary in pieces and writes dh, dw and dbias whole.
  * The gradients of the logits are rounded to the type where they enter a product (f32: h, w and they are two f16 numbers each, 22
- * bits together); all sums, maxima and logarithms are f32.
+ * bits together for what is within 2^-18 of the largest: of h and of w over the tensor, of the logits' gradients over softmax - onehot
+ * = 1, whatever a row's d_loss is; below it the error stays 2^-40 of that largest).  With reduction 0 dW takes h times the
+ * row's share of the largest d_loss, rounded to a power of two: an element 2^-29 of the largest in h and d_loss together has 11 bits.
+ * All sums, maxima and logarithms are f32.
  * Base addresses of h and w are 16-byte aligned, rows a multiple of 16 and less than 2^23 bytes apart, hidden a multiple of 8 (pad with
  * zeros), dh and dw 16-byte aligned with rows a multiple of 4 elements apart, the workspace 256-byte aligned; tsg_xent_workspace says how much.  n_rows >= 1. */
 typedef struct tsg_xent_desc {

@@ -1,0 +1,80 @@
+"""Gradients of the cross entropy where upstream gradients are small, large or of very different size per row, against the 64-bit
+form, judged row by row.
+
+Tolerances as in test_gpu_ops.py: 2 u for the two roundings of 16-bit types (u = eps / 2), 1e-5 for f32, and for f16 results
+half of its fixed step, 2^-25, per element."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_ops import bound_of, entropy_case, plain_cross_entropy, rel
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def rows_within(got, want, dt, factor=1.0):
+    """Every row for itself."""
+    got, want = got.detach().double().cpu(), want.double()
+    assert torch.isfinite(got).all()
+    err, norm = (got - want).norm(dim=1), want.norm(dim=1)
+    fixed = 2.0 ** -25 * math.sqrt(want.shape[1]) if dt == torch.float16 else 0.0
+    over = err - factor * ((1e-5 if dt == torch.float32 else torch.finfo(dt).eps + 2e-6) * norm + fixed)
+    worst = int(over.argmax())
+    assert float(over[worst]) <= 0.0, (worst, float(err[worst]), float(norm[worst]))
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('t,v,k', [(61, 1000, 256), (150, 3001, 100), (2500, 9001, 64)])
+def test_cross_entropy_rows_of_very_different_upstream_gradients(dt, t, v, k):
+    """reduction 'none' with upstream gradients over 12 decades (f16, whose dh has to hold them: 7), in no order, some negative,
+    some zero."""
+    from ts_trajgen_amd import ops
+    h, w, b, target = entropy_case(dt, t, v, k, seed=t)
+    low, high = (-3, 4) if dt == torch.float16 else (-12, 0)
+    g = torch.Generator().manual_seed(t)
+    up = torch.logspace(low, high, t)[torch.randperm(t, generator=g)] * (1 - 2 * (torch.rand(t, generator=g) < 0.3).float())
+    up[::17] = 0.0
+    rows = ops.linear_cross_entropy(h, w, target, bias=b, reduction='none')
+    got = torch.autograd.grad(rows, [h, w, b], up.to(DEV))
+    _, dh, dw, db = plain_cross_entropy(h, w, b, target, -100, up)
+    rows_within(got[0], dh, dt)
+    rows_within(got[1], dw, dt)
+    assert rel(got[2], db) < bound_of(dt, db)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_cross_entropy_one_large_upstream_gradient_over_small_ones(dt):
+    """One row of 1 among rows of 1e-6 whose targets nothing else says anything about: their rows of dW are those rows' alone but
+    for the large row's probabilities."""
+    from ts_trajgen_amd import ops
+    t, v, k = 200, 1500, 64
+    h, w, b, target = entropy_case(dt, t, v, k, seed=3, ignored=0.0)
+    target = torch.arange(t).to(DEV)
+    up = torch.full((t,), 1e-6 if dt != torch.float16 else 1.0)
+    up[7] = 1.0 if dt != torch.float16 else 1e4
+    rows = ops.linear_cross_entropy(h, w, target, bias=b, reduction='none')
+    got = torch.autograd.grad(rows, [h, w, b], up.to(DEV))
+    _, dh, dw, db = plain_cross_entropy(h, w, b, target, -100, up)
+    rows_within(got[0], dh, dt)
+    rows_within(got[1], dw, dt)
+    assert rel(got[2], db) < bound_of(dt, db)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('by', [1e-30, 1e30])
+def test_cross_entropy_tiny_and_huge_upstream_gradients(dt, by):
+    """All of one size, at the ends of f32 (bf16 and f32; f16 results hold neither)."""
+    from ts_trajgen_amd import ops
+    if dt == torch.float16:
+        by = {1e-30: 2.0 ** -8, 1e30: 2.0 ** 14}[by]
+    h, w, b, target = entropy_case(dt, 90, 700, 64, seed=6)
+    up = torch.rand(90, generator=torch.Generator().manual_seed(1)) * by + by
+    rows = ops.linear_cross_entropy(h, w, target, bias=b, reduction='none')
+    got = torch.autograd.grad(rows, [h, w, b], up.to(DEV))
+    _, dh, dw, db = plain_cross_entropy(h, w, b, target, -100, up)
+    rows_within(got[0], dh, dt)
+    rows_within(got[1], dw, dt)
+    assert rel(got[2], db) < bound_of(dt, db)

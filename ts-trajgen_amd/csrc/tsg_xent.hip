@@ -14,8 +14,8 @@
 // x 2^e = hi + lo with e from the tensor's largest magnitude (hi, lo: 22 bits together; an element 2^-18 below the
 // largest still has them all), and a product is three passes, hi hi + hi lo + lo hi, summed in f32: the dropped term is
 // 2^-22 relative, next to f32's own 2^-24 per addition, at a third of the f16 rate (833 TFLOP/s) against 157 of the f32
-// matrix cores.  dz is rounded to the operand type (bf16: 2^-9 relative); it is scaled by 2^15 over the largest |g|
-// first, so that probabilities down to 1e-9 stay above f16's subnormals; for f32 it is hi + lo as well.  Errors of dh and dW
+// matrix cores.  dz is rounded to the operand type (bf16: 2^-9 relative); it is brought to 2^15 for a
+// whole probability first, so that those down to 1e-9 stay above f16's subnormals; for f32 it is hi + lo as well.  Errors of dh and dW
 // against 64 bits, 16-bit types, 100 drawn shapes: at most 1.32 times those of 32-bit sums rounded once (1.47 for a pair of rows).
 // 16384 states x 50021 entries x 1024 wide, bf16 (1.68 TFLOP a product): statistics 1.65 ms (1020 TFLOP/s), dz 2.00 ms (840), dW 1.65 ms (1020),
 // dh 1.24 ms (1355); a large bf16 matrix product of the library: 1129.  8192 x 40307 x 256, f32: 0.61, 0.89, 0.55 and 0.48 ms, the f32 rate of the
@@ -48,16 +48,23 @@ __device__ __forceinline__ float scale_of(unsigned bits) {
   return ldexpf(1.0f, s);
 }
 
-// dz is held as (softmax - onehot) g 2^15 / largest |g|: under 'sum' and 'mean', where all g are alike, the target's entry is then -2^15 but for
-// its own probability, and a constant rounding of g does not go into every row of the gradients (errors up to 2.6 times 32-bit sums rounded
-// once, with a power of two as the scale).  dz_unit: what one of dz stands for.
-__device__ __forceinline__ float dz_scale(unsigned gmax) {
-  const float v = __uint_as_float(gmax);
-  return !(v > 0.0f) ? 1.0f : v < 0x1p-100f ? 0x1p115f : 0x1p15f / v;
-}
-__device__ __forceinline__ float dz_unit(unsigned gmax) {
-  const float v = __uint_as_float(gmax);
-  return !(v > 0.0f) ? 1.0f : v < 0x1p-100f ? 0x1p-115f : v * 0x1p-15f;
+// dz of a row is held as (softmax - onehot) q 2^15 with q in (1/2, 1] and g = q 2^-k largest |g|, k the row's own.  A row whose g is small
+// beside the others' would lose its probabilities below f16's smallest number in units that all rows share (f32, g of 1e-7 of the largest:
+// dh off by 1.4e-3).  k comes back where dh is written; for dW the states are multiplied by 2^-k instead (xent_fold_kernel).  Under 'sum' and
+// 'mean', where all g are alike, q = 1 and k = 0: the target's entry is -2^15 but for its own probability, no constant rounding of g goes into
+// every row of the gradients, and the states are read as they are.
+struct DzUnit {  // what one of dz stands for, m 2^e; apart, so that neither end of f32 is passed on the way
+  float m;
+  int e;
+  __device__ __forceinline__ float of(float sum, int k = 0) const { return ldexpf(sum * m, e - k); }
+};
+// other: what the second operand of the sum was multiplied by, or null
+__device__ __forceinline__ DzUnit dz_unit(unsigned gmax, const float* other = nullptr) {
+  DzUnit u = {1.0f, 0};
+  if (gmax) u.m = frexpf(__uint_as_float(gmax), &u.e);
+  u.e -= 15;
+  if (other) u.m /= *other;
+  return u;
 }
 // what a magnitude says to a common scale: one that is not finite spoils its own row, not the others' precision
 __device__ __forceinline__ float weight_of(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.0f; }
@@ -76,7 +83,11 @@ struct XentArgs {
   float2* part;                 // forward: [vocab tiles][rows]
   float* zt;                    // forward: [rows] the target's logit
   float2* stat;                 // [rows] maximum, log2 of the sum
-  float* g;                     // backward: [rows] gradient of the row's loss, 0 for rows left out
+  float* g;                     // backward: [rows] q 2^15 with the sign of g, 0 for rows left out
+  int* shift;                   // backward: [rows] k
+  const char* hd;               // the states as dW reads them: h, or h 2^-k times *hd_by
+  long hd_row, hd_plane;
+  const float* hd_by;           // or null: 1
   unsigned long long* used;     // backward: bit t % 64 of word t / 64: g_t != 0
   char* dz;                     // [rows][ldz] 16-bit; f32: lo plane dz_plane further on
   long ldz, dz_plane;           // elements, bytes
@@ -306,7 +317,7 @@ __global__ __launch_bounds__(1024) void xent_reduce_kernel(XentArgs a, const flo
   if (out) *out = (float)(mean ? sum / (double)n : sum);
 }
 
-// g_t and the largest |g_t|, one workgroup.  reduction 0: d_loss per row; 1: one gradient for the sum; 2: for the mean
+// q_t, k_t and the largest |g_t|, one workgroup.  reduction 0: d_loss per row; 1: one gradient for the sum; 2: for the mean
 __global__ __launch_bounds__(1024) void xent_grad_kernel(XentArgs a, const float* d_loss, int reduction) {
   __shared__ float top[16];
   __shared__ int c[16];
@@ -332,9 +343,23 @@ __global__ __launch_bounds__(1024) void xent_grad_kernel(XentArgs a, const float
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x) return;
-  for (int w = 1; w < 16; ++w) m = fmaxf(m, top[w]);
-  *a.gmax = __float_as_uint(m);
+  for (int w = 0; w < 16; ++w) m = fmaxf(m, top[w]);
+  if (threadIdx.x == 0) *a.gmax = __float_as_uint(m);
+  int em;
+  const float mm = frexpf(m, &em);
+  for (int t = threadIdx.x; t < a.rows; t += 1024) {  // its own rows again
+    const float g = a.g[t];
+    float q = g;
+    int k = 0;
+    if (g != 0.0f && fabsf(g) < INFINITY) {
+      int e;
+      q = frexpf(g, &e) / mm;
+      if (fabsf(q) > 1.0f) q *= 0.5f, ++e;
+      k = em - e;
+    }
+    a.g[t] = q * 0x1p15f;
+    a.shift[t] = k;
+  }
 }
 
 template <typename D, typename T, bool SPLIT>
@@ -348,13 +373,12 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dz_kernel(XentArgs a, i
   Acc<T> z;
   logits<D, T, SPLIT>(a, z, lds, m0, tn * T::TN, wave, lane);
   const int wm = wave / T::WN * 32 * T::XM, wn = wave % T::WN * 32 * T::XN;
-  const float gs = dz_scale(*a.gmax);
 #pragma unroll
   for (int y = 0; y < T::XN; ++y) {
     const int n = wn + 32 * y + (lane & 31), t = tn * T::TN + n;
     const bool in = t < a.rows;
     const float2 st = in ? a.stat[t] : make_float2(0.0f, INFINITY);
-    const float g = in ? a.g[t] * gs : 0.0f;
+    const float g = in ? a.g[t] : 0.0f;
     const long target = in ? a.target[t] : -1;
     const int at = target >= 0 && target < a.vocab ? (int)target - (m0 + wm + 4 * h) : -1;
 #pragma unroll
@@ -367,6 +391,12 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dz_kernel(XentArgs a, i
       }
   }
   if (a.db_part) {
+    float of_row[T::XN];  // 2^-k
+#pragma unroll
+    for (int y = 0; y < T::XN; ++y) {
+      const int t = tn * T::TN + wn + 32 * y + (lane & 31);
+      of_row[y] = t < a.rows ? ldexpf(1.0f, -a.shift[t]) : 0.0f;
+    }
     // sums over the states: 16 registers x 32 lanes, halving the registers with four bits of the lane
     float* join = reinterpret_cast<float*>(lds);  // [WN][TM]
 #pragma unroll
@@ -374,9 +404,9 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dz_kernel(XentArgs a, i
       float sums[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        sums[i] = z[x][0][i];
+        sums[i] = z[x][0][i] * of_row[0];
 #pragma unroll
-        for (int y = 1; y < T::XN; ++y) sums[i] += z[x][y][i];
+        for (int y = 1; y < T::XN; ++y) sums[i] = __builtin_fmaf(z[x][y][i], of_row[y], sums[i]);
       }
 #pragma unroll
       for (int n = 8; n > 0; n >>= 1) {
@@ -443,10 +473,9 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dw_kernel(XentArgs a, i
   Acc<T> acc;
   zero_acc<T>(acc);
   const Operand A = {a.dz + (t0 * a.ldz + tm * T::TM) * 2, a.ldz * 2, a.dz_plane, len, (int)a.ldz - tm * T::TM, nullptr};
-  const Operand B = {a.h + t0 * a.h_row + (long)tn * T::TN * 2, a.h_row, a.h_plane, len, a.hidden - tn * T::TN, a.used + t0 / 64};
+  const Operand B = {a.hd + t0 * a.hd_row + (long)tn * T::TN * 2, a.hd_row, a.hd_plane, len, a.hidden - tn * T::TN, a.used + t0 / 64};
   if (len > 0) product<D, T, true, true, true>(acc, lds, A, B, len, SPLIT ? 3 : 1, wave, lane);
-  float by = dz_unit(*a.gmax);
-  if (SPLIT) by /= a.scales[0];
+  const DzUnit unit = dz_unit(*a.gmax, a.hd_by);
   const int wm = wave / T::WN * 32 * T::XM, wn = wave % T::WN * 32 * T::XN;
 #pragma unroll
   for (int x = 0; x < T::XM; ++x)
@@ -457,7 +486,7 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dw_kernel(XentArgs a, i
         const int m = tm * T::TM + wm + 32 * x + (i & 3) + 8 * (i >> 2) + 4 * h, k = tn * T::TN + wn + 32 * y + (lane & 31);
         if (m < a.vc && k < a.hidden) {
           if (a.dw_part) a.dw_part[((long)split_id * a.vc + m) * a.hidden + k] = acc[x][y][i];
-          else reinterpret_cast<OUT*>(a.dw + (long)(a.v0 + m) * a.dw_row)[k] = (OUT)(acc[x][y][i] * by);
+          else reinterpret_cast<OUT*>(a.dw + (long)(a.v0 + m) * a.dw_row)[k] = (OUT)unit.of(acc[x][y][i]);
         }
       }
 }
@@ -495,11 +524,11 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void xent_dh_kernel(XentArgs a, i
       }
 }
 
-// A gradient from its stretches' sums: [splits][n / hidden][hidden] f32 -> rows of OUT, by dz_unit and 1 / *other.
+// A gradient from its stretches' sums: [splits][n / hidden][hidden] f32 -> rows of OUT, in units of dz and, per row, of 2^-shift.
 // Four elements per thread; PARTS of the workgroup's waves share the stretches (1 or 4).
 template <typename OUT, int PARTS>
 __global__ __launch_bounds__(256) void xent_join_grad_kernel(const float* from, int splits, long n, int hidden, OUT* out, long out_row, const unsigned* gmax,
-                                                             const float* other) {
+                                                             const float* other, const int* shift) {
   constexpr int WIDE = 256 / PARTS;
   __shared__ float4 join[PARTS][WIDE];
   const int part = threadIdx.x / WIDE, lane = threadIdx.x % WIDE;
@@ -522,10 +551,10 @@ __global__ __launch_bounds__(256) void xent_join_grad_kernel(const float* from, 
     }
   }
   if (i >= n) return;
-  float by = dz_unit(*gmax);
-  if (__is_same(OUT, float)) by /= *other;
+  const DzUnit unit = dz_unit(*gmax, other);
+  const int k = shift ? shift[i / hidden] : 0;
   OUT* to = out + (i / hidden) * out_row + i % hidden;
-  OUT v[4] = {(OUT)(s.x * by), (OUT)(s.y * by), (OUT)(s.z * by), (OUT)(s.w * by)};
+  OUT v[4] = {(OUT)unit.of(s.x, k), (OUT)unit.of(s.y, k), (OUT)unit.of(s.z, k), (OUT)unit.of(s.w, k)};
   if (sizeof(OUT) == 4) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(v);
   else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(v);
 }
@@ -541,7 +570,7 @@ template <typename OUT> __global__ __launch_bounds__(256) void xent_db_out_kerne
   __syncthreads();
   if (part || v >= a.vc) return;
   s = (join[0][lane] + join[1][lane]) + (join[2][lane] + join[3][lane]);
-  db[a.v0 + v] = (OUT)(s * dz_unit(*a.gmax));
+  db[a.v0 + v] = (OUT)dz_unit(*a.gmax).of(s);
 }
 
 // ---- f32 operands: largest magnitudes, then the two planes
@@ -614,10 +643,83 @@ __global__ __launch_bounds__(256) void xent_planes_kernel(Planes a) {
   }
 }
 
+// ---- the states times 2^-k of their rows, for dW where upstream gradients differ: a power of two and exact, until it reaches the type's
+// smallest numbers.  f16 and f32's planes begin at 2^15 for the largest state, so an element 2^-29 of the largest in state and gradient
+// together still has 11 bits; bf16 reaches further by itself.
+struct Fold {
+  const char* h;
+  long row;             // bytes
+  int rows, chunks;     // of 8 elements
+  const float* g;       // rows that are left out (0) may hold anything: they have no say
+  const int* shift;
+  float* amax;          // [blocks], f16 only
+  const float* scale;   // f32 only: what the forward multiplied its planes by
+  float* by;            // f16 only, out: what the states were multiplied by
+  char* out;
+  long plane;           // f32 only
+};
+template <typename D> __device__ __forceinline__ void fold_load(const Fold& a, long i, float (&v)[8]) {
+  typedef typename D::type T;
+  const T* x = reinterpret_cast<const T*>(a.h + (i / a.chunks) * a.row) + (i % a.chunks) * 8;
+  T e[8];
+#pragma unroll
+  for (int b = 0; b < (int)sizeof(T) * 8; b += 16) *reinterpret_cast<uint4*>(reinterpret_cast<char*>(e) + b) = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(x) + b);
+#pragma unroll
+  for (int n = 0; n < 8; ++n) v[n] = (float)e[n];
+}
+__global__ __launch_bounds__(256) void xent_fold_max_kernel(Fold a) {
+  __shared__ float join[4];
+  float m = 0.0f;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < (long)a.rows * a.chunks; i += (long)gridDim.x * 256) {
+    if (a.g[i / a.chunks] == 0.0f) continue;
+    float v[8];
+    fold_load<TsgF16>(a, i, v);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) m = fmaxf(m, weight_of(v[n]));
+  }
+  m = tsg_wave_max(m);
+  if ((threadIdx.x & 63) == 0) join[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) a.amax[blockIdx.x] = fmaxf(fmaxf(join[0], join[1]), fmaxf(join[2], join[3]));
+}
+template <typename D> __global__ __launch_bounds__(256) void xent_fold_kernel(Fold a) {
+  constexpr bool SPLIT = __is_same(D, TsgF32);
+  typedef typename D::type T;
+  float by = SPLIT ? *a.scale : 1.0f;
+  if constexpr (__is_same(D, TsgF16)) {
+    __shared__ float join[4];
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) m = fmaxf(m, a.amax[i]);
+    m = tsg_wave_max(m);
+    if ((threadIdx.x & 63) == 0) join[threadIdx.x >> 6] = m;
+    __syncthreads();
+    by = scale_of(__float_as_uint(fmaxf(fmaxf(join[0], join[1]), fmaxf(join[2], join[3]))));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.by = by;
+  }
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < (long)a.rows * a.chunks; i += (long)gridDim.x * 256) {
+    float v[8];
+    fold_load<D>(a, i, v);
+    const int k = a.shift[i / a.chunks];
+    tsg_u4 hi, lo;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) v[n] = ldexpf(v[n] * by, -k);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      if constexpr (SPLIT) {
+        hi[n] = tsg_pack2<TsgF16>(v[2 * n], v[2 * n + 1]);
+        lo[n] = tsg_pack2<TsgF16>(v[2 * n] - (float)(_Float16)v[2 * n], v[2 * n + 1] - (float)(_Float16)v[2 * n + 1]);
+      } else {
+        hi[n] = tsg_pack2<D>(v[2 * n], v[2 * n + 1]);
+      }
+    }
+    *reinterpret_cast<tsg_u4*>(a.out + i * 16) = hi;
+    if constexpr (SPLIT) *reinterpret_cast<tsg_u4*>(a.out + a.plane + i * 16) = lo;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------ host side
 struct Layout {
-  size_t gmax, amax, planes, h_plane, w_plane, part, zt, g, used, dz, dz_plane, db, dh, total;
-  size_t dw;
+  size_t gmax, amax, planes, h_plane, w_plane, part, zt, g, shift, used, fold, fold_amax, fold_by, dz, dz_plane, db, dh, dw, total;
   int vc, splits, split_len, dh_shape, dw_shape, dw_splits, dw_len;
 };
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -666,7 +768,13 @@ Layout layout_of(const tsg_xent_desc* d, bool backward) {
     l.dz_plane = f32 ? up256(T * vc * 2) : 0;
     l.dz = take(f32 ? 2 * l.dz_plane : T * vc * 2);
     l.g = take(T * 4);
+    l.shift = take(T * 4);
     l.used = take((T + 63) / 64 * 8);
+    if (d->reduction == 0) {
+      l.fold = take(f32 ? 2 * l.h_plane : T * K * 2);
+      l.fold_amax = take(PLANE_BLOCKS * 4);
+      l.fold_by = take(4);
+    }
     l.db = d->bias ? take((size_t)tsg_cdiv(T, 64) * vc * 4) : 0;
     // dh has few tiles and a long sum: cut it until the chip is full, in stretches of 128 entries at least
     l.dh_shape = T >= 2048 ? BIG : T > 64 ? MID : FEW;
@@ -756,6 +864,27 @@ void make_planes(const tsg_xent_desc* d, const XentArgs& a, const Layout& l, boo
   hipLaunchKernelGGL(xent_planes_kernel, grid, dim3(256), 0, s, p);
 }
 
+// upstream gradients per row differ: dW's states carry 2^-k
+void make_fold(const tsg_xent_desc* d, XentArgs& a, const Layout& l, hipStream_t s) {
+  char* ws = (char*)d->workspace;
+  Fold f = {};
+  f.h = (const char*)d->h, f.row = d->h_row * (d->dtype == TSG_F32 ? 4 : 2), f.rows = a.rows, f.chunks = d->hidden / 8;
+  f.g = a.g, f.shift = a.shift, f.amax = (float*)(ws + l.fold_amax), f.scale = d->scales, f.by = (float*)(ws + l.fold_by);
+  f.out = ws + l.fold, f.plane = (long)l.h_plane;
+  const int64_t want = ((int64_t)f.rows * f.chunks + 255) / 256;
+  const dim3 grid((unsigned)(want > PLANE_BLOCKS ? PLANE_BLOCKS : want)), block(256);
+  a.hd = f.out, a.hd_row = d->hidden * 2L, a.hd_plane = d->dtype == TSG_F32 ? f.plane : 0;
+  if (d->dtype == TSG_F32) {
+    hipLaunchKernelGGL(xent_fold_kernel<TsgF32>, grid, block, 0, s, f);
+  } else if (d->dtype == TSG_BF16) {
+    hipLaunchKernelGGL(xent_fold_kernel<TsgBf16>, grid, block, 0, s, f);
+  } else {
+    hipLaunchKernelGGL(xent_fold_max_kernel, grid, block, 0, s, f);
+    hipLaunchKernelGGL(xent_fold_kernel<TsgF16>, grid, block, 0, s, f);
+    a.hd_by = f.by;
+  }
+}
+
 // f(Tile<...>) for the shape
 template <typename F> void with_tile(int shape, F f) {
   if (shape == BIG) f(Big());
@@ -794,14 +923,14 @@ template <typename D, typename OUT> void backward_piece(XentArgs a, const tsg_xe
     hipLaunchKernelGGL((xent_dh_kernel<D, T, SPLIT>), dim3((unsigned)(tr * tk * l.splits)), dim3(64 * T::WAVES), 0, s, a, tr, tk);
   });
   if (d->bias) hipLaunchKernelGGL(xent_db_out_kernel<OUT>, dim3(tsg_cdiv(a.vc, 64)), dim3(256), 0, s, a, (OUT*)d->dbias, tt);
-  auto join = [&](const float* from, int splits, long n, OUT* out, long out_row, const float* other) {
+  auto join = [&](const float* from, int splits, long n, OUT* out, long out_row, const float* other, const int* shift) {
     if (splits >= 16)
-      hipLaunchKernelGGL((xent_join_grad_kernel<OUT, 4>), dim3((unsigned)((n / 4 + 63) / 64)), dim3(256), 0, s, from, splits, n, a.hidden, out, out_row, a.gmax, other);
+      hipLaunchKernelGGL((xent_join_grad_kernel<OUT, 4>), dim3((unsigned)((n / 4 + 63) / 64)), dim3(256), 0, s, from, splits, n, a.hidden, out, out_row, a.gmax, other, shift);
     else
-      hipLaunchKernelGGL((xent_join_grad_kernel<OUT, 1>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, from, splits, n, a.hidden, out, out_row, a.gmax, other);
+      hipLaunchKernelGGL((xent_join_grad_kernel<OUT, 1>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, from, splits, n, a.hidden, out, out_row, a.gmax, other, shift);
   };
-  if (a.dw_part) join(a.dw_part, l.dw_splits, (long)a.vc * a.hidden, (OUT*)d->dw + (long)a.v0 * d->dw_row, d->dw_row, a.scales);
-  if (a.v0 + a.vc >= a.vocab) join(a.dh_part, l.splits, (long)a.rows * a.hidden, (OUT*)d->dh, d->dh_row, SPLIT ? a.scales + 1 : nullptr);
+  if (a.dw_part) join(a.dw_part, l.dw_splits, (long)a.vc * a.hidden, (OUT*)d->dw + (long)a.v0 * d->dw_row, d->dw_row, a.hd_by, nullptr);
+  if (a.v0 + a.vc >= a.vocab) join(a.dh_part, l.splits, (long)a.rows * a.hidden, (OUT*)d->dh, d->dh_row, SPLIT ? a.scales + 1 : nullptr, a.shift);
 }
 
 }  // namespace
@@ -843,7 +972,9 @@ extern "C" int tsg_xent_backward(const tsg_xent_desc* d, void* stream) {
   char* ws = (char*)d->workspace;
   XentArgs a = args_of(d, l);
   a.g = (float*)(ws + l.g);
+  a.shift = (int*)(ws + l.shift);
   a.used = (unsigned long long*)(ws + l.used);
+  a.hd = a.h, a.hd_row = a.h_row, a.hd_plane = a.h_plane, a.hd_by = d->dtype == TSG_F32 ? d->scales : nullptr;
   a.dz = ws + l.dz, a.dz_plane = (long)l.dz_plane;
   a.db_part = d->bias ? (float*)(ws + l.db) : nullptr;
   a.dh_part = (float*)(ws + l.dh);
@@ -854,6 +985,7 @@ extern "C" int tsg_xent_backward(const tsg_xent_desc* d, void* stream) {
   a.ldz = l.vc;
   if (d->dtype == TSG_F32) make_planes(d, a, l, true, s);
   hipLaunchKernelGGL(xent_grad_kernel, dim3(1), dim3(1024), 0, s, a, d->d_loss, d->reduction);
+  if (d->reduction == 0) make_fold(d, a, l, s);
   for (int64_t v0 = 0; v0 < d->n_vocab; v0 += l.vc) {
     a.v0 = (int)v0;
     a.vc = (int)(d->n_vocab - v0 < l.vc ? d->n_vocab - v0 : l.vc);
