@@ -556,7 +556,8 @@ int tsg_gat_train_backward_rng(const tsg_gat_train* d, const tsg_gat_dropout* r,
  * stats [heads][n_q][2] f32 is written by the forward (a row's largest q.k, and the base-2 logarithm of the sum of
  * exp(scale (q.k - largest)); 0 and +inf where a row sees nothing) and read, with out, by the backward, which writes
  * delta [heads][n_q].
- * 16-bit types: p and the gradients of the scores are rounded to the type where they enter a product, all sums are f32.  Elements
+ * 16-bit types: p and the gradients of the scores are rounded to the type where they enter a product, all sums are f32.  (f16:
+ * carried by powers of two per row or key, so that small or large d_out and v leave them their 11 bits.)  Elements
  * that are not finite reach the rows that see them and no others (where one is infinite, a sum over it may be NaN).
  * workspace: what tsg_attn_workspace says, 16-byte aligned, for the forward with few rows over many keys and for the
  * backward of few long sequences; 0 bytes = none needed. */
