@@ -122,3 +122,20 @@ def test_encoder_entries_with_a_generator_refuse_before_any_launch():
             d = _lib.GatTrain()
             setattr(d, mask, 4096)
             assert entry(C.byref(d), C.byref(ok), None) < 0
+
+
+def test_live_dropouts_of_function_g_need_a_step():
+    """The same step draws the same masks, so a caller who gives none would train on one mask for ever."""
+    from ts_trajgen_amd.generator.function_g_fc import FunctionGFC
+    conf = {'road_emb_size': 8, 'time_emb_size': 8, 'hidden_size': 16, 'lstm_layer_num': 1, 'dropout_p': 0.5, 'dis_weight': 0.5}
+    m = FunctionGFC(conf, {'road_num': 20, 'road_pad': 19, 'time_size': 20, 'time_pad': 19}).train(True)
+    loc, ptr = torch.zeros(4, dtype=torch.int64), torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(ValueError, match='step'):
+        m.trajectory_loss(loc, loc, ptr)
+    with pytest.raises(RuntimeError, match='HIP device'):       # the parameters are not on a device: the next check
+        m.trajectory_loss(loc, loc, ptr, step=0)
+    with pytest.raises(RuntimeError, match='HIP device'):
+        m.train(False).trajectory_loss(loc, loc, ptr)
+    m.dropout_p = 0.0
+    with pytest.raises(RuntimeError, match='HIP device'):
+        m.train(True).trajectory_loss(loc, loc, ptr)

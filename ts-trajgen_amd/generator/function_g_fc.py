@@ -70,16 +70,20 @@ class FunctionGFC(nn.Module):
         """softmax of forward() over the candidates (function_g_fc.py:189-204)."""
         return self.predict_g(trace_loc, trace_time, des, candidate_set, candidate_dis, trace_mask)
 
-    def trajectory_loss(self, trace_loc, trace_time, seq_ptr, target=None, reduction='mean', seed=0, step=0):
+    def trajectory_loss(self, trace_loc, trace_time, seq_ptr, target=None, reduction='mean', seed=0, step=None):
         """Cross entropy of the next road at every position of packed trajectories, over all roads (the score of
         function_g_fc.py:155-184 before its gather, at every prefix at once).
 
         trace_loc and trace_time hold the trajectories one behind the other ([n] integers), seq_ptr ([n_seq + 1] int32)
         their starts.  target ([n] int64, -100 = not counted) defaults to the next road of the same trajectory; positions of
         no trajectory never count.  In training mode the dropouts of function_g_fc.py:160,182 are live, drawn from the
-        counter (seed, site 0 and 1, step): give every training step its own step.  hidden_size is at most 512
-        (ops.causal_attention).  In inference mode torch's recurrence has no backward.  The call waits for the
+        counter (seed, site 0 and 1, step): every training step needs a step of its own, and a call without one is refused.
+        hidden_size is at most 512 (ops.causal_attention).  In inference mode torch's recurrence has no backward.  The call waits for the
         device once: it looks at the lengths and ids."""
+        drop = self.dropout_p if self.training else 0.0
+        if drop and step is None:
+            raise ValueError('trajectory_loss: the dropouts are live, give every training step a step of its own (the same step '
+                             'drops the same elements)')
         dev = self.out_fc.weight.device
         if dev.type != 'cuda':
             raise RuntimeError('FunctionGFC.trajectory_loss needs its parameters on a HIP device (no CPU fallback)')
@@ -106,7 +110,6 @@ class FunctionGFC(nn.Module):
         if target is None:
             target = torch.where(pos == lens[seq] - 1, torch.full_like(loc, -100), torch.roll(loc, -1))
         target = torch.where(inside, target.to(dev), torch.full_like(loc, -100))
-        drop = self.dropout_p if self.training else 0.0
         x = torch.cat([self.road_emb(loc), self.time_emb(tim)], dim=1)
         if drop:
             x = ops.dropout(x, drop, seed, site=0, step=step)
