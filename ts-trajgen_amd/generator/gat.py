@@ -253,8 +253,11 @@ class GATLayerImp3(nn.Module):
         cfg.update({'m_in': None, 'm_proj': None, 'm_att': None} if rng is not None else
                    {'m_in': m_in.reshape(n, fin), 'm_proj': m_proj.reshape(n, nh * fo),
                     'm_att': m_att.reshape(e, nh)[order].contiguous()})
-        out = _GATTrainFn.apply(x, self.linear_proj.weight, self.skip_proj.weight, self.scoring_fn_source,
-                                self.scoring_fn_target, self.bias, cfg)
+        args = (x, self.linear_proj.weight, self.skip_proj.weight, self.scoring_fn_source, self.scoring_fn_target, self.bias)
+        if rng is not None:
+            from ..ops import _inputs
+            args = _inputs(*args)
+        out = _GATTrainFn.apply(*args, cfg)
         return out, edge_index
 
     def forward(self, data):

@@ -6,7 +6,8 @@
 
 They take tensors on a HIP device (f32, bf16 or f16), run on torch's current stream of that device, allocate their results and
 workspaces through torch's allocator and never synchronise, so they can be captured in a graph (forward and backward
-together; drop eager results that still hold an autograd graph of the same leaves first, which is checked).  Wrong shapes, types or
+together; drop eager results that still hold an autograd graph of the same leaves first, which is checked for leaves that these
+operators took themselves; or a forward under no_grad).  Wrong shapes, types or
 devices raise ValueError / TypeError / RuntimeError before anything is launched; there is no CPU fallback.  Gradients are
 first order: differentiating a gradient raises.
 """
@@ -97,6 +98,13 @@ def _enter(ctx, *inputs):
         _LIVE.add(ctx)
 
 
+def _inputs(*tensors):
+    """As an operator's node takes them: under no_grad no backward follows, and a node has nothing to note or keep for one."""
+    if torch.is_grad_enabled():
+        return tensors
+    return [t.detach() if t is not None and t.requires_grad else t for t in tensors]
+
+
 def _save(ctx, *tensors):
     """Everything a backward reads goes through autograd's saved tensors: hooks may move it or bring it back from elsewhere (then
     the operands may be written meanwhile), and a backward that does not keep its graph lets go of it."""
@@ -170,7 +178,7 @@ def dropout(x, p, seed, site=0, step=0):
     p, seed, site = float(p), int(seed), int(site)
     step = step if torch.is_tensor(step) else int(step)
     check_rng('dropout', p, seed, site, step, dev)
-    return _Dropout.apply(x, p, seed, site, step)
+    return _Dropout.apply(*_inputs(x), p, seed, site, step)
 
 
 # -------------------------------------------------------------------------------------------------------- attention
@@ -296,7 +304,7 @@ def causal_attention(q, k, v, seq_ptr, kv_ptr=None, scale=None):
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError('causal_attention: scale is positive, got %r' % scale)
-    return _CausalAttention.apply(q, k, v, seq_ptr, kv_ptr, scale)
+    return _CausalAttention.apply(*_inputs(q, k, v), seq_ptr, kv_ptr, scale)
 
 
 # ---------------------------------------------------------------------------------------------------- cross entropy
@@ -385,4 +393,4 @@ def linear_cross_entropy(h, weight, target, bias=None, ignore_index=-100, reduct
         raise ValueError('linear_cross_entropy: target is int64 [rows], got %s %s' % (target.dtype, tuple(target.shape)))
     if reduction not in REDUCTIONS:
         raise ValueError("linear_cross_entropy: reduction is 'none', 'sum' or 'mean', got %r" % (reduction,))
-    return _LinearCrossEntropy.apply(h, weight, bias, target, int(ignore_index), REDUCTIONS[reduction])
+    return _LinearCrossEntropy.apply(*_inputs(h, weight, bias), target, int(ignore_index), REDUCTIONS[reduction])
