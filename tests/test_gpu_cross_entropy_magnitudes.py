@@ -78,3 +78,29 @@ def test_cross_entropy_tiny_and_huge_upstream_gradients(dt, by):
     rows_within(got[0], dh, dt)
     rows_within(got[1], dw, dt)
     assert rel(got[2], db) < bound_of(dt, db)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_cross_entropy_rows_of_different_upstream_gradients_over_several_pieces(dt):
+    """30000 rows x 8001 entries: two pieces of the vocabulary in 16 bits, three in f32."""
+    from ts_trajgen_amd import ops
+    t, v, k = 30000, 8001, 16
+    g = torch.Generator(device=DEV).manual_seed(1)
+    h = torch.randn(t, k, generator=g, device=DEV).to(dt).requires_grad_(True)
+    w = (torch.randn(v, k, generator=g, device=DEV) * 0.3).to(dt).requires_grad_(True)
+    b = (torch.randn(v, generator=g, device=DEV) * 0.3).to(dt).requires_grad_(True)
+    target = torch.randint(0, v, (t,), generator=g, device=DEV)
+    low, high = (-3, 3) if dt == torch.float16 else (-12, 0)
+    up = torch.logspace(low, high, t, device=DEV)[torch.randperm(t, generator=g, device=DEV)]
+    rows = ops.linear_cross_entropy(h, w, target, bias=b, reduction='none')
+    got = torch.autograd.grad(rows, [h, w, b], up)
+    with torch.no_grad():
+        dz = torch.log_softmax(h.double() @ w.double().t() + b.double(), dim=1)
+        assert rel(rows, -dz.gather(1, target.unsqueeze(1)).squeeze(1)) < 1e-5
+        dz.exp_()
+        dz[torch.arange(t, device=DEV), target] -= 1.0
+        dz *= up.double().unsqueeze(1)
+        dh, dw, db = (x.cpu() for x in (dz @ w.double(), dz.t() @ h.double(), dz.sum(0)))
+    rows_within(got[0], dh, dt)
+    rows_within(got[1], dw, dt)
+    assert rel(got[2], db) < bound_of(dt, db)

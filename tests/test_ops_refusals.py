@@ -139,3 +139,18 @@ def test_live_dropouts_of_function_g_need_a_step():
     m.dropout_p = 0.0
     with pytest.raises(RuntimeError, match='HIP device'):
         m.train(True).trajectory_loss(loc, loc, ptr)
+
+
+@pytest.mark.parametrize('dtype,rows,vocab,hidden', [(0, 8192, 40307, 256), (1, 16384, 50021, 1024), (2, 16384, 50021, 512), (1, 65536, 131072, 512)])
+@pytest.mark.parametrize('reduction', [0, 2])
+def test_cross_entropy_workspace_is_a_fraction_of_the_logits(dtype, rows, vocab, hidden, reduction):
+    """The logits' gradient exists for a piece of the vocabulary at a time: 384 MiB, next to what grows with h and W alone
+    (f32: their two planes; dh in f32; with reduction 0 h once more; dW in f32 where its rows are cut, of one piece)."""
+    d = _lib.XentDesc()
+    d.dtype, d.hidden, d.reduction, d.n_rows, d.n_vocab = dtype, hidden, reduction, rows, vocab
+    fwd, bwd = C.c_size_t(), C.c_size_t()
+    assert _lib.lib().tsg_xent_workspace(C.byref(d), C.byref(fwd), C.byref(bwd)) == 0
+    each = 4 if dtype == 0 else 2
+    logits = rows * vocab * each
+    assert bwd.value < 0.5 * logits and fwd.value < 0.1 * logits
+    assert bwd.value < (384 << 20) + 4 * hidden * (8 * vocab + 12 * rows)

@@ -1,9 +1,9 @@
 // Softmax cross entropy over a large vocabulary from the states themselves: z_tv = h_t . w_v + b_v, loss_t = log sum_v
 // exp(z_tv) - z_t,target, without the [rows][vocabulary] logits ever being kept.
 //
-// forward   products of 128 vocabulary rows x 128 states; their epilogue leaves (maximum, sum of exp) per state and
-//           128 vocabulary rows, and the target's logit; a small kernel joins them.
-// backward  the vocabulary is taken in pieces.  Per piece the products are computed once more, their epilogue turns them into
+// forward   products in tiles of 256, 128 or 64 vocabulary rows by as many states (shape_of); their epilogue leaves (maximum, sum of
+//           exp) per state and tile, and the target's logit; a small kernel joins them.
+// backward  the vocabulary is taken in pieces (DZ_BUDGET).  Per piece the products are computed once more, their epilogue turns them into
 //           dz_tv = g_t (softmax_tv - [v == target_t]) in 16 bits, and two further products read that:
 //           dW = dz^T h (whole for the piece) and dh += dz W (summed over the pieces in f32).  db comes from dz before
 //           its rounding.  8 T V K operations instead of the 6 of a form that keeps the logits.
@@ -724,8 +724,6 @@ struct Layout {
 };
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// dz of a piece takes at most `budget` bytes (but 128 vocabulary rows at least): large pieces fill the chip, small ones keep
-// the workspace small.
 // The largest tile that still gives every CU a workgroup (256 x 256 fill one, of 128 x 128 two fit), else the next
 enum Shape { FEW, MID, BIG };
 Shape shape_of(int64_t m, int64_t n, int64_t times = 1) {
@@ -734,7 +732,11 @@ Shape shape_of(int64_t m, int64_t n, int64_t times = 1) {
   return FEW;
 }
 constexpr int PLANE_BLOCKS = 512;
-constexpr size_t DZ_BUDGET = (size_t)2 << 30;
+// dz of a piece takes at most this much (but 256 vocabulary rows at least): large pieces fill the chip, small ones keep the memory of a call
+// far below the logits'.  Forward and backward, with the gradients, of 8192 x 40307 x 256, f32 (logits 1.32 GB) and 16384 x 50021 x 1024, bf16
+// (1.64 GB): 128 MiB 5.56 and 7.48 ms, 304 and 405 MB; 256 MiB 2.93 and 6.99 ms, 499 and 498 MB; 384 MiB 2.83 and 6.99 ms, 571 and 665 MB;
+// all in one piece 2.70 and 6.95 ms, 1634 and 1844 MB.
+constexpr size_t DZ_BUDGET = (size_t)384 << 20;
 
 Layout layout_of(const tsg_xent_desc* d, bool backward) {
   Layout l = {};
