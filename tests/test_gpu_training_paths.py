@@ -208,3 +208,21 @@ def test_function_g_of_other_widths(hidden):
     for (k, w), r in zip(m.named_parameters(), ref.parameters()):
         if r.grad is not None:
             assert float((w.grad.double().cpu() - r.grad).norm() / r.grad.norm()) <= 2e-5, k
+
+
+@pytest.mark.parametrize('auto', [torch.float16, torch.bfloat16])
+def test_function_g_under_autocast(auto):
+    """The recurrence then runs in 16 bits, and out_fc goes with it as torch's own linear would.  Logits are 64 products of states below 1
+    and weights below 1/8: three roundings of 2^-11 on each are 64 / 8 * 3 * 2^-11 = 0.012, and states off by 8 * 2^-11 (four
+    roundings a step, halved by every forget gate) 64 / 8 * 2^-8 = 0.03; a loss is the difference of two: 0.1 (the recurrence is
+    f16 under both)."""
+    loc, tim, ptr = trajectories([12, 40, 2])
+    m = function_g().to(DEV).train(True)
+    want = m.trajectory_loss(loc, tim, ptr).detach()
+    with torch.autocast('cuda', auto):
+        got = m.trajectory_loss(loc, tim, ptr)
+    assert got.dtype == torch.float32 and abs(float(got.detach()) - float(want)) <= 0.1
+    got.backward()
+    for k, w in m.named_parameters():
+        if not k.startswith('intra_attn'):
+            assert w.grad.dtype == torch.float32 and torch.isfinite(w.grad).all() and float(w.grad.abs().max()) > 0.0

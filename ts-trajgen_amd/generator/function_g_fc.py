@@ -120,4 +120,5 @@ class FunctionGFC(nn.Module):
         a = ops.causal_attention(q, q, q, ptr, scale=1.0).squeeze(1)
         if drop:
             a = ops.dropout(a, drop, seed, site=1, step=step)
-        return ops.linear_cross_entropy(a, self.out_fc.weight, target, bias=self.out_fc.bias, reduction=reduction)
+        # one type: under autocast the recurrence's, as a linear layer would have it
+        return ops.linear_cross_entropy(a, self.out_fc.weight.to(a.dtype), target, bias=self.out_fc.bias.to(a.dtype), reduction=reduction)
