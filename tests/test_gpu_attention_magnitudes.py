@@ -65,3 +65,13 @@ def test_attention_f16_gradients_of_large_values():
         got, want, _, _ = attention_grads(torch.float16, [2300], 2, 1, 64, [by], seed=5, v_by=v_by)
         for what, a, e in zip(('dq', 'dk', 'dv'), got, want):
             assert rel(a, e) < bound_of(torch.float16, e), (v_by, what, rel(a, e), bound_of(torch.float16, e))
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('by', [1e-3, 1.0])
+@pytest.mark.parametrize('heads,kv_heads,dim', [(16, 1, 64), (16, 1, 128), (32, 2, 128), (16, 1, 256)])
+def test_attention_gradients_of_short_sequences_under_many_heads(dt, by, heads, kv_heads, dim):
+    """Fewer than 1024 positions in the mean, but walks long enough to be cut into stretches: both at once."""
+    got, want, _, _ = attention_grads(dt, [500, 700], heads, kv_heads, dim, [by, by], seed=heads + dim)
+    for what, a, e in zip(('dq', 'dk', 'dv'), got, want):
+        assert rel(a, e) < bound_of(dt, e), (what, rel(a, e), bound_of(dt, e))
