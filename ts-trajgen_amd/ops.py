@@ -116,9 +116,9 @@ def _saved(what, ctx):
     """The saved tensors.  What a hook brings back has other addresses and strides; other shapes, types or devices would be read
     as what they are not."""
     tensors = ctx.saved_tensors
-    for t, like in zip(tensors, ctx.like):
-        if like is not None and (t.shape, t.dtype, t.device) != like:
-            raise RuntimeError('%s: a saved tensor %s came back as %s' % (what, like, (t.shape, t.dtype, t.device)))
+    now = [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+    if now != ctx.like:
+        raise RuntimeError('%s: saved tensors %s came back as %s' % (what, ctx.like, now))
     return tensors
 
 
@@ -233,8 +233,9 @@ class _CausalAttention(torch.autograd.Function):
             ws = _workspace(d, sizes[0], dev)  # noqa: F841  (held until the launches are on the stream)
             _call('tsg_attn_forward', d, dev)
             if train:
-                ctx.need, ctx.scale = sizes[1], scale
-                _save(ctx, ql, kl, vl, q_ptr, k_ptr, out, stats, rest)
+                ctx.need, ctx.desc = sizes[1], d
+                ctx.strides = ql.stride(), kl.stride(), vl.stride(), out.stride()
+                _save(ctx, ql, kl, vl, q_ptr, None if k_ptr is q_ptr else k_ptr, out, stats, rest)
         else:
             out.zero_()
         ctx.size = n_q, k.shape[0], heads, k.shape[1], dim, wide, per
@@ -250,12 +251,21 @@ class _CausalAttention(torch.autograd.Function):
         dv = torch.empty_like(dk)
         if ctx.need is not None:
             q, k, v, q_ptr, k_ptr, out, stats, rest = _saved('causal_attention', ctx)
-            q, k, v, out, gl = [_laid_out(t, per, wide) for t in (q, k, v, out, d_out)]
+            # the forward's sizes; every address anew, and the strides where a hook brought back others
+            d, at = _lib.AttnDesc.from_buffer_copy(ctx.desc), [t.data_ptr() for t in (q, k, v, out)]
+            if (at[0] | at[1] | at[2] | at[3]) & 15 or (q.stride(), k.stride(), v.stride(), out.stride()) != ctx.strides:
+                q, k, v, out = [_laid_out(t, per, wide) for t in (q, k, v, out)]
+                at = [t.data_ptr() for t in (q, k, v, out)]
+                (d.q_row, d.q_head), (d.k_row, d.k_head), (d.v_row, d.v_head), (d.out_row, d.out_head) = [
+                    t.stride()[:2] for t in (q, k, v, out)]
+            q_ptr, stats = q_ptr.contiguous(), stats.contiguous()
+            k_ptr = q_ptr if k_ptr is None else k_ptr.contiguous()
             rest = None if rest is None else rest.contiguous()
-            stats, q_ptr, k_ptr = stats.contiguous(), q_ptr.contiguous(), k_ptr.contiguous()
-            d = _attn_desc(q, k, v, q_ptr, k_ptr, ctx.scale, out, stats, rest)
+            d.q, d.k, d.v, d.out = at
+            d.q_ptr, d.k_ptr, d.stats, d.out_rest = q_ptr.data_ptr(), k_ptr.data_ptr(), stats.data_ptr(), _ptr(rest)
+            gl = _laid_out(d_out, per, wide)
             d.d_out, d.dq, d.dk, d.dv = gl.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-            d.delta = stats.data_ptr() + 8 * heads * n_q
+            d.delta = d.stats + 8 * heads * n_q
             d.d_out_row, d.d_out_head = gl.stride(0), gl.stride(1)
             d.dq_row, d.dk_row, d.dv_row = heads * wide, kv_heads * wide, kv_heads * wide
             d.dq_head = d.dk_head = d.dv_head = wide
@@ -321,15 +331,6 @@ def _rows_for(x, wide):
     return x.clone(memory_format=torch.contiguous_format)
 
 
-def _xent_desc(h, w, bias, target, ignore, reduction, store, loss):
-    rows, wide = h.shape
-    at = store.data_ptr()        # [rows][2] stats, [rows] losses, [2] scales of f32 operands
-    return _lib.XentDesc(DTYPES[h.dtype], wide, reduction, 0, rows, w.shape[0], ignore, h.data_ptr(), w.data_ptr(), _ptr(bias),
-                         max(h.stride(0), wide), max(w.stride(0), wide), target.data_ptr(),
-                         loss.data_ptr() if loss is not None and reduction == 0 else at + 8 * rows, _ptr(loss), at,
-                         at + 12 * rows if h.dtype == torch.float32 else None)
-
-
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, w, bias, target, ignore, reduction):
@@ -340,28 +341,35 @@ class _LinearCrossEntropy(torch.autograd.Function):
         tl = target.contiguous()
         store = torch.empty(3 * rows + 2, dtype=torch.float32, device=dev)
         loss = torch.empty(rows if reduction == 0 else (), dtype=torch.float32, device=dev)
-        d = _xent_desc(hl, wl, bl, tl, ignore, reduction, store, loss)
+        at = store.data_ptr()        # [rows][2] stats, [rows] losses, [2] scales of f32 operands
+        d = _lib.XentDesc(DTYPES[h.dtype], wide, reduction, 0, rows, w.shape[0], ignore, hl.data_ptr(), wl.data_ptr(), _ptr(bl),
+                          max(hl.stride(0), wide), max(wl.stride(0), wide), tl.data_ptr(),
+                          loss.data_ptr() if reduction == 0 else at + 8 * rows, loss.data_ptr(), at,
+                          at + 12 * rows if h.dtype == torch.float32 else None)
         sizes = _sizes('tsg_xent_workspace', d)
         ws = _workspace(d, sizes[0], dev)  # noqa: F841
         _call('tsg_xent_forward', d, dev)
         if any(ctx.needs_input_grad[:3]):
-            ctx.cfg = h.shape[1], wide, ignore, reduction, sizes[1]
+            ctx.cfg, ctx.desc = (h.shape[1], wide, sizes[1]), d
             _save(ctx, hl, wl, bl, tl, store)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss):
-        width, wide, ignore, reduction, need = ctx.cfg
+        width, wide, need = ctx.cfg
         h, w, bias, target, store = _saved('linear_cross_entropy', ctx)
-        dev = h.device
+        dev, rows, dt = h.device, h.shape[0], h.dtype
         h, w, target, store = _rows_for(h, wide), _rows_for(w, wide), target.contiguous(), store.contiguous()
         bias = None if bias is None else bias.contiguous()
         d_loss = d_loss.contiguous()
-        dh = torch.empty((h.shape[0], wide), dtype=h.dtype, device=dev)
-        dw = torch.empty((w.shape[0], wide), dtype=h.dtype, device=dev)
-        db = None if bias is None else torch.empty(w.shape[0], dtype=h.dtype, device=dev)
-        d = _xent_desc(h, w, bias, target, ignore, reduction, store, None)
+        dh = torch.empty((rows, wide), dtype=dt, device=dev)
+        dw = torch.empty((w.shape[0], wide), dtype=dt, device=dev)
+        db = None if bias is None else torch.empty(w.shape[0], dtype=dt, device=dev)
+        d = _lib.XentDesc.from_buffer_copy(ctx.desc)         # the forward's sizes; every address and stride anew
+        d.h, d.w, d.bias, d.target, d.stats = h.data_ptr(), w.data_ptr(), _ptr(bias), target.data_ptr(), store.data_ptr()
+        d.h_row, d.w_row = max(h.stride(0), wide), max(w.stride(0), wide)
+        d.row_loss, d.loss, d.scales = None, None, d.stats + 12 * rows if dt == torch.float32 else None
         d.d_loss, d.dh, d.dw, d.dbias = d_loss.data_ptr(), dh.data_ptr(), dw.data_ptr(), _ptr(db)
         d.dh_row = d.dw_row = wide
         ws = _workspace(d, need, dev)  # noqa: F841
