@@ -75,3 +75,31 @@ def test_attention_gradients_of_short_sequences_under_many_heads(dt, by, heads, 
     got, want, _, _ = attention_grads(dt, [500, 700], heads, kv_heads, dim, [by, by], seed=heads + dim)
     for what, a, e in zip(('dq', 'dk', 'dv'), got, want):
         assert rel(a, e) < bound_of(dt, e), (what, rel(a, e), bound_of(dt, e))
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('dim', [64, 128, 256])
+def test_attention_gradients_in_a_captured_graph(dt, dim):
+    """Replayed with upstream gradients of another size each time, between eager calls."""
+    from ts_trajgen_amd import ops
+    lens = [77, 600, 5]
+    p = torch.tensor(ptr(lens), dtype=torch.int32, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(dim)
+    q, k, v = (torch.randn(sum(lens), h, dim, generator=g, device=DEV).to(dt).requires_grad_(True) for h in (8, 1, 1))
+    base = torch.randn(sum(lens), 8, dim, generator=g, device=DEV)
+    do = torch.zeros(sum(lens), 8, dim, device=DEV, dtype=dt)
+
+    def step():
+        out = ops.causal_attention(q, k, v, p)
+        return (out.detach(),) + torch.autograd.grad(out, [q, k, v], do)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for by in (1e-4, 1.0, 5e3, 1e-2):
+        do.copy_(base * by)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, e in zip(captured, step()):
+            assert torch.equal(a, e)

@@ -104,3 +104,42 @@ def test_cross_entropy_rows_of_different_upstream_gradients_over_several_pieces(
     rows_within(got[0], dh, dt)
     rows_within(got[1], dw, dt)
     assert rel(got[2], db) < bound_of(dt, db)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_cross_entropy_upstream_gradients_of_zero_and_single_rows(dt):
+    from ts_trajgen_amd import ops
+    h, w, b, target = entropy_case(dt, 80, 600, 72, seed=2, ignored=0.0)
+    rows = ops.linear_cross_entropy(h, w, target, bias=b, reduction='none')
+    for g in torch.autograd.grad(rows, [h, w, b], torch.zeros(80, device=DEV), retain_graph=True):
+        assert float(g.abs().sum()) == 0.0
+    up = torch.zeros(80)
+    up[61] = -3e-5 if dt != torch.float16 else -3.0        # one row alone: its gradients are what a call of it alone gives
+    got = torch.autograd.grad(rows, [h, w, b], up.to(DEV))
+    _, *want = plain_cross_entropy(h, w, b, target, -100, up)
+    for a, e in zip(got, want):
+        assert rel(a, e) < bound_of(dt, e)
+    assert float(got[0][:61].abs().sum()) == 0.0 and float(got[0][62:].abs().sum()) == 0.0
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_cross_entropy_per_row_in_a_captured_graph(dt):
+    """Replayed with other upstream gradients of other sizes each time, between eager calls."""
+    from ts_trajgen_amd import ops
+    h, w, b, target = entropy_case(dt, 100, 700, 64, seed=10)
+    up = torch.zeros(100, device=DEV)
+
+    def step():
+        rows = ops.linear_cross_entropy(h, w, target, bias=b, reduction='none')
+        return (rows.detach(),) + torch.autograd.grad(rows, [h, w, b], up)
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = step()
+    for n in range(4):
+        up.copy_(torch.logspace(-3 - n, 2 * n, 100))
+        g.replay()
+        torch.cuda.synchronize()
+        for a, e in zip(captured, step()):
+            assert torch.equal(a, e)

@@ -156,3 +156,24 @@ def test_encoder_tensors_that_a_hook_changed_are_refused():
             out, _ = layer((torch.randn(9, 8, device=DEV, requires_grad=True), edges))
         with pytest.raises(RuntimeError, match='saved tensor'):
             out.sum().backward()
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_under_checkpoints_the_forward_runs_again(dt):
+    from torch.utils.checkpoint import checkpoint
+    from ts_trajgen_amd import ops
+    g = torch.Generator().manual_seed(9)
+    p = torch.tensor([0, 40, 43, N], dtype=torch.int32, device=DEV)
+    x = torch.randn(N, 2, 36, generator=g).to(dt).to(DEV).requires_grad_(True)
+    w = torch.randn(VOCAB, 72, generator=g).to(dt).to(DEV).requires_grad_(True)
+    target = torch.randint(0, VOCAB, (N,), generator=g).to(DEV)
+
+    def loss(x, w):
+        a = ops.causal_attention(x * 1.0, x * 0.5, x, p)
+        return ops.linear_cross_entropy(ops.dropout(a.reshape(N, 72), 0.3, 5, 2, 7), w, target)
+    want = torch.autograd.grad(loss(x, w), [x, w])
+    for reentrant in (False, True):
+        for t in (x, w):
+            t.grad = None
+        checkpoint(loss, x, w, use_reentrant=reentrant).backward()
+        assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
