@@ -143,3 +143,20 @@ def test_cross_entropy_per_row_in_a_captured_graph(dt):
         torch.cuda.synchronize()
         for a, e in zip(captured, step()):
             assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('t,v,k,reduction', [(2048, 1300, 64, 'mean'), (5000, 300, 256, 'none'), (20000, 2049, 100, 'sum'), (2100, 257, 512, 'mean')])
+def test_cross_entropy_many_rows_over_few_entries(dt, t, v, k, reduction):
+    """dW has a handful of tiles and a long sum there, which is cut into stretches of the rows."""
+    from ts_trajgen_amd import ops
+    h, w, b, target = entropy_case(dt, t, v, k, seed=t, ignored=0.1)
+    g = torch.Generator().manual_seed(t)
+    loss = ops.linear_cross_entropy(h, w, target, bias=b, reduction=reduction)
+    up = torch.rand(t, generator=g) + 0.5 if reduction == 'none' else torch.tensor(1.7)
+    got = torch.autograd.grad(loss, [h, w, b], up.to(DEV))
+    n = float((target != -100).sum())
+    d_row = up if reduction == 'none' else torch.full((t,), 1.7 / (n if reduction == 'mean' else 1.0))
+    _, *want = plain_cross_entropy(h, w, b, target, -100, d_row)
+    for a, e in zip(got, want):
+        assert rel(a, e) < bound_of(dt, e)

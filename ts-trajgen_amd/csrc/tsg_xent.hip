@@ -3,7 +3,7 @@
 //
 // forward   products in tiles of 256, 128 or 64 vocabulary rows by as many states (shape_of); their epilogue leaves (maximum, sum of
 //           exp) per state and tile, and the target's logit; a small kernel joins them.
-// backward  the vocabulary is taken in pieces (DZ_BUDGET).  Per piece the products are computed once more, their epilogue turns them into
+// backward  the vocabulary is taken in pieces (DZ_LEAST, DZ_MOST).  Per piece the products are computed once more, their epilogue turns them into
 //           dz_tv = g_t (softmax_tv - [v == target_t]) in 16 bits, and two further products read that:
 //           dW = dz^T h (whole for the piece) and dh += dz W (summed over the pieces in f32).  db comes from dz before
 //           its rounding.  8 T V K operations instead of the 6 of a form that keeps the logits.
@@ -732,11 +732,14 @@ Shape shape_of(int64_t m, int64_t n, int64_t times = 1) {
   return FEW;
 }
 constexpr int PLANE_BLOCKS = 512;
-// dz of a piece takes at most this much (but 256 vocabulary rows at least): large pieces fill the chip, small ones keep the memory of a call
-// far below the logits'.  Forward and backward, with the gradients, of 8192 x 40307 x 256, f32 (logits 1.32 GB) and 16384 x 50021 x 1024, bf16
-// (1.64 GB): 128 MiB 5.56 and 7.48 ms, 304 and 405 MB; 256 MiB 2.93 and 6.99 ms, 499 and 498 MB; 384 MiB 2.83 and 6.99 ms, 571 and 665 MB;
-// all in one piece 2.70 and 6.95 ms, 1634 and 1844 MB.
-constexpr size_t DZ_BUDGET = (size_t)384 << 20;
+// dz of a piece takes at most a quarter of the logits, within these bounds (but 256 vocabulary rows at least): large pieces fill the chip, small
+// ones keep the memory of a call far below the logits'.  Forward and backward, and the peak with the gradients, by the bound:
+//                               128 MiB          256              384              768              2 GiB
+//   8192 x 40307 x 256, f32     5.56 ms 0.30 GB  2.93 0.50        2.83 0.57        2.75 0.90        2.70 1.63 (all in one piece; logits 1.32 GB)
+//   16384 x 50021 x 1024, bf16  7.48    0.41     6.99 0.50        6.99 0.67        7.19 1.24        6.95 1.84 (likewise; 1.64 GB)
+//   67062 x 11096 x 256, f32                     9.58 0.51        8.43 0.65        7.30 1.06        6.94 1.83 (2.98 GB)
+//   30000 x 500000 x 128, f32                    130  0.88        115  1.03        107  1.43        101  2.74 (60 GB)
+constexpr size_t DZ_LEAST = (size_t)384 << 20, DZ_MOST = (size_t)2 << 30;
 
 Layout layout_of(const tsg_xent_desc* d, bool backward) {
   Layout l = {};
@@ -759,7 +762,9 @@ Layout layout_of(const tsg_xent_desc* d, bool backward) {
     l.zt = take(T * 4);
   } else {
     const size_t each = f32 ? 4 : 2;
-    size_t vc = DZ_BUDGET / (T * each) / 256 * 256;
+    size_t budget = T * V * each / 4;
+    budget = budget < DZ_LEAST ? DZ_LEAST : budget > DZ_MOST ? DZ_MOST : budget;
+    size_t vc = budget / (T * each) / 256 * 256;
     if (vc < 256) vc = 256;
     const size_t all = (V + 63) / 64 * 64;
     if (vc > all) vc = all;
@@ -789,15 +794,21 @@ Layout layout_of(const tsg_xent_desc* d, bool backward) {
     l.splits = (int)((vc + l.split_len - 1) / l.split_len);
     l.dh = take((size_t)l.splits * T * K * 4);
     // dW of a narrow state has few tiles too (40307 x 256: 158 of 256 x 256): cut the rows where that leaves the CUs less idle, each
-    // cut priced at 2 % for the sums it writes and reads again
+    // cut priced at 2 % for the sums it writes and reads again.  A narrow piece has a handful (1280 x 256: 5): cut until they fill the chip
+    // once, in stretches of 512 rows at least; the small tiles it would take else are slow over a long sum
+    // (67062 rows, f32: 1280 x 256 in 64 x 64 tiles 3115 us; 2304 x 256, twice the products, cut: 274).
     l.dw_shape = shape_of((int64_t)vc, (int64_t)K);
     l.dw_splits = 1;
     const int64_t big = (int64_t)tsg_cdiv(vc, Big::TM) * tsg_cdiv(K, Big::TN);
-    if (big < 768 && big >= 32 && T >= 2048) {
-      double best = 1e9;
-      for (int c = 1; c <= 8 && T / c >= 1024; ++c) {
-        const double cost = (double)((big * c + 255) / 256) / c + 0.02 * c;
-        if (cost < best) best = cost, l.dw_splits = c;
+    if (big < 768 && T >= 2048) {
+      if (big >= 32) {
+        double best = 1e9;
+        for (int c = 1; c <= 8 && T / c >= 1024; ++c) {
+          const double cost = (double)((big * c + 255) / 256) / c + 0.02 * c;
+          if (cost < best) best = cost, l.dw_splits = c;
+        }
+      } else {
+        l.dw_splits = (int)(T / 512 < (size_t)(256 / big) ? T / 512 : 256 / big);
       }
       l.dw_shape = BIG;
     }
