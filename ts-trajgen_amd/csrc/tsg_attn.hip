@@ -18,8 +18,8 @@
 // The backward is two kernels, one per output side (dq; dk and dv), each recomputing the scores: seven products instead
 // of five, no atomics, and results that do not depend on the order of workgroups.
 // 4 sequences of 2.5-4 k positions, 16 heads over 4, 128 wide, bf16: forward 236 us (775 TFLOP/s), dq 301 us (910, three products), dk and dv
-// 458 us (800, four products) and 29 us for joining the stretches; a large bf16 matrix product of the library: 1129.  Bound by the vector
-// work between the products (exponentials, packing, masks) and by LDS reads, with the matrix cores busy under half of the time.
+// 458 us (800, four products) and 29 us for joining the stretches; a large bf16 matrix product of the library: 1129.  Matrix cores busy 37, 46 and
+// 38 % of the time, vector units (exponentials, packing, masks) 39, 36 and 29 %, both at once 10-14 %, LDS 20-31 %, 1.5-1.7 waves a SIMD at work.
 #include "tsg_mma.h"
 
 namespace {
@@ -814,7 +814,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void attn_dkv_
 // 4 m + e, so that one load serves four products and a lane's results are 16 bytes side by side.
 // Buffers bound the operands: rows behind the interval and chunks behind the width read as zeros.
 // 2048 sequences of 2-64 positions, 256 wide: forward 80 us, dq 113 us, dk and dv 138 us; the operands and results alone are 110 us of a large
-// copy.  Bound by the matrix cores' f32 rate on blocks of which about half is masked, and by the loads' latency.
+// copy, but each kernel reads all operands again.  Bound by the loads: the matrix cores work 24-29 % of the time, vector units 16-20 %.
 struct Rows16 {  // one block of 16 rows, 64 columns
   __amdgpu_buffer_rsrc_t d;
   unsigned row, col, stride;  // the lane's byte offsets: its row fragment, its column fragment

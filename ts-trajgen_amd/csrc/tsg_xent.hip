@@ -17,9 +17,11 @@
 // matrix cores.  dz is rounded to the operand type (bf16: 2^-9 relative); it is brought to 2^15 for a
 // whole probability first, so that those down to 1e-9 stay above f16's subnormals; for f32 it is hi + lo as well.  Errors of dh and dW
 // against 64 bits, 16-bit types, 100 drawn shapes: at most 1.32 times those of 32-bit sums rounded once (1.47 for a pair of rows).
-// 16384 states x 50021 entries x 1024 wide, bf16 (1.68 TFLOP a product): statistics 1.65 ms (1020 TFLOP/s), dz 2.00 ms (840), dW 1.65 ms (1020),
-// dh 1.24 ms (1355); a large bf16 matrix product of the library: 1129.  8192 x 40307 x 256, f32: 0.61, 0.89, 0.55 and 0.48 ms, the f32 rate of the
-// library's product (153 TFLOP/s) would take 1.10 ms each.  The first two pay for exponentials in their epilogues and dz for writing them.
+// 16384 states x 50021 entries x 1024 wide, bf16 (1.68 TFLOP a product; five pieces): statistics 1.65-1.74 ms (970-1020 TFLOP/s), dz 1.91 ms (880),
+// dW 1.62 ms (1040), dh 1.42 ms (1180); a large bf16 matrix product of the library: 1129.  8192 x 40307 x 256, f32 (four pieces): 0.61, 0.88, 0.60
+// and 0.53 ms, the f32 rate of the library's product (153 TFLOP/s) would take 1.10 ms each.  The first two pay for their epilogues, which nothing
+// runs under: a 256 x 256 tile is one workgroup a CU, whose waves leave the products together (5000 x 40307 x 512, f16: matrix cores 27 % of
+// the time, vector units 36 %, both 1 %).
 // All sums, maxima and logarithms are f32.  Nothing depends on the order of workgroups: no floating-point atomics.
 #include "tsg_mma.h"
 

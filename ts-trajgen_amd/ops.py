@@ -381,7 +381,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
 def linear_cross_entropy(h, weight, target, bias=None, ignore_index=-100, reduction='mean'):
     """Cross entropy of softmax(h weight^T + bias) against target, differentiable in h, weight and bias, without the
-    [rows][vocabulary] logits being kept (they exist in pieces of the vocabulary, in the backward only).
+    [rows][vocabulary] logits being kept (their gradient exists in pieces of the vocabulary, in the backward only: a quarter of the logits,
+    between 384 MiB and 2 GiB).
 
     h [rows][hidden], weight [vocabulary][hidden] (function G's out_fc.weight, function_g_fc.py:134), bias [vocabulary] or
     None, all of one type (f32, bf16 or f16); target int64 [rows].  The loss is f32: per row ('none'), their sum
