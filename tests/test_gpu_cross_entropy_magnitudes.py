@@ -160,3 +160,16 @@ def test_cross_entropy_many_rows_over_few_entries(dt, t, v, k, reduction):
     _, *want = plain_cross_entropy(h, w, b, target, -100, d_row)
     for a, e in zip(got, want):
         assert rel(a, e) < bound_of(dt, e)
+
+
+@pytest.mark.parametrize('h_by,w_by', [(1e-36, 1.0), (1e-3, 1e-33), (1e18, 1e-18)])
+def test_cross_entropy_states_and_weights_at_the_ends_of_f32(h_by, w_by):
+    """Their planes are brought to f16's range by powers of two as far out as 2^126, which come off the gradients without passing through
+    f32's smallest numbers on the way."""
+    from ts_trajgen_amd import ops
+    h, w, b, target = entropy_case(torch.float32, 70, 500, 64, seed=6, h_by=h_by, w_by=w_by / 8, ignored=0.1)
+    loss = ops.linear_cross_entropy(h, w, target, bias=b, reduction='sum')
+    got = torch.autograd.grad(loss, [h, w, b])
+    _, *want = plain_cross_entropy(h, w, b, target, -100, torch.ones(70))
+    for a, e in zip(got, want):
+        rows_within(a if a.dim() == 2 else a.unsqueeze(0), e if e.dim() == 2 else e.unsqueeze(0), torch.float32)

@@ -60,12 +60,13 @@ struct DzUnit {  // what one of dz stands for, m 2^e; apart, so that neither end
   int e;
   __device__ __forceinline__ float of(float sum, int k = 0) const { return ldexpf(sum * m, e - k); }
 };
-// other: what the second operand of the sum was multiplied by, or null
+// other: what the second operand of the sum was multiplied by, a power of two, or null
 __device__ __forceinline__ DzUnit dz_unit(unsigned gmax, const float* other = nullptr) {
   DzUnit u = {1.0f, 0};
+  int e = 1;
   if (gmax) u.m = frexpf(__uint_as_float(gmax), &u.e);
-  u.e -= 15;
-  if (other) u.m /= *other;
+  if (other) frexpf(*other, &e);  // 2^(e - 1)
+  u.e -= 15 + e - 1;
   return u;
 }
 // what a magnitude says to a common scale: one that is not finite spoils its own row, not the others' precision

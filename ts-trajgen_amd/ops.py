@@ -208,6 +208,7 @@ def _sizes(entry, d):
 
 def _workspace(d, need, dev):
     if not need:
+        d.workspace, d.workspace_bytes = None, 0
         return None
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     d.workspace, d.workspace_bytes = ws.data_ptr(), need
